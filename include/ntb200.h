@@ -442,6 +442,92 @@ int ntb200_bias_add_channels(int dtype, void* x, const void* bias, int64_t batch
                              void* stream);
 int ntb200_sum_channels(int dtype, const void* grad, void* out, int64_t batch, int64_t channels, int64_t inner,
                         void* stream);
+/* ---- the residual feed-forward block: norm, linear with activation and residual, distillation loss -----------------
+ * No counterpart in the reference.  Operators that need scratch take it as `workspace` (16-byte aligned, at least
+ * ..._workspace_bytes), allocate nothing and keep nothing, so a call can be captured into any number of graphs as long
+ * as each graph has a workspace of its own.  Row strides are in elements; rows have a column stride of 1.
+ *
+ * ntb200_rms_norm: h = x + residual (h = x without one), rstd = (mean(h^2) + eps)^-1/2, y = h * rstd * weight for each
+ * of `rows` rows.  Sums and the norm use the unrounded fp32 h; y and h are rounded once.  F32, F16, BF16; y and h are
+ * contiguous.  residual, h and rstd may be NULL; h may be the residual or x itself (same row stride).
+ * ntb200_rms_norm_int8: the same y as Int8 rows with one scale each: with u = h * weight and A = max |u|,
+ * q = rint(u * 127 / A) and scale = A * rstd / 127, so y = q * scale.  A row of zeros has scale 0; a row with a NaN or
+ * an infinity has a scale that is not finite.
+ * ntb200_quantize_rows: q = rint(x * 127 / A), scale = A / 127 without any norm (hidden activations; weights, once).
+ * ntb200_rms_norm_backward: from h and rstd of the forward call, grad_y = dL/dy and grad_h = dL/dh over the residual
+ * stream (NULL: nothing arrives there): grad_x = dL/dx, which is also the residual's gradient, and grad_weight (may be
+ * NULL, then no workspace is needed).  grad_x may be grad_y or grad_h itself (contiguous). */
+int ntb200_rms_norm(int dtype, const void* x, int64_t x_row_stride, const void* residual, int64_t residual_row_stride,
+                    const void* weight, void* y, void* h, float* rstd, int64_t rows, int64_t cols, double eps, void* stream);
+int ntb200_rms_norm_int8(int dtype, const void* x, int64_t x_row_stride, const void* residual, int64_t residual_row_stride,
+                         const void* weight, int8_t* q, float* scale, void* h, int64_t rows, int64_t cols, double eps,
+                         void* stream);
+int ntb200_quantize_rows(int dtype, const void* x, int64_t x_row_stride, int8_t* q, float* scale, int64_t rows, int64_t cols,
+                         void* stream);
+size_t ntb200_rms_norm_backward_workspace_bytes(int64_t rows, int64_t cols);
+int ntb200_rms_norm_backward(int dtype, const void* h, int64_t h_row_stride, const void* weight, const float* rstd,
+                             const void* grad_y, int64_t grad_y_row_stride, const void* grad_h, int64_t grad_h_row_stride,
+                             void* grad_x, void* grad_weight, void* workspace, int64_t rows, int64_t cols, void* stream);
+
+/* y = act(x w + bias) + residual, x [m, k], w [k, n] (any non-negative strides, a transposed view included), in one GEMM
+ * whose epilogue does the rest on the fp32 sums; pre (may be NULL) receives x w + bias for the backward pass.
+ * dtype F32 / F16 / BF16: everything has that type.  dtype I8: x and w are Int8 with a scale for each row of x and each
+ * column of w (fp32), the product is exact in s32, and bias, residual, pre and y have out_dtype (F32 / F16 / BF16).
+ * GELU is z Phi(z) with the normal distribution's Phi, GELU_TANH its usual tanh form, SILU z / (1 + e^-z).
+ * y may be the residual itself (same row stride).  16-bit and Int8 products always run on the tensor cores: operands
+ * whose rows do not start on 16 bytes are copied into the workspace first. */
+typedef enum ntb200_activation {
+    NTB200_ACT_NONE = 0,
+    NTB200_ACT_RELU = 1,
+    NTB200_ACT_GELU = 2,
+    NTB200_ACT_GELU_TANH = 3,
+    NTB200_ACT_SILU = 4
+} ntb200_activation;
+typedef struct ntb200_linear_desc {
+    int32_t dtype, out_dtype, activation, reserved;
+    int64_t m, n, k;
+    const void* x; int64_t x_row_stride, x_col_stride;
+    const void* w; int64_t w_row_stride, w_col_stride;
+    const float* x_scale;      /* [m], I8 only */
+    const float* w_scale;      /* [n], I8 only */
+    const void* bias;          /* [n] or NULL */
+    const void* residual; int64_t residual_row_stride;
+    void* y; int64_t y_row_stride;
+    void* pre; int64_t pre_row_stride;
+} ntb200_linear_desc;
+size_t ntb200_linear_act_workspace_bytes(const ntb200_linear_desc* desc);
+int ntb200_linear_act(const ntb200_linear_desc* desc, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Backward pass of ntb200_linear_act for F32 / F16 / BF16: with gz = grad_out * act'(pre), grad_x = gz w^T [m, k],
+ * grad_w = x^T gz [k, n] (or [n, k] with grad_w_transposed, for weights kept as [out, in]) and grad_bias = column sums of
+ * gz; each may be NULL.  The residual's gradient is grad_out itself.  pre may be NULL when the activation is NONE.  gz is
+ * rounded to the operands' type for the two products (the bias gradient sums it unrounded). */
+typedef struct ntb200_linear_backward_desc {
+    int32_t dtype, activation, grad_w_transposed, reserved;
+    int64_t m, n, k;
+    const void* x; int64_t x_row_stride, x_col_stride;
+    const void* w; int64_t w_row_stride, w_col_stride;
+    const void* pre; int64_t pre_row_stride;
+    const void* grad_out; int64_t grad_out_row_stride;
+    void* grad_x;
+    void* grad_w;
+    void* grad_bias;
+} ntb200_linear_backward_desc;
+size_t ntb200_linear_act_backward_workspace_bytes(const ntb200_linear_backward_desc* desc);
+int ntb200_linear_act_backward(const ntb200_linear_backward_desc* desc, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Distillation from a teacher's `top` largest logits of each row: teacher [rows, top] values and index [rows, top] their
+ * columns (I32 or I64); an entry whose column lies outside [0, vocab), or whose value is -inf, is not there.  With
+ * p = softmax over the row's entries of teacher / T and q = softmax(logits / T) over all columns,
+ *   row_loss = T^2 sum_j p_j (log p_j - log q_{i_j}),   *loss = sum over rows of row_weight * row_loss,
+ *   grad = d loss / d logits = row_weight T (q - p)   (a column named twice takes the sum of its p).
+ * A row without entries or with weight 0 has loss 0 and a gradient of zeros.  row_weight [rows] fp32, NULL: 1 / rows (the
+ * mean).  grad may be NULL (loss only) or the logits themselves.  At most 1024 entries per row. */
+int ntb200_distill_topk(int dtype, const void* logits, int64_t logits_row_stride, int teacher_dtype, const void* teacher,
+                        int index_dtype, const void* index, const float* row_weight, void* grad, int64_t grad_row_stride,
+                        float* row_loss, float* loss, int64_t rows, int64_t vocab, int64_t top, double temperature,
+                        void* stream);
+
 /* dst[rows, cols] (contiguous) = src viewed with the given element strides: Tensor::contiguous(). */
 int ntb200_copy_strided_2d(int dtype, void* dst, const void* src, int64_t batch, int64_t rows, int64_t cols,
                            int64_t src_batch_stride, int64_t src_row_stride, int64_t src_col_stride, void* stream);

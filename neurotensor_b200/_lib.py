@@ -47,6 +47,30 @@ class GemmEpilogue(ctypes.Structure):
     _fields_ = [("relu_out", _vp), ("relu_mask_src", _vp)]
 
 
+ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU = range(5)
+
+
+class LinearDesc(ctypes.Structure):
+    """ntb200_linear_desc."""
+    _fields_ = [(n, ctypes.c_int32) for n in ("dtype", "out_dtype", "activation", "reserved")] + \
+               [("m", _i64), ("n", _i64), ("k", _i64),
+                ("x", _vp), ("x_row_stride", _i64), ("x_col_stride", _i64),
+                ("w", _vp), ("w_row_stride", _i64), ("w_col_stride", _i64),
+                ("x_scale", _vp), ("w_scale", _vp), ("bias", _vp),
+                ("residual", _vp), ("residual_row_stride", _i64),
+                ("y", _vp), ("y_row_stride", _i64), ("pre", _vp), ("pre_row_stride", _i64)]
+
+
+class LinearBackwardDesc(ctypes.Structure):
+    """ntb200_linear_backward_desc."""
+    _fields_ = [(n, ctypes.c_int32) for n in ("dtype", "activation", "grad_w_transposed", "reserved")] + \
+               [("m", _i64), ("n", _i64), ("k", _i64),
+                ("x", _vp), ("x_row_stride", _i64), ("x_col_stride", _i64),
+                ("w", _vp), ("w_row_stride", _i64), ("w_col_stride", _i64),
+                ("pre", _vp), ("pre_row_stride", _i64), ("grad_out", _vp), ("grad_out_row_stride", _i64),
+                ("grad_x", _vp), ("grad_w", _vp), ("grad_bias", _vp)]
+
+
 ALLGATHER_FN = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t)
 
 # name -> (restype, argtypes); every symbol include/ntb200.h declares
@@ -136,6 +160,17 @@ SIGNATURES = {
     "ntb200_sum_channels": (_ci, [_ci, _vp, _vp, _i64, _i64, _i64, _vp]),
     "ntb200_sgd_step": (_ci, [_ci, _vp, _vp, _i64, ctypes.c_double, _vp]),
     "ntb200_adam_step": (_ci, [_ci, _vp, _vp, _vp, _vp, _i64] + [ctypes.c_double] * 4 + [_i64, _vp]),
+    "ntb200_rms_norm": (_ci, [_ci, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, ctypes.c_double, _vp]),
+    "ntb200_rms_norm_int8": (_ci, [_ci, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, ctypes.c_double, _vp]),
+    "ntb200_quantize_rows": (_ci, [_ci, _vp, _i64, _vp, _vp, _i64, _i64, _vp]),
+    "ntb200_rms_norm_backward_workspace_bytes": (_sz, [_i64, _i64]),
+    "ntb200_rms_norm_backward": (_ci, [_ci, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _vp]),
+    "ntb200_linear_act_workspace_bytes": (_sz, [ctypes.POINTER(LinearDesc)]),
+    "ntb200_linear_act": (_ci, [ctypes.POINTER(LinearDesc), _vp, _sz, _vp]),
+    "ntb200_linear_act_backward_workspace_bytes": (_sz, [ctypes.POINTER(LinearBackwardDesc)]),
+    "ntb200_linear_act_backward": (_ci, [ctypes.POINTER(LinearBackwardDesc), _vp, _sz, _vp]),
+    "ntb200_distill_topk": (_ci, [_ci, _vp, _i64, _ci, _vp, _ci, _vp, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _i64,
+                                  ctypes.c_double, _vp]),
     "ntb200_copy_strided_2d": (_ci, [_ci, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp]),
     "ntb200_convert": (_ci, [_ci, _vp, _ci, _vp, _i64, _vp]),
 }

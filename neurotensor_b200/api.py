@@ -975,3 +975,307 @@ def matmult_host(a, b, c, transpose_a=False, transpose_b=False, accumulate=True)
     check(lib().ntb200_matmult_host(ca, pa, pb, pc, batches, am, ak, bk, bn, int(transpose_a), int(transpose_b),
                                     int(bool(accumulate))))
     return c
+
+
+# ---- the residual feed-forward block: norm, linear with activation and residual, distillation loss -------------------
+
+_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+_ACTIVATIONS = {"none": _lib.ACT_NONE, None: _lib.ACT_NONE, "relu": _lib.ACT_RELU, "gelu": _lib.ACT_GELU,
+                "gelu_tanh": _lib.ACT_GELU_TANH, "silu": _lib.ACT_SILU}
+
+
+def _on_device(what, first, *others):
+    """Every operand on the first one's device, and that device current: the C ABI works on the current one."""
+    if not first.is_cuda:
+        raise ValueError("neurotensor_b200 operates on CUDA tensors only (there is no CPU path)")
+    dev = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != dev:
+            raise ValueError("%s: every tensor must be on the same CUDA device" % what)
+    if dev != torch.cuda.current_device():
+        raise ValueError("%s: the tensors are on cuda:%d but cuda:%d is the current device" % (what, dev, torch.cuda.current_device()))
+
+
+def _rows_of(t):
+    """(tensor, rows, row stride) of `t` seen as rows of its last dim; a layout that has no row stride is made contiguous."""
+    if t.dim() == 2:
+        rows, rs = t.shape[0], t.stride(0)
+    elif t.dim() == 1:
+        rows, rs = 1, t.shape[0]
+    elif t.is_contiguous():
+        rows, rs = t.numel() // max(1, t.shape[-1]), t.shape[-1]
+    else:
+        return _rows_of(t.reshape(-1, t.shape[-1]))
+    if t.shape[-1] != 1 and t.stride(-1) != 1 or (rows > 1 and rs < t.shape[-1]):
+        return _rows_of(t.contiguous())
+    return t, rows, rs
+
+
+def _activation(name):
+    try:
+        return _ACTIVATIONS[name]
+    except (KeyError, TypeError):
+        raise ValueError("Expected the activation to be one of none, relu, gelu, gelu_tanh, silu but got %r" % (name,))
+
+
+def _norm_operands(what, x, weight, residual):
+    if x.dtype not in _FLOATS:
+        raise ValueError("%s: expected Float32, Float16 or BFloat16 but got %s" % (what, x.dtype))
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError("%s: expected rows of at least one element but got shape %s" % (what, tuple(x.shape)))
+    if weight is not None and (weight.dim() != 1 or weight.shape[0] != x.shape[-1] or weight.dtype != x.dtype):
+        raise ValueError("%s: expected a weight of %d values of %s but got %s of %s"
+                         % (what, x.shape[-1], x.dtype, tuple(weight.shape), weight.dtype))
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+        raise ValueError("%s: expected a residual of shape %s and %s but got %s and %s"
+                         % (what, tuple(x.shape), x.dtype, tuple(residual.shape), residual.dtype))
+
+
+def rms_norm(x, weight, eps=1e-6, residual=None):
+    """h = x + residual, y = h * rstd * weight over the last dim, rstd = (mean(h^2) + eps)^-1/2.
+    Returns (y, h, rstd): h is x itself without a residual, rstd (fp32, one per row) is what rms_norm_backward takes.
+    The norm uses the unrounded sum h."""
+    _norm_operands("rms_norm", x, weight, residual)
+    _on_device("rms_norm", x, weight, residual)
+    xr, rows, x_rs = _rows_of(x)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    h, rr, r_rs = x, None, 0
+    if residual is not None:
+        h = torch.empty_like(y)
+        rr, _, r_rs = _rows_of(residual)
+    w = weight if weight.stride(0) == 1 else weight.contiguous()
+    check(lib().ntb200_rms_norm(dtype_code(x), xr.data_ptr(), x_rs, None if rr is None else rr.data_ptr(), r_rs, w.data_ptr(),
+                                y.data_ptr(), None if rr is None else h.data_ptr(), rstd.data_ptr(), rows, x.shape[-1], eps,
+                                _stream()))
+    return y, h, rstd
+
+
+def rms_norm_int8(x, weight, eps=1e-6, residual=None):
+    """rms_norm whose output leaves as Int8 rows with one fp32 scale each (y = q * scale): what linear_int8 reads.
+    Returns (q, scale, h)."""
+    _norm_operands("rms_norm_int8", x, weight, residual)
+    _on_device("rms_norm_int8", x, weight, residual)
+    xr, rows, x_rs = _rows_of(x)
+    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    h, rr, r_rs = x, None, 0
+    if residual is not None:
+        h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        rr, _, r_rs = _rows_of(residual)
+    w = weight if weight.stride(0) == 1 else weight.contiguous()
+    check(lib().ntb200_rms_norm_int8(dtype_code(x), xr.data_ptr(), x_rs, None if rr is None else rr.data_ptr(), r_rs, w.data_ptr(),
+                                     q.data_ptr(), scale.data_ptr(), None if rr is None else h.data_ptr(), rows, x.shape[-1], eps,
+                                     _stream()))
+    return q, scale, h
+
+
+def quantize_rows(x):
+    """(q, scale): every row of the last dim as Int8 with one fp32 scale, x ~ q * scale, scale = max |row| / 127.
+    For hidden activations, and once for weights kept as [out, in]."""
+    _norm_operands("quantize_rows", x, None, None)
+    _on_device("quantize_rows", x)
+    xr, rows, x_rs = _rows_of(x)
+    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    check(lib().ntb200_quantize_rows(dtype_code(x), xr.data_ptr(), x_rs, q.data_ptr(), scale.data_ptr(), rows, x.shape[-1], _stream()))
+    return q, scale
+
+
+def rms_norm_backward(h, weight, rstd, grad_y, grad_h=None, want_weight=True):
+    """(grad_x, grad_weight) of rms_norm from its h and rstd.  grad_h is the gradient that arrives over the residual
+    stream h; grad_x is also the gradient of the residual.  grad_weight is None unless wanted."""
+    _norm_operands("rms_norm_backward", h, weight, None)
+    for t, name in ((grad_y, "grad_y"), (grad_h, "grad_h")):
+        if t is not None and (t.shape != h.shape or t.dtype != h.dtype):
+            raise ValueError("rms_norm_backward: expected %s of shape %s and %s but got %s and %s"
+                             % (name, tuple(h.shape), h.dtype, tuple(t.shape), t.dtype))
+    if rstd.shape != h.shape[:-1] or rstd.dtype != torch.float32:
+        raise ValueError("rms_norm_backward: expected rstd of shape %s in Float32 but got %s in %s"
+                         % (tuple(h.shape[:-1]), tuple(rstd.shape), rstd.dtype))
+    _on_device("rms_norm_backward", h, weight, rstd, grad_y, grad_h)
+    cols = h.shape[-1]
+    hr, rows, h_rs = _rows_of(h)
+    gr, _, g_rs = _rows_of(grad_y)
+    sr, _, s_rs = _rows_of(grad_h) if grad_h is not None else (None, 0, 0)
+    w = weight if weight.stride(0) == 1 else weight.contiguous()
+    rs = rstd if rstd.is_contiguous() else rstd.contiguous()
+    gx = torch.empty(h.shape, dtype=h.dtype, device=h.device)
+    gw = ws = None
+    if want_weight:
+        gw = torch.empty(cols, dtype=h.dtype, device=h.device)
+        ws = torch.empty(max(1, lib().ntb200_rms_norm_backward_workspace_bytes(rows, cols)), dtype=torch.uint8, device=h.device)
+    check(lib().ntb200_rms_norm_backward(dtype_code(h), hr.data_ptr(), h_rs, w.data_ptr(), rs.data_ptr(), gr.data_ptr(), g_rs,
+                                         None if sr is None else sr.data_ptr(), s_rs, gx.data_ptr(),
+                                         None if gw is None else gw.data_ptr(), None if ws is None else ws.data_ptr(), rows, cols,
+                                         _stream()))
+    return gx, gw
+
+
+def _linear_desc(what, x, w, bias, activation, residual, transpose_w, dtype):
+    """Checked ntb200_linear_desc without its outputs, the output's shape, and the tensors it points into."""
+    if x.dim() < 1 or w.dim() != 2:
+        raise ValueError("%s: expected rows of x and a 2-D weight but got %dD and %dD" % (what, x.dim(), w.dim()))
+    k, n = (w.shape[1], w.shape[0]) if transpose_w else (w.shape[0], w.shape[1])
+    if x.shape[-1] != k:
+        raise ValueError("%s: expected the weight to take %d inputs when it took %d" % (what, x.shape[-1], k))
+    shape = x.shape[:-1] + (n,)
+    if bias is not None and (bias.dim() != 1 or bias.shape[0] != n or bias.dtype != dtype):
+        raise ValueError("%s: expected a bias of %d values of %s but got %s of %s" % (what, n, dtype, tuple(bias.shape), bias.dtype))
+    if residual is not None and (residual.shape != shape or residual.dtype != dtype):
+        raise ValueError("%s: expected a residual of shape %s and %s but got %s and %s"
+                         % (what, tuple(shape), dtype, tuple(residual.shape), residual.dtype))
+    _on_device(what, x, w, bias, residual)
+    xr, rows, x_rs = _rows_of(x)
+    d = _lib.LinearDesc()
+    d.dtype, d.out_dtype, d.activation = _TORCH_TO_CODE[x.dtype], _TORCH_TO_CODE[dtype], _activation(activation)
+    d.m, d.n, d.k = rows, n, k
+    d.x, d.x_row_stride, d.x_col_stride = xr.data_ptr(), x_rs, 1
+    s0, s1 = w.stride()
+    d.w, d.w_row_stride, d.w_col_stride = w.data_ptr(), (s1 if transpose_w else s0), (s0 if transpose_w else s1)
+    keep = [xr]
+    if bias is not None:
+        b = bias if bias.stride(0) == 1 else bias.contiguous()
+        d.bias = b.data_ptr()
+        keep.append(b)
+    if residual is not None:
+        rr, _, r_rs = _rows_of(residual)
+        d.residual, d.residual_row_stride = rr.data_ptr(), r_rs
+        keep.append(rr)
+    return d, shape, keep
+
+
+def _run_linear(d, y):
+    d.y, d.y_row_stride = y.data_ptr(), d.n
+    need = lib().ntb200_linear_act_workspace_bytes(ctypes.byref(d))
+    ws = torch.empty(need, dtype=torch.uint8, device=y.device) if need else None
+    check(lib().ntb200_linear_act(ctypes.byref(d), None if ws is None else ws.data_ptr(), need, _stream()))
+
+
+def linear_act(x, w, bias=None, activation="none", residual=None, transpose_w=False, want_pre=False):
+    """act(x.w + bias) + residual in one GEMM: the bias, the activation (none, relu, gelu, gelu_tanh, silu) and the
+    residual are applied to the fp32 sums in its epilogue and rounded once.  w is [in, out] like functional::linear's
+    weight, or [out, in] with transpose_w.  Float32, Float16, BFloat16.
+    want_pre: returns (y, pre) with pre = x.w + bias, which linear_act_backward takes."""
+    if x.dtype not in _FLOATS or w.dtype != x.dtype:
+        raise ValueError("linear_act: expected both tensors to be Float32, Float16 or BFloat16 alike but got %s and %s" % (x.dtype, w.dtype))
+    d, shape, keep = _linear_desc("linear_act", x, w, bias, activation, residual, transpose_w, x.dtype)
+    y = torch.empty(shape, dtype=x.dtype, device=x.device)
+    if want_pre:
+        pre = torch.empty_like(y)
+        d.pre, d.pre_row_stride = pre.data_ptr(), d.n
+        _run_linear(d, y)
+        return y, pre
+    _run_linear(d, y)
+    return y
+
+
+def linear_int8(q, scale, w, w_scale, bias=None, activation="none", residual=None, transpose_w=False, dtype=torch.bfloat16):
+    """act((q.w) * scale * w_scale + bias) + residual for Int8 rows q with a scale each (rms_norm_int8, quantize_rows)
+    and an Int8 weight with a scale for each output; the product is exact.  The result, bias and residual have `dtype`."""
+    if q.dtype != torch.int8 or w.dtype != torch.int8:
+        raise ValueError("linear_int8: expected Int8 operands but got %s and %s" % (q.dtype, w.dtype))
+    if dtype not in _FLOATS:
+        raise ValueError("linear_int8: expected an output of Float32, Float16 or BFloat16 but got %s" % (dtype,))
+    d, shape, keep = _linear_desc("linear_int8", q, w, bias, activation, residual, transpose_w, dtype)
+    if scale.shape != q.shape[:-1] or scale.dtype != torch.float32:
+        raise ValueError("linear_int8: expected scales of shape %s in Float32 but got %s in %s"
+                         % (tuple(q.shape[:-1]), tuple(scale.shape), scale.dtype))
+    if w_scale.dim() != 1 or w_scale.shape[0] != d.n or w_scale.dtype != torch.float32:
+        raise ValueError("linear_int8: expected %d weight scales in Float32 but got %s in %s" % (d.n, tuple(w_scale.shape), w_scale.dtype))
+    if d.k > 131071:
+        raise ValueError("linear_int8: Int8 sums are exact up to 131071 inputs but got %d" % d.k)
+    _on_device("linear_int8", q, scale, w_scale)
+    s = scale if scale.is_contiguous() else scale.contiguous()
+    v = w_scale if w_scale.stride(0) == 1 else w_scale.contiguous()
+    d.x_scale, d.w_scale = s.data_ptr(), v.data_ptr()
+    y = torch.empty(shape, dtype=dtype, device=q.device)
+    _run_linear(d, y)
+    return y
+
+
+def linear_act_backward(x, w, pre, grad_out, activation="none", transpose_w=False, want_x=True, want_w=True, want_bias=True):
+    """(grad_x, grad_w, grad_bias) of linear_act: gz = grad_out * act'(pre), grad_x = gz.w^T, grad_w = x^T.gz (shaped like
+    w), grad_bias = column sums of gz.  The residual's gradient is grad_out itself.  pre may be None without an activation."""
+    act = _activation(activation)
+    if x.dtype not in _FLOATS or w.dtype != x.dtype or grad_out.dtype != x.dtype or (pre is not None and pre.dtype != x.dtype):
+        raise ValueError("linear_act_backward: expected tensors of one dtype, Float32, Float16 or BFloat16, but got %s, %s and %s"
+                         % (x.dtype, w.dtype, grad_out.dtype))
+    if w.dim() != 2 or x.dim() < 1:
+        raise ValueError("linear_act_backward: expected rows of x and a 2-D weight but got %dD and %dD" % (x.dim(), w.dim()))
+    k, n = (w.shape[1], w.shape[0]) if transpose_w else (w.shape[0], w.shape[1])
+    shape = x.shape[:-1] + (n,)
+    if x.shape[-1] != k or grad_out.shape != shape or (pre is not None and pre.shape != shape):
+        raise ValueError("linear_act_backward: shapes %s, %s and %s do not belong together"
+                         % (tuple(x.shape), tuple(w.shape), tuple(grad_out.shape)))
+    if pre is None and act != _lib.ACT_NONE:
+        raise ValueError("linear_act_backward: the pre-activation is needed for %s" % activation)
+    _on_device("linear_act_backward", x, w, pre, grad_out)
+    if n == 0 or k == 0:
+        raise ValueError("linear_act_backward: expected a weight with elements but got shape %s" % (tuple(w.shape),))
+    xr, rows, x_rs = _rows_of(x)
+    gr, _, g_rs = _rows_of(grad_out)
+    d = _lib.LinearBackwardDesc()
+    d.dtype, d.activation, d.grad_w_transposed = _TORCH_TO_CODE[x.dtype], act, int(bool(transpose_w))
+    d.m, d.n, d.k = rows, n, k
+    d.x, d.x_row_stride, d.x_col_stride = xr.data_ptr(), x_rs, 1
+    s0, s1 = w.stride()
+    d.w, d.w_row_stride, d.w_col_stride = w.data_ptr(), (s1 if transpose_w else s0), (s0 if transpose_w else s1)
+    d.grad_out, d.grad_out_row_stride = gr.data_ptr(), g_rs
+    if act != _lib.ACT_NONE:
+        pr, _, p_rs = _rows_of(pre)
+        d.pre, d.pre_row_stride = pr.data_ptr(), p_rs
+    gx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_x else None
+    gw = torch.empty(w.shape, dtype=x.dtype, device=x.device) if want_w else None
+    gb = torch.empty(n, dtype=x.dtype, device=x.device) if want_bias else None
+    d.grad_x, d.grad_w, d.grad_bias = (None if t is None else t.data_ptr() for t in (gx, gw, gb))
+    need = lib().ntb200_linear_act_backward_workspace_bytes(ctypes.byref(d))
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    check(lib().ntb200_linear_act_backward(ctypes.byref(d), None if ws is None else ws.data_ptr(), need, _stream()))
+    return gx, gw, gb
+
+
+def distill_topk(logits, teacher, index, temperature=1.0, row_weight=None, want_grad=True, out_grad=None):
+    """Divergence of softmax(logits / T) from a teacher known by its top logits: `teacher` holds their values, `index`
+    their columns (a column outside the vocabulary, -1 for instance, or a value of -inf marks an entry that is not there).
+    Returns (loss, row_loss, grad): loss = sum of row_weight * row_loss (mean over rows by default), grad = d loss /
+    d logits (None unless wanted).  out_grad: where the gradient goes; the logits themselves will do."""
+    what = "distill_topk"
+    if logits.dtype not in _FLOATS or teacher.dtype not in _FLOATS:
+        raise ValueError("%s: expected Float32, Float16 or BFloat16 logits but got %s and %s" % (what, logits.dtype, teacher.dtype))
+    if index.dtype not in (torch.int32, torch.int64):
+        raise ValueError("%s: expected Int32 or Int64 columns but got %s" % (what, index.dtype))
+    if logits.dim() < 1 or logits.shape[-1] < 1 or teacher.dim() < 1 or teacher.shape[:-1] != logits.shape[:-1] or index.shape != teacher.shape:
+        raise ValueError("%s: shapes %s, %s and %s do not belong together"
+                         % (what, tuple(logits.shape), tuple(teacher.shape), tuple(index.shape)))
+    top = teacher.shape[-1]
+    if not 1 <= top <= 1024:
+        raise ValueError("%s: expected 1 to 1024 teacher entries per row but got %d" % (what, top))
+    if not 0 < temperature < 1e30:
+        raise ValueError("%s: the temperature must be positive and finite but got %r" % (what, temperature))
+    if row_weight is not None and (row_weight.shape != logits.shape[:-1] or row_weight.dtype != torch.float32):
+        raise ValueError("%s: expected row weights of shape %s in Float32 but got %s in %s"
+                         % (what, tuple(logits.shape[:-1]), tuple(row_weight.shape), row_weight.dtype))
+    if out_grad is not None and (out_grad.shape != logits.shape or out_grad.dtype != logits.dtype):
+        raise ValueError("%s: expected out_grad to be shaped and typed like the logits" % what)
+    _on_device(what, logits, teacher, index, row_weight, out_grad)
+    sr, rows, s_rs = _rows_of(logits)
+    t = teacher if teacher.is_contiguous() else teacher.contiguous()
+    i = index if index.is_contiguous() else index.contiguous()
+    rw = row_weight if row_weight is None or row_weight.is_contiguous() else row_weight.contiguous()
+    grad, g_rs = None, 0
+    if want_grad or out_grad is not None:
+        if out_grad is None:
+            grad, g_rs = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device), logits.shape[-1]
+        else:
+            grad, _, g_rs = _rows_of(out_grad)
+            if grad.data_ptr() != out_grad.data_ptr():
+                raise ValueError("%s: out_grad needs rows with a stride" % what)
+            grad = out_grad
+    row_loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=logits.device)
+    loss = torch.empty((), dtype=torch.float32, device=logits.device)
+    check(lib().ntb200_distill_topk(_TORCH_TO_CODE[logits.dtype], sr.data_ptr(), s_rs, _TORCH_TO_CODE[t.dtype], t.data_ptr(),
+                                    _TORCH_TO_CODE[i.dtype], i.data_ptr(), None if rw is None else rw.data_ptr(),
+                                    None if grad is None else grad.data_ptr(), g_rs, row_loss.data_ptr(), loss.data_ptr(), rows,
+                                    logits.shape[-1], top, float(temperature), _stream()))
+    return loss, row_loss, grad

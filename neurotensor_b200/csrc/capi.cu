@@ -110,8 +110,20 @@ size_t scratch_keep_limit() {
 }
 }  // namespace
 
+thread_local ScratchArena* t_arena = nullptr;
+ScratchArena::ScratchArena(void* b, size_t n) : base(static_cast<char*>(b)), bytes(n), outer(t_arena) { t_arena = this; }
+ScratchArena::~ScratchArena() { t_arena = outer; }
+
 int scratch_acquire(void** out, size_t bytes, cudaStream_t stream) {
     *out = nullptr;
+    if (t_arena) {
+        const size_t at = (t_arena->used + 255) & ~size_t(255);
+        if (at > t_arena->bytes || bytes > t_arena->bytes - at)
+            return fail(NTB200_ERR_ALLOC, "the workspace of %zu bytes is too small (%zu more bytes wanted)", t_arena->bytes, bytes);
+        *out = t_arena->base + at;
+        t_arena->used = at + bytes;
+        return NTB200_OK;
+    }
     if (bytes == 0) bytes = 256;
     bytes = (bytes + ((size_t(1) << 20) - 1)) & ~((size_t(1) << 20) - 1);   // whole MiB: a slightly larger next call still fits
     g_scratch_acquires.fetch_add(1, std::memory_order_relaxed);
@@ -162,6 +174,7 @@ int scratch_acquire(void** out, size_t bytes, cudaStream_t stream) {
 
 void scratch_release(void* ptr, cudaStream_t stream) {
     if (!ptr) return;
+    if (t_arena) return;   // the caller's block: its pieces live until the call ends
     {
         std::lock_guard<std::mutex> lk(g_scratch_mu);
         for (auto& b : g_scratch)

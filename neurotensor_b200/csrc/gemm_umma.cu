@@ -35,6 +35,7 @@
 #include <mutex>
 
 #include "internal.h"
+#include "linear_epilogue.cuh"
 #include "sm100_ptx.cuh"
 
 namespace ntb200 {
@@ -88,6 +89,7 @@ struct UmmaParams {
     uint32_t s_stage_tx;         // bytes the TMA loads of one stage deliver
     long long relu_out_offset;   // second output: max(C, 0)
     long long mask_offset;       // input h: the result is zeroed where h < 0 (ReLU backward)
+    LinearParams linear;         // the kernels' kLinear instantiations: everything after the product
 };
 
 // Tensor maps of the peer-mapped copies of C (TMA-store epilogue of ntb200_gemm_push); only the first n_peers are valid.
@@ -210,12 +212,39 @@ __device__ __forceinline__ void drain_partial(uint32_t taddr, float (&run)[HC], 
             run[cc * 32 + j] = first ? __uint_as_float(v[j]) : run[cc * 32 + j] + __uint_as_float(v[j]);
     }
 }
-template <int HC>
+template <int HC, bool kLinear>
 __device__ __forceinline__ void store_running(const UmmaParams& p, const float (&run)[HC], int b, int row, int col_base) {
     if (row >= p.m) return;
 #pragma unroll
-    for (int cc = 0; cc < HC / 32; ++cc)
-        if (col_base + cc * 32 < p.n) store_chunk_f32(p, b, row, col_base + cc * 32, &run[cc * 32]);
+    for (int cc = 0; cc < HC / 32; ++cc) {
+        if (col_base + cc * 32 >= p.n) continue;
+        if constexpr (kLinear) {
+            float f[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) f[j] = run[cc * 32 + j];
+            linear_finish32(p.linear, p.n, row, col_base + cc * 32, f);
+        } else {
+            store_chunk_f32(p, b, row, col_base + cc * 32, &run[cc * 32]);
+        }
+    }
+}
+
+// Epilogue of the kLinear instantiations (Float16 / BFloat16 / Int8 operands): each thread owns a row of the tile.
+template <int BN, bool kInt>
+__device__ __forceinline__ void epilogue_linear(const UmmaParams& p, uint32_t tmem_acc, int row, int n0) {
+#pragma unroll 1
+    for (int cc = 0; cc < BN / 32; ++cc) {
+        const int col0 = n0 + cc * 32;
+        if (col0 >= p.n) break;  // uniform across the CTA
+        uint32_t v[32];
+        tmem_ld_32x32b_x32(tmem_acc + uint32_t(cc * 32), v);
+        tmem_ld_wait();
+        if (row >= p.m) continue;
+        float f[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) f[j] = kInt ? __int2float_rn(int(v[j])) : __uint_as_float(v[j]);
+        linear_finish32(p.linear, p.n, row, col0, f);
+    }
 }
 
 // Epilogue of one 128-row accumulator slice: thread `row` of the tile reads its TMEM lane 32 columns at a time,
@@ -657,7 +686,7 @@ __device__ __forceinline__ void epilogue_plain(const UmmaParams& p, const CUtens
     }
 }
 
-template <MmaKind kKind, int BN, bool kSplit>
+template <MmaKind kKind, int BN, bool kSplit, bool kLinear = false>
 __global__ void __launch_bounds__(kSplit ? kThreadsSplit : kThreads, 1)
 umma_gemm_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
                  const __grid_constant__ CUtensorMap tma_a_lo, const __grid_constant__ CUtensorMap tma_b_lo,
@@ -838,7 +867,7 @@ umma_gemm_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
                 if (lane == 0) mbar_arrive(tempty_bar(acc));
                 if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
             }
-            if (alive) store_running<HC>(p, run, b, mi * kBM + row_in_tile, ni * BN + half * HC);
+            if (alive) store_running<HC, kLinear>(p, run, b, mi * kBM + row_in_tile, ni * BN + half * HC);
         }
     } else {
         // ------------------------------------------------------------------ epilogue
@@ -856,8 +885,12 @@ umma_gemm_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
                 break;
             }
             tcgen05_fence_after();
-            epilogue_tile<BN>(p, tmem_base + (uint32_t(quad * 32) << 16) + uint32_t(acc * BN), b,
-                              mi * kBM + row_in_tile, ni * BN);
+            if constexpr (kLinear)
+                epilogue_linear<BN, kKind == MmaKind::i8>(p, tmem_base + (uint32_t(quad * 32) << 16) + uint32_t(acc * BN),
+                                                          mi * kBM + row_in_tile, ni * BN);
+            else
+                epilogue_tile<BN>(p, tmem_base + (uint32_t(quad * 32) << 16) + uint32_t(acc * BN), b,
+                                  mi * kBM + row_in_tile, ni * BN);
             tcgen05_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(tempty_bar(acc));
@@ -897,7 +930,7 @@ struct PairTile {
 
 // kEpi = 8 (16- and 8-bit outputs through TMA stores, no second output): two epilogue warps per lane quadrant, each
 // taking 128 of the tile's 256 columns, for shallow K where the epilogue, not the main loop, bounds a tile.
-template <MmaKind kKind, bool kSplit, int kEpi = 4>
+template <MmaKind kKind, bool kSplit, int kEpi = 4, bool kLinear = false>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kSplit ? kThreadsSplit : 64 + 32 * kEpi, 1)
 umma_gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
                       const __grid_constant__ CUtensorMap tma_a_lo, const __grid_constant__ CUtensorMap tma_b_lo,
@@ -1080,7 +1113,7 @@ umma_gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
                 if (lane == 0) mbar_arrive_leader(tempty_bar(acc));
                 if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
             }
-            if (alive) store_running<HC>(p, run, b, mi * 256 + row_in_tile, ni * BN + half * HC);
+            if (alive) store_running<HC, kLinear>(p, run, b, mi * 256 + row_in_tile, ni * BN + half * HC);
         }
     } else {
         // ------------------------------------------------------------------ epilogue (both CTAs)
@@ -1101,7 +1134,12 @@ umma_gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
             // a 16-bit C with nothing fused takes the lean epilogue (NTB200_GENERAL_EPILOGUE=1 sets p.lean_ok to 0)
             const bool plain = p.tma_store && p.lean_ok && !p.bias && !p.accumulate && !p.has_mask && !p.has_relu_out &&
                                p.n_peers == 0 && p.out_kind != kOutI8;
-            if constexpr (!kSplit && kEpi == 16) {
+            if constexpr (kLinear) {
+                constexpr int kCols = BN * 4 / kEpi;       // kEpi / 4 warps per lane quadrant share the tile's columns
+                const int part = (warp - 2) >> 2;
+                epilogue_linear<kCols, kKind == MmaKind::i8>(p, tmem_base + (uint32_t(quad * 32) << 16) + uint32_t(acc * BN + part * kCols),
+                                                             mi * 256 + row_in_tile, ni * BN + part * kCols);
+            } else if constexpr (!kSplit && kEpi == 16) {
                 const int quarter = (warp - 2) >> 2;   // four warps per lane quadrant, 64 columns (one 128-byte sub-tile) each
                 if (plain)
                     epilogue_plain<1, false>(p, &tma_c, tmem_base + (uint32_t(quad * 32) << 16) + uint32_t(acc * BN + quarter * 64),
@@ -1950,7 +1988,7 @@ bool plan_store(void* c, CUtensorMapDataType dt, int es_bytes, int64_t m, int64_
     return encode_cached(out, dt, c, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B) == CUDA_SUCCESS;
 }
 
-template <MmaKind kKind, int BN, bool kSplit>
+template <MmaKind kKind, int BN, bool kSplit, bool kLinear = false>
 int launch_instance(const Maps& m, const UmmaParams& p_in, int grid, int a_rows_staged, cudaStream_t stream) {
     using T = Tile<BN, kSplit>;
     UmmaParams p = p_in;
@@ -1969,11 +2007,11 @@ int launch_instance(const Maps& m, const UmmaParams& p_in, int grid, int a_rows_
     if (dev_i < 0 || dev_i >= 64) dev_i = 0;
     if (!attr_set[dev_i].load(std::memory_order_acquire)) {
         const uint32_t max_smem = T::kRingBudget + T::kBarrierBytes + 1024;
-        cudaError_t e = cudaFuncSetAttribute(umma_gemm_kernel<kKind, BN, kSplit>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(max_smem));
+        cudaError_t e = cudaFuncSetAttribute(umma_gemm_kernel<kKind, BN, kSplit, kLinear>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(max_smem));
         if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(umma_gemm_kernel)");
         attr_set[dev_i].store(true, std::memory_order_release);
     }
-    umma_gemm_kernel<kKind, BN, kSplit><<<grid, kSplit ? kThreadsSplit : kThreads, smem, stream>>>(m.a.map, m.b.map, m.a_lo.map, m.b_lo.map, p);
+    umma_gemm_kernel<kKind, BN, kSplit, kLinear><<<grid, kSplit ? kThreadsSplit : kThreads, smem, stream>>>(m.a.map, m.b.map, m.a_lo.map, m.b_lo.map, p);
     count_launch();
     NTB200_CUDA(cudaGetLastError());
     return NTB200_OK;
@@ -2021,11 +2059,11 @@ int active_clusters_query(const void* kernel, uint32_t smem_bytes, int cluster_s
     return n;
 }
 
-template <MmaKind kKind, bool kSplit, int kEpi = 4>
+template <MmaKind kKind, bool kSplit, int kEpi = 4, bool kLinear = false>
 int launch_pair_instance(const Maps& m, const UmmaParams& p, cudaStream_t stream) {
     // Shallow K, plain TMA-store epilogue: the instantiations with eight or sixteen epilogue warps (the epilogue, not
     // the main loop, bounds a tile, and its throughput grows with the warps that run it)
-    if constexpr (!kSplit && kEpi == 4) {
+    if constexpr (!kSplit && kEpi == 4 && !kLinear) {
         if (p.tma_store && !p.has_relu_out && p.k_blocks <= 6 && !g_four_epilogue_warps) {
             static const int forced = [] { const char* e = getenv("NTB200_EPILOGUE_WARPS"); return e ? atoi(e) : 0; }();
             // A C with nothing fused leaves through the lean epilogue, and with it four warps (two chunks in flight, no
@@ -2040,19 +2078,28 @@ int launch_pair_instance(const Maps& m, const UmmaParams& p, cudaStream_t stream
         }
     }
     constexpr uint32_t smem = PairTile<kSplit>::kSmemBytes;
-    cudaError_t e = cudaFuncSetAttribute(umma_gemm_pair_kernel<kKind, kSplit, kEpi>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+    cudaError_t e = cudaFuncSetAttribute(umma_gemm_pair_kernel<kKind, kSplit, kEpi, kLinear>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
     if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(umma_gemm_pair_kernel)");
     static int cached[64] = {0};  // per instantiation, per device
     int dev = 0;
     (void)cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64) dev = 0;
     if (cached[dev] == 0)
-        cached[dev] = resident_pairs_query(reinterpret_cast<const void*>(umma_gemm_pair_kernel<kKind, kSplit, kEpi>), smem);
+        cached[dev] = resident_pairs_query(reinterpret_cast<const void*>(umma_gemm_pair_kernel<kKind, kSplit, kEpi, kLinear>), smem);
     const int pairs = std::min(p.total_tiles, cached[dev]);
-    umma_gemm_pair_kernel<kKind, kSplit, kEpi><<<2 * pairs, kSplit ? kThreadsSplit : 64 + 32 * kEpi, smem, stream>>>(m.a.map, m.b.map, m.a_lo.map, m.b_lo.map, m.c, m.relu, m.peers, p);
+    umma_gemm_pair_kernel<kKind, kSplit, kEpi, kLinear><<<2 * pairs, kSplit ? kThreadsSplit : 64 + 32 * kEpi, smem, stream>>>(m.a.map, m.b.map, m.a_lo.map, m.b_lo.map, m.c, m.relu, m.peers, p);
     count_launch();
     NTB200_CUDA(cudaGetLastError());
     return NTB200_OK;
+}
+
+// The kLinear instantiations, by tile.
+template <MmaKind kKind, bool kSplit>
+int launch_linear(const Maps& m, const UmmaParams& p, bool use_pair, int bn, int grid, int a_rows_staged, cudaStream_t stream) {
+    if (use_pair) return launch_pair_instance<kKind, kSplit, kSplit ? 4 : 8, true>(m, p, stream);
+    if (bn == 256) return launch_instance<kKind, 256, kSplit, true>(m, p, grid, a_rows_staged, stream);
+    if (bn == 128) return launch_instance<kKind, 128, kSplit, true>(m, p, grid, a_rows_staged, stream);
+    return launch_instance<kKind, 64, kSplit, true>(m, p, grid, a_rows_staged, stream);
 }
 
 // ---- Float32 as three TF32 products ------------------------------------------------------------------
@@ -2273,6 +2320,13 @@ int launch_planned(const GemmArgs& g, const Planned& pl, const Side& a, const Si
                     "(problem of at least 74 tiles of 256 x 256, 16-byte aligned rows)");
     const int grid = int(std::min<int64_t>(p.total_tiles, sms));
     note_route(pl.route);
+    if (g.linear) {
+        p.linear = *g.linear;
+        p.tma_store = 0;
+        if (pl.kind == MmaKind::tf32) return launch_linear<MmaKind::tf32, true>(maps, p, use_pair, bn, grid, a_rows_staged, stream);
+        if (pl.kind == MmaKind::i8) return launch_linear<MmaKind::i8, false>(maps, p, use_pair, bn, grid, a_rows_staged, stream);
+        return launch_linear<MmaKind::f16, false>(maps, p, use_pair, bn, grid, a_rows_staged, stream);
+    }
     if (pl.kind == MmaKind::tf32) {
         if (use_pair) return launch_pair_instance<MmaKind::tf32, true>(maps, p, stream);
         if (bn == 256) return launch_instance<MmaKind::tf32, 256, true>(maps, p, grid, a_rows_staged, stream);
@@ -2424,7 +2478,7 @@ int launch_int_limbs(const GemmArgs& g, cudaStream_t stream) {
 const bool g_no_splitk = [] { const char* e = getenv("NTB200_NO_SPLITK"); return e && e[0] == '1'; }();
 
 int pick_k_splits(const GemmArgs& g) {
-    if (g_no_splitk || g.no_alloc || g.batch != 1 || g.m > kBM || g.relu_out || g.mask_src || g.n_peers > 0) return 1;
+    if (g_no_splitk || g.no_alloc || g.batch != 1 || g.m > kBM || g.relu_out || g.mask_src || g.n_peers > 0 || g.linear) return 1;
     if (g.k % 64 != 0 || g.n % 4 != 0) return 1;
     // measured: no gain (or a loss, once the partial tiles weigh against the weights) below 4096 deep or 32 MB of weights
     if (g.k < 4096 || g.n * g.k < (int64_t(1) << 24)) return 1;
@@ -2460,7 +2514,7 @@ F16Plan plan_f16_tiles(const GemmArgs& g, int es = 2) {
     const int block_k = 128 / es;  // 8-bit operands: 128 deep K blocks, the same four MMAs and the same cycles
     const double kb = double((g.k + block_k - 1) / block_k);
     const bool fused = g.relu_out || g.mask_src || g.n_peers > 0;
-    const bool may_split = es == 2 && !g_no_splitk && !g.no_alloc && g.batch == 1 && !fused && g.n % 4 == 0;   // the reduce kernel is 16-bit
+    const bool may_split = es == 2 && !g_no_splitk && !g.linear && !g.no_alloc && g.batch == 1 && !fused && g.n % 4 == 0;   // the reduce kernel is 16-bit
     const double dram_us = double(g.batch) * (double(g.m) * g.k + double(g.k) * g.n + double(g.m) * g.n) * es / 4.5e6;
     struct Cand { bool pair; int bn; double fixed_us, us_per_k_block; };   // launch + fill + last epilogue; main loop
     const Cand cands[] = {{true, 256, 11.0, 0.35}, {false, 256, 13.0, 0.39}, {false, 128, 10.0, 0.34}, {false, 64, 10.0, 0.30}};
@@ -2620,7 +2674,7 @@ int cluster_k_capacity(int bn, int slices) {
 
 ClusterKPlan plan_cluster_k(const GemmArgs& g, int es) {
     ClusterKPlan best{0, 0, 1e30, false};
-    if (g_no_cluster_k || g.no_alloc || g.batch != 1 || g.relu_out || g.mask_src || g.n_peers > 0) return best;
+    if (g_no_cluster_k || g.no_alloc || g.batch != 1 || g.relu_out || g.mask_src || g.n_peers > 0 || g.linear) return best;
     if (g.k < 2048 || g.n * g.k < (int64_t(1) << 23)) return best;
     const int block_k = 128 / es;
     const int k_blocks = int((g.k + block_k - 1) / block_k);
@@ -2727,7 +2781,7 @@ struct PairClusterPlan {
 PairClusterPlan plan_pair_cluster_k(const GemmArgs& g, int es) {
     PairClusterPlan best{0, 1e30, false};
     static const bool disabled = [] { const char* e = getenv("NTB200_NO_PAIR_CLUSTER_K"); return e && e[0] == '1'; }();
-    if (disabled || g_disable_pair || es != 2 || g.no_alloc || g.batch != 1 || g.relu_out || g.mask_src || g.n_peers > 0) return best;
+    if (disabled || g_disable_pair || es != 2 || g.no_alloc || g.batch != 1 || g.relu_out || g.mask_src || g.n_peers > 0 || g.linear) return best;
     if (g.m <= kBM || g.n <= 128) return best;
     const int block_k = 128 / es;
     const int k_blocks = int((g.k + block_k - 1) / block_k);
@@ -2818,6 +2872,21 @@ bool umma_cluster_k_would_run(const GemmArgs& g) {
     if (g.dtype != NTB200_F16 && g.dtype != NTB200_BF16) return false;
     if (g.m > kBM || operands_stageable(g) != nullptr) return false;
     return plan_cluster_k(g, 2).valid;
+}
+
+size_t umma_scratch_bytes(const GemmArgs& g) {
+    if (g.m <= 0 || g.n <= 0 || g.k <= 0) return 0;
+    const int es = int(dtype_size(g.dtype));
+    if (es > 2) return 0;
+    int splits = 1;
+    if (es == 2) {
+        const F16Plan plan = plan_f16_tiles(g);
+        splits = plan.valid ? plan.splits : pick_k_splits(g);
+    }
+    size_t bytes = splits > 1 ? size_t(splits) * size_t(g.m) * size_t(g.n) * sizeof(float) : 0;
+    const PairClusterPlan pk = plan_pair_cluster_k(g, es);
+    if (pk.valid) bytes = std::max(bytes, size_t((g.m + 255) / 256) * size_t((g.n + 255) / 256) * 2 * pk.slices * kExchangeRegion * sizeof(float4));
+    return bytes ? bytes + 512 : 0;
 }
 
 bool umma_supported(const GemmArgs& g, const char** why) {

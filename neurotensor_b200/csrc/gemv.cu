@@ -189,6 +189,12 @@ int launch_gemv_rows(const GemmArgs& g, bool kn_layout, cudaStream_t stream) {
 
 // One 2-D problem with one or two rows, 16-bit floats, K-contiguous A, weights contiguous along N or along K with
 // 16-byte aligned rows, plain epilogue.
+size_t gemv_scratch_bytes(const GemmArgs& g) {
+    if (g.m > kGemvMaxRows || g.k <= 0) return 0;
+    const long long slab = kSlabKN < kSlabNK ? kSlabKN : kSlabNK;
+    return size_t((g.k + slab - 1) / slab) * kGemvMaxRows * size_t(g.n) * sizeof(float) + 256;
+}
+
 bool gemv_supported(const GemmArgs& g) {
     static const bool disabled = [] { const char* e = getenv("NTB200_NO_GEMV"); return e && e[0] == '1'; }();   // A/B measurements
     if (disabled) return false;

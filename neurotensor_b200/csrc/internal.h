@@ -29,6 +29,30 @@ void keep_pool_memory();  // once per device: the stream-ordered pool retains fr
 int scratch_acquire(void** ptr, size_t bytes, cudaStream_t stream);
 void scratch_release(void* ptr, cudaStream_t stream);
 
+// While one is alive on this host thread, scratch_acquire hands out pieces of the caller's block instead of the
+// library's own: operators that take a workspace can then be captured into any number of graphs.
+struct ScratchArena {
+    ScratchArena(void* base, size_t bytes);
+    ~ScratchArena();
+    ScratchArena(const ScratchArena&) = delete;
+    ScratchArena& operator=(const ScratchArena&) = delete;
+    char* base;
+    size_t bytes, used = 0;
+    ScratchArena* outer;
+};
+
+// What the epilogue of ntb200_linear_act does with each product (device pointers, strides in elements):
+// z = product [* row_scale col_scale] + bias; pre = z; y = act(z) + residual.
+struct LinearParams {
+    const float* row_scale; const float* col_scale;   // both or neither
+    const void* bias;
+    const void* residual; long long residual_rs;
+    void* y; long long y_rs;
+    void* pre; long long pre_rs;
+    int act, out_dtype;
+    int vec_ok;                                       // every pointer and row starts on 16 bytes
+};
+
 // A GEMM after validation: C[b] = (accumulate ? C[b] : 0) + bias + A[b].B[b]; strides in elements.
 struct GemmArgs {
     int dtype;
@@ -54,12 +78,15 @@ struct GemmArgs {
     // the caller may not allocate: only routes that need no scratch memory (no operand copies, no K slices, no
     // weight-streaming partial sums)
     int no_alloc = 0;
+    // ntb200_linear_act: everything after the product (c is then y); tcgen05 route only
+    const LinearParams* linear = nullptr;
 };
 
 // tcgen05 route.  Returns NTB200_ERR_UNSUPPORTED (without touching the error text) when the operands
 // cannot be expressed as TMA tensor maps, so the caller can route elsewhere.
 bool umma_supported(const GemmArgs& g, const char** why);
 int launch_umma_gemm(const GemmArgs& g, cudaStream_t stream);
+size_t umma_scratch_bytes(const GemmArgs& g);   // upper bound of the scratch launch_umma_gemm takes for 16- and 8-bit operands
 // Few rows of 16-bit floats against a large weight matrix: would the automatic route slice K over a thread-block
 // cluster (one launch, weights read once at close to the HBM rate)?
 bool umma_cluster_k_would_run(const GemmArgs& g);
@@ -91,6 +118,7 @@ int launch_conv2d_dkernel_implicit(const Conv2dShape& s, const void* x, const vo
 // One or two rows of 16-bit floats against a large weight matrix: CUDA-core kernels that stream the weights.
 bool gemv_supported(const GemmArgs& g);
 int launch_gemv(const GemmArgs& g, cudaStream_t stream);
+size_t gemv_scratch_bytes(const GemmArgs& g);   // upper bound of its scratch
 
 // CUDA-core route: every dtype, every stride pattern.
 int launch_simt_gemm(const GemmArgs& g, cudaStream_t stream);

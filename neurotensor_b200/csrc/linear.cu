@@ -1,0 +1,397 @@
+// ntb200_linear_act and its backward pass: y = act(x w [* scales] + bias) + residual.
+//
+// The product runs on the tcgen05 kernels of gemm_umma.cu, whose epilogue does everything that follows the product on
+// the fp32 accumulator (linear_epilogue.cuh): one launch, one rounding, no intermediate in memory but the
+// pre-activation that the backward pass asks for.  Operands that TMA cannot address (rows that do not start on 16
+// bytes) are copied once into padded rows in the caller's workspace; a small Float32 product runs on the exact
+// CUDA-core kernel and is finished by an elementwise pass.
+#include <algorithm>
+
+#include "internal.h"
+#include "linear_epilogue.cuh"
+#include "row_ops.cuh"
+
+namespace ntb200 {
+namespace {
+
+bool linear_float(int d) { return d == NTB200_F32 || d == NTB200_F16 || d == NTB200_BF16; }
+bool on16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+size_t round256(size_t b) { return (b + 255) & ~size_t(255); }
+
+// y = act(z + bias) + residual, pre = z + bias, from an fp32 product (or none: z null, K = 0).
+__global__ void linear_finish_kernel(const float* __restrict__ z, const LinearParams l, long long m, int n) {
+    const long long total = m * n;
+    for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
+        const long long row = i / n;
+        const int col = int(i - row * n);
+        float v = z ? z[i] : 0.f;
+        if (l.bias) v += lin_load(l.bias, col, l.out_dtype);
+        if (l.pre) lin_store(l.pre, row * l.pre_rs + col, v, l.out_dtype);
+        v = l.out_dtype == NTB200_F32 ? act_value<false>(l.act, v) : act_value<true>(l.act, v);
+        if (l.residual) v += lin_load(l.residual, row * l.residual_rs + col, l.out_dtype);
+        lin_store(l.y, row * l.y_rs + col, v, l.out_dtype);
+    }
+}
+
+// dst[r][c] = src[r * rs + c * cs], rows of dst ld elements apart (a multiple of 16 bytes), E bytes per element.
+// One 16-byte store per thread; neighbouring threads read neighbouring elements where cs is 1.
+template <class U>
+__global__ void pad_rows_kernel(const U* __restrict__ src, long long rs, long long cs, U* __restrict__ dst, long long ld, long long rows,
+                                long long cols) {
+    constexpr int V = 16 / sizeof(U);
+    const long long per_row = ld / V, total = rows * per_row;
+    for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
+        const long long r = i / per_row, c0 = (i - r * per_row) * V;
+        Pack<U, V> o;
+#pragma unroll
+        for (int j = 0; j < V; ++j) o.e[j] = c0 + j < cols ? src[r * rs + (c0 + j) * cs] : U(0);
+        *reinterpret_cast<Pack<U, V>*>(dst + r * ld + c0) = o;
+    }
+}
+
+// gz = gy act'(pre), and the column sums of gz of one slab of rows per blockIdx.y (partial: [slabs, n]).  32 x 8 threads,
+// each on V columns of every eighth row of the slab; the sums use gz before it is rounded.
+template <class T, int V>
+__global__ void __launch_bounds__(256) act_backward_kernel(const T* __restrict__ gy, long long gy_rs, const T* __restrict__ pre, long long pre_rs,
+                                                           T* __restrict__ gz, long long gz_rs, float* __restrict__ partial, long long m,
+                                                           int n, int act, long long slab_rows) {
+    __shared__ float red[8][32 * V + 1];
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+    const int col = (blockIdx.x * 32 + x) * V;
+    const long long r0 = blockIdx.y * slab_rows, r1 = min(m, r0 + slab_rows);
+    float sum[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) sum[i] = 0.f;
+    if (col < n) {
+#pragma unroll 2
+        for (long long r = r0 + y; r < r1; r += 8) {
+            const Pack<T, V> g = *reinterpret_cast<const Pack<T, V>*>(gy + r * gy_rs + col);
+            Pack<T, V> o;
+            if (pre) {
+                const Pack<T, V> z = *reinterpret_cast<const Pack<T, V>*>(pre + r * pre_rs + col);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float v = g.up(i) * act_slope<sizeof(T) == 2>(act, z.up(i));
+                    sum[i] += v;
+                    o.set(i, v);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) sum[i] += g.up(i);
+                o = g;
+            }
+            if (gz) *reinterpret_cast<Pack<T, V>*>(gz + r * gz_rs + col) = o;
+        }
+    }
+    if (!partial) return;
+#pragma unroll
+    for (int i = 0; i < V; ++i) red[y][x * V + i] = sum[i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 32 * V; i += 256) {
+        const int c = blockIdx.x * 32 * V + i;
+        if (c >= n) continue;
+        float v = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v += red[k][i];
+        partial[(long long)blockIdx.y * n + c] = v;
+    }
+}
+
+template <class T>
+__global__ void __launch_bounds__(256) join_slabs_kernel(const float* __restrict__ partial, T* __restrict__ out, int slabs, int n) {
+    __shared__ float s[8][33];
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5, c = blockIdx.x * 32 + x;
+    float v = 0.f;
+    if (c < n)
+        for (int i = y; i < slabs; i += 8) v += partial[(long long)i * n + c];
+    s[y][x] = v;
+    __syncthreads();
+    if (y == 0 && c < n) {
+        for (int i = 1; i < 8; ++i) v += s[i][x];
+        out[c] = RowType<T>::down(v);
+    }
+}
+
+// Slabs of rows of the bias gradient's partial sums: enough blocks for the GPU, at least 64 rows each.
+long long act_slabs(int64_t m, int64_t n, int vec) {
+    const int64_t col_blocks = (n + 32 * vec - 1) / (32 * vec);
+    int64_t slabs = std::max<int64_t>(1, std::min<int64_t>((m + 63) / 64, (148 * 8 + col_blocks - 1) / col_blocks));
+    return std::min<int64_t>(slabs, 65535);
+}
+
+// A GEMM operand as [mn, k] with element strides.
+struct Operand {
+    const void* p;
+    int64_t mn, k, mn_s, k_s;
+};
+bool tma_ready(const Operand& o, int es) {
+    if (!on16(o.p)) return false;
+    return ((o.k_s == 1 || o.k == 1) && (o.mn == 1 || o.mn_s * es % 16 == 0)) || ((o.mn_s == 1 || o.mn == 1) && (o.k == 1 || o.k_s * es % 16 == 0));
+}
+// Bytes of the padded copy (0: none needed).
+size_t padded_bytes(const Operand& o, int es) {
+    if (tma_ready(o, es)) return 0;
+    const bool along_k = o.k_s <= o.mn_s;
+    const int64_t rows = along_k ? o.mn : o.k, cols = along_k ? o.k : o.mn, v = 16 / es;
+    return round256(size_t(rows) * size_t((cols + v - 1) / v * v) * size_t(es));
+}
+int pad_operand(Operand& o, int es, cudaStream_t stream) {
+    const size_t bytes = padded_bytes(o, es);
+    if (bytes == 0) return NTB200_OK;
+    void* copy = nullptr;
+    if (int rc = scratch_acquire(&copy, bytes, stream)) return rc;
+    const bool along_k = o.k_s <= o.mn_s;
+    const int64_t rows = along_k ? o.mn : o.k, cols = along_k ? o.k : o.mn, v = 16 / es, ld = (cols + v - 1) / v * v;
+    const int64_t rs = along_k ? o.mn_s : o.k_s, cs = along_k ? o.k_s : o.mn_s;
+    const int blocks = int(std::min<int64_t>((rows * (ld / v) + 255) / 256, int64_t(sm_count()) * 16));
+    if (es == 1) pad_rows_kernel<uint8_t><<<blocks, 256, 0, stream>>>(static_cast<const uint8_t*>(o.p), rs, cs, static_cast<uint8_t*>(copy), ld, rows, cols);
+    else pad_rows_kernel<uint16_t><<<blocks, 256, 0, stream>>>(static_cast<const uint16_t*>(o.p), rs, cs, static_cast<uint16_t*>(copy), ld, rows, cols);
+    count_launch();
+    NTB200_CUDA(cudaGetLastError());
+    o.p = copy;
+    o.mn_s = along_k ? ld : 1;
+    o.k_s = along_k ? 1 : ld;
+    return NTB200_OK;
+}
+
+GemmArgs gemm_of(int dtype, const Operand& a, const Operand& b, void* c, int64_t c_rs) {
+    GemmArgs g{};
+    g.dtype = dtype;
+    g.f16_rounding = NTB200_F16_ROUND_ONCE;
+    g.m = a.mn; g.n = b.mn; g.k = a.k; g.batch = 1;
+    g.a = a.p; g.a_rs = a.mn_s; g.a_cs = a.k_s; g.a_bs = 0;
+    g.b = b.p; g.b_rs = b.k_s; g.b_cs = b.mn_s; g.b_bs = 0;
+    g.c = c; g.c_rs = c_rs; g.c_bs = 0;
+    return g;
+}
+
+bool small_f32(const GemmArgs& g) { return double(g.m) * double(g.n) * double(g.k) < 6.0e7; }   // as ntb200_gemm routes it
+
+// One plain product of the backward pass: its scratch beyond padded copies.
+size_t product_bytes(const GemmArgs& g) {
+    if (g.dtype == NTB200_F32) return small_f32(g) ? 0 : 2 * size_t(g.m + g.n) * size_t(g.k + 3) * 4 + 1024;
+    return umma_scratch_bytes(g) + gemv_scratch_bytes(g) + 1024;
+}
+int plain_product(int dtype, Operand a, Operand b, void* c, int64_t c_rs, cudaStream_t stream) {
+    if (a.mn == 0 || b.mn == 0) return NTB200_OK;
+    if (dtype != NTB200_F32 && a.k > 0) {
+        if (int rc = pad_operand(a, 2, stream)) return rc;
+        if (int rc = pad_operand(b, 2, stream)) return rc;
+    }
+    return route_gemm(gemm_of(dtype, a, b, c, c_rs), NTB200_ROUTE_AUTO, stream);
+}
+
+int check_linear(const ntb200_linear_desc* d) {
+    const char* what = "linear_act";
+    if (!d) return fail(NTB200_ERR_INVALID_ARG, "%s: null descriptor", what);
+    const bool int8 = d->dtype == NTB200_I8;
+    if (!int8 && !linear_float(d->dtype))
+        return fail(NTB200_ERR_UNSUPPORTED, "%s: Float32, Float16, BFloat16 and Int8 only, got %s", what, dtype_name(d->dtype));
+    if (!linear_float(d->out_dtype) || (!int8 && d->out_dtype != d->dtype))
+        return fail(NTB200_ERR_INVALID_ARG, "%s: the output of %s operands cannot be %s", what, dtype_name(d->dtype), dtype_name(d->out_dtype));
+    if (d->activation < NTB200_ACT_NONE || d->activation > NTB200_ACT_SILU)
+        return fail(NTB200_ERR_INVALID_ARG, "%s: unknown activation %d", what, d->activation);
+    if (d->m < 0 || d->n < 0 || d->k < 0 || d->m > (int64_t(1) << 30) || d->n > (int64_t(1) << 30) || d->k > (int64_t(1) << 30))
+        return fail(NTB200_ERR_INVALID_ARG, "%s: bad extent", what);
+    if (int8 && d->k > 131071) return fail(NTB200_ERR_INVALID_ARG, "%s: Int8 sums are exact up to K = 131071, got %lld", what, (long long)d->k);
+    if (d->x_row_stride < 0 || d->x_col_stride < 0 || d->w_row_stride < 0 || d->w_col_stride < 0)
+        return fail(NTB200_ERR_INVALID_ARG, "%s: negative stride", what);
+    if (d->m > 1 && (d->y_row_stride < d->n || (d->pre && d->pre_row_stride < d->n) || (d->residual && d->residual_row_stride < d->n)))
+        return fail(NTB200_ERR_INVALID_ARG, "%s: a row stride is shorter than a row", what);
+    if (d->m == 0 || d->n == 0) return NTB200_OK;
+    if (!d->y || (d->k > 0 && (!d->x || !d->w)) || (int8 && (!d->x_scale || !d->w_scale)))
+        return fail(NTB200_ERR_INVALID_ARG, "%s: null pointer", what);
+    if (!int8 && (d->x_scale || d->w_scale)) return fail(NTB200_ERR_INVALID_ARG, "%s: scales belong to Int8 operands", what);
+    if (d->pre && (d->pre == d->y || d->pre == d->residual))
+        return fail(NTB200_ERR_INVALID_ARG, "%s: the pre-activation needs memory of its own", what);
+    if (d->residual && d->residual == d->y && d->residual_row_stride != d->y_row_stride)
+        return fail(NTB200_ERR_INVALID_ARG, "%s: an output in the residual's place must have its row stride", what);
+    return NTB200_OK;
+}
+
+Operand x_of(const ntb200_linear_desc& d) { return Operand{d.x, d.m, d.k, d.x_row_stride, d.x_col_stride}; }
+Operand w_of(const ntb200_linear_desc& d) { return Operand{d.w, d.n, d.k, d.w_col_stride, d.w_row_stride}; }
+
+int check_backward(const ntb200_linear_backward_desc* d) {
+    const char* what = "linear_act_backward";
+    if (!d) return fail(NTB200_ERR_INVALID_ARG, "%s: null descriptor", what);
+    if (!linear_float(d->dtype)) return fail(NTB200_ERR_UNSUPPORTED, "%s: Float32, Float16 and BFloat16 only, got %s", what, dtype_name(d->dtype));
+    if (d->activation < NTB200_ACT_NONE || d->activation > NTB200_ACT_SILU)
+        return fail(NTB200_ERR_INVALID_ARG, "%s: unknown activation %d", what, d->activation);
+    if (d->m < 0 || d->n <= 0 || d->k <= 0 || d->m > (int64_t(1) << 30) || d->n > (int64_t(1) << 30) || d->k > (int64_t(1) << 30))
+        return fail(NTB200_ERR_INVALID_ARG, "%s: bad extent", what);
+    if (d->x_row_stride < 0 || d->x_col_stride < 0 || d->w_row_stride < 0 || d->w_col_stride < 0)
+        return fail(NTB200_ERR_INVALID_ARG, "%s: negative stride", what);
+    if (d->m > 1 && (d->grad_out_row_stride < d->n || (d->pre && d->pre_row_stride < d->n)))
+        return fail(NTB200_ERR_INVALID_ARG, "%s: a row stride is shorter than a row", what);
+    if (d->m == 0) return NTB200_OK;
+    if (!d->grad_out || (d->activation != NTB200_ACT_NONE && !d->pre) || (d->grad_x && !d->w) || (d->grad_w && !d->x))
+        return fail(NTB200_ERR_INVALID_ARG, "%s: null pointer", what);
+    return NTB200_OK;
+}
+
+// How the backward pass forms gz: its row stride (rows start on 16 bytes), whether it is grad_out itself, and whether
+// grad_out and pre can be read 16 bytes at a time.
+struct GzPlan { int64_t ld; bool own; bool vec; long long slabs; };
+GzPlan plan_gz(const ntb200_linear_backward_desc& d) {
+    const int es = int(dtype_size(d.dtype)), v = 16 / es;
+    const bool act = d.activation != NTB200_ACT_NONE;
+    const bool rows16 = on16(d.grad_out) && (d.m == 1 || d.grad_out_row_stride * es % 16 == 0);
+    GzPlan p;
+    p.vec = d.n % v == 0 && rows16 && (!act || (on16(d.pre) && (d.m == 1 || d.pre_row_stride * es % 16 == 0)));
+    p.own = act || (!rows16 && d.dtype != NTB200_F32);
+    p.ld = p.own ? (d.n + v - 1) / v * v : d.grad_out_row_stride;
+    p.slabs = act_slabs(d.m, d.n, p.vec ? v : 1);
+    return p;
+}
+
+template <class T>
+int launch_gz(const ntb200_linear_backward_desc& d, const GzPlan& p, void* gz, float* partial, cudaStream_t stream) {
+    constexpr int kVec = 16 / sizeof(T);
+    const long long per = (d.m + p.slabs - 1) / p.slabs;
+    const int slabs = int((d.m + per - 1) / per);
+    const T* gy = static_cast<const T*>(d.grad_out);
+    const T* pre = d.activation != NTB200_ACT_NONE ? static_cast<const T*>(d.pre) : nullptr;
+    const int v = p.vec ? kVec : 1;
+    const dim3 grid(unsigned((d.n + 32 * v - 1) / (32 * v)), unsigned(slabs));
+    if (p.vec)
+        act_backward_kernel<T, kVec><<<grid, 256, 0, stream>>>(gy, d.grad_out_row_stride, pre, d.pre_row_stride, static_cast<T*>(gz), p.ld, partial, d.m, int(d.n), d.activation, per);
+    else
+        act_backward_kernel<T, 1><<<grid, 256, 0, stream>>>(gy, d.grad_out_row_stride, pre, d.pre_row_stride, static_cast<T*>(gz), p.ld, partial, d.m, int(d.n), d.activation, per);
+    count_launch();
+    NTB200_CUDA(cudaGetLastError());
+    if (partial) {
+        join_slabs_kernel<T><<<unsigned((d.n + 31) / 32), 256, 0, stream>>>(partial, static_cast<T*>(d.grad_bias), slabs, int(d.n));
+        count_launch();
+        NTB200_CUDA(cudaGetLastError());
+    }
+    return NTB200_OK;
+}
+
+// The two products of the backward pass over gz: operands in the order GemmArgs wants them.
+void backward_operands(const ntb200_linear_backward_desc& d, const void* gz, int64_t ld, Operand (&dx)[2], Operand (&dw)[2]) {
+    dx[0] = Operand{gz, d.m, d.n, ld, 1};                               // gx[m, k] = gz[m, n] . w[k, n]^T
+    dx[1] = Operand{d.w, d.k, d.n, d.w_row_stride, d.w_col_stride};
+    dw[0] = Operand{d.x, d.k, d.m, d.x_col_stride, d.x_row_stride};     // gw[k, n] = x^T . gz
+    dw[1] = Operand{gz, d.n, d.m, 1, ld};
+    if (d.grad_w_transposed) std::swap(dw[0], dw[1]);                   // gw[n, k] = gz^T . x
+}
+
+}  // namespace
+}  // namespace ntb200
+
+using namespace ntb200;
+
+extern "C" {
+
+size_t ntb200_linear_act_workspace_bytes(const ntb200_linear_desc* d) {
+    if (check_linear(d) || d->m == 0 || d->n == 0 || d->k == 0) return 0;
+    if (d->dtype == NTB200_F32) {
+        const GemmArgs g = gemm_of(d->dtype, x_of(*d), w_of(*d), d->y, d->y_row_stride);
+        return small_f32(g) ? round256(size_t(d->m) * size_t(d->n) * 4) : 2 * size_t(d->m + d->n) * size_t(d->k + 3) * 4 + 1024;
+    }
+    const int es = int(dtype_size(d->dtype));
+    GemmArgs g = gemm_of(d->dtype, x_of(*d), w_of(*d), d->y, d->y_row_stride);
+    const LinearParams l{};
+    g.linear = &l;
+    return padded_bytes(x_of(*d), es) + padded_bytes(w_of(*d), es) + umma_scratch_bytes(g);
+}
+
+int ntb200_linear_act(const ntb200_linear_desc* d, void* workspace, size_t workspace_bytes, void* stream) {
+    if (int rc = check_linear(d)) return rc;
+    if (d->m == 0 || d->n == 0) return NTB200_OK;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (workspace_bytes > 0 && (!workspace || !on16(workspace)))
+        return fail(NTB200_ERR_INVALID_ARG, "linear_act: the workspace must start on 16 bytes");
+    const ScratchArena arena(workspace, workspace_bytes);
+    const int oes = int(dtype_size(d->out_dtype));
+    LinearParams l{};
+    l.row_scale = d->x_scale; l.col_scale = d->w_scale;
+    l.bias = d->bias;
+    l.residual = d->residual; l.residual_rs = d->residual_row_stride;
+    l.y = d->y; l.y_rs = d->y_row_stride;
+    l.pre = d->pre; l.pre_rs = d->pre_row_stride;
+    l.act = d->activation; l.out_dtype = d->out_dtype;
+    auto rows16 = [&](const void* p, int64_t rs) { return !p || (on16(p) && (d->m == 1 || rs * oes % 16 == 0)); };
+    l.vec_ok = rows16(l.y, l.y_rs) && rows16(l.residual, l.residual_rs) && rows16(l.pre, l.pre_rs) && on16(l.bias) && on16(l.col_scale);
+    Operand x = x_of(*d), w = w_of(*d);
+    GemmArgs g = gemm_of(d->dtype, x, w, d->y, d->y_row_stride);
+    if (d->k == 0 || (d->dtype == NTB200_F32 && small_f32(g))) {
+        void* z = nullptr;
+        if (d->k > 0) {
+            if (int rc = scratch_acquire(&z, size_t(d->m) * size_t(d->n) * 4, s)) return rc;
+            g.c = z; g.c_rs = d->n;
+            if (int rc = launch_simt_gemm(g, s)) return rc;
+        }
+        const int blocks = int(std::min<int64_t>((d->m * d->n + 255) / 256, int64_t(sm_count()) * 16));
+        linear_finish_kernel<<<blocks, 256, 0, s>>>(static_cast<const float*>(z), l, d->m, int(d->n));
+        count_launch();
+        NTB200_CUDA(cudaGetLastError());
+        return NTB200_OK;
+    }
+    if (d->dtype != NTB200_F32) {
+        const int es = int(dtype_size(d->dtype));
+        if (int rc = pad_operand(x, es, s)) return rc;
+        if (int rc = pad_operand(w, es, s)) return rc;
+        g = gemm_of(d->dtype, x, w, d->y, d->y_row_stride);
+    }
+    g.linear = &l;
+    return launch_umma_gemm(g, s);
+}
+
+size_t ntb200_linear_act_backward_workspace_bytes(const ntb200_linear_backward_desc* d) {
+    if (check_backward(d) || d->m == 0) return 0;
+    const int es = int(dtype_size(d->dtype));
+    const GzPlan p = plan_gz(*d);
+    size_t bytes = 1024;
+    if (p.own) bytes += round256(size_t(d->m) * size_t(p.ld) * size_t(es));
+    if (d->grad_bias) bytes += round256(size_t(p.slabs) * size_t(d->n) * 4);
+    Operand dx[2], dw[2];
+    backward_operands(*d, p.own ? nullptr : d->grad_out, p.ld, dx, dw);
+    for (const auto* o : {dx, dw}) {
+        if (o == dx ? !d->grad_x : !d->grad_w) continue;
+        if (d->dtype != NTB200_F32) bytes += padded_bytes(o[0], es) + padded_bytes(o[1], es);
+        bytes += product_bytes(gemm_of(d->dtype, o[0], o[1], nullptr, o[1].mn));
+    }
+    return bytes;
+}
+
+int ntb200_linear_act_backward(const ntb200_linear_backward_desc* d, void* workspace, size_t workspace_bytes, void* stream) {
+    if (int rc = check_backward(d)) return rc;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (workspace_bytes > 0 && (!workspace || !on16(workspace)))
+        return fail(NTB200_ERR_INVALID_ARG, "linear_act_backward: the workspace must start on 16 bytes");
+    const size_t es = dtype_size(d->dtype);
+    if (d->m == 0) {   // no rows: the weights' gradients are sums of nothing
+        if (d->grad_w) NTB200_CUDA(cudaMemsetAsync(d->grad_w, 0, size_t(d->k) * size_t(d->n) * es, s));
+        if (d->grad_bias) NTB200_CUDA(cudaMemsetAsync(d->grad_bias, 0, size_t(d->n) * es, s));
+        return NTB200_OK;
+    }
+    const ScratchArena arena(workspace, workspace_bytes);
+    const GzPlan p = plan_gz(*d);
+    const void* gz = d->grad_out;
+    void* own = nullptr;
+    float* partial = nullptr;
+    if (p.own) {
+        if (int rc = scratch_acquire(&own, size_t(d->m) * size_t(p.ld) * es, s)) return rc;
+        gz = own;
+    }
+    if (d->grad_bias)
+        if (int rc = scratch_acquire(reinterpret_cast<void**>(&partial), size_t(p.slabs) * size_t(d->n) * 4, s)) return rc;
+    if (p.own || partial) {
+        int rc;
+        if (d->dtype == NTB200_F32) rc = launch_gz<float>(*d, p, own, partial, s);
+        else if (d->dtype == NTB200_F16) rc = launch_gz<__half>(*d, p, own, partial, s);
+        else rc = launch_gz<__nv_bfloat16>(*d, p, own, partial, s);
+        if (rc) return rc;
+    }
+    Operand dx[2], dw[2];
+    backward_operands(*d, gz, p.ld, dx, dw);
+    if (d->grad_x)
+        if (int rc = plain_product(d->dtype, dx[0], dx[1], d->grad_x, d->k, s)) return rc;
+    if (d->grad_w)
+        if (int rc = plain_product(d->dtype, dw[0], dw[1], d->grad_w, d->grad_w_transposed ? d->k : d->n, s)) return rc;
+    return NTB200_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,516 @@
+// Root-mean-square norm with the residual's addition, its backward pass, and the quantisation of rows to Int8.
+//
+//   h = x + r        rstd = (mean(h^2) + eps)^-1/2        y = h rstd w
+//   Int8:   u = h w,  A = max |u|,  q = rint(u 127 / A),  scale = A rstd / 127        (y = q scale; rstd cancels out of q)
+//   backward, given h, rstd, gy = dL/dy and gh = dL/dh over the residual stream:
+//           g = gy w,  xhat = h rstd,  gx = rstd (g - xhat mean(g xhat)) + gh,  gw = sum over rows of gy xhat
+//
+// All sums run in fp32 on the unrounded h; y, h and gx are rounded once, when they are stored.  These kernels move
+// bytes: 8 per element for a 16-bit forward pass with residual (x, r in; y, h out), as many for the backward pass.
+#include <algorithm>
+
+#include "internal.h"
+#include "row_ops.cuh"
+
+namespace ntb200 {
+namespace {
+
+enum RowOut : int { kSame = 0, kInt8 = 1 };
+
+struct RowArgs {
+    const void* x; long long x_rs;
+    const void* r; long long r_rs;      // null: no residual
+    const void* w;                      // null: no norm, quantise the row itself
+    void* y;                            // [rows, cols], type of x or int8
+    void* h; float* stat;               // stat: rstd (16 / 32-bit output) or the row's scale (Int8 output)
+    long long rows; int cols;
+    float eps;
+};
+
+// q = rint(u * 127 / A), clamped; a row of zeros gives zeros, a NaN gives 0 (its row's scale is NaN, so the product
+// that reads it still is).  A below 2^-100 is scaled up first: 127 / A would overflow.
+struct Quant {
+    float up, inv;
+    __device__ __forceinline__ explicit Quant(float top) {
+        up = top < 0x1p-100f ? 0x1p100f : 1.f;
+        inv = top > 0.f ? __fdiv_rn(127.f, __fmul_rn(top, up)) : (top == 0.f ? 0.f : top);
+    }
+    __device__ __forceinline__ int operator()(float u) const {
+        const int q = __float2int_rn(__fmul_rn(__fmul_rn(u, up), inv));
+        return max(-127, min(127, q));
+    }
+};
+
+// G threads (a power of two, 32 or more) hold one row in registers, P vectors of V elements each; a block of
+// max(G, 256) threads takes blockDim / G rows at a time.  One pass over memory: load, reduce, scale, store.
+template <class T, int V, int P, int kOut>
+__global__ void __launch_bounds__(1024) norm_rows_kernel(const RowArgs a, int G) {
+    __shared__ float s_sum[2][32], s_top[2][32];
+    const int groups = blockDim.x / G, group = threadIdx.x / G, t = threadIdx.x - group * G;
+    const int warps = G >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, first_warp = group * warps;
+    const int nv = a.cols / V;
+    const Pack<T, V>* w = static_cast<const Pack<T, V>*>(a.w);
+    int flip = 0;
+    for (long long base = (long long)blockIdx.x * groups; base < a.rows; base += (long long)gridDim.x * groups, flip ^= 1) {
+        const long long row = base + group;
+        const bool live = row < a.rows;
+        const Pack<T, V>* x = reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(a.x) + (live ? row : 0) * a.x_rs);
+        const Pack<T, V>* r = reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(a.r) + (live && a.r ? row : 0) * a.r_rs);
+        float f[P * V];
+        Pack<T, V> px[P], pr[P];
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            const int c = t + p * G;
+            if (live && c < nv) {
+                px[p] = x[c];
+                if (a.r) pr[p] = r[c];
+            }
+        }
+        float sum = 0.f, top = 0.f;
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            const int c = t + p * G;
+            const bool in = live && c < nv;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                float v = in ? px[p].up(i) : 0.f;
+                if (a.r && in) v = __fadd_rn(v, pr[p].up(i));
+                f[p * V + i] = v;
+                if (a.w) sum += v * v;
+            }
+            if (a.h && in) {
+                Pack<T, V> o;
+#pragma unroll
+                for (int i = 0; i < V; ++i) o.set(i, f[p * V + i]);
+                reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.h) + row * a.cols)[c] = o;
+            }
+            if (kOut == kInt8 && in) {
+                if (a.w) {
+                    const Pack<T, V> pw = w[c];
+#pragma unroll
+                    for (int i = 0; i < V; ++i) f[p * V + i] = __fmul_rn(f[p * V + i], pw.up(i));
+                }
+#pragma unroll
+                for (int i = 0; i < V; ++i) top = max_nan(top, fabsf(f[p * V + i]));
+            }
+        }
+        sum = warp_sum(sum);
+        if (kOut == kInt8) top = warp_max_nan(top);
+        if (warps > 1) {
+            if (lane == 0) {
+                s_sum[flip][warp] = sum;
+                if (kOut == kInt8) s_top[flip][warp] = top;
+            }
+            __syncthreads();   // the two buffers alternate, so one barrier per row is enough
+            sum = lane < warps ? s_sum[flip][first_warp + lane] : 0.f;
+            sum = warp_sum(sum);
+            if (kOut == kInt8) {
+                top = lane < warps ? s_top[flip][first_warp + lane] : 0.f;
+                top = warp_max_nan(top);
+            }
+        }
+        const float rstd = a.w ? __frsqrt_rn(sum / float(a.cols) + a.eps) : 1.f;
+        if (!live) continue;
+        if (kOut == kInt8) {
+            const Quant quant(top);
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+                const int c = t + p * G;
+                if (c >= nv) continue;
+                Pack<int8_t, V> o;
+#pragma unroll
+                for (int i = 0; i < V; ++i) o.e[i] = int8_t(quant(f[p * V + i]));
+                reinterpret_cast<Pack<int8_t, V>*>(static_cast<int8_t*>(a.y) + row * a.cols)[c] = o;
+            }
+            if (t == 0) a.stat[row] = __fdiv_rn(__fmul_rn(top, rstd), 127.f);
+        } else {
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+                const int c = t + p * G;
+                if (c >= nv) continue;
+                const Pack<T, V> pw = w[c];
+                Pack<T, V> o;
+#pragma unroll
+                for (int i = 0; i < V; ++i) o.set(i, f[p * V + i] * rstd * pw.up(i));
+                reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.y) + row * a.cols)[c] = o;
+            }
+            if (a.stat && t == 0) a.stat[row] = rstd;
+        }
+    }
+}
+
+template <int kThreads>
+__device__ __forceinline__ void block_sum_top(float& sum, float& top) {
+    __shared__ float s_sum[kThreads / 32], s_top[kThreads / 32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    sum = warp_sum(sum);
+    top = warp_max_nan(top);
+    __syncthreads();
+    if (lane == 0) { s_sum[warp] = sum; s_top[warp] = top; }
+    __syncthreads();
+    sum = warp_sum(lane < kThreads / 32 ? s_sum[lane] : 0.f);
+    top = warp_max_nan(lane < kThreads / 32 ? s_top[lane] : 0.f);
+}
+
+// Rows too long for a block's registers: the row is read twice (the second time from L2).  Every element is read and
+// written by one thread, so h may be x or r here as well.
+template <class T, int kOut>
+__global__ void __launch_bounds__(1024) norm_long_rows_kernel(const RowArgs a) {
+    const T* w = static_cast<const T*>(a.w);
+    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T* x = static_cast<const T*>(a.x) + row * a.x_rs;
+        const T* r = a.r ? static_cast<const T*>(a.r) + row * a.r_rs : nullptr;
+        float sum = 0.f, top = 0.f;
+        for (int c = threadIdx.x; c < a.cols; c += 1024) {
+            float v = RowType<T>::up(x[c]);
+            if (r) v = __fadd_rn(v, RowType<T>::up(r[c]));
+            if (w) sum += v * v;
+            if (kOut == kInt8) top = max_nan(top, fabsf(w ? __fmul_rn(v, RowType<T>::up(w[c])) : v));
+        }
+        block_sum_top<1024>(sum, top);
+        const float rstd = w ? __frsqrt_rn(sum / float(a.cols) + a.eps) : 1.f;
+        const Quant quant(top);
+        for (int c = threadIdx.x; c < a.cols; c += 1024) {
+            float v = RowType<T>::up(x[c]);
+            if (r) v = __fadd_rn(v, RowType<T>::up(r[c]));
+            if (a.h) static_cast<T*>(a.h)[row * a.cols + c] = RowType<T>::down(v);
+            if (kOut == kInt8)
+                static_cast<int8_t*>(a.y)[row * a.cols + c] = int8_t(quant(w ? __fmul_rn(v, RowType<T>::up(w[c])) : v));
+            else
+                static_cast<T*>(a.y)[row * a.cols + c] = RowType<T>::down(v * rstd * RowType<T>::up(w[c]));
+        }
+        if (threadIdx.x == 0) {
+            if (kOut == kInt8) a.stat[row] = __fdiv_rn(__fmul_rn(top, rstd), 127.f);
+            else if (a.stat) a.stat[row] = rstd;
+        }
+    }
+}
+
+struct BackArgs {
+    const void* h; long long h_rs;
+    const void* w; const float* rstd;
+    const void* gy; long long gy_rs;
+    const void* gh; long long gh_rs;    // null: nothing arrives over the residual stream
+    void* gx; float* partial;           // partial: [grid, cols] sums of gy xhat, one row per block; null: no weight gradient
+    long long rows; int cols;
+};
+
+// The same layout; each thread keeps the sums of gy xhat of its columns in registers over all rows its block takes.
+template <class T, int V, int P>
+__global__ void __launch_bounds__(1024) norm_backward_kernel(const BackArgs a, int G) {
+    extern __shared__ float s_gw[];      // [groups - 1][cols] while the groups of a block are joined
+    __shared__ float s_dot[2][32];
+    const int groups = blockDim.x / G, group = threadIdx.x / G, t = threadIdx.x - group * G;
+    const int warps = G >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, first_warp = group * warps;
+    const int nv = a.cols / V;
+    const Pack<T, V>* w = static_cast<const Pack<T, V>*>(a.w);
+    float gw[P * V];
+#pragma unroll
+    for (int i = 0; i < P * V; ++i) gw[i] = 0.f;
+    int flip = 0;
+    for (long long base = (long long)blockIdx.x * groups; base < a.rows; base += (long long)gridDim.x * groups, flip ^= 1) {
+        const long long row = base + group;
+        const bool live = row < a.rows;
+        const Pack<T, V>* h = reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(a.h) + (live ? row : 0) * a.h_rs);
+        const Pack<T, V>* gy = reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(a.gy) + (live ? row : 0) * a.gy_rs);
+        const Pack<T, V>* gh = reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(a.gh) + (live && a.gh ? row : 0) * a.gh_rs);
+        const float rstd = live ? a.rstd[row] : 0.f;
+        Pack<T, V> ph[P], pg[P], pr[P];
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            const int c = t + p * G;
+            if (live && c < nv) {
+                ph[p] = h[c];
+                pg[p] = gy[c];
+                if (a.gh) pr[p] = gh[c];
+            }
+        }
+        float dot = 0.f;
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            const int c = t + p * G;
+            if (!live || c >= nv) continue;
+            const Pack<T, V> pw = w[c];
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float gx = pg[p].up(i) * (ph[p].up(i) * rstd);
+                gw[p * V + i] += gx;
+                dot += gx * pw.up(i);
+            }
+        }
+        dot = warp_sum(dot);
+        if (warps > 1) {
+            if (lane == 0) s_dot[flip][warp] = dot;
+            __syncthreads();
+            dot = warp_sum(lane < warps ? s_dot[flip][first_warp + lane] : 0.f);
+        }
+        if (!live) continue;
+        dot /= float(a.cols);
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            const int c = t + p * G;
+            if (c >= nv) continue;
+            const Pack<T, V> pw = w[c];
+            Pack<T, V> o;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                float v = rstd * (pg[p].up(i) * pw.up(i) - ph[p].up(i) * rstd * dot);
+                if (a.gh) v += pr[p].up(i);
+                o.set(i, v);
+            }
+            reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.gx) + row * a.cols)[c] = o;
+        }
+    }
+    if (!a.partial) return;
+    // join the block's groups in their order, then one row of partial sums per block
+    __syncthreads();
+    if (group > 0) {
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            const int c = t + p * G;
+            if (c < nv)
+#pragma unroll
+                for (int i = 0; i < V; ++i) s_gw[(group - 1) * a.cols + c * V + i] = gw[p * V + i];
+        }
+    }
+    __syncthreads();
+    if (group == 0) {
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            const int c = t + p * G;
+            if (c >= nv) continue;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                float v = gw[p * V + i];
+                for (int g = 1; g < groups; ++g) v += s_gw[(g - 1) * a.cols + c * V + i];
+                a.partial[(long long)blockIdx.x * a.cols + c * V + i] = v;
+            }
+        }
+    }
+}
+
+// Rows too long for registers: gx row by row (two passes over the row) ...
+template <class T>
+__global__ void __launch_bounds__(1024) norm_backward_long_kernel(const BackArgs a) {
+    const T* w = static_cast<const T*>(a.w);
+    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T* h = static_cast<const T*>(a.h) + row * a.h_rs;
+        const T* gy = static_cast<const T*>(a.gy) + row * a.gy_rs;
+        const T* gh = a.gh ? static_cast<const T*>(a.gh) + row * a.gh_rs : nullptr;
+        const float rstd = a.rstd[row];
+        float dot = 0.f, none = 0.f;
+        for (int c = threadIdx.x; c < a.cols; c += 1024)
+            dot += RowType<T>::up(gy[c]) * RowType<T>::up(w[c]) * (RowType<T>::up(h[c]) * rstd);
+        block_sum_top<1024>(dot, none);
+        dot /= float(a.cols);
+        for (int c = threadIdx.x; c < a.cols; c += 1024) {
+            float v = rstd * (RowType<T>::up(gy[c]) * RowType<T>::up(w[c]) - RowType<T>::up(h[c]) * rstd * dot);
+            if (gh) v += RowType<T>::up(gh[c]);
+            static_cast<T*>(a.gx)[row * a.cols + c] = RowType<T>::down(v);
+        }
+    }
+}
+// ... and the weight gradient's partial sums column by column, one slab of rows per blockIdx.y.
+template <class T>
+__global__ void norm_weight_long_kernel(const BackArgs a, long long slab_rows) {
+    const int c = blockIdx.x * blockDim.x + threadIdx.x;
+    if (c >= a.cols) return;
+    const long long r0 = blockIdx.y * slab_rows, r1 = min(a.rows, r0 + slab_rows);
+    float v = 0.f;
+    for (long long row = r0; row < r1; ++row)
+        v += RowType<T>::up(static_cast<const T*>(a.gy)[row * a.gy_rs + c]) *
+             (RowType<T>::up(static_cast<const T*>(a.h)[row * a.h_rs + c]) * a.rstd[row]);
+    a.partial[(long long)blockIdx.y * a.cols + c] = v;
+}
+
+// out[c] = sum over the slabs of partial[s][c], in a fixed order: 8 threads per column take every eighth slab.
+template <class T>
+__global__ void __launch_bounds__(256) sum_partials_kernel(const float* __restrict__ partial, T* __restrict__ out, int slabs, int cols) {
+    __shared__ float s[8][33];
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5, c = blockIdx.x * 32 + x;
+    float v = 0.f;
+    if (c < cols)
+        for (int i = y; i < slabs; i += 8) v += partial[(long long)i * cols + c];
+    s[y][x] = v;
+    __syncthreads();
+    if (y == 0 && c < cols) {
+        for (int i = 1; i < 8; ++i) v += s[i][x];
+        out[c] = RowType<T>::down(v);
+    }
+}
+
+bool aligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
+
+// How a row is laid over threads: V elements per vector (16 bytes where every row starts on 16 bytes, else one), P
+// vectors per thread, G threads per row.  G = 0: too long for registers.
+struct RowPlan { int v, p, g; };
+RowPlan plan_row(int cols, int vec, bool vec_ok) {
+    RowPlan r{vec_ok ? vec : 1, 0, 0};
+    const int nv = cols / r.v;
+    const int most = vec_ok ? 4 : 16;
+    for (int p = vec_ok ? 1 : 4; p <= most; p *= 2)
+        for (int g = 32; g <= (p == most ? 1024 : 256); g *= 2)
+            if ((long long)p * g >= nv) return RowPlan{r.v, p, g};
+    return r;
+}
+
+template <class T, int kOut>
+int launch_rows(const RowArgs& a, bool vec_ok, cudaStream_t stream) {
+    constexpr int kVec = 16 / sizeof(T);
+    const RowPlan pl = plan_row(a.cols, kVec, vec_ok);
+    const int sms = sm_count();
+    if (pl.g == 0) {
+        const int grid = int(std::min<long long>(a.rows, 2ll * sms));
+        norm_long_rows_kernel<T, kOut><<<grid, 1024, 0, stream>>>(a);
+    } else {
+        const int threads = std::max(pl.g, 256), groups = threads / pl.g;
+        const long long want = (a.rows + groups - 1) / groups;
+        const int grid = int(std::min<long long>(want, (long long)sms * 16));
+#define NTB200_ROWS(VV, PP) norm_rows_kernel<T, VV, PP, kOut><<<grid, threads, 0, stream>>>(a, pl.g)
+        if (pl.v > 1) {
+            if (pl.p == 1) NTB200_ROWS(kVec, 1);
+            else if (pl.p == 2) NTB200_ROWS(kVec, 2);
+            else NTB200_ROWS(kVec, 4);
+        } else {
+            if (pl.p == 4) NTB200_ROWS(1, 4);
+            else if (pl.p == 8) NTB200_ROWS(1, 8);
+            else NTB200_ROWS(1, 16);
+        }
+#undef NTB200_ROWS
+    }
+    count_launch();
+    NTB200_CUDA(cudaGetLastError());
+    return NTB200_OK;
+}
+
+constexpr int64_t kMaxCols = int64_t(1) << 30;
+
+// Slabs of the weight gradient's partial sums, and so the grid of the backward kernel: depends on sizes alone, so that
+// the workspace can be sized before the call.
+int backward_slabs(int64_t rows) { return int(std::max<int64_t>(1, std::min<int64_t>(rows, 2 * 148))); }
+
+template <class T>
+int launch_backward(const BackArgs& a, void* grad_weight, bool vec_ok, cudaStream_t stream) {
+    constexpr int kVec = 16 / sizeof(T);
+    const RowPlan pl = plan_row(a.cols, kVec, vec_ok);
+    int slabs = backward_slabs(a.rows);
+    if (pl.g == 0) {
+        if (a.partial) {   // before gx, which may take the place of gy
+            const long long per = (a.rows + slabs - 1) / slabs;
+            slabs = int((a.rows + per - 1) / per);
+            norm_weight_long_kernel<T><<<dim3(unsigned((a.cols + 255) / 256), unsigned(slabs)), 256, 0, stream>>>(a, per);
+            count_launch();
+        }
+        norm_backward_long_kernel<T><<<int(std::min<long long>(a.rows, 2ll * sm_count())), 1024, 0, stream>>>(a);
+        count_launch();
+    } else {
+        const int threads = std::max(pl.g, 256), groups = threads / pl.g;
+        slabs = int(std::min<long long>(slabs, (a.rows + groups - 1) / groups));
+        // at most 7 groups of 1024 columns: 28 KB
+        const size_t smem = a.partial ? size_t(groups - 1) * a.cols * sizeof(float) : 0;
+#define NTB200_BACK(VV, PP) norm_backward_kernel<T, VV, PP><<<slabs, threads, smem, stream>>>(a, pl.g)
+        if (pl.v > 1) {
+            if (pl.p == 1) NTB200_BACK(kVec, 1);
+            else if (pl.p == 2) NTB200_BACK(kVec, 2);
+            else NTB200_BACK(kVec, 4);
+        } else {
+            if (pl.p == 4) NTB200_BACK(1, 4);
+            else if (pl.p == 8) NTB200_BACK(1, 8);
+            else NTB200_BACK(1, 16);
+        }
+#undef NTB200_BACK
+        count_launch();
+    }
+    NTB200_CUDA(cudaGetLastError());
+    if (a.partial) {
+        sum_partials_kernel<T><<<unsigned((a.cols + 31) / 32), 256, 0, stream>>>(a.partial, static_cast<T*>(grad_weight), slabs, a.cols);
+        count_launch();
+        NTB200_CUDA(cudaGetLastError());
+    }
+    return NTB200_OK;
+}
+
+#define NTB200_ROW_SWITCH(dtype, ...)                                                       \
+    switch (dtype) {                                                                        \
+        case NTB200_F32: { using T = float; return __VA_ARGS__; }                           \
+        case NTB200_F16: { using T = __half; return __VA_ARGS__; }                          \
+        default: { using T = __nv_bfloat16; return __VA_ARGS__; }                           \
+    }
+
+int check_rows(const char* what, int dtype, int64_t rows, int64_t cols) {
+    if (dtype != NTB200_F32 && dtype != NTB200_F16 && dtype != NTB200_BF16)
+        return fail(NTB200_ERR_UNSUPPORTED, "%s: Float32, Float16 and BFloat16 only, got %s", what, dtype_name(dtype));
+    if (rows < 0 || cols <= 0 || cols > kMaxCols) return fail(NTB200_ERR_INVALID_ARG, "%s: bad extent", what);
+    return NTB200_OK;
+}
+
+}  // namespace
+}  // namespace ntb200
+
+using namespace ntb200;
+
+extern "C" {
+
+static int norm_forward(const char* what, int dtype, const void* x, int64_t x_rs, const void* r, int64_t r_rs, const void* w, void* y,
+                        bool int8, void* h, float* stat, int64_t rows, int64_t cols, double eps, void* stream) {
+    if (int rc = check_rows(what, dtype, rows, cols)) return rc;
+    if (rows == 0) return NTB200_OK;
+    if (!x || !y || (int8 && !stat)) return fail(NTB200_ERR_INVALID_ARG, "%s: null pointer", what);
+    if (!(eps >= 0)) return fail(NTB200_ERR_INVALID_ARG, "%s: epsilon must not be negative", what);
+    if ((rows > 1 && x_rs < cols) || (r && rows > 1 && r_rs < cols))
+        return fail(NTB200_ERR_INVALID_ARG, "%s: a row stride is shorter than a row", what);
+    const int es = int(dtype_size(dtype));
+    const bool vec_ok = cols * es % 16 == 0 && x_rs * es % 16 == 0 && (!r || r_rs * es % 16 == 0) && aligned(x, 16) && aligned(r, 16) &&
+                        aligned(w, 16) && aligned(y, int8 ? size_t(16 / es) : 16) && aligned(h, 16);
+    const RowArgs a{x, x_rs, r, r_rs, w, y, h, stat, rows, int(cols), float(eps)};
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (int8) { NTB200_ROW_SWITCH(dtype, (launch_rows<T, kInt8>(a, vec_ok, s))) }
+    NTB200_ROW_SWITCH(dtype, (launch_rows<T, kSame>(a, vec_ok, s)))
+}
+
+int ntb200_rms_norm(int dtype, const void* x, int64_t x_row_stride, const void* residual, int64_t residual_row_stride, const void* weight,
+                    void* y, void* h, float* rstd, int64_t rows, int64_t cols, double eps, void* stream) {
+    if (rows > 0 && !weight) return fail(NTB200_ERR_INVALID_ARG, "rms_norm: null pointer");
+    return norm_forward("rms_norm", dtype, x, x_row_stride, residual, residual_row_stride, weight, y, false, h, rstd, rows, cols, eps, stream);
+}
+
+int ntb200_rms_norm_int8(int dtype, const void* x, int64_t x_row_stride, const void* residual, int64_t residual_row_stride,
+                         const void* weight, int8_t* q, float* scale, void* h, int64_t rows, int64_t cols, double eps, void* stream) {
+    if (rows > 0 && !weight) return fail(NTB200_ERR_INVALID_ARG, "rms_norm_int8: null pointer");
+    return norm_forward("rms_norm_int8", dtype, x, x_row_stride, residual, residual_row_stride, weight, q, true, h, scale, rows, cols, eps,
+                        stream);
+}
+
+int ntb200_quantize_rows(int dtype, const void* x, int64_t x_row_stride, int8_t* q, float* scale, int64_t rows, int64_t cols, void* stream) {
+    return norm_forward("quantize_rows", dtype, x, x_row_stride, nullptr, 0, nullptr, q, true, nullptr, scale, rows, cols, 0.0, stream);
+}
+
+size_t ntb200_rms_norm_backward_workspace_bytes(int64_t rows, int64_t cols) {
+    if (rows <= 0 || cols <= 0) return 0;
+    return size_t(backward_slabs(rows)) * size_t(cols) * sizeof(float);
+}
+
+int ntb200_rms_norm_backward(int dtype, const void* h, int64_t h_row_stride, const void* weight, const float* rstd, const void* grad_y,
+                             int64_t grad_y_row_stride, const void* grad_h, int64_t grad_h_row_stride, void* grad_x, void* grad_weight,
+                             void* workspace, int64_t rows, int64_t cols, void* stream) {
+    const char* what = "rms_norm_backward";
+    if (int rc = check_rows(what, dtype, rows, cols)) return rc;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (rows == 0) {
+        if (grad_weight) NTB200_CUDA(cudaMemsetAsync(grad_weight, 0, size_t(cols) * dtype_size(dtype), s));
+        return NTB200_OK;
+    }
+    if (!h || !weight || !rstd || !grad_y || !grad_x || (grad_weight && !workspace))
+        return fail(NTB200_ERR_INVALID_ARG, "%s: null pointer", what);
+    if (rows > 1 && (h_row_stride < cols || grad_y_row_stride < cols || (grad_h && grad_h_row_stride < cols)))
+        return fail(NTB200_ERR_INVALID_ARG, "%s: a row stride is shorter than a row", what);
+    const int es = int(dtype_size(dtype));
+    const bool vec_ok = cols * es % 16 == 0 && h_row_stride * es % 16 == 0 && grad_y_row_stride * es % 16 == 0 &&
+                        (!grad_h || grad_h_row_stride * es % 16 == 0) && aligned(h, 16) && aligned(weight, 16) && aligned(grad_y, 16) &&
+                        aligned(grad_h, 16) && aligned(grad_x, 16);
+    const BackArgs a{h, h_row_stride, weight, rstd, grad_y, grad_y_row_stride, grad_h, grad_h_row_stride, grad_x,
+                     grad_weight ? static_cast<float*>(workspace) : nullptr, rows, int(cols)};
+    NTB200_ROW_SWITCH(dtype, (launch_backward<T>(a, grad_weight, vec_ok, s)))
+}
+
+}  // extern "C"

@@ -1,0 +1,50 @@
+// Pieces the row-wise kernels (norm, row quantiser, distillation loss) share: 16-byte vector loads of any float type
+// into fp32 registers and back, NaN-propagating maxima, block reductions.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstdint>
+
+namespace ntb200 {
+
+template <class T> struct RowType;
+template <> struct RowType<float> {
+    static __device__ __forceinline__ float up(float v) { return v; }
+    static __device__ __forceinline__ float down(float v) { return v; }
+};
+template <> struct RowType<__half> {
+    static __device__ __forceinline__ float up(__half v) { return __half2float(v); }
+    static __device__ __forceinline__ __half down(float v) { return __float2half_rn(v); }
+};
+template <> struct RowType<__nv_bfloat16> {
+    static __device__ __forceinline__ float up(__nv_bfloat16 v) { return __bfloat162float(v); }
+    static __device__ __forceinline__ __nv_bfloat16 down(float v) { return __float2bfloat16_rn(v); }
+};
+
+// V consecutive elements: V * sizeof(T) is 16, 8, 4 or 2 bytes, and addresses are aligned to that.
+template <class T, int V>
+struct __align__(sizeof(T) * V) Pack {
+    T e[V];
+    __device__ __forceinline__ float up(int i) const { return RowType<T>::up(e[i]); }
+    __device__ __forceinline__ void set(int i, float v) { e[i] = RowType<T>::down(v); }
+};
+
+__device__ __forceinline__ float max_nan(float a, float b) {   // NaN if either is NaN
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+__device__ __forceinline__ float warp_max_nan(float v) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
+}  // namespace ntb200
