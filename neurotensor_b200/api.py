@@ -14,6 +14,7 @@ passed as strides and are never copied when one of the last two strides is 1.  S
 raise ValueError (the reference throws std::invalid_argument) before anything is launched.
 """
 import ctypes
+import math
 
 import torch
 
@@ -984,8 +985,12 @@ _ACTIVATIONS = {"none": _lib.ACT_NONE, None: _lib.ACT_NONE, "relu": _lib.ACT_REL
                 "gelu_tanh": _lib.ACT_GELU_TANH, "silu": _lib.ACT_SILU}
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream    # torch.cuda.current_stream(i).cuda_stream without building an object
+
+
 def _on_device(what, first, *others):
-    """Every operand on the first one's device, and that device current: the C ABI works on the current one."""
+    """The raw current stream of the operands' device, after checking that they share it and that it is current (the C
+    ABI works on the current device)."""
     if not first.is_cuda:
         raise ValueError("neurotensor_b200 operates on CUDA tensors only (there is no CPU path)")
     dev = first.get_device()
@@ -994,21 +999,26 @@ def _on_device(what, first, *others):
             raise ValueError("%s: every tensor must be on the same CUDA device" % what)
     if dev != torch.cuda.current_device():
         raise ValueError("%s: the tensors are on cuda:%d but cuda:%d is the current device" % (what, dev, torch.cuda.current_device()))
+    return _raw_stream(dev)
 
 
 def _rows_of(t):
     """(tensor, rows, row stride) of `t` seen as rows of its last dim; a layout that has no row stride is made contiguous."""
+    if t.is_contiguous():
+        n = t.shape[-1]
+        return t, (t.numel() // n if n else math.prod(t.shape[:-1])), n
+    n = t.shape[-1]
     if t.dim() == 2:
-        rows, rs = t.shape[0], t.stride(0)
-    elif t.dim() == 1:
-        rows, rs = 1, t.shape[0]
-    elif t.is_contiguous():
-        rows, rs = t.numel() // max(1, t.shape[-1]), t.shape[-1]
-    else:
-        return _rows_of(t.reshape(-1, t.shape[-1]))
-    if t.shape[-1] != 1 and t.stride(-1) != 1 or (rows > 1 and rs < t.shape[-1]):
+        rs = t.stride(0)
+        if (t.stride(1) == 1 or n == 1) and rs >= n:
+            return t, t.shape[0], rs
         return _rows_of(t.contiguous())
-    return t, rows, rs
+    if t.dim() < 2 or t.stride(-1) != 1:
+        return _rows_of(t.contiguous())
+    try:
+        return _rows_of(t.view(-1, n))
+    except RuntimeError:
+        return _rows_of(t.contiguous())
 
 
 def _activation(name):
@@ -1036,18 +1046,18 @@ def rms_norm(x, weight, eps=1e-6, residual=None):
     Returns (y, h, rstd): h is x itself without a residual, rstd (fp32, one per row) is what rms_norm_backward takes.
     The norm uses the unrounded sum h."""
     _norm_operands("rms_norm", x, weight, residual)
-    _on_device("rms_norm", x, weight, residual)
+    stream = _on_device("rms_norm", x, weight, residual)
+    shape = x.shape
     xr, rows, x_rs = _rows_of(x)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    y = x.new_empty(shape)
+    rstd = x.new_empty(shape[:-1], dtype=torch.float32)
     h, rr, r_rs = x, None, 0
     if residual is not None:
-        h = torch.empty_like(y)
+        h = x.new_empty(shape)
         rr, _, r_rs = _rows_of(residual)
-    w = weight if weight.stride(0) == 1 else weight.contiguous()
-    check(lib().ntb200_rms_norm(dtype_code(x), xr.data_ptr(), x_rs, None if rr is None else rr.data_ptr(), r_rs, w.data_ptr(),
-                                y.data_ptr(), None if rr is None else h.data_ptr(), rstd.data_ptr(), rows, x.shape[-1], eps,
-                                _stream()))
+    w = weight if weight.is_contiguous() else weight.contiguous()
+    check(lib().ntb200_rms_norm(_TORCH_TO_CODE[x.dtype], xr.data_ptr(), x_rs, None if rr is None else rr.data_ptr(), r_rs, w.data_ptr(),
+                                y.data_ptr(), None if rr is None else h.data_ptr(), rstd.data_ptr(), rows, shape[-1], eps, stream))
     return y, h, rstd
 
 
@@ -1055,18 +1065,18 @@ def rms_norm_int8(x, weight, eps=1e-6, residual=None):
     """rms_norm whose output leaves as Int8 rows with one fp32 scale each (y = q * scale): what linear_int8 reads.
     Returns (q, scale, h)."""
     _norm_operands("rms_norm_int8", x, weight, residual)
-    _on_device("rms_norm_int8", x, weight, residual)
+    stream = _on_device("rms_norm_int8", x, weight, residual)
     xr, rows, x_rs = _rows_of(x)
-    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    q = x.new_empty(x.shape, dtype=torch.int8)
+    scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
     h, rr, r_rs = x, None, 0
     if residual is not None:
-        h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        h = x.new_empty(x.shape)
         rr, _, r_rs = _rows_of(residual)
-    w = weight if weight.stride(0) == 1 else weight.contiguous()
-    check(lib().ntb200_rms_norm_int8(dtype_code(x), xr.data_ptr(), x_rs, None if rr is None else rr.data_ptr(), r_rs, w.data_ptr(),
+    w = weight if weight.is_contiguous() else weight.contiguous()
+    check(lib().ntb200_rms_norm_int8(_TORCH_TO_CODE[x.dtype], xr.data_ptr(), x_rs, None if rr is None else rr.data_ptr(), r_rs, w.data_ptr(),
                                      q.data_ptr(), scale.data_ptr(), None if rr is None else h.data_ptr(), rows, x.shape[-1], eps,
-                                     _stream()))
+                                     stream))
     return q, scale, h
 
 
@@ -1074,11 +1084,11 @@ def quantize_rows(x):
     """(q, scale): every row of the last dim as Int8 with one fp32 scale, x ~ q * scale, scale = max |row| / 127.
     For hidden activations, and once for weights kept as [out, in]."""
     _norm_operands("quantize_rows", x, None, None)
-    _on_device("quantize_rows", x)
+    stream = _on_device("quantize_rows", x)
     xr, rows, x_rs = _rows_of(x)
-    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    check(lib().ntb200_quantize_rows(dtype_code(x), xr.data_ptr(), x_rs, q.data_ptr(), scale.data_ptr(), rows, x.shape[-1], _stream()))
+    q = x.new_empty(x.shape, dtype=torch.int8)
+    scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    check(lib().ntb200_quantize_rows(_TORCH_TO_CODE[x.dtype], xr.data_ptr(), x_rs, q.data_ptr(), scale.data_ptr(), rows, x.shape[-1], stream))
     return q, scale
 
 
@@ -1093,27 +1103,27 @@ def rms_norm_backward(h, weight, rstd, grad_y, grad_h=None, want_weight=True):
     if rstd.shape != h.shape[:-1] or rstd.dtype != torch.float32:
         raise ValueError("rms_norm_backward: expected rstd of shape %s in Float32 but got %s in %s"
                          % (tuple(h.shape[:-1]), tuple(rstd.shape), rstd.dtype))
-    _on_device("rms_norm_backward", h, weight, rstd, grad_y, grad_h)
+    stream = _on_device("rms_norm_backward", h, weight, rstd, grad_y, grad_h)
     cols = h.shape[-1]
     hr, rows, h_rs = _rows_of(h)
     gr, _, g_rs = _rows_of(grad_y)
     sr, _, s_rs = _rows_of(grad_h) if grad_h is not None else (None, 0, 0)
-    w = weight if weight.stride(0) == 1 else weight.contiguous()
+    w = weight if weight.is_contiguous() else weight.contiguous()
     rs = rstd if rstd.is_contiguous() else rstd.contiguous()
-    gx = torch.empty(h.shape, dtype=h.dtype, device=h.device)
+    gx = h.new_empty(h.shape)
     gw = ws = None
     if want_weight:
-        gw = torch.empty(cols, dtype=h.dtype, device=h.device)
-        ws = torch.empty(max(1, lib().ntb200_rms_norm_backward_workspace_bytes(rows, cols)), dtype=torch.uint8, device=h.device)
-    check(lib().ntb200_rms_norm_backward(dtype_code(h), hr.data_ptr(), h_rs, w.data_ptr(), rs.data_ptr(), gr.data_ptr(), g_rs,
+        gw = h.new_empty(cols)
+        ws = h.new_empty(max(1, lib().ntb200_rms_norm_backward_workspace_bytes(rows, cols)), dtype=torch.uint8)
+    check(lib().ntb200_rms_norm_backward(_TORCH_TO_CODE[h.dtype], hr.data_ptr(), h_rs, w.data_ptr(), rs.data_ptr(), gr.data_ptr(), g_rs,
                                          None if sr is None else sr.data_ptr(), s_rs, gx.data_ptr(),
                                          None if gw is None else gw.data_ptr(), None if ws is None else ws.data_ptr(), rows, cols,
-                                         _stream()))
+                                         stream))
     return gx, gw
 
 
 def _linear_desc(what, x, w, bias, activation, residual, transpose_w, dtype):
-    """Checked ntb200_linear_desc without its outputs, the output's shape, and the tensors it points into."""
+    """Checked ntb200_linear_desc without its outputs and scales, the output's shape, the tensors it points into, the stream."""
     if x.dim() < 1 or w.dim() != 2:
         raise ValueError("%s: expected rows of x and a 2-D weight but got %dD and %dD" % (what, x.dim(), w.dim()))
     k, n = (w.shape[1], w.shape[0]) if transpose_w else (w.shape[0], w.shape[1])
@@ -1125,31 +1135,34 @@ def _linear_desc(what, x, w, bias, activation, residual, transpose_w, dtype):
     if residual is not None and (residual.shape != shape or residual.dtype != dtype):
         raise ValueError("%s: expected a residual of shape %s and %s but got %s and %s"
                          % (what, tuple(shape), dtype, tuple(residual.shape), residual.dtype))
-    _on_device(what, x, w, bias, residual)
+    act = _activation(activation)
+    stream = _on_device(what, x, w, bias, residual)
     xr, rows, x_rs = _rows_of(x)
-    d = _lib.LinearDesc()
-    d.dtype, d.out_dtype, d.activation = _TORCH_TO_CODE[x.dtype], _TORCH_TO_CODE[dtype], _activation(activation)
-    d.m, d.n, d.k = rows, n, k
-    d.x, d.x_row_stride, d.x_col_stride = xr.data_ptr(), x_rs, 1
-    s0, s1 = w.stride()
-    d.w, d.w_row_stride, d.w_col_stride = w.data_ptr(), (s1 if transpose_w else s0), (s0 if transpose_w else s1)
     keep = [xr]
+    b = r = None
+    r_rs = 0
     if bias is not None:
-        b = bias if bias.stride(0) == 1 else bias.contiguous()
-        d.bias = b.data_ptr()
-        keep.append(b)
+        bc = bias if bias.is_contiguous() else bias.contiguous()
+        b = bc.data_ptr()
+        keep.append(bc)
     if residual is not None:
         rr, _, r_rs = _rows_of(residual)
-        d.residual, d.residual_row_stride = rr.data_ptr(), r_rs
+        r = rr.data_ptr()
         keep.append(rr)
-    return d, shape, keep
+    w_ks, w_ns = w.stride()
+    if transpose_w:
+        w_ks, w_ns = w_ns, w_ks
+    d = _lib.LinearDesc(_TORCH_TO_CODE[x.dtype], _TORCH_TO_CODE[dtype], act, 0, rows, n, k, xr.data_ptr(), x_rs, 1, w.data_ptr(), w_ks, w_ns,
+                        None, None, b, r, r_rs)
+    return d, shape, keep, stream
 
 
-def _run_linear(d, y):
+def _run_linear(d, y, stream):
     d.y, d.y_row_stride = y.data_ptr(), d.n
-    need = lib().ntb200_linear_act_workspace_bytes(ctypes.byref(d))
-    ws = torch.empty(need, dtype=torch.uint8, device=y.device) if need else None
-    check(lib().ntb200_linear_act(ctypes.byref(d), None if ws is None else ws.data_ptr(), need, _stream()))
+    ref = ctypes.byref(d)
+    need = lib().ntb200_linear_act_workspace_bytes(ref)
+    ws = y.new_empty(need, dtype=torch.uint8) if need else None
+    check(lib().ntb200_linear_act(ref, None if ws is None else ws.data_ptr(), need, stream))
 
 
 def linear_act(x, w, bias=None, activation="none", residual=None, transpose_w=False, want_pre=False):
@@ -1159,14 +1172,14 @@ def linear_act(x, w, bias=None, activation="none", residual=None, transpose_w=Fa
     want_pre: returns (y, pre) with pre = x.w + bias, which linear_act_backward takes."""
     if x.dtype not in _FLOATS or w.dtype != x.dtype:
         raise ValueError("linear_act: expected both tensors to be Float32, Float16 or BFloat16 alike but got %s and %s" % (x.dtype, w.dtype))
-    d, shape, keep = _linear_desc("linear_act", x, w, bias, activation, residual, transpose_w, x.dtype)
-    y = torch.empty(shape, dtype=x.dtype, device=x.device)
+    d, shape, keep, stream = _linear_desc("linear_act", x, w, bias, activation, residual, transpose_w, x.dtype)
+    y = x.new_empty(shape)
     if want_pre:
-        pre = torch.empty_like(y)
+        pre = x.new_empty(shape)
         d.pre, d.pre_row_stride = pre.data_ptr(), d.n
-        _run_linear(d, y)
+        _run_linear(d, y, stream)
         return y, pre
-    _run_linear(d, y)
+    _run_linear(d, y, stream)
     return y
 
 
@@ -1177,7 +1190,7 @@ def linear_int8(q, scale, w, w_scale, bias=None, activation="none", residual=Non
         raise ValueError("linear_int8: expected Int8 operands but got %s and %s" % (q.dtype, w.dtype))
     if dtype not in _FLOATS:
         raise ValueError("linear_int8: expected an output of Float32, Float16 or BFloat16 but got %s" % (dtype,))
-    d, shape, keep = _linear_desc("linear_int8", q, w, bias, activation, residual, transpose_w, dtype)
+    d, shape, keep, stream = _linear_desc("linear_int8", q, w, bias, activation, residual, transpose_w, dtype)
     if scale.shape != q.shape[:-1] or scale.dtype != torch.float32:
         raise ValueError("linear_int8: expected scales of shape %s in Float32 but got %s in %s"
                          % (tuple(q.shape[:-1]), tuple(scale.shape), scale.dtype))
@@ -1187,10 +1200,10 @@ def linear_int8(q, scale, w, w_scale, bias=None, activation="none", residual=Non
         raise ValueError("linear_int8: Int8 sums are exact up to 131071 inputs but got %d" % d.k)
     _on_device("linear_int8", q, scale, w_scale)
     s = scale if scale.is_contiguous() else scale.contiguous()
-    v = w_scale if w_scale.stride(0) == 1 else w_scale.contiguous()
+    v = w_scale if w_scale.is_contiguous() else w_scale.contiguous()
     d.x_scale, d.w_scale = s.data_ptr(), v.data_ptr()
-    y = torch.empty(shape, dtype=dtype, device=q.device)
-    _run_linear(d, y)
+    y = q.new_empty(shape, dtype=dtype)
+    _run_linear(d, y, stream)
     return y
 
 
@@ -1210,28 +1223,27 @@ def linear_act_backward(x, w, pre, grad_out, activation="none", transpose_w=Fals
                          % (tuple(x.shape), tuple(w.shape), tuple(grad_out.shape)))
     if pre is None and act != _lib.ACT_NONE:
         raise ValueError("linear_act_backward: the pre-activation is needed for %s" % activation)
-    _on_device("linear_act_backward", x, w, pre, grad_out)
+    stream = _on_device("linear_act_backward", x, w, pre, grad_out)
     if n == 0 or k == 0:
         raise ValueError("linear_act_backward: expected a weight with elements but got shape %s" % (tuple(w.shape),))
     xr, rows, x_rs = _rows_of(x)
     gr, _, g_rs = _rows_of(grad_out)
-    d = _lib.LinearBackwardDesc()
-    d.dtype, d.activation, d.grad_w_transposed = _TORCH_TO_CODE[x.dtype], act, int(bool(transpose_w))
-    d.m, d.n, d.k = rows, n, k
-    d.x, d.x_row_stride, d.x_col_stride = xr.data_ptr(), x_rs, 1
-    s0, s1 = w.stride()
-    d.w, d.w_row_stride, d.w_col_stride = w.data_ptr(), (s1 if transpose_w else s0), (s0 if transpose_w else s1)
-    d.grad_out, d.grad_out_row_stride = gr.data_ptr(), g_rs
+    pr, p_rs = None, 0
     if act != _lib.ACT_NONE:
         pr, _, p_rs = _rows_of(pre)
-        d.pre, d.pre_row_stride = pr.data_ptr(), p_rs
-    gx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_x else None
-    gw = torch.empty(w.shape, dtype=x.dtype, device=x.device) if want_w else None
-    gb = torch.empty(n, dtype=x.dtype, device=x.device) if want_bias else None
-    d.grad_x, d.grad_w, d.grad_bias = (None if t is None else t.data_ptr() for t in (gx, gw, gb))
-    need = lib().ntb200_linear_act_backward_workspace_bytes(ctypes.byref(d))
-    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-    check(lib().ntb200_linear_act_backward(ctypes.byref(d), None if ws is None else ws.data_ptr(), need, _stream()))
+    gx = x.new_empty(x.shape) if want_x else None
+    gw = x.new_empty(w.shape) if want_w else None
+    gb = x.new_empty(n) if want_bias else None
+    w_ks, w_ns = w.stride()
+    if transpose_w:
+        w_ks, w_ns = w_ns, w_ks
+    d = _lib.LinearBackwardDesc(_TORCH_TO_CODE[x.dtype], act, int(bool(transpose_w)), 0, rows, n, k, xr.data_ptr(), x_rs, 1, w.data_ptr(), w_ks, w_ns,
+                                None if pr is None else pr.data_ptr(), p_rs, gr.data_ptr(), g_rs,
+                                *(None if t is None else t.data_ptr() for t in (gx, gw, gb)))
+    ref = ctypes.byref(d)
+    need = lib().ntb200_linear_act_backward_workspace_bytes(ref)
+    ws = x.new_empty(need, dtype=torch.uint8) if need else None
+    check(lib().ntb200_linear_act_backward(ref, None if ws is None else ws.data_ptr(), need, stream))
     return gx, gw, gb
 
 
@@ -1258,7 +1270,7 @@ def distill_topk(logits, teacher, index, temperature=1.0, row_weight=None, want_
                          % (what, tuple(logits.shape[:-1]), tuple(row_weight.shape), row_weight.dtype))
     if out_grad is not None and (out_grad.shape != logits.shape or out_grad.dtype != logits.dtype):
         raise ValueError("%s: expected out_grad to be shaped and typed like the logits" % what)
-    _on_device(what, logits, teacher, index, row_weight, out_grad)
+    stream = _on_device(what, logits, teacher, index, row_weight, out_grad)
     sr, rows, s_rs = _rows_of(logits)
     t = teacher if teacher.is_contiguous() else teacher.contiguous()
     i = index if index.is_contiguous() else index.contiguous()
@@ -1266,16 +1278,16 @@ def distill_topk(logits, teacher, index, temperature=1.0, row_weight=None, want_
     grad, g_rs = None, 0
     if want_grad or out_grad is not None:
         if out_grad is None:
-            grad, g_rs = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device), logits.shape[-1]
+            grad, g_rs = logits.new_empty(logits.shape), logits.shape[-1]
         else:
             grad, _, g_rs = _rows_of(out_grad)
             if grad.data_ptr() != out_grad.data_ptr():
                 raise ValueError("%s: out_grad needs rows with a stride" % what)
             grad = out_grad
-    row_loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=logits.device)
-    loss = torch.empty((), dtype=torch.float32, device=logits.device)
+    row_loss = logits.new_empty(logits.shape[:-1], dtype=torch.float32)
+    loss = logits.new_empty((), dtype=torch.float32)
     check(lib().ntb200_distill_topk(_TORCH_TO_CODE[logits.dtype], sr.data_ptr(), s_rs, _TORCH_TO_CODE[t.dtype], t.data_ptr(),
                                     _TORCH_TO_CODE[i.dtype], i.data_ptr(), None if rw is None else rw.data_ptr(),
                                     None if grad is None else grad.data_ptr(), g_rs, row_loss.data_ptr(), loss.data_ptr(), rows,
-                                    logits.shape[-1], top, float(temperature), _stream()))
+                                    logits.shape[-1], top, temperature, stream))
     return loss, row_loss, grad

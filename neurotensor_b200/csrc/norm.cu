@@ -11,6 +11,7 @@
 
 #include "internal.h"
 #include "row_ops.cuh"
+#include "sm100_ptx.cuh"
 
 namespace ntb200 {
 namespace {
@@ -186,6 +187,162 @@ __global__ void __launch_bounds__(1024) norm_long_rows_kernel(const RowArgs a) {
     }
 }
 
+// ---- many rows: each group of G threads streams its rows through a ring of shared-memory stages --------------------
+// A group takes rows first, first + step, ...; one thread of it keeps `stages` rows on their way with untiled bulk
+// copies (one per tensor and row) while the group reduces and writes the row that has landed.  Loads in flight cost no
+// registers and no barrier, so the memory system always has the next rows to fetch.  A row is read from its stage into
+// registers before the barrier of its reduction; the thread that passes that barrier refills the stage.
+struct RowRing {
+    uint32_t data, bars;             // shared-memory addresses of this group's stages and their barriers
+    uint32_t row_bytes;
+    int tensors, stages;
+    __device__ __forceinline__ uint32_t at(int stage, int tensor) const { return data + uint32_t(stage * tensors + tensor) * row_bytes; }
+    __device__ __forceinline__ uint32_t bar(int stage) const { return bars + 8u * uint32_t(stage); }
+};
+
+template <class T, int V>
+__device__ __forceinline__ Pack<T, V> ld_shared_pack(uint32_t addr) {
+    static_assert(sizeof(Pack<T, V>) == 16, "16-byte vectors");
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return *reinterpret_cast<Pack<T, V>*>(&v);
+}
+
+// The G threads of a group meet: a warp by itself, more than one warp on a named barrier of their own.
+__device__ __forceinline__ void group_sync(int group, int G) {
+    if (G == 32) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(G) : "memory");
+}
+
+struct RingShape { int G, stages; unsigned int* status; };
+
+// Start of a ring kernel: barriers initialised, the group's first rows on their way.
+template <class Load>
+__device__ __forceinline__ RowRing ring_start(const RingShape& rs, uint32_t smem, uint32_t bars, int group, int t, int tensors, uint32_t row_bytes,
+                                              long long row, long long step, long long rows, const Load& load) {
+    RowRing ring{smem + uint32_t(group * rs.stages * tensors) * row_bytes, bars + 8u * uint32_t(group * rs.stages), row_bytes, tensors, rs.stages};
+    if (t == 0) {
+        for (int s = 0; s < rs.stages; ++s) mbar_init(ring.bar(s), 1);
+        fence_barrier_init();
+        fence_proxy_async_smem();
+        for (int s = 0; s < rs.stages && row + s * step < rows; ++s) load(ring, s, row + s * step);
+    }
+    return ring;
+}
+
+// A wait that ran out: the device status word is raised, the block's groups see the flag behind their next barrier,
+// and each group's copying thread waits (bounded again) for the copies still on their way before the block ends.
+__device__ __forceinline__ void ring_gave_up(const RingShape& rs, volatile uint32_t* abort_flag, unsigned int where) {
+    *abort_flag = 1;
+    atomicExch(rs.status, 0x100u | where);
+}
+__device__ __forceinline__ void ring_drain(const RowRing& ring, int stage, uint32_t phase, long long row, long long step, long long rows) {
+    volatile uint32_t never = 0;
+    for (int s = 0; s < ring.stages && row < rows; ++s, row += step) {
+        (void)mbar_wait(ring.bar(stage), phase, &never);
+        if (++stage == ring.stages) { stage = 0; phase ^= 1u; }
+    }
+}
+
+template <class T, int P, int kOut, bool kResidual>
+__global__ void __launch_bounds__(512) norm_ring_kernel(const RowArgs a, const RingShape rs) {
+    constexpr int V = 16 / sizeof(T);
+    extern __shared__ __align__(128) uint8_t ring_mem[];
+    __shared__ __align__(8) unsigned long long s_bar[128];
+    __shared__ float s_sum[2][32], s_top[2][32];
+    __shared__ uint32_t s_abort;
+    const int G = rs.G, groups = blockDim.x / G, group = threadIdx.x / G, t = threadIdx.x - group * G;
+    const int warps = G >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, first_warp = group * warps;
+    const int nv = a.cols / V;
+    const long long step = (long long)gridDim.x * groups;
+    long long row = (long long)blockIdx.x * groups + group;
+    if (threadIdx.x == 0) s_abort = 0;
+    auto load = [&](const RowRing& ring, int s, long long r) {
+        mbar_expect_tx(ring.bar(s), ring.row_bytes * uint32_t(ring.tensors));
+        bulk_load(ring.at(s, 0), static_cast<const T*>(a.x) + r * a.x_rs, ring.row_bytes, ring.bar(s));
+        if (kResidual) bulk_load(ring.at(s, 1), static_cast<const T*>(a.r) + r * a.r_rs, ring.row_bytes, ring.bar(s));
+    };
+    const RowRing ring = ring_start(rs, smem_u32(ring_mem), smem_u32(s_bar), group, t, kResidual ? 2 : 1, uint32_t(a.cols) * uint32_t(sizeof(T)), row, step,
+                                    a.rows, load);
+    const Pack<T, V>* w = static_cast<const Pack<T, V>*>(a.w);
+    __syncthreads();
+    int flip = 0, stage = 0;
+    uint32_t phase = 0;
+    for (; row < a.rows; row += step, flip ^= 1) {
+        if (!mbar_wait(ring.bar(stage), phase, &s_abort)) ring_gave_up(rs, &s_abort, 0x41);
+        float f[P * V];
+        float sum = 0.f, top = 0.f;
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            const int c = t + p * G;
+            if (c < nv) {
+                const Pack<T, V> x = ld_shared_pack<T, V>(ring.at(stage, 0) + uint32_t(c) * 16u);
+                if (kResidual) {
+                    const Pack<T, V> r = ld_shared_pack<T, V>(ring.at(stage, 1) + uint32_t(c) * 16u);
+                    Pack<T, V> o;
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        f[p * V + i] = __fadd_rn(x.up(i), r.up(i));
+                        o.set(i, f[p * V + i]);
+                    }
+                    reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.h) + row * a.cols)[c] = o;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) f[p * V + i] = x.up(i);
+                }
+                if (a.w) {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) sum += f[p * V + i] * f[p * V + i];
+                }
+                if (kOut == kInt8) {
+                    if (a.w) {
+                        const Pack<T, V> pw = w[c];
+#pragma unroll
+                        for (int i = 0; i < V; ++i) f[p * V + i] = __fmul_rn(f[p * V + i], pw.up(i));
+                    }
+#pragma unroll
+                    for (int i = 0; i < V; ++i) top = max_nan(top, fabsf(f[p * V + i]));
+                }
+            }
+        }
+        sum = warp_sum(sum);
+        if (kOut == kInt8) top = warp_max_nan(top);
+        if (warps > 1 && lane == 0) {
+            s_sum[flip][warp] = sum;
+            if (kOut == kInt8) s_top[flip][warp] = top;
+        }
+        group_sync(group, G);     // the row is in registers and its partial sums are in place
+        if (*static_cast<volatile uint32_t*>(&s_abort)) break;
+        if (t == 0 && row + ring.stages * step < a.rows) load(ring, stage, row + ring.stages * step);
+        if (++stage == ring.stages) { stage = 0; phase ^= 1u; }
+        if (warps > 1) {
+            sum = warp_sum(lane < warps ? s_sum[flip][first_warp + lane] : 0.f);
+            if (kOut == kInt8) top = warp_max_nan(lane < warps ? s_top[flip][first_warp + lane] : 0.f);
+        }
+        const float rstd = a.w ? __frsqrt_rn(sum / float(a.cols) + a.eps) : 1.f;
+        const Quant quant(top);
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            const int c = t + p * G;
+            if (c >= nv) continue;
+            if (kOut == kInt8) {
+                Pack<int8_t, V> o;
+#pragma unroll
+                for (int i = 0; i < V; ++i) o.e[i] = int8_t(quant(f[p * V + i]));
+                reinterpret_cast<Pack<int8_t, V>*>(static_cast<int8_t*>(a.y) + row * a.cols)[c] = o;
+            } else {
+                const Pack<T, V> pw = w[c];
+                Pack<T, V> o;
+#pragma unroll
+                for (int i = 0; i < V; ++i) o.set(i, f[p * V + i] * rstd * pw.up(i));
+                reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.y) + row * a.cols)[c] = o;
+            }
+        }
+        if (t == 0 && a.stat) a.stat[row] = kOut == kInt8 ? __fdiv_rn(__fmul_rn(top, rstd), 127.f) : rstd;
+    }
+    if (t == 0 && s_abort) ring_drain(ring, stage, phase, row, step, a.rows);
+}
+
 struct BackArgs {
     const void* h; long long h_rs;
     const void* w; const float* rstd;
@@ -289,6 +446,112 @@ __global__ void __launch_bounds__(1024) norm_backward_kernel(const BackArgs a, i
     }
 }
 
+// The backward pass over the ring: h, gy and gh (kStream) of a row land together.
+template <class T, int P, bool kStream>
+__global__ void __launch_bounds__(512) norm_backward_ring_kernel(const BackArgs a, const RingShape rs) {
+    constexpr int V = 16 / sizeof(T);
+    extern __shared__ __align__(128) uint8_t ring_mem[];
+    __shared__ __align__(8) unsigned long long s_bar[128];
+    __shared__ float s_dot[2][32];
+    __shared__ uint32_t s_abort;
+    const int G = rs.G, groups = blockDim.x / G, group = threadIdx.x / G, t = threadIdx.x - group * G;
+    const int warps = G >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, first_warp = group * warps;
+    const int nv = a.cols / V;
+    const long long step = (long long)gridDim.x * groups;
+    long long row = (long long)blockIdx.x * groups + group;
+    if (threadIdx.x == 0) s_abort = 0;
+    auto load = [&](const RowRing& ring, int s, long long r) {
+        mbar_expect_tx(ring.bar(s), ring.row_bytes * uint32_t(ring.tensors));
+        bulk_load(ring.at(s, 0), static_cast<const T*>(a.h) + r * a.h_rs, ring.row_bytes, ring.bar(s));
+        bulk_load(ring.at(s, 1), static_cast<const T*>(a.gy) + r * a.gy_rs, ring.row_bytes, ring.bar(s));
+        if (kStream) bulk_load(ring.at(s, 2), static_cast<const T*>(a.gh) + r * a.gh_rs, ring.row_bytes, ring.bar(s));
+    };
+    const RowRing ring = ring_start(rs, smem_u32(ring_mem), smem_u32(s_bar), group, t, kStream ? 3 : 2, uint32_t(a.cols) * uint32_t(sizeof(T)), row, step,
+                                    a.rows, load);
+    Pack<T, V> w[P];
+    float gw[P * V];
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        if (t + p * G < nv) w[p] = static_cast<const Pack<T, V>*>(a.w)[t + p * G];
+#pragma unroll
+        for (int i = 0; i < V; ++i) gw[p * V + i] = 0.f;
+    }
+    __syncthreads();
+    int flip = 0, stage = 0;
+    uint32_t phase = 0;
+    const float inv_cols = 1.f / float(a.cols);
+    for (; row < a.rows; row += step, flip ^= 1) {
+        const float rstd = a.rstd[row];
+        if (!mbar_wait(ring.bar(stage), phase, &s_abort)) ring_gave_up(rs, &s_abort, 0x42);
+        Pack<T, V> h[P], gy[P], gh[P];
+        float dot = 0.f;
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            const int c = t + p * G;
+            if (c < nv) {
+                h[p] = ld_shared_pack<T, V>(ring.at(stage, 0) + uint32_t(c) * 16u);
+                gy[p] = ld_shared_pack<T, V>(ring.at(stage, 1) + uint32_t(c) * 16u);
+                if (kStream) gh[p] = ld_shared_pack<T, V>(ring.at(stage, 2) + uint32_t(c) * 16u);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float g = gy[p].up(i) * (h[p].up(i) * rstd);
+                    gw[p * V + i] += g;
+                    dot += g * w[p].up(i);
+                }
+            }
+        }
+        dot = warp_sum(dot);
+        if (warps > 1 && lane == 0) s_dot[flip][warp] = dot;
+        group_sync(group, G);
+        if (*static_cast<volatile uint32_t*>(&s_abort)) break;
+        if (t == 0 && row + ring.stages * step < a.rows) load(ring, stage, row + ring.stages * step);
+        if (++stage == ring.stages) { stage = 0; phase ^= 1u; }
+        if (warps > 1) dot = warp_sum(lane < warps ? s_dot[flip][first_warp + lane] : 0.f);
+        const float c0 = rstd * dot * inv_cols;
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            const int c = t + p * G;
+            if (c >= nv) continue;
+            Pack<T, V> o;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                float v = rstd * (gy[p].up(i) * w[p].up(i) - h[p].up(i) * c0);
+                if (kStream) v += gh[p].up(i);
+                o.set(i, v);
+            }
+            reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.gx) + row * a.cols)[c] = o;
+        }
+    }
+    if (t == 0 && s_abort) ring_drain(ring, stage, phase, row, step, a.rows);
+    if (!a.partial) return;
+    // the ring is empty: join the block's groups in their order there, then one row of partial sums per block
+    __syncthreads();
+    float* s_gw = reinterpret_cast<float*>(ring_mem);
+    if (group > 0) {
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            const int c = t + p * G;
+            if (c < nv)
+#pragma unroll
+                for (int i = 0; i < V; ++i) s_gw[(group - 1) * a.cols + c * V + i] = gw[p * V + i];
+        }
+    }
+    __syncthreads();
+    if (group == 0) {
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            const int c = t + p * G;
+            if (c >= nv) continue;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                float v = gw[p * V + i];
+                for (int g = 1; g < groups; ++g) v += s_gw[(g - 1) * a.cols + c * V + i];
+                a.partial[(long long)blockIdx.x * a.cols + c * V + i] = v;
+            }
+        }
+    }
+}
+
 // Rows too long for registers: gx row by row (two passes over the row) ...
 template <class T>
 __global__ void __launch_bounds__(1024) norm_backward_long_kernel(const BackArgs a) {
@@ -349,14 +612,64 @@ RowPlan plan_row(int cols, int vec, bool vec_ok) {
     const int nv = cols / r.v;
     const int most = vec_ok ? 4 : 16;
     for (int p = vec_ok ? 1 : 4; p <= most; p *= 2)
-        for (int g = 32; g <= (p == most ? 1024 : 256); g *= 2)
+        for (int g = 32; g <= (vec_ok || p == most ? 1024 : 256); g *= 2)
             if ((long long)p * g >= nv) return RowPlan{r.v, p, g};
     return r;
+}
+
+// The ring's shape for rows of `tensors` x cols elements: blocks of 512 threads (128 registers each), two vectors per
+// thread (one for rows of up to 32 vectors, four where a row needs all 512 threads), as many stages as 200 KB of shared
+// memory hold, up to 8.  stages < 2: no ring, the row is too long.
+constexpr int kRingThreads = 512;
+struct RingPlan { int p, g, stages; uint32_t smem; };
+RingPlan plan_ring(int cols, int vec, int es, int tensors) {
+    const int nv = cols / vec;
+    RingPlan r{nv <= 32 ? 1 : 2, 32, 0, 0};
+    while (r.g < kRingThreads && r.p * r.g < nv) r.g *= 2;
+    if (r.p * r.g < nv) r.p = 4;
+    if (r.p * r.g < nv) return r;
+    const uint32_t stage = uint32_t(tensors) * uint32_t(cols) * uint32_t(es), groups = uint32_t(kRingThreads / r.g);
+    r.stages = int(std::min<uint32_t>(8, 200u * 1024u / (stage * groups)));
+    r.smem = stage * groups * uint32_t(std::max(r.stages, 1));
+    return r;
+}
+
+// Kernel attributes are per device and kernel, and only ever raised.
+int allow_smem(const void* kernel, uint32_t bytes) {
+    if (bytes <= 40 * 1024) return NTB200_OK;   // the 48 KB every kernel may have, less static shared memory
+    NTB200_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)));
+    return NTB200_OK;
+}
+
+template <class T, int P, int kOut, bool kResidual>
+int launch_ring(const RowArgs& a, const RingPlan& r, cudaStream_t stream) {
+    auto kernel = norm_ring_kernel<T, P, kOut, kResidual>;
+    if (int rc = allow_smem(reinterpret_cast<const void*>(kernel), r.smem)) return rc;
+    const int groups = kRingThreads / r.g;
+    const int grid = int(std::min<long long>((a.rows + groups - 1) / groups, sm_count()));
+    kernel<<<grid, kRingThreads, r.smem, stream>>>(a, RingShape{r.g, r.stages, device_status_word()});
+    count_launch();
+    NTB200_CUDA(cudaGetLastError());
+    return NTB200_OK;
 }
 
 template <class T, int kOut>
 int launch_rows(const RowArgs& a, bool vec_ok, cudaStream_t stream) {
     constexpr int kVec = 16 / sizeof(T);
+    if (vec_ok && (a.h || !a.r)) {
+        const RingPlan r = plan_ring(a.cols, kVec, int(sizeof(T)), a.r ? 2 : 1);
+        // each group has several rows to stream
+        if (r.stages >= 2 && a.rows >= 4ll * sm_count() * (kRingThreads / r.g)) {
+            if (a.r) {
+                if (r.p == 1) return launch_ring<T, 1, kOut, true>(a, r, stream);
+                if (r.p == 2) return launch_ring<T, 2, kOut, true>(a, r, stream);
+                return launch_ring<T, 4, kOut, true>(a, r, stream);
+            }
+            if (r.p == 1) return launch_ring<T, 1, kOut, false>(a, r, stream);
+            if (r.p == 2) return launch_ring<T, 2, kOut, false>(a, r, stream);
+            return launch_ring<T, 4, kOut, false>(a, r, stream);
+        }
+    }
     const RowPlan pl = plan_row(a.cols, kVec, vec_ok);
     const int sms = sm_count();
     if (pl.g == 0) {
@@ -389,12 +702,32 @@ constexpr int64_t kMaxCols = int64_t(1) << 30;
 // the workspace can be sized before the call.
 int backward_slabs(int64_t rows) { return int(std::max<int64_t>(1, std::min<int64_t>(rows, 2 * 148))); }
 
+template <class T, int P, bool kStream>
+int launch_backward_ring(const BackArgs& a, const RingPlan& r, int grid, cudaStream_t stream) {
+    auto kernel = norm_backward_ring_kernel<T, P, kStream>;
+    const uint32_t smem = std::max(r.smem, uint32_t(kRingThreads / r.g - 1) * uint32_t(a.cols) * 4u);
+    if (int rc = allow_smem(reinterpret_cast<const void*>(kernel), smem)) return rc;
+    kernel<<<grid, kRingThreads, smem, stream>>>(a, RingShape{r.g, r.stages, device_status_word()});
+    count_launch();
+    return NTB200_OK;
+}
+
 template <class T>
 int launch_backward(const BackArgs& a, void* grad_weight, bool vec_ok, cudaStream_t stream) {
     constexpr int kVec = 16 / sizeof(T);
     const RowPlan pl = plan_row(a.cols, kVec, vec_ok);
     int slabs = backward_slabs(a.rows);
-    if (pl.g == 0) {
+    const RingPlan r = vec_ok ? plan_ring(a.cols, kVec, int(sizeof(T)), a.gh ? 3 : 2) : RingPlan{};
+    const int ring_groups = r.g ? kRingThreads / r.g : 1;
+    if (r.stages >= 2 && a.rows >= 4ll * sm_count() * ring_groups) {
+        slabs = std::min(slabs, sm_count());
+        int rc;
+        if (a.gh) rc = r.p == 1 ? launch_backward_ring<T, 1, true>(a, r, slabs, stream)
+                     : r.p == 2 ? launch_backward_ring<T, 2, true>(a, r, slabs, stream) : launch_backward_ring<T, 4, true>(a, r, slabs, stream);
+        else rc = r.p == 1 ? launch_backward_ring<T, 1, false>(a, r, slabs, stream)
+                : r.p == 2 ? launch_backward_ring<T, 2, false>(a, r, slabs, stream) : launch_backward_ring<T, 4, false>(a, r, slabs, stream);
+        if (rc) return rc;
+    } else if (pl.g == 0) {
         if (a.partial) {   // before gx, which may take the place of gy
             const long long per = (a.rows + slabs - 1) / slabs;
             slabs = int((a.rows + per - 1) / per);

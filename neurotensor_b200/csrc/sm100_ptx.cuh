@@ -92,6 +92,12 @@ __device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const void* tmap,
         : "memory");
 }
 
+// Untiled copy global -> shared of `bytes` (a multiple of 16; both addresses 16-byte aligned), completion on an mbarrier.
+__device__ __forceinline__ void bulk_load(uint32_t smem_dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(smem_dst), "l"(__cvta_generic_to_global(src)), "r"(bytes), "r"(bar) : "memory");
+}
+
 // The same load issued by either CTA of a pair working as one cta_group::2 MMA: the data lands in the issuing CTA's
 // shared memory, the byte count is credited to the barrier at `bar` in the pair's EVEN CTA (the MMA leader).
 constexpr uint32_t kPeerBitMask = 0xFEFFFFFFu;  // clears the bit that selects the odd CTA of a pair in a shared::cluster address

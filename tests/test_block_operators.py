@@ -167,7 +167,8 @@ def test_distill_refusals():
 
 # ---- norm -----------------------------------------------------------------------------------------------------------
 
-NORM_SHAPES = [(1, 1), (3, 5), (7, 64), (130, 200), (1, 4096), (37, 1999), (5, 8192), (3, 16384), (2, 16383), (2, 40000), (300, 33), (1000, 256)]
+NORM_SHAPES = [(1, 1), (3, 5), (7, 64), (130, 200), (1, 4096), (37, 1999), (5, 8192), (3, 16384), (2, 16383), (2, 40000), (300, 33), (1000, 256),
+               (9700, 64), (9600, 264), (2600, 2048), (1300, 4104), (700, 8192), (650, 16384)]     # enough rows to stream
 
 
 def norm_inputs(rows, n, dtype, residual, seed=0):
@@ -496,7 +497,7 @@ def test_linear_layouts():
         x = big[0, :, :96]
         place = rbig[0].clone()
         want = api.linear_act(x, w, b, "gelu", residual=place[:, :72])
-        d, _, keep = api._linear_desc("linear_act", x, w, b, "gelu", place[:, :72], False, dtype)
+        d, _, keep, _ = api._linear_desc("linear_act", x, w, b, "gelu", place[:, :72], False, dtype)
         d.y, d.y_row_stride = place.data_ptr(), 90
         need = _lib.lib().ntb200_linear_act_workspace_bytes(ctypes.byref(d))
         ws = torch.empty(max(need, 1), dtype=torch.uint8, device="cuda")
@@ -515,7 +516,7 @@ def test_linear_layouts():
 def test_linear_needs_its_workspace():
     from neurotensor_b200 import _lib, api
     x, w = torch.zeros(64, 33, dtype=F16, device="cuda"), torch.zeros(33, 40, dtype=F16, device="cuda")
-    d, _, keep = api._linear_desc("linear_act", x, w, None, "none", None, False, F16)
+    d, _, keep, _ = api._linear_desc("linear_act", x, w, None, "none", None, False, F16)
     y = torch.empty(64, 40, dtype=F16, device="cuda")
     d.y, d.y_row_stride = y.data_ptr(), 40
     assert _lib.lib().ntb200_linear_act_workspace_bytes(ctypes.byref(d)) >= 64 * 40 * 2
