@@ -686,6 +686,109 @@ __device__ __forceinline__ void epilogue_plain(const UmmaParams& p, const CUtens
     }
 }
 
+// Epilogue of the kLinear pair kernel for 16-bit outputs whose rows TMA can address: one warp's 32 rows x kCols columns as
+// sub-tiles of 64 columns, staged like epilogue_tile_tma's.  The residual comes in by TMA as well, into the very
+// buffer its sum leaves from: row-per-thread reads of 32 different rows would cost as much as row-per-thread stores.
+// `staging` holds two sub-tiles: without a pre-activation output both residual sub-tiles are on their way before the
+// accumulator is complete (linear_residual_prefetch); with one, buffer 0 is the pre-activation's, buffer 1 is y's, and
+// the second sub-tile waits until the first has left.
+template <int kCols>
+__device__ __forceinline__ void linear_residual_prefetch(const UmmaParams& p, const CUtensorMap* tma_res, uint32_t staging, uint32_t bar, int row0, int lane,
+                                                         int n0) {
+    if (n0 >= p.n) return;
+    if (lane == 0) {
+        tma_store_wait_read();   // the previous tile's sub-tiles have left
+        const bool both = !p.linear.pre && n0 + 64 < p.n;
+        mbar_expect_tx(bar, both ? 8192u : 4096u);
+        tma_load_3d(staging + (p.linear.pre ? 4096u : 0u), tma_res, bar, n0, row0, 0);
+        if (both) tma_load_3d(staging + 4096u, tma_res, bar, n0 + 64, row0, 0);
+    }
+    __syncwarp();
+}
+
+template <int kCols, bool kInt>
+__device__ __forceinline__ bool epilogue_linear_tma(const UmmaParams& p, const CUtensorMap* tma_y, const CUtensorMap* tma_pre, const CUtensorMap* tma_res,
+                                                    uint32_t tmem_acc, uint32_t staging, uint32_t bar, uint32_t& phase, int row0, int lane, int n0,
+                                                    volatile uint32_t* abort_flag) {
+    static_assert(kCols == 128, "two sub-tiles of 64 columns per warp");
+    if (n0 >= p.n) return true;   // uniform across the warp
+    const LinearParams& l = p.linear;
+    const bool pre = l.pre != nullptr, res = l.residual != nullptr;
+    const int dt = l.out_dtype;
+    const float rs = l.row_scale && row0 + lane < p.m ? l.row_scale[row0 + lane] : 1.f;
+    if (!res) {
+        if (lane == 0) tma_store_wait_read();
+        __syncwarp();
+    }
+    auto wait_residual = [&]() {
+        const bool ok = __all_sync(0xffffffffu, mbar_wait(bar, phase, abort_flag));
+        if (ok) phase ^= 1u;
+        return ok;
+    };
+    if (res && !wait_residual()) return false;
+#pragma unroll 1
+    for (int cc = 0; cc < 4; ++cc) {
+        const int col0 = n0 + cc * 32;
+        if (col0 >= p.n) break;
+        const int sub = cc >> 1, in_sub = cc & 1;
+        uint32_t v[32];
+        tmem_ld_32x32b_x32(tmem_acc + uint32_t(cc * 32), v);
+        if (pre && cc == 2) {   // both buffers again: the first sub-tile has to leave first
+            if (lane == 0) {
+                tma_store_wait_read();
+                if (res) {
+                    mbar_expect_tx(bar, 4096u);
+                    tma_load_3d(staging + 4096u, tma_res, bar, n0 + 64, row0, 0);
+                }
+            }
+            __syncwarp();
+            if (res && !wait_residual()) { tmem_ld_wait(); return false; }
+        }
+        tmem_ld_wait();
+        float f[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) f[j] = kInt ? __int2float_rn(int(v[j])) : __uint_as_float(v[j]);
+        linear_scale_bias32(l, p.n, col0, rs, col0 + 32 <= p.n && l.vec_ok, f);
+        const uint32_t row_pre = staging + uint32_t(lane) * 128u;
+        const uint32_t row_y = staging + (pre ? 4096u : uint32_t(sub) * 4096u) + uint32_t(lane) * 128u;
+        auto put = [&](uint32_t row, const float (&o)[32]) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const uint32_t chunk = uint32_t(in_sub * 4 + q) ^ uint32_t(lane & 7);
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row + (chunk << 4)), "r"(lin_pack2(o[8 * q], o[8 * q + 1], dt)),
+                             "r"(lin_pack2(o[8 * q + 2], o[8 * q + 3], dt)), "r"(lin_pack2(o[8 * q + 4], o[8 * q + 5], dt)),
+                             "r"(lin_pack2(o[8 * q + 6], o[8 * q + 7], dt)) : "memory");
+            }
+        };
+        if (pre) put(row_pre, f);
+        act_values<true>(l.act, f);
+        if (res) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const uint32_t chunk = uint32_t(in_sub * 4 + q) ^ uint32_t(lane & 7);
+                uint32_t w[4];
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(row_y + (chunk << 4)) : "memory");
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    f[8 * q + 2 * j] += lin_up16(w[j] & 0xffffu, dt);
+                    f[8 * q + 2 * j + 1] += lin_up16(w[j] >> 16, dt);
+                }
+            }
+        }
+        put(row_y, f);
+        if (in_sub == 1 || col0 + 32 >= p.n) {   // the sub-tile is complete, or C ends inside it (the stores clip)
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                if (pre) tma_store_3d(tma_pre, staging, n0 + sub * 64, row0, 0);
+                tma_store_3d(tma_y, staging + (pre ? 4096u : uint32_t(sub) * 4096u), n0 + sub * 64, row0, 0);
+                tma_store_commit();
+            }
+        }
+    }
+    return true;
+}
+
 template <MmaKind kKind, int BN, bool kSplit, bool kLinear = false>
 __global__ void __launch_bounds__(kSplit ? kThreadsSplit : kThreads, 1)
 umma_gemm_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
@@ -952,6 +1055,7 @@ umma_gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
     auto tempty_bar = [&](int a) { return bar_base + 8u * (2 * kStages + 2 + a); };
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(bar_gen + 8 * (2 * kStages + 4));
     volatile uint32_t* abort_flag = tmem_slot + 1;
+    auto residual_bar = [&](int w) { return bar_base + 8u * (2 * kStages + 5 + w); };   // kLinear: one per epilogue warp
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_cta_rank();
@@ -967,6 +1071,8 @@ umma_gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
             mbar_init(tfull_bar(a), 1);
             mbar_init(tempty_bar(a), kSplit ? 16 : 2 * kEpi);   // one arrival per epilogue warp of both CTAs
         }
+        if constexpr (kLinear && !kSplit)
+            for (int w = 0; w < kEpi; ++w) mbar_init(residual_bar(w), 1);
         *abort_flag = 0;
         fence_barrier_init();
         fence_proxy_async_smem();
@@ -1120,10 +1226,19 @@ umma_gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
         const int quad = warp & 3;
         const int row_in_tile = int(rank) * 128 + quad * 32 + lane;
         int acc = 0;
-        uint32_t acc_phase = 0;
+        uint32_t acc_phase = 0, residual_phase = 0;
+        bool residual_pending = false;   // kLinear: a residual sub-tile is on its way
         for (int t = pair; t < p.total_tiles; t += npairs) {
             int b, mi, ni;
             tile_coords(p, t, b, mi, ni);
+            if constexpr (kLinear && !kSplit) {
+                if (p.tma_store && p.linear.residual) {
+                    const int n0 = ni * BN + ((warp - 2) >> 2) * 128;
+                    linear_residual_prefetch<128>(p, &tma_peers.m[0], staging_base + uint32_t(warp - 2) * 8192u, residual_bar(warp - 2),
+                                                  mi * 256 + int(rank) * 128 + quad * 32, lane, n0);
+                    residual_pending = n0 < p.n;
+                }
+            }
             bool ok = mbar_wait(tfull_bar(acc), acc_phase, abort_flag);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) {
@@ -1137,6 +1252,20 @@ umma_gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
             if constexpr (kLinear) {
                 constexpr int kCols = BN * 4 / kEpi;       // kEpi / 4 warps per lane quadrant share the tile's columns
                 const int part = (warp - 2) >> 2;
+                if constexpr (!kSplit) {
+                    if (p.tma_store) {
+                        residual_pending = false;   // waited for inside
+                        if (!epilogue_linear_tma<kCols, kKind == MmaKind::i8>(
+                                p, &tma_c, &tma_relu, &tma_peers.m[0], tmem_base + (uint32_t(quad * 32) << 16) + uint32_t(acc * BN + part * kCols),
+                                staging_base + uint32_t(warp - 2) * 8192u, residual_bar(warp - 2), residual_phase,
+                                mi * 256 + int(rank) * 128 + quad * 32, lane, ni * BN + part * kCols, abort_flag)) {
+                            if (lane == 0) raise_timeout(abort_flag, 0x17);
+                            residual_pending = p.linear.residual != nullptr;
+                            break;
+                        }
+                    }
+                }
+                if (kSplit || !p.tma_store)
                 epilogue_linear<kCols, kKind == MmaKind::i8>(p, tmem_base + (uint32_t(quad * 32) << 16) + uint32_t(acc * BN + part * kCols),
                                                              mi * 256 + row_in_tile, ni * BN + part * kCols);
             } else if constexpr (!kSplit && kEpi == 16) {
@@ -1187,6 +1316,11 @@ umma_gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
             __syncwarp();
             if (lane == 0) mbar_arrive_leader(tempty_bar(acc));
             if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+        }
+        if constexpr (kLinear && !kSplit) {   // gave up with a residual sub-tile on its way: it lands before the CTA leaves
+            volatile uint32_t never = 0;
+            if (residual_pending && lane == 0) (void)mbar_wait(residual_bar(warp - 2), residual_phase, &never);
+            __syncwarp();
         }
         if (p.tma_store && lane == 0) tma_store_wait_all();   // the last tiles' stores are complete before the CTA leaves
     }
@@ -1244,7 +1378,7 @@ __device__ __forceinline__ float4 ld_shared_f4(uint32_t addr) {
     return v;
 }
 
-template <int S, int U>
+template <int S, int U, bool kLinear, bool kInt>
 __device__ __forceinline__ void cluster_reduce_store(const UmmaParams& p, const ClusterKParams& cp, uint32_t tile_base, int rows,
                                                      int m_base, int n_base, int col_first, int cols_mine, uint32_t rank_first,
                                                      uint32_t rank_stride, int my_slice) {
@@ -1271,10 +1405,26 @@ __device__ __forceinline__ void cluster_reduce_store(const UmmaParams& p, const 
             const int col = n_base + gcol[u];
             if (i >= items || col >= p.n) continue;
             float4 acc = v[u][0];
-#pragma unroll
-            for (int sl = 1; sl < S; ++sl) { acc.x += v[u][sl].x; acc.y += v[u][sl].y; acc.z += v[u][sl].z; acc.w += v[u][sl].w; }
-            float f[4] = {acc.x, acc.y, acc.z, acc.w};
+            float f[4];
             const int grow = m_base + row[u];
+            if constexpr (kInt) {   // the slices' s32 sums stay whole numbers until they are one
+                int s[4] = {__float_as_int(acc.x), __float_as_int(acc.y), __float_as_int(acc.z), __float_as_int(acc.w)};
+#pragma unroll
+                for (int sl = 1; sl < S; ++sl) {
+                    s[0] += __float_as_int(v[u][sl].x); s[1] += __float_as_int(v[u][sl].y);
+                    s[2] += __float_as_int(v[u][sl].z); s[3] += __float_as_int(v[u][sl].w);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) f[j] = __int2float_rn(s[j]);
+            } else {
+#pragma unroll
+                for (int sl = 1; sl < S; ++sl) { acc.x += v[u][sl].x; acc.y += v[u][sl].y; acc.z += v[u][sl].z; acc.w += v[u][sl].w; }
+                f[0] = acc.x; f[1] = acc.y; f[2] = acc.z; f[3] = acc.w;
+            }
+            if constexpr (kLinear) {
+                linear_finish4(p.linear, p.n, grow, col, f);
+                continue;
+            }
             uint16_t* dst = static_cast<uint16_t*>(p.c) + (long long)grow * p.c_rs + col;
             const uint16_t* bias = static_cast<const uint16_t*>(p.bias);
             uint32_t r[4];
@@ -1297,7 +1447,7 @@ __device__ __forceinline__ void cluster_reduce_store(const UmmaParams& p, const 
     }
 }
 
-template <int BN>
+template <int BN, MmaKind kKind = MmaKind::f16, bool kLinear = false>
 __global__ void __launch_bounds__(kThreads, 1)
 umma_gemm_cluster_k_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b, const ClusterKParams cp) {
     using T = Tile<BN, false>;
@@ -1406,8 +1556,8 @@ umma_gemm_cluster_k_kernel(const __grid_constant__ CUtensorMap tma_a, const __gr
                 const uint64_t b_desc = make_smem_desc_sw128(a_addr + p.s_a_bytes, p.b_lbo, 1024);
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    umma<MmaKind::f16, 1>(tmem_base, a_desc + uint64_t(k * p.a_kstep), b_desc + uint64_t(k * p.b_kstep), p.idesc,
-                                          ((kb - kb_begin) | k) != 0);
+                    umma<kKind, 1>(tmem_base, a_desc + uint64_t(k * p.a_kstep), b_desc + uint64_t(k * p.b_kstep), p.idesc,
+                                   ((kb - kb_begin) | k) != 0);
                 umma_commit<1>(empty_bar(stage));
                 if (++stage == kStages) { stage = 0; phase ^= 1u; }
             }
@@ -1452,9 +1602,9 @@ umma_gemm_cluster_k_kernel(const __grid_constant__ CUtensorMap tma_a, const __gr
         const int rows = min(kBM, p.m - m0);
         const int col_first = int(rank) * cols_mine;
         switch (cp.slices) {
-            case 2: cluster_reduce_store<2, 8>(p, cp, smem_base, rows, m0, n0, col_first, cols_mine, 0u, 1u, int(rank)); break;
-            case 4: cluster_reduce_store<4, 4>(p, cp, smem_base, rows, m0, n0, col_first, cols_mine, 0u, 1u, int(rank)); break;
-            default: cluster_reduce_store<8, 2>(p, cp, smem_base, rows, m0, n0, col_first, cols_mine, 0u, 1u, int(rank)); break;
+            case 2: cluster_reduce_store<2, 8, kLinear, kKind == MmaKind::i8>(p, cp, smem_base, rows, m0, n0, col_first, cols_mine, 0u, 1u, int(rank)); break;
+            case 4: cluster_reduce_store<4, 4, kLinear, kKind == MmaKind::i8>(p, cp, smem_base, rows, m0, n0, col_first, cols_mine, 0u, 1u, int(rank)); break;
+            default: cluster_reduce_store<8, 2, kLinear, kKind == MmaKind::i8>(p, cp, smem_base, rows, m0, n0, col_first, cols_mine, 0u, 1u, int(rank)); break;
         }
     }
     // nobody leaves while a neighbour may still read its shared memory
@@ -1777,11 +1927,11 @@ umma_gemm_pair_cluster_k_kernel(const __grid_constant__ CUtensorMap tma_a, const
             }
             __syncthreads();
             // the staged sums leave with bias, previous C and one rounding, coalesced along the rows
-            cluster_reduce_store<1, 8>(p, cp, smem_base, rows, m0, n0_pair, slice * cols_mine, cols_mine, 0u, 0u, 0);
+            cluster_reduce_store<1, 8, false, false>(p, cp, smem_base, rows, m0, n0_pair, slice * cols_mine, cols_mine, 0u, 0u, 0);
         } else if (cp.slices == 2) {
-            cluster_reduce_store<2, 8>(p, cp, smem_base, rows, m0, n0_pair, slice * cols_mine, cols_mine, half, 2u, slice);
+            cluster_reduce_store<2, 8, false, false>(p, cp, smem_base, rows, m0, n0_pair, slice * cols_mine, cols_mine, half, 2u, slice);
         } else {
-            cluster_reduce_store<4, 4>(p, cp, smem_base, rows, m0, n0_pair, slice * cols_mine, cols_mine, half, 2u, slice);
+            cluster_reduce_store<4, 4, false, false>(p, cp, smem_base, rows, m0, n0_pair, slice * cols_mine, cols_mine, half, 2u, slice);
         }
     }
     tcgen05_fence_before();
@@ -2300,7 +2450,7 @@ int launch_planned(const GemmArgs& g, const Planned& pl, const Side& a, const Si
     maps.relu = maps.a.map;
     p.tma_store = 0;
     const bool out16 = pl.out_kind == kOutF16 || pl.out_kind == kOutBF16;
-    if (use_pair && !pl.split && (out16 || pl.out_kind == kOutI8) && !g_direct_stores) {
+    if (use_pair && !pl.split && (out16 || pl.out_kind == kOutI8) && !g_direct_stores && !g.linear) {
         const int64_t relu_rs = g.relu_rs ? g.relu_rs : g.c_rs, relu_bs = g.relu_rs ? g.relu_bs : g.c_bs;
         const bool peers_relu = g.peers_get_relu && g.relu_out;
         bool ok = plan_store(g.c, pl.dt, out16 ? 2 : 1, g.m, g.n, g.batch, g.c_rs, g.c_bs, &maps.c);
@@ -2322,7 +2472,13 @@ int launch_planned(const GemmArgs& g, const Planned& pl, const Side& a, const Si
     note_route(pl.route);
     if (g.linear) {
         p.linear = *g.linear;
-        p.tma_store = 0;
+        const LinearParams& l = p.linear;
+        const bool l16 = l.out_dtype == NTB200_F16 || l.out_dtype == NTB200_BF16;
+        const CUtensorMapDataType ldt = l.out_dtype == NTB200_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+        p.has_relu_out = l.pre != nullptr;   // the kernel prefetches the second output's tensor map
+        p.tma_store = use_pair && l16 && l.vec_ok && !g_direct_stores && plan_store(l.y, ldt, 2, g.m, g.n, 1, l.y_rs, 0, &maps.c) &&
+                      (!l.pre || plan_store(l.pre, ldt, 2, g.m, g.n, 1, l.pre_rs, 0, &maps.relu)) &&
+                      (!l.residual || plan_store(const_cast<void*>(l.residual), ldt, 2, g.m, g.n, 1, l.residual_rs, 0, &maps.peers.m[0]));
         if (pl.kind == MmaKind::tf32) return launch_linear<MmaKind::tf32, true>(maps, p, use_pair, bn, grid, a_rows_staged, stream);
         if (pl.kind == MmaKind::i8) return launch_linear<MmaKind::i8, false>(maps, p, use_pair, bn, grid, a_rows_staged, stream);
         return launch_linear<MmaKind::f16, false>(maps, p, use_pair, bn, grid, a_rows_staged, stream);
@@ -2478,7 +2634,7 @@ int launch_int_limbs(const GemmArgs& g, cudaStream_t stream) {
 const bool g_no_splitk = [] { const char* e = getenv("NTB200_NO_SPLITK"); return e && e[0] == '1'; }();
 
 int pick_k_splits(const GemmArgs& g) {
-    if (g_no_splitk || g.no_alloc || g.batch != 1 || g.m > kBM || g.relu_out || g.mask_src || g.n_peers > 0 || g.linear) return 1;
+    if (g_no_splitk || g.no_alloc || g.batch != 1 || g.m > kBM || g.relu_out || g.mask_src || g.n_peers > 0) return 1;
     if (g.k % 64 != 0 || g.n % 4 != 0) return 1;
     // measured: no gain (or a loss, once the partial tiles weigh against the weights) below 4096 deep or 32 MB of weights
     if (g.k < 4096 || g.n * g.k < (int64_t(1) << 24)) return 1;
@@ -2514,7 +2670,7 @@ F16Plan plan_f16_tiles(const GemmArgs& g, int es = 2) {
     const int block_k = 128 / es;  // 8-bit operands: 128 deep K blocks, the same four MMAs and the same cycles
     const double kb = double((g.k + block_k - 1) / block_k);
     const bool fused = g.relu_out || g.mask_src || g.n_peers > 0;
-    const bool may_split = es == 2 && !g_no_splitk && !g.linear && !g.no_alloc && g.batch == 1 && !fused && g.n % 4 == 0;   // the reduce kernel is 16-bit
+    const bool may_split = es == 2 && !g_no_splitk && !g.no_alloc && g.batch == 1 && !fused && g.n % 4 == 0;   // the reduce kernel is 16-bit
     const double dram_us = double(g.batch) * (double(g.m) * g.k + double(g.k) * g.n + double(g.m) * g.n) * es / 4.5e6;
     struct Cand { bool pair; int bn; double fixed_us, us_per_k_block; };   // launch + fill + last epilogue; main loop
     const Cand cands[] = {{true, 256, 11.0, 0.35}, {false, 256, 13.0, 0.39}, {false, 128, 10.0, 0.34}, {false, 64, 10.0, 0.30}};
@@ -2571,6 +2727,22 @@ __global__ void splitk_reduce_kernel(const float* __restrict__ partial, int spli
     }
 }
 
+// The same for ntb200_linear_act: the partial tiles of a row are added in order, then everything after the product.
+__global__ void splitk_linear_kernel(const float* __restrict__ partial, int splits, long long slab, int m, int n, const LinearParams l) {
+    const int n4 = n >> 2;
+    const long long idx = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+    if (idx >= (long long)m * n4) return;
+    const int row = int(idx / n4), col = int(idx % n4) * 4;
+    const float* src = partial + (long long)row * n + col;
+    float4 acc = *reinterpret_cast<const float4*>(src);
+    for (int s = 1; s < splits; ++s) {
+        const float4 v = *reinterpret_cast<const float4*>(src + s * slab);
+        acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+    }
+    float f[4] = {acc.x, acc.y, acc.z, acc.w};
+    linear_finish4(l, n, row, col, f);
+}
+
 int launch_f16_split_k(const GemmArgs& g, const Planned& pl16, int splits, const TileChoice* choice, cudaStream_t stream) {
     const int64_t slab = g.m * g.n, kslice = g.k / splits;
     float* partial = nullptr;
@@ -2580,6 +2752,7 @@ int launch_f16_split_k(const GemmArgs& g, const Planned& pl16, int splits, const
     part.k = kslice;
     part.c = partial; part.c_rs = g.n; part.c_bs = slab;
     part.bias = nullptr; part.accumulate = 0;
+    part.linear = nullptr;
     Planned pl = pl16;
     pl.out_kind = kOutF32;
     pl.route = g.dtype == NTB200_F16 ? "umma_f16_splitk" : "umma_bf16_splitk";
@@ -2591,7 +2764,9 @@ int launch_f16_split_k(const GemmArgs& g, const Planned& pl16, int splits, const
         uint16_t* c = static_cast<uint16_t*>(g.c);
         const uint16_t* bias = static_cast<const uint16_t*>(g.bias);
         const int wide_stores = (reinterpret_cast<uintptr_t>(g.c) % 8 == 0 && g.c_rs % 4 == 0) ? 1 : 0;
-        if (g.dtype == NTB200_F16)
+        if (g.linear)
+            splitk_linear_kernel<<<blocks, 256, 0, stream>>>(partial, splits, slab, int(g.m), int(g.n), *g.linear);
+        else if (g.dtype == NTB200_F16)
             splitk_reduce_kernel<kOutF16><<<blocks, 256, 0, stream>>>(partial, splits, slab, int(g.m), int(g.n), c, g.c_rs, bias,
                                                                      g.bias_rs, g.bias_cs, g.accumulate, wide_stores);
         else
@@ -2610,7 +2785,7 @@ int launch_f16_split_k(const GemmArgs& g, const Planned& pl16, int splits, const
 // Returns NTB200_ERR_UNSUPPORTED (nothing launched, error text untouched) when the shape does not fit the scheme.
 const bool g_no_cluster_k = [] { const char* e = getenv("NTB200_NO_CLUSTER_K"); return e && e[0] == '1'; }();
 
-template <int BN>
+template <int BN, MmaKind kKind = MmaKind::f16, bool kLinear = false>
 int launch_cluster_k_instance(const Maps& maps, ClusterKParams cp, int a_rows_staged, int clusters, cudaStream_t stream) {
     using T = Tile<BN, false>;
     UmmaParams& p = cp.u;
@@ -2621,7 +2796,7 @@ int launch_cluster_k_instance(const Maps& maps, ClusterKParams cp, int a_rows_st
     const uint32_t ring = uint32_t(p.s_stages) * p.s_stage_bytes + T::kABytes;
     if (uint32_t(cp.rows_live) * uint32_t(cp.pitch) * 4u > ring) return NTB200_ERR_UNSUPPORTED;   // the partial tile lives in the ring
     const uint32_t smem = ring + T::kBarrierBytes + 1024;
-    auto kernel = umma_gemm_cluster_k_kernel<BN>;
+    auto kernel = umma_gemm_cluster_k_kernel<BN, kKind, kLinear>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
     if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(umma_gemm_cluster_k_kernel)");
     cudaLaunchConfig_t cfg = {};
@@ -2674,7 +2849,7 @@ int cluster_k_capacity(int bn, int slices) {
 
 ClusterKPlan plan_cluster_k(const GemmArgs& g, int es) {
     ClusterKPlan best{0, 0, 1e30, false};
-    if (g_no_cluster_k || g.no_alloc || g.batch != 1 || g.relu_out || g.mask_src || g.n_peers > 0 || g.linear) return best;
+    if (g_no_cluster_k || g.no_alloc || g.batch != 1 || g.relu_out || g.mask_src || g.n_peers > 0) return best;
     if (g.k < 2048 || g.n * g.k < (int64_t(1) << 23)) return best;
     const int block_k = 128 / es;
     const int k_blocks = int((g.k + block_k - 1) / block_k);
@@ -2743,9 +2918,20 @@ int launch_f16_cluster_k(const GemmArgs& g, const Planned& pl16, const ClusterKP
     cp.pitch = bn + 4;
     cp.rows_live = int(std::min<int64_t>(kBM, (g.m + 31) / 32 * 32));   // every M tile but the last is full
     cp.c_wide_ok = (reinterpret_cast<uintptr_t>(g.c) % 8 == 0 && g.c_rs % 4 == 0) ? 1 : 0;
-    const int rc = bn == 256 ? launch_cluster_k_instance<256>(maps, cp, a_rows_staged, p.total_tiles, stream)
-                             : launch_cluster_k_instance<128>(maps, cp, a_rows_staged, p.total_tiles, stream);
-    if (rc == NTB200_OK) note_route(g.dtype == NTB200_F16 ? "umma_f16_clusterk" : "umma_bf16_clusterk");
+    int rc;
+    if (g.linear) {
+        p.linear = *g.linear;
+        if (pl16.kind == MmaKind::i8)
+            rc = bn == 256 ? launch_cluster_k_instance<256, MmaKind::i8, true>(maps, cp, a_rows_staged, p.total_tiles, stream)
+                           : launch_cluster_k_instance<128, MmaKind::i8, true>(maps, cp, a_rows_staged, p.total_tiles, stream);
+        else
+            rc = bn == 256 ? launch_cluster_k_instance<256, MmaKind::f16, true>(maps, cp, a_rows_staged, p.total_tiles, stream)
+                           : launch_cluster_k_instance<128, MmaKind::f16, true>(maps, cp, a_rows_staged, p.total_tiles, stream);
+    } else {
+        rc = bn == 256 ? launch_cluster_k_instance<256>(maps, cp, a_rows_staged, p.total_tiles, stream)
+                       : launch_cluster_k_instance<128>(maps, cp, a_rows_staged, p.total_tiles, stream);
+    }
+    if (rc == NTB200_OK) note_route(g.dtype == NTB200_I8 ? "umma_i8_clusterk" :g.dtype == NTB200_F16 ? "umma_f16_clusterk" : "umma_bf16_clusterk");
     return rc;
 }
 
@@ -2917,6 +3103,13 @@ int launch_umma_gemm(const GemmArgs& g, cudaStream_t stream) {
     if (is_i8) {
         plan = plan_f16_tiles(g, 1);
         if (plan.valid && !tune_int("NTB200_OLD_PLAN")) choice = &plan.tile;
+        if (g.linear && g.m <= kBM) {   // few rows: K slices inside a cluster, as for 16 bits below
+            const ClusterKPlan ck = plan_cluster_k(g, es);
+            if (ck.valid) {
+                const int rc = launch_f16_cluster_k(g, pl, ck, stream);
+                if (rc != NTB200_ERR_UNSUPPORTED) return rc;
+            }
+        }
     } else {
         int splits = pick_k_splits(g);
         plan = plan_f16_tiles(g);

@@ -342,7 +342,8 @@ def test_norm_in_place_of_the_stream(n):
 # ---- linear ---------------------------------------------------------------------------------------------------------
 
 LINEAR_SHAPES = [(1, 1, 1), (1, 64, 8), (3, 7, 5), (5, 40, 33), (16, 512, 256), (33, 100, 130), (128, 4096, 2048), (129, 72, 200),
-                 (200, 257, 300), (300, 640, 513), (1, 4096, 4096), (64, 4096, 4096), (256, 4096, 512), (1100, 136, 1032)]
+                 (200, 257, 300), (300, 640, 513), (1, 4096, 4096), (64, 4096, 4096), (256, 4096, 512), (1100, 136, 1032),
+                 (2600, 72, 4104), (2600, 72, 4103)]      # several tiles per CTA pair
 
 
 def linear_tolerance(x64, w64, k, dtype, y64, extra=0.0):
@@ -438,7 +439,7 @@ def test_linear_gradients_are_differences(act):
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("m,k,n", [(1, 1, 1), (3, 7, 5), (8, 512, 256), (33, 100, 130), (129, 272, 200), (300, 641, 513), (1, 4096, 4096), (16, 4096, 2048),
-                                   (1100, 144, 1040)])
+                                   (1100, 144, 1040), (2600, 80, 4104)])
 def test_linear_int8(m, k, n, dtype, act):
     from neurotensor_b200 import api
     gen = generator(m + 7 * k + 31 * n)
