@@ -12,6 +12,7 @@
 
 #include "internal.h"
 #include "row_ops.cuh"
+#include "sm100_ptx.cuh"
 
 namespace ntb200 {
 namespace {
@@ -75,7 +76,296 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
     return warp_sum(lane < kThreads / 32 ? red[lane] : 0.f);
 }
 
-// One block per row.
+// ---- one cluster per row: the row stays in shared memory ------------------------------------------------------------
+// The C blocks of a cluster hold one row, a piece each, fetched once by untiled bulk copies in four parts; maximum, sum and
+// gradient then come from shared memory, and only (max, sum, teacher's share) of each piece crosses the cluster.  A block
+// that re-read its row from L2 instead took 623 us for 4096 x 131072 bf16 logits: the rows in flight (592 x 256 KB) do not
+// fit L2, so the second read went to memory again.  Pieces are at most 72 KB where C <= 8 allows it, so that three blocks
+// per SM overlap loading, arithmetic and storing.
+// Rows need not start on 16 bytes: the piece's whole 16-byte granules are copied, the elements of a cut first or last
+// granule are loaded one by one, and what else lies in those two granules is set to -inf, which adds nothing.
+constexpr int kPieceThreads = 256, kParts = 4, kMaxCluster = 8;
+
+// Behind the piece in dynamic shared memory: three arrays of `top` entries (the teacher's probabilities, the student's
+// logits at the same places, the columns within this piece, -1: not there or in another block's piece).
+struct PieceShared {
+    float red[3][kPieceThreads / 32];
+    float4 share[kMaxCluster];           // (max, sum, sum p (x - max), sum p) of every block's piece, by rank
+    unsigned long long bar[kParts];
+    uint32_t abort_flag;
+};
+
+// Two maxima, or up to three sums, over the block in one exchange.
+__device__ __forceinline__ void piece_max2(float& u, float& v, PieceShared& sh) {
+    constexpr int W = kPieceThreads / 32;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        u = fmaxf(u, __shfl_xor_sync(0xffffffffu, u, o));
+        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    }
+    if (lane == 0) { sh.red[0][warp] = u; sh.red[1][warp] = v; }
+    __syncthreads();
+    u = sh.red[0][0]; v = sh.red[1][0];
+#pragma unroll
+    for (int i = 1; i < W; ++i) { u = fmaxf(u, sh.red[0][i]); v = fmaxf(v, sh.red[1][i]); }
+    __syncthreads();
+}
+template <int N>
+__device__ __forceinline__ void piece_sums(float (&u)[N], PieceShared& sh) {
+    constexpr int W = kPieceThreads / 32;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        u[k] = warp_sum(u[k]);
+        if (lane == 0) sh.red[k][warp] = u[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        u[k] = sh.red[k][0];
+#pragma unroll
+        for (int i = 1; i < W; ++i) u[k] += sh.red[k][i];
+    }
+    __syncthreads();
+}
+
+// The largest of V elements.  16-bit types compare two at a time, which changes no value (NaN is ignored either way and
+// shows in the sum).
+template <class T, int V>
+__device__ __forceinline__ float pack_max(const Pack<T, V>& x) {
+    if constexpr (sizeof(T) == 4) {
+        float top = x.up(0);
+#pragma unroll
+        for (int k = 1; k < V; ++k) top = fmaxf(top, x.up(k));
+        return top;
+    } else {
+        using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+        const T2* p = reinterpret_cast<const T2*>(x.e);
+        T2 top = p[0];
+#pragma unroll
+        for (int k = 1; k < V / 2; ++k) top = __hmax2(top, p[k]);
+        return fmaxf(RowType<T>::up(top.x), RowType<T>::up(top.y));
+    }
+}
+
+__device__ __forceinline__ void st_cluster_f4(uint32_t local_addr, uint32_t cta_rank, float4 v) {
+    asm volatile(
+        "{\n\t.reg .b32 remote;\n\t"
+        "mapa.shared::cluster.u32 remote, %0, %1;\n\t"
+        "st.shared::cluster.v4.f32 [remote], {%2, %3, %4, %5};\n\t}"
+        ::"r"(local_addr), "r"(cta_rank), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+}
+
+template <class T>
+__global__ void __launch_bounds__(kPieceThreads, 3) distill_piece_kernel(const DistillArgs a, int C, int piece, bool same_align, unsigned int* status) {
+    constexpr int V = 16 / sizeof(T);
+    extern __shared__ __align__(128) uint8_t piece_mem[];
+    __shared__ PieceShared sh;
+    float* sh_p = reinterpret_cast<float*>(piece_mem + (size_t(piece) * sizeof(T) + 32));
+    float* sh_x = sh_p + a.top;
+    int* sh_at = reinterpret_cast<int*>(sh_x + a.top);
+    const int tid = threadIdx.x, lane = tid & 31;
+    const uint32_t rank = C > 1 ? cluster_cta_rank() : 0u;
+    const long long row = blockIdx.x / C;
+    const float c = kLog2e / a.temp;
+    const int first = int(rank) * piece, count = max(0, min(piece, a.vocab - first));
+    const T* s = static_cast<const T*>(a.s) + row * a.s_rs + first;
+    T* grad = a.grad ? static_cast<T*>(a.grad) + row * a.g_rs + first : nullptr;
+    const float weight = a.weight ? a.weight[row] : a.even_weight;
+    // granules of 16 bytes: element e of the piece sits at e + lead; granules [g0, g1) are whole
+    const int lead = int((reinterpret_cast<uintptr_t>(s) & 15) / sizeof(T));
+    const int granules = count ? (lead + count + V - 1) / V : 0;
+    const int g0 = lead ? 1 : 0, g1 = (lead + count) / V;
+    auto zeros = [&]() {
+        if (!grad) return;
+        const bool wide = same_align && g1 > g0;
+        const int w0 = wide ? g0 * V - lead : 0, w1 = wide ? g1 * V - lead : 0;   // elements written 16 bytes at a time
+        Pack<T, V> zero;
+#pragma unroll
+        for (int k = 0; k < V; ++k) zero.set(k, 0.f);
+        for (int v = g0 + tid; wide && v < g1; v += kPieceThreads) reinterpret_cast<Pack<T, V>*>(grad - lead)[v] = zero;
+        for (int v = tid; v < count - (w1 - w0); v += kPieceThreads) grad[v < w0 ? v : v + (w1 - w0)] = RowType<T>::down(0.f);
+    };
+    if (weight == 0.f) {
+        zeros();
+        if (rank == 0 && tid == 0) a.row_loss[row] = 0.f;
+        return;
+    }
+    T* mem = reinterpret_cast<T*>(piece_mem);
+    const int part = g1 > g0 ? (g1 - g0 + kParts - 1) / kParts : 0;   // granules per part
+    if (tid == 0) {
+        sh.abort_flag = 0;
+        for (int i = 0; i < kParts; ++i) mbar_init(smem_u32(&sh.bar[i]), 1);
+        fence_barrier_init();
+        fence_proxy_async_smem();
+        for (int i = 0; i < kParts; ++i) {
+            const int b = g0 + i * part, e = min(g1, b + part);
+            if (b >= e) continue;
+            mbar_expect_tx(smem_u32(&sh.bar[i]), uint32_t(e - b) * 16u);
+            bulk_load(smem_u32(piece_mem) + uint32_t(b) * 16u, s + (b * V - lead), uint32_t(e - b) * 16u, smem_u32(&sh.bar[i]));
+        }
+    }
+    if (tid < V && granules) {   // the cut granules
+        if (g0 == 1) mem[tid] = tid >= lead && tid - lead < count ? s[tid - lead] : RowType<T>::down(-INFINITY);
+        if (granules > g1 && (granules - 1 >= g0)) {
+            const int e = (granules - 1) * V + tid - lead;
+            mem[(granules - 1) * V + tid] = e < count ? s[e] : RowType<T>::down(-INFINITY);
+        }
+    }
+    // the teacher's entries, in every block
+    float tmax = -INFINITY;
+    int present = 0;
+    for (int j = tid; j < a.top; j += kPieceThreads) {
+        const long long i = a.idx64 ? static_cast<const long long*>(a.idx)[row * a.top + j] : static_cast<const int*>(a.idx)[row * a.top + j];
+        const float t = i >= 0 && i < a.vocab ? teacher_value(a, row * a.top + j) : -INFINITY;
+        sh_at[j] = t != -INFINITY && i >= first && i < first + count ? int(i - first) : -1;
+        sh_p[j] = t;
+        present |= t != -INFINITY;
+        tmax = fmaxf(tmax, t);
+    }
+    present = __syncthreads_or(present);
+    if (C > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // this block runs: its shared memory may be written
+    bool landed = true;
+    auto wait_part = [&](int i) {
+        if (g0 + i * part < min(g1, g0 + (i + 1) * part)) landed = mbar_wait(smem_u32(&sh.bar[i]), 0, &sh.abort_flag) && landed;
+    };
+    float m = -INFINITY;
+    if (granules > g1 && granules - 1 >= g0 && tid < V) m = RowType<T>::up(mem[(granules - 1) * V + tid]);
+    if (g0 == 1 && tid < V) m = fmaxf(m, RowType<T>::up(mem[tid]));
+    for (int i = 0; i < kParts; ++i) {
+        wait_part(i);
+        for (int v = g0 + i * part + tid; v < min(g1, g0 + (i + 1) * part); v += kPieceThreads) {
+            m = fmaxf(m, pack_max(reinterpret_cast<const Pack<T, V>*>(mem)[v]));
+        }
+    }
+    if (!landed && lane == 0) {
+        sh.abort_flag = 1;
+        atomicExch(status, 0x151u);
+    }
+    piece_max2(tmax, m, sh);
+    const float ref = m == -INFINITY ? 0.f : m, mc = ref * c;
+    float sums[2] = {0.f, 0.f};          // the teacher's and the student's
+    for (int j = tid; j < a.top; j += kPieceThreads) sums[0] += sh_p[j] == -INFINITY ? 0.f : exp2f((sh_p[j] - tmax) * c);
+    float z0 = 0.f, z1 = 0.f;
+#pragma unroll 2
+    for (int v = tid; v < granules; v += kPieceThreads) {
+        const Pack<T, V> x = reinterpret_cast<const Pack<T, V>*>(mem)[v];
+#pragma unroll
+        for (int k = 0; k < V; k += 2) {
+            z0 += exp2_hw(sizeof(T) == 4 ? (x.up(k) - ref) * c : fmaf(x.up(k), c, -mc));
+            z1 += exp2_hw(sizeof(T) == 4 ? (x.up(k + 1) - ref) * c : fmaf(x.up(k + 1), c, -mc));
+        }
+    }
+    sums[1] = z0 + z1;
+    piece_sums(sums, sh);
+    const float tsum = sums[0], z = sums[1];
+    // probabilities
+    float parts[3] = {0.f, 0.f, 0.f};    // sum p log p, sum p and sum p (x - m) of this piece
+    const float log2t = log2f(tsum);
+    for (int j = tid; j < a.top; j += kPieceThreads) {
+        const float t = sh_p[j];
+        float p = 0.f;
+        if (t != -INFINITY) {
+            const float lt = (t - tmax) * c;
+            p = exp2f(lt) / tsum;
+            if (p != 0.f) parts[0] += p * (lt - log2t);
+        }
+        sh_p[j] = p;
+        if (sh_at[j] >= 0 && p != 0.f) {
+            const float x = RowType<T>::up(mem[sh_at[j] + lead]);
+            sh_x[j] = x;
+            parts[1] += p;
+            parts[2] += p * ((x - ref) * c);
+        } else if (sh_at[j] >= 0) {
+            sh_x[j] = RowType<T>::up(mem[sh_at[j] + lead]);
+        }
+    }
+    piece_sums(parts, sh);
+    const float entropy = parts[0], own_p = parts[1], own_x = parts[2];
+    if (C > 1) {
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (tid < C) st_cluster_f4(smem_u32(&sh.share[rank]), uint32_t(tid), make_float4(m, z, own_x, own_p));
+        cluster_sync_all();
+    } else {
+        if (tid == 0) sh.share[0] = make_float4(m, z, own_x, own_p);
+        __syncthreads();
+    }
+    if (sh.abort_flag) {   // a copy did not land in time (the status word tells): it may still, so the block waits once more
+        volatile uint32_t never = 0;
+        if (tid == 0)
+            for (int i = 0; i < kParts; ++i)
+                if (g0 + i * part < min(g1, g0 + (i + 1) * part)) (void)mbar_wait(smem_u32(&sh.bar[i]), 0, &never);
+        __syncthreads();
+        return;
+    }
+    float gm = -INFINITY, gz = 0.f, cross = 0.f;
+    for (int i = 0; i < C; ++i) gm = fmaxf(gm, sh.share[i].x);
+    for (int i = 0; i < C; ++i) {
+        const float4 q = sh.share[i];
+        const float d = q.x == -INFINITY ? 0.f : (q.x - gm) * c;
+        gz += q.x == -INFINITY && gm != -INFINITY ? 0.f : q.y * exp2f(d);
+        cross += q.z + q.w * d;          // sum p (x - gm) c
+    }
+    if (gm == -INFINITY) gz = NAN;       // every column of the student masked out
+    if (!present) {
+        zeros();
+        if (rank == 0 && tid == 0) a.row_loss[row] = 0.f;
+        return;
+    }
+    if (rank == 0 && tid == 0) a.row_loss[row] = a.temp * a.temp * (entropy - cross + log2f(gz)) / kLog2e;
+    if (!grad) return;
+    const float coef = weight * a.temp, scale = coef / gz;
+    // q times its factor: for 16-bit gradients one multiply-add and one exponential, the factor inside the exponent
+    const bool fold = sizeof(T) == 2 && scale > 0.f;
+    const float off = fold ? fmaf(-gm, c, log2f(scale)) : -gm * c, mul = fold ? 1.f : scale;
+    auto value = [&](float x) { return (sizeof(T) == 4 ? exp2_hw((x - gm) * c) : exp2_hw(fmaf(x, c, off))) * mul; };
+    if (same_align && fold) {
+        Pack<T, V>* gv = reinterpret_cast<Pack<T, V>*>(grad - lead);
+#pragma unroll 2
+        for (int v = g0 + tid; v < g1; v += kPieceThreads) {
+            const Pack<T, V> x = reinterpret_cast<const Pack<T, V>*>(mem)[v];
+            float o[V];
+#pragma unroll
+            for (int k = 0; k < V; ++k) o[k] = exp2_hw(fmaf(x.up(k), c, off));
+            Pack<T, V> q;
+            q.put(o);
+            gv[v] = q;
+        }
+    } else if (same_align) {
+        Pack<T, V>* gv = reinterpret_cast<Pack<T, V>*>(grad - lead);
+        for (int v = g0 + tid; v < g1; v += kPieceThreads) {
+            const Pack<T, V> x = reinterpret_cast<const Pack<T, V>*>(mem)[v];
+            Pack<T, V> o;
+#pragma unroll
+            for (int k = 0; k < V; ++k) o.set(k, value(x.up(k)));
+            gv[v] = o;
+        }
+    }
+    if (same_align) {
+        if (tid < V && granules) {
+            if (g0 == 1 && tid >= lead && tid - lead < count) grad[tid - lead] = RowType<T>::down(value(RowType<T>::up(mem[tid])));
+            const int e = (granules - 1) * V + tid - lead;
+            if (granules > g1 && granules - 1 >= g0 && e < count) grad[e] = RowType<T>::down(value(RowType<T>::up(mem[e + lead])));
+        }
+    } else {
+        for (int v = tid; v < count; v += kPieceThreads) grad[v] = RowType<T>::down(value(RowType<T>::up(mem[v + lead])));
+    }
+    __syncthreads();
+    for (int j = tid; j < a.top; j += kPieceThreads) {
+        const int at = sh_at[j];
+        if (at < 0) continue;
+        bool one = true;
+        for (int k = 0; k < j; ++k) one = one && sh_at[k] != at;
+        if (!one) continue;
+        float p = sh_p[j];
+        for (int k = j + 1; k < a.top; ++k)
+            if (sh_at[k] == at) p += sh_p[k];
+        grad[at] = RowType<T>::down(scale * exp2f((sh_x[j] - gm) * c) - coef * p);
+    }
+}
+
+// One block per row, the row read twice: rows too long for eight blocks' shared memory.
 template <class T, int V, int kThreads>
 __global__ void __launch_bounds__(kThreads) distill_kernel(const DistillArgs a) {
     __shared__ RowShared<kThreads> sh;
@@ -204,12 +494,52 @@ __global__ void __launch_bounds__(1024) distill_total_kernel(const float* __rest
     if (threadIdx.x == 0) *loss = v;
 }
 
+// Blocks per row: the smallest power of two whose pieces are at most 72 KB (three blocks per SM), more while the rows leave
+// SMs without a block and pieces stay above 8 KB; then whatever fits a block's shared memory.  0: the row does not.
+int cluster_size(long long rows, int vocab, int es) {
+    constexpr long long kMany = 72 * 1024, kMost = 200 * 1024;
+    const long long bytes = (long long)vocab * es;
+    int C = 1;
+    while (C < kMaxCluster && (bytes > kMany * C || (rows * C * 2 <= sm_count() && bytes > 16 * 1024 * C))) C *= 2;
+    return bytes > kMost * C ? 0 : C;
+}
+
 template <class T>
 int launch_distill(const DistillArgs& a, bool vec_ok, float* loss, cudaStream_t stream) {
     constexpr int kVec = 16 / sizeof(T);
-    const int grid = int(std::min<long long>(a.rows, 1ll << 30));
-    if (vec_ok) distill_kernel<T, kVec, 512><<<grid, 512, 0, stream>>>(a);
-    else distill_kernel<T, 1, 512><<<grid, 512, 0, stream>>>(a);
+    const int C = cluster_size(a.rows, a.vocab, int(sizeof(T)));
+    if (C > 0 && a.rows * C < (1ll << 31)) {
+        const int piece = int(((long long)a.vocab + C - 1) / C + 63) / 64 * 64;
+        const uint32_t smem = uint32_t(piece) * uint32_t(sizeof(T)) + 32u + 12u * uint32_t(a.top);
+        const bool same_align = a.grad && (reinterpret_cast<uintptr_t>(a.grad) - reinterpret_cast<uintptr_t>(a.s)) % 16 == 0 &&
+                                ((a.g_rs - a.s_rs) * (long long)sizeof(T)) % 16 == 0;
+        auto kernel = distill_piece_kernel<T>;
+        static std::atomic<bool> set[64];
+        int dev = 0;
+        (void)cudaGetDevice(&dev);
+        if (dev < 0 || dev >= 64) dev = 0;
+        if (!set[dev].load(std::memory_order_acquire)) {
+            NTB200_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 213 * 1024));
+            set[dev].store(true, std::memory_order_release);
+        }
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(unsigned(a.rows * C), 1, 1);
+        cfg.blockDim = dim3(kPieceThreads, 1, 1);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = stream;
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = unsigned(C);
+        attr.val.clusterDim.y = 1;
+        attr.val.clusterDim.z = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        NTB200_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, C, piece, same_align, device_status_word()));
+    } else {
+        const int grid = int(std::min<long long>(a.rows, 1ll << 30));
+        if (vec_ok) distill_kernel<T, kVec, 512><<<grid, 512, 0, stream>>>(a);
+        else distill_kernel<T, 1, 512><<<grid, 512, 0, stream>>>(a);
+    }
     count_launch();
     NTB200_CUDA(cudaGetLastError());
     distill_total_kernel<<<1, 1024, 0, stream>>>(a.row_loss, a.weight, a.even_weight, a.rows, loss);

@@ -212,38 +212,72 @@ __device__ __forceinline__ void drain_partial(uint32_t taddr, float (&run)[HC], 
             run[cc * 32 + j] = first ? __uint_as_float(v[j]) : run[cc * 32 + j] + __uint_as_float(v[j]);
     }
 }
-template <int HC, bool kLinear>
+template <int HC>
 __device__ __forceinline__ void store_running(const UmmaParams& p, const float (&run)[HC], int b, int row, int col_base) {
     if (row >= p.m) return;
 #pragma unroll
-    for (int cc = 0; cc < HC / 32; ++cc) {
-        if (col_base + cc * 32 >= p.n) continue;
-        if constexpr (kLinear) {
-            float f[32];
+    for (int cc = 0; cc < HC / 32; ++cc)
+        if (col_base + cc * 32 < p.n) store_chunk_f32(p, b, row, col_base + cc * 32, &run[cc * 32]);
+}
+// Epilogue of the kLinear instantiations where TMA cannot move y, pre or the residual, and of their single-CTA tiles: the
+// products go through a kRows x 32 fp32 block of shared memory per warp and leave by rows.  A thread that stored its own
+// row would touch 32 rows per instruction; on [333, 1001] x [1001, 1030], whose rows start on 4 bytes, that took 47 us.
+// `wait` waits for the accumulator: what the first chunk needs besides it is requested before.
+constexpr uint32_t kStagedBlock = 16 * 33 * 4;      // 16 rows per warp; the pair kernel's staging buffer holds 32
+template <int kRows, int kDt>
+__device__ __forceinline__ void finish_chunk(const UmmaParams& p, const float (&f)[32], float* staged, int row0, int lane, int col0, const LinearAhead& a) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) f[j] = run[cc * 32 + j];
-            linear_finish32(p.linear, p.n, row, col_base + cc * 32, f);
-        } else {
-            store_chunk_f32(p, b, row, col_base + cc * 32, &run[cc * 32]);
-        }
+    for (int first = 0; first < 32; first += kRows) {
+        if (row0 + first >= p.m) break;   // uniform across the warp
+        __syncwarp();                     // the previous block's readers are done
+        if (kRows == 32 || (lane & ~(kRows - 1)) == first)
+#pragma unroll
+            for (int j = 0; j < 32; ++j) staged[(lane - first) * 33 + j] = f[j];
+        __syncwarp();
+        linear_finish_block<kDt, kRows>(p.linear, p.m, p.n, staged, row0, first, col0, lane, a);
     }
 }
-
-// Epilogue of the kLinear instantiations (Float16 / BFloat16 / Int8 operands): each thread owns a row of the tile.
-template <int BN, bool kInt>
-__device__ __forceinline__ void epilogue_linear(const UmmaParams& p, uint32_t tmem_acc, int row, int n0) {
+template <int BN, bool kInt, int kRows, int kDt, class Wait>
+__device__ __forceinline__ bool epilogue_linear(const UmmaParams& p, uint32_t tmem_acc, float* staged, int row0, int lane, int n0, const Wait& wait) {
+    LinearAhead ahead;
+    linear_load_ahead<kDt>(p.linear, p.m, p.n, row0, n0, lane, ahead);
+    if (!wait()) return false;
+    if (row0 >= p.m) return true;   // uniform across the warp
 #pragma unroll 1
     for (int cc = 0; cc < BN / 32; ++cc) {
         const int col0 = n0 + cc * 32;
         if (col0 >= p.n) break;  // uniform across the CTA
         uint32_t v[32];
         tmem_ld_32x32b_x32(tmem_acc + uint32_t(cc * 32), v);
+        if (cc > 0) linear_load_ahead<kDt>(p.linear, p.m, p.n, row0, col0, lane, ahead);
         tmem_ld_wait();
-        if (row >= p.m) continue;
         float f[32];
 #pragma unroll
         for (int j = 0; j < 32; ++j) f[j] = kInt ? __int2float_rn(int(v[j])) : __uint_as_float(v[j]);
-        linear_finish32(p.linear, p.n, row, col0, f);
+        finish_chunk<kRows, kDt>(p, f, staged, row0, lane, col0, ahead);
+    }
+    return true;
+}
+template <int BN, bool kInt, int kRows, class Wait>
+__device__ __forceinline__ bool epilogue_linear(const UmmaParams& p, uint32_t tmem_acc, float* staged, int row0, int lane, int n0, const Wait& wait) {
+    if (p.linear.out_dtype == NTB200_F16) return epilogue_linear<BN, kInt, kRows, NTB200_F16>(p, tmem_acc, staged, row0, lane, n0, wait);
+    if (kInt && p.linear.out_dtype == NTB200_F32) return epilogue_linear<BN, kInt, kRows, NTB200_F32>(p, tmem_acc, staged, row0, lane, n0, wait);
+    return epilogue_linear<BN, kInt, kRows, NTB200_BF16>(p, tmem_acc, staged, row0, lane, n0, wait);
+}
+// The Float32 split kernels' running sums.
+template <int HC>
+__device__ __forceinline__ void finish_running(const UmmaParams& p, const float (&run)[HC], float* staged, int row0, int lane, int col_base) {
+    if (row0 >= p.m) return;
+#pragma unroll
+    for (int cc = 0; cc < HC / 32; ++cc) {
+        const int col0 = col_base + cc * 32;
+        if (col0 >= p.n) continue;
+        LinearAhead ahead;
+        linear_load_ahead<NTB200_F32>(p.linear, p.m, p.n, row0, col0, lane, ahead);
+        float f[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) f[j] = run[cc * 32 + j];
+        finish_chunk<16, NTB200_F32>(p, f, staged, row0, lane, col0, ahead);
     }
 }
 
@@ -789,8 +823,10 @@ __device__ __forceinline__ bool epilogue_linear_tma(const UmmaParams& p, const C
     return true;
 }
 
+// kLinear: eight epilogue warps, each on half of the tile's columns (a problem on single-CTA tiles has few of them per SM,
+// so the epilogue's latency is not hidden).
 template <MmaKind kKind, int BN, bool kSplit, bool kLinear = false>
-__global__ void __launch_bounds__(kSplit ? kThreadsSplit : kThreads, 1)
+__global__ void __launch_bounds__(kSplit || kLinear ? kThreadsSplit : kThreads, 1)
 umma_gemm_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
                  const __grid_constant__ CUtensorMap tma_a_lo, const __grid_constant__ CUtensorMap tma_b_lo,
                  const UmmaParams p) {
@@ -820,7 +856,7 @@ umma_gemm_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(tfull_bar(a), 1);
-            mbar_init(tempty_bar(a), kSplit ? 8 : 4);   // one arrival per epilogue warp
+            mbar_init(tempty_bar(a), kSplit || kLinear ? 8 : 4);   // one arrival per epilogue warp
         }
         *abort_flag = 0;
         fence_barrier_init();
@@ -970,7 +1006,13 @@ umma_gemm_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
                 if (lane == 0) mbar_arrive(tempty_bar(acc));
                 if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
             }
-            if (alive) store_running<HC, kLinear>(p, run, b, mi * kBM + row_in_tile, ni * BN + half * HC);
+            if (alive) {
+                if constexpr (kLinear)
+                    finish_running<HC>(p, run, reinterpret_cast<float*>(bar_gen + T::kBarrierBytes + uint32_t(warp - 2) * kStagedBlock),
+                                       mi * kBM + quad * 32, lane, ni * BN + half * HC);
+                else
+                    store_running<HC>(p, run, b, mi * kBM + row_in_tile, ni * BN + half * HC);
+            }
         }
     } else {
         // ------------------------------------------------------------------ epilogue
@@ -981,17 +1023,23 @@ umma_gemm_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
         for (int t = blockIdx.x; t < p.total_tiles; t += gridDim.x) {
             int b, mi, ni;
             tile_coords(p, t, b, mi, ni);
-            bool ok = mbar_wait(tfull_bar(acc), acc_phase, abort_flag);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) {
-                if (lane == 0) raise_timeout(abort_flag, 5);
+            auto wait = [&]() {
+                const bool ok = __all_sync(0xffffffffu, mbar_wait(tfull_bar(acc), acc_phase, abort_flag));
+                if (ok) tcgen05_fence_after();
+                else if (lane == 0) raise_timeout(abort_flag, 5);
+                return ok;
+            };
+            if constexpr (kLinear) {
+                const int half = (warp - 2) >> 2;
+                if (!epilogue_linear<BN / 2, kKind == MmaKind::i8, 16>(
+                        p, tmem_base + (uint32_t(quad * 32) << 16) + uint32_t(acc * BN + half * (BN / 2)),
+                        reinterpret_cast<float*>(bar_gen + T::kBarrierBytes + uint32_t(warp - 2) * kStagedBlock), mi * kBM + quad * 32, lane,
+                        ni * BN + half * (BN / 2), wait))
+                    break;
+            } else if (!wait()) {
                 break;
             }
-            tcgen05_fence_after();
-            if constexpr (kLinear)
-                epilogue_linear<BN, kKind == MmaKind::i8>(p, tmem_base + (uint32_t(quad * 32) << 16) + uint32_t(acc * BN),
-                                                          mi * kBM + row_in_tile, ni * BN);
-            else
+            if constexpr (!kLinear)
                 epilogue_tile<BN>(p, tmem_base + (uint32_t(quad * 32) << 16) + uint32_t(acc * BN), b,
                                   mi * kBM + row_in_tile, ni * BN);
             tcgen05_fence_before();
@@ -1219,7 +1267,13 @@ umma_gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
                 if (lane == 0) mbar_arrive_leader(tempty_bar(acc));
                 if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
             }
-            if (alive) store_running<HC, kLinear>(p, run, b, mi * 256 + row_in_tile, ni * BN + half * HC);
+            if (alive) {
+                if constexpr (kLinear)
+                    finish_running<HC>(p, run, reinterpret_cast<float*>(bar_gen + 256 + uint32_t(warp - 2) * kStagedBlock),
+                                       mi * 256 + int(rank) * 128 + quad * 32, lane, ni * BN + half * HC);
+                else
+                    store_running<HC>(p, run, b, mi * 256 + row_in_tile, ni * BN + half * HC);
+            }
         }
     } else {
         // ------------------------------------------------------------------ epilogue (both CTAs)
@@ -1249,10 +1303,10 @@ umma_gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
             // a 16-bit C with nothing fused takes the lean epilogue (NTB200_GENERAL_EPILOGUE=1 sets p.lean_ok to 0)
             const bool plain = p.tma_store && p.lean_ok && !p.bias && !p.accumulate && !p.has_mask && !p.has_relu_out &&
                                p.n_peers == 0 && p.out_kind != kOutI8;
-            if constexpr (kLinear) {
+            if constexpr (kLinear && !kSplit) {
                 constexpr int kCols = BN * 4 / kEpi;       // kEpi / 4 warps per lane quadrant share the tile's columns
                 const int part = (warp - 2) >> 2;
-                if constexpr (!kSplit) {
+                {
                     if (p.tma_store) {
                         residual_pending = false;   // waited for inside
                         if (!epilogue_linear_tma<kCols, kKind == MmaKind::i8>(
@@ -1265,9 +1319,11 @@ umma_gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
                         }
                     }
                 }
-                if (kSplit || !p.tma_store)
-                epilogue_linear<kCols, kKind == MmaKind::i8>(p, tmem_base + (uint32_t(quad * 32) << 16) + uint32_t(acc * BN + part * kCols),
-                                                             mi * 256 + row_in_tile, ni * BN + part * kCols);
+                if (!p.tma_store)
+                    (void)epilogue_linear<kCols, kKind == MmaKind::i8, 32>(
+                        p, tmem_base + (uint32_t(quad * 32) << 16) + uint32_t(acc * BN + part * kCols),
+                        reinterpret_cast<float*>(smem_gen + kStages * kPairStageBytes + uint32_t(warp - 2) * 8192u),
+                        mi * 256 + int(rank) * 128 + quad * 32, lane, ni * BN + part * kCols, [] { return true; });
             } else if constexpr (!kSplit && kEpi == 16) {
                 const int quarter = (warp - 2) >> 2;   // four warps per lane quadrant, 64 columns (one 128-byte sub-tile) each
                 if (plain)
@@ -2148,20 +2204,23 @@ int launch_instance(const Maps& m, const UmmaParams& p_in, int grid, int a_rows_
     p.s_a_bytes = uint32_t(a_rows_staged) * 128u;
     p.s_stage_bytes = copies * (p.s_a_bytes + T::kBBytes);
     p.s_stage_tx = p.s_stage_bytes;
-    p.s_stages = int(std::min<uint32_t>(uint32_t(T::kMaxStages), (T::kRingBudget - T::kABytes) / p.s_stage_bytes));
-    const uint32_t smem = uint32_t(p.s_stages) * p.s_stage_bytes + T::kABytes + T::kBarrierBytes + 1024;
+    constexpr uint32_t kStaged = kLinear ? 8u * kStagedBlock : 0u;   // a staged block for each epilogue warp
+    constexpr uint32_t kRing = T::kRingBudget;
+    static_assert(kRing + T::kBarrierBytes + 1024 + kStaged <= 232448u, "shared memory of one SM");
+    p.s_stages = int(std::min<uint32_t>(uint32_t(T::kMaxStages), (kRing - T::kABytes) / p.s_stage_bytes));
+    const uint32_t smem = uint32_t(p.s_stages) * p.s_stage_bytes + T::kABytes + T::kBarrierBytes + 1024 + kStaged;
     // the attribute is per device and per instantiation: the largest size this instantiation can ask for, set once
     static std::atomic<bool> attr_set[64];
     int dev_i = 0;
     (void)cudaGetDevice(&dev_i);
     if (dev_i < 0 || dev_i >= 64) dev_i = 0;
     if (!attr_set[dev_i].load(std::memory_order_acquire)) {
-        const uint32_t max_smem = T::kRingBudget + T::kBarrierBytes + 1024;
+        const uint32_t max_smem = kRing + T::kBarrierBytes + 1024 + kStaged;
         cudaError_t e = cudaFuncSetAttribute(umma_gemm_kernel<kKind, BN, kSplit, kLinear>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(max_smem));
         if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(umma_gemm_kernel)");
         attr_set[dev_i].store(true, std::memory_order_release);
     }
-    umma_gemm_kernel<kKind, BN, kSplit, kLinear><<<grid, kSplit ? kThreadsSplit : kThreads, smem, stream>>>(m.a.map, m.b.map, m.a_lo.map, m.b_lo.map, p);
+    umma_gemm_kernel<kKind, BN, kSplit, kLinear><<<grid, kSplit || kLinear ? kThreadsSplit : kThreads, smem, stream>>>(m.a.map, m.b.map, m.a_lo.map, m.b_lo.map, p);
     count_launch();
     NTB200_CUDA(cudaGetLastError());
     return NTB200_OK;
@@ -2227,7 +2286,8 @@ int launch_pair_instance(const Maps& m, const UmmaParams& p, cudaStream_t stream
             if (warps == 8) return launch_pair_instance<kKind, kSplit, 8>(m, p, stream);
         }
     }
-    constexpr uint32_t smem = PairTile<kSplit>::kSmemBytes;
+    constexpr uint32_t smem = PairTile<kSplit>::kSmemBytes + (kLinear && kSplit ? 8u * kStagedBlock : 0u);
+    static_assert(smem <= 232448u, "shared memory of one SM");
     cudaError_t e = cudaFuncSetAttribute(umma_gemm_pair_kernel<kKind, kSplit, kEpi, kLinear>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
     if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(umma_gemm_pair_kernel)");
     static int cached[64] = {0};  // per instantiation, per device
@@ -2402,8 +2462,9 @@ int launch_planned(const GemmArgs& g, const Planned& pl, const Side& a, const Si
     p.tiles_m = use_pair ? int((g.m + 255) / 256) : int(tiles_m);
     p.tiles_n = int((g.n + bn - 1) / bn);
     p.k_blocks = int((g.k + block_k - 1) / block_k);
-    // Float32 split: hand over a partial sum every `g_split_chunk_blocks` K blocks (32 k each)
-    p.chunk_blocks = pl.split ? g_split_chunk_blocks : p.k_blocks;
+    // Float32 split: hand over a partial sum every `g_split_chunk_blocks` K blocks (32 k each); every second one for
+    // ntb200_linear_act, whose relative error at K = 1024 falls from 1.4e-6 to that of an fp32 product
+    p.chunk_blocks = pl.split ? (g.linear ? 2 : g_split_chunk_blocks) : p.k_blocks;
     p.group_m = 8;
     p.total_tiles = int(int64_t(p.tiles_m) * p.tiles_n * g.batch);
     p.block_k = block_k;

@@ -51,10 +51,11 @@ __global__ void pad_rows_kernel(const U* __restrict__ src, long long rs, long lo
 
 // gz = gy act'(pre), and the column sums of gz of one slab of rows per blockIdx.y (partial: [slabs, n]).  32 x 8 threads,
 // each on V columns of every eighth row of the slab; the sums use gz before it is rounded.
-template <class T, int V>
-__global__ void __launch_bounds__(256) act_backward_kernel(const T* __restrict__ gy, long long gy_rs, const T* __restrict__ pre, long long pre_rs,
+// kAct is the activation, decided once per launch: a switch per value costs as much as the slope.
+template <class T, int V, int kAct>
+__global__ void __launch_bounds__(256, 4) act_backward_kernel(const T* __restrict__ gy, long long gy_rs, const T* __restrict__ pre, long long pre_rs,
                                                            T* __restrict__ gz, long long gz_rs, float* __restrict__ partial, long long m,
-                                                           int n, int act, long long slab_rows) {
+                                                           int n, long long slab_rows) {
     __shared__ float red[8][32 * V + 1];
     const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
     const int col = (blockIdx.x * 32 + x) * V;
@@ -63,18 +64,19 @@ __global__ void __launch_bounds__(256) act_backward_kernel(const T* __restrict__
 #pragma unroll
     for (int i = 0; i < V; ++i) sum[i] = 0.f;
     if (col < n) {
-#pragma unroll 2
+#pragma unroll 4
         for (long long r = r0 + y; r < r1; r += 8) {
             const Pack<T, V> g = *reinterpret_cast<const Pack<T, V>*>(gy + r * gy_rs + col);
             Pack<T, V> o;
-            if (pre) {
+            if constexpr (kAct != NTB200_ACT_NONE) {
                 const Pack<T, V> z = *reinterpret_cast<const Pack<T, V>*>(pre + r * pre_rs + col);
+                float v[V];
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    const float v = g.up(i) * act_slope<sizeof(T) == 2>(act, z.up(i));
-                    sum[i] += v;
-                    o.set(i, v);
+                    v[i] = g.up(i) * act_slope<sizeof(T) == 2>(kAct, z.up(i));
+                    sum[i] += v[i];
                 }
+                o.put(v);
             } else {
 #pragma unroll
                 for (int i = 0; i < V; ++i) sum[i] += g.up(i);
@@ -112,10 +114,10 @@ __global__ void __launch_bounds__(256) join_slabs_kernel(const float* __restrict
     }
 }
 
-// Slabs of rows of the bias gradient's partial sums: enough blocks for the GPU, at least 64 rows each.
+// Slabs of rows of the bias gradient's partial sums: four blocks per SM, all resident at once, of at least 64 rows each.
 long long act_slabs(int64_t m, int64_t n, int vec) {
     const int64_t col_blocks = (n + 32 * vec - 1) / (32 * vec);
-    int64_t slabs = std::max<int64_t>(1, std::min<int64_t>((m + 63) / 64, (148 * 8 + col_blocks - 1) / col_blocks));
+    int64_t slabs = std::max<int64_t>(1, std::min<int64_t>((m + 63) / 64, 148 * 4 / std::min<int64_t>(col_blocks, 148 * 4)));
     return std::min<int64_t>(slabs, 65535);
 }
 
@@ -174,11 +176,20 @@ size_t product_bytes(const GemmArgs& g) {
 }
 int plain_product(int dtype, Operand a, Operand b, void* c, int64_t c_rs, cudaStream_t stream) {
     if (a.mn == 0 || b.mn == 0) return NTB200_OK;
-    if (dtype != NTB200_F32 && a.k > 0) {
+    if (dtype != NTB200_F32) {
         if (int rc = pad_operand(a, 2, stream)) return rc;
         if (int rc = pad_operand(b, 2, stream)) return rc;
     }
-    return route_gemm(gemm_of(dtype, a, b, c, c_rs), NTB200_ROUTE_AUTO, stream);
+    GemmArgs g = gemm_of(dtype, a, b, c, c_rs);
+    // Rows that TMA cannot store would leave a plain GEMM element by element, thread by thread: ntb200_linear_act's
+    // epilogue moves them by rows.  Large Float32 products take its finer partial sums.
+    LinearParams l{};
+    l.y = c; l.y_rs = c_rs; l.act = NTB200_ACT_NONE; l.out_dtype = dtype;
+    if (dtype == NTB200_F32 ? !small_f32(g) : c_rs % 8 != 0 || !on16(c)) {
+        g.linear = &l;
+        return launch_umma_gemm(g, stream);
+    }
+    return route_gemm(g, NTB200_ROUTE_AUTO, stream);
 }
 
 int check_linear(const ntb200_linear_desc* d) {
@@ -254,10 +265,22 @@ int launch_gz(const ntb200_linear_backward_desc& d, const GzPlan& p, void* gz, f
     const T* pre = d.activation != NTB200_ACT_NONE ? static_cast<const T*>(d.pre) : nullptr;
     const int v = p.vec ? kVec : 1;
     const dim3 grid(unsigned((d.n + 32 * v - 1) / (32 * v)), unsigned(slabs));
-    if (p.vec)
-        act_backward_kernel<T, kVec><<<grid, 256, 0, stream>>>(gy, d.grad_out_row_stride, pre, d.pre_row_stride, static_cast<T*>(gz), p.ld, partial, d.m, int(d.n), d.activation, per);
-    else
-        act_backward_kernel<T, 1><<<grid, 256, 0, stream>>>(gy, d.grad_out_row_stride, pre, d.pre_row_stride, static_cast<T*>(gz), p.ld, partial, d.m, int(d.n), d.activation, per);
+#define NTB200_GZ(VV, AA) \
+    act_backward_kernel<T, VV, AA><<<grid, 256, 0, stream>>>(gy, d.grad_out_row_stride, pre, d.pre_row_stride, static_cast<T*>(gz), p.ld, partial, d.m, int(d.n), per)
+#define NTB200_GZ_ACT(AA)              \
+    case AA:                           \
+        if (p.vec) NTB200_GZ(kVec, AA); \
+        else NTB200_GZ(1, AA);         \
+        break
+    switch (d.activation) {
+        NTB200_GZ_ACT(NTB200_ACT_NONE);
+        NTB200_GZ_ACT(NTB200_ACT_RELU);
+        NTB200_GZ_ACT(NTB200_ACT_GELU);
+        NTB200_GZ_ACT(NTB200_ACT_GELU_TANH);
+        NTB200_GZ_ACT(NTB200_ACT_SILU);
+    }
+#undef NTB200_GZ_ACT
+#undef NTB200_GZ
     count_launch();
     NTB200_CUDA(cudaGetLastError());
     if (partial) {

@@ -5,6 +5,7 @@
 #include <cuda_fp16.h>
 
 #include "internal.h"
+#include "row_ops.cuh"
 
 namespace ntb200 {
 
@@ -12,7 +13,7 @@ namespace ntb200 {
 // a hundredth of half a Float16 step); Float32 results use the full-precision functions.
 template <bool kFast>
 __device__ __forceinline__ float sigmoid_times(float z, float u) {   // z / (1 + e^-u)
-    if constexpr (kFast) return __fdividef(z, 1.f + __expf(-u));
+    if constexpr (kFast) return z * rcp_hw(1.f + exp2_hw(-1.4426950408889634f * u));
     return z / (1.f + expf(-u));
 }
 
@@ -22,8 +23,9 @@ constexpr float kGeluCubic = 0.044715f;
 // Phi(z) = erfc(-z / sqrt 2) / 2 for results of 16 bits, e = e^(-z^2 / 2).  Phi(-a) = e t P(t) with t = 1 / (1 + 0.36 a): P is
 // a degree-6 fit of erfcx(a / sqrt 2) / (2 t), relative error below 1.1e-6 over 0 <= a <= 14 (least squares reweighted
 // towards the minimax, evaluated in fp32), so the tail keeps its relative precision.  15 instructions; erfcf takes 40.
+__device__ __forceinline__ float gauss_fast(float z) { return exp2_hw(-0.72134752044448170f * z * z); }   // e^(-z^2 / 2)
 __device__ __forceinline__ float phi_fast(float z, float e) {
-    const float t = __fdividef(1.f, 1.f + 0.36f * fabsf(z));
+    const float t = rcp_hw(1.f + 0.36f * fabsf(z));
     const float q = e * t * (0.14371304f + t * (0.14177254f + t * (0.13971882f + t * (0.026550606f + t * (0.1809521f + t * (-0.17976327f + t * 0.047055867f))))));
     return z < 0.f ? q : 1.f - q;
 }
@@ -44,7 +46,7 @@ __device__ __forceinline__ float act_value(int act, float z) {
     if constexpr (!kFast) return act_value_full(act, z);
     switch (act) {
         case NTB200_ACT_RELU: return z < 0.f ? 0.f : z;
-        case NTB200_ACT_GELU: return z * phi_fast(z, __expf(-0.5f * z * z));
+        case NTB200_ACT_GELU: return z * phi_fast(z, gauss_fast(z));
         case NTB200_ACT_GELU_TANH: return sigmoid_times<true>(z, kGeluScale * (z + kGeluCubic * z * z * z));
         case NTB200_ACT_SILU: return sigmoid_times<true>(z, z);
         default: return z;
@@ -56,9 +58,11 @@ __device__ __forceinline__ float act_slope(int act, float z) {
     switch (act) {
         case NTB200_ACT_RELU: return z < 0.f ? 0.f : 1.f;
         case NTB200_ACT_GELU: {
-            const float e = kFast ? __expf(-0.5f * z * z) : expf(-0.5f * z * z);
-            if constexpr (kFast) return phi_fast(z, e) + z * e * 0.39894228040143268f;
-            return 0.5f * erfcf(z * -0.70710678118654752f) + z * e * 0.39894228040143268f;
+            if constexpr (kFast) {
+                const float e = gauss_fast(z);
+                return fmaf(z * 0.39894228040143268f, e, phi_fast(z, e));
+            }
+            return 0.5f * erfcf(z * -0.70710678118654752f) + z * expf(-0.5f * z * z) * 0.39894228040143268f;
         }
         case NTB200_ACT_GELU_TANH: {
             if (fabsf(z) > 20.f) return z > 0.f ? 1.f : 0.f;   // the tails, before z^3 can overflow
@@ -139,19 +143,6 @@ __device__ __forceinline__ void lin_add32(const void* p, long long i, int dtype,
         }
     }
 }
-__device__ __forceinline__ void lin_store32(void* p, long long i, int dtype, const float (&v)[32]) {
-    if (dtype == NTB200_F32) {
-        float4* d = reinterpret_cast<float4*>(static_cast<float*>(p) + i);
-#pragma unroll
-        for (int q = 0; q < 8; ++q) d[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-        return;
-    }
-    uint4* d = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i);
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-        d[q] = make_uint4(lin_pack2(v[8 * q], v[8 * q + 1], dtype), lin_pack2(v[8 * q + 2], v[8 * q + 3], dtype),
-                          lin_pack2(v[8 * q + 4], v[8 * q + 5], dtype), lin_pack2(v[8 * q + 6], v[8 * q + 7], dtype));
-}
 
 // Scales and bias of 32 consecutive products of one row; wide: every column is there and the vectors start on 16 bytes.
 __device__ __forceinline__ void linear_scale_bias32(const LinearParams& l, int n, int col0, float rs, bool wide, float (&f)[32]) {
@@ -214,30 +205,75 @@ __device__ __forceinline__ void linear_finish4(const LinearParams& l, int n, int
         }
 }
 
-// 32 consecutive products of one row, columns col0 ..: everything after the product, stored.
-__device__ __forceinline__ void linear_finish32(const LinearParams& l, int n, int row, int col0, float (&f)[32]) {
-    const int dt = l.out_dtype;
-    const bool full = col0 + 32 <= n && l.vec_ok;
-    linear_scale_bias32(l, n, col0, l.row_scale ? l.row_scale[row] : 1.f, full, f);
-    const long long y0 = (long long)row * l.y_rs + col0, r0 = (long long)row * l.residual_rs + col0, p0 = (long long)row * l.pre_rs + col0;
-    if (full) {
-        if (l.pre) lin_store32(l.pre, p0, dt, f);
-        if (dt == NTB200_F32) act_values<false>(l.act, f);
-        else act_values<true>(l.act, f);
-        if (l.residual) lin_add32(l.residual, r0, dt, f);
-        lin_store32(l.y, y0, dt, f);
-        return;
-    }
-    if (l.pre) {
+// One element of y's type.
+template <int kDt>
+__device__ __forceinline__ float lin_get(const char* p) {
+    if constexpr (kDt == NTB200_F32) return *reinterpret_cast<const float*>(p);
+    else return lin_up16(*reinterpret_cast<const uint16_t*>(p), kDt);
+}
+template <int kDt>
+__device__ __forceinline__ void lin_set(char* p, float v) {
+    if constexpr (kDt == NTB200_F32) *reinterpret_cast<float*>(p) = v;
+    else *reinterpret_cast<uint16_t*>(p) = uint16_t(lin_pack2(v, 0.f, kDt));
+}
+
+// What a warp needs besides the products of 32 rows x 32 columns, lane = column: the column's scale and bias and the
+// residuals of its 32 rows.  Loaded before the products are there, all loads on their way together.
+struct LinearAhead {
+    float cs, bias, res[32];
+};
+template <int kDt>
+__device__ __forceinline__ void linear_load_ahead(const LinearParams& l, int m, int n, int row0, int col0, int lane, LinearAhead& a) {
+    constexpr int es = kDt == NTB200_F32 ? 4 : 2;
+    const int col = col0 + lane;
+    const bool in = col < n;
+    a.cs = l.col_scale && in ? l.col_scale[col] : 1.f;
+    a.bias = l.bias && in ? lin_get<kDt>(static_cast<const char*>(l.bias) + (long long)col * es) : 0.f;
+    if (l.residual && in) {
+        const char* p = static_cast<const char*>(l.residual) + ((long long)row0 * l.residual_rs + col) * es;
+        const long long step = l.residual_rs * es;
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
-            if (col0 + j < n) lin_store(l.pre, p0 + j, f[j], dt);
-    }
-    if (dt == NTB200_F32) act_values<false>(l.act, f);
-    else act_values<true>(l.act, f);
+        for (int r = 0; r < 32; ++r) {
+            a.res[r] = row0 + r < m ? lin_get<kDt>(p) : 0.f;
+            p += step;
+        }
+    } else {
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
-        if (col0 + j < n) lin_store(l.y, y0 + j, f[j] + (l.residual ? lin_load(l.residual, r0 + j, dt) : 0.f), dt);
+        for (int r = 0; r < 32; ++r) a.res[r] = 0.f;
+    }
+}
+
+// kRows x 32 products staged in shared memory (row pitch 33 floats; rows first .. first + kRows of the warp's 32), finished
+// by a warp with lane = column: pre and y leave in runs of 32 elements of a row, whatever their alignment.
+template <int kDt, int kRows>
+__device__ __forceinline__ void linear_finish_block(const LinearParams& l, int m, int n, const float* staged, int row0, int first, int col0, int lane,
+                                                    const LinearAhead& a) {
+    constexpr int es = kDt == NTB200_F32 ? 4 : 2;
+    const int col = col0 + lane;
+    const bool in = col < n;
+    char* y = static_cast<char*>(l.y) + ((long long)(row0 + first) * l.y_rs + col) * es;
+    char* pre = static_cast<char*>(l.pre) + ((long long)(row0 + first) * l.pre_rs + col) * es;
+    const long long y_step = l.y_rs * es, pre_step = l.pre_rs * es;
+#pragma unroll
+    for (int r0 = 0; r0 < kRows; r0 += 8) {
+        if (row0 + first + r0 >= m) break;   // uniform across the warp
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int r = first + r0 + i;
+            f[i] = staged[(r0 + i) * 33 + lane];
+            if (l.row_scale) f[i] *= (row0 + r < m ? l.row_scale[row0 + r] : 0.f) * a.cs;
+            f[i] += a.bias;
+            if (l.pre && in && row0 + r < m) lin_set<kDt>(pre, f[i]);
+            pre += pre_step;
+        }
+        act_values<kDt != NTB200_F32>(l.act, f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (in && row0 + first + r0 + i < m) lin_set<kDt>(y, f[i] + a.res[first + r0 + i]);
+            y += y_step;
+        }
+    }
 }
 
 }  // namespace ntb200

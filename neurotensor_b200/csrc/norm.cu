@@ -28,17 +28,29 @@ struct RowArgs {
     float eps;
 };
 
-// q = rint(u * 127 / A), clamped; a row of zeros gives zeros, a NaN gives 0 (its row's scale is NaN, so the product
-// that reads it still is).  A below 2^-100 is scaled up first: 127 / A would overflow.
+// q = rint(u * 127 / A), which lies within +-127 but for roundings; a row of zeros gives zeros, a NaN gives 0 (its row's
+// scale is NaN, so the product that reads it still is).  A below 2^-100 is scaled up first: 127 / A would overflow.
 struct Quant {
     float up, inv;
     __device__ __forceinline__ explicit Quant(float top) {
         up = top < 0x1p-100f ? 0x1p100f : 1.f;
         inv = top > 0.f ? __fdiv_rn(127.f, __fmul_rn(top, up)) : (top == 0.f ? 0.f : top);
     }
-    __device__ __forceinline__ int operator()(float u) const {
-        const int q = __float2int_rn(__fmul_rn(__fmul_rn(u, up), inv));
-        return max(-127, min(127, q));
+    // V values, packed.  127 (1 + 2^-22) at most reaches the conversion, so it needs no clamp; x * 1 is exact.
+    template <int V>
+    __device__ __forceinline__ void put(Pack<int8_t, V>& o, const float* u) const {
+        int q[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) q[i] = __float2int_rn(__fmul_rn(up == 1.f ? u[i] : __fmul_rn(u[i], up), inv));
+        if constexpr (V % 4 == 0) {
+            uint32_t* w = reinterpret_cast<uint32_t*>(o.e);
+#pragma unroll
+            for (int i = 0; i < V; i += 4)
+                w[i / 4] = __byte_perm(__byte_perm(uint32_t(q[i]), uint32_t(q[i + 1]), 0x0040), __byte_perm(uint32_t(q[i + 2]), uint32_t(q[i + 3]), 0x0040), 0x5410);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) o.e[i] = int8_t(q[i]);
+        }
     }
 };
 
@@ -81,8 +93,7 @@ __global__ void __launch_bounds__(1024) norm_rows_kernel(const RowArgs a, int G)
             }
             if (a.h && in) {
                 Pack<T, V> o;
-#pragma unroll
-                for (int i = 0; i < V; ++i) o.set(i, f[p * V + i]);
+                o.put(f + p * V);
                 reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.h) + row * a.cols)[c] = o;
             }
             if (kOut == kInt8 && in) {
@@ -119,8 +130,7 @@ __global__ void __launch_bounds__(1024) norm_rows_kernel(const RowArgs a, int G)
                 const int c = t + p * G;
                 if (c >= nv) continue;
                 Pack<int8_t, V> o;
-#pragma unroll
-                for (int i = 0; i < V; ++i) o.e[i] = int8_t(quant(f[p * V + i]));
+                quant.put(o, f + p * V);
                 reinterpret_cast<Pack<int8_t, V>*>(static_cast<int8_t*>(a.y) + row * a.cols)[c] = o;
             }
             if (t == 0) a.stat[row] = __fdiv_rn(__fmul_rn(top, rstd), 127.f);
@@ -131,8 +141,10 @@ __global__ void __launch_bounds__(1024) norm_rows_kernel(const RowArgs a, int G)
                 if (c >= nv) continue;
                 const Pack<T, V> pw = w[c];
                 Pack<T, V> o;
+                float v[V];
 #pragma unroll
-                for (int i = 0; i < V; ++i) o.set(i, f[p * V + i] * rstd * pw.up(i));
+                for (int i = 0; i < V; ++i) v[i] = f[p * V + i] * rstd * pw.up(i);
+                o.put(v);
                 reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.y) + row * a.cols)[c] = o;
             }
             if (a.stat && t == 0) a.stat[row] = rstd;
@@ -176,7 +188,12 @@ __global__ void __launch_bounds__(1024) norm_long_rows_kernel(const RowArgs a) {
             if (r) v = __fadd_rn(v, RowType<T>::up(r[c]));
             if (a.h) static_cast<T*>(a.h)[row * a.cols + c] = RowType<T>::down(v);
             if (kOut == kInt8)
-                static_cast<int8_t*>(a.y)[row * a.cols + c] = int8_t(quant(w ? __fmul_rn(v, RowType<T>::up(w[c])) : v));
+            {
+                const float u = w ? __fmul_rn(v, RowType<T>::up(w[c])) : v;
+                Pack<int8_t, 1> o;
+                quant.put(o, &u);
+                static_cast<int8_t*>(a.y)[row * a.cols + c] = o.e[0];
+            }
             else
                 static_cast<T*>(a.y)[row * a.cols + c] = RowType<T>::down(v * rstd * RowType<T>::up(w[c]));
         }
@@ -281,10 +298,8 @@ __global__ void __launch_bounds__(512) norm_ring_kernel(const RowArgs a, const R
                     const Pack<T, V> r = ld_shared_pack<T, V>(ring.at(stage, 1) + uint32_t(c) * 16u);
                     Pack<T, V> o;
 #pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        f[p * V + i] = __fadd_rn(x.up(i), r.up(i));
-                        o.set(i, f[p * V + i]);
-                    }
+                    for (int i = 0; i < V; ++i) f[p * V + i] = __fadd_rn(x.up(i), r.up(i));
+                    o.put(f + p * V);
                     reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.h) + row * a.cols)[c] = o;
                 } else {
 #pragma unroll
@@ -327,14 +342,15 @@ __global__ void __launch_bounds__(512) norm_ring_kernel(const RowArgs a, const R
             if (c >= nv) continue;
             if (kOut == kInt8) {
                 Pack<int8_t, V> o;
-#pragma unroll
-                for (int i = 0; i < V; ++i) o.e[i] = int8_t(quant(f[p * V + i]));
+                quant.put(o, f + p * V);
                 reinterpret_cast<Pack<int8_t, V>*>(static_cast<int8_t*>(a.y) + row * a.cols)[c] = o;
             } else {
                 const Pack<T, V> pw = w[c];
                 Pack<T, V> o;
+                float v[V];
 #pragma unroll
-                for (int i = 0; i < V; ++i) o.set(i, f[p * V + i] * rstd * pw.up(i));
+                for (int i = 0; i < V; ++i) v[i] = f[p * V + i] * rstd * pw.up(i);
+                o.put(v);
                 reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.y) + row * a.cols)[c] = o;
             }
         }
@@ -513,12 +529,13 @@ __global__ void __launch_bounds__(512) norm_backward_ring_kernel(const BackArgs 
             const int c = t + p * G;
             if (c >= nv) continue;
             Pack<T, V> o;
+            float v[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                float v = rstd * (gy[p].up(i) * w[p].up(i) - h[p].up(i) * c0);
-                if (kStream) v += gh[p].up(i);
-                o.set(i, v);
+                v[i] = rstd * (gy[p].up(i) * w[p].up(i) - h[p].up(i) * c0);
+                if (kStream) v[i] += gh[p].up(i);
             }
+            o.put(v);
             reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.gx) + row * a.cols)[c] = o;
         }
     }

@@ -5,6 +5,7 @@
 #include <cuda_fp16.h>
 
 #include <cstdint>
+#include <type_traits>
 
 namespace ntb200 {
 
@@ -28,7 +29,38 @@ struct __align__(sizeof(T) * V) Pack {
     T e[V];
     __device__ __forceinline__ float up(int i) const { return RowType<T>::up(e[i]); }
     __device__ __forceinline__ void set(int i, float v) { e[i] = RowType<T>::down(v); }
+    // all of them, rounded; 16-bit values two at a time (one conversion instruction a pair)
+    __device__ __forceinline__ void put(const float* v) {
+        if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+            uint32_t* w = reinterpret_cast<uint32_t*>(e);
+#pragma unroll
+            for (int i = 0; i < V; i += 2) {
+                if constexpr (std::is_same<T, __half>::value) {
+                    const __half2 h = __floats2half2_rn(v[i], v[i + 1]);
+                    w[i / 2] = *reinterpret_cast<const uint32_t*>(&h);
+                } else {
+                    const __nv_bfloat162 h = __floats2bfloat162_rn(v[i], v[i + 1]);
+                    w[i / 2] = *reinterpret_cast<const uint32_t*>(&h);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) e[i] = RowType<T>::down(v[i]);
+        }
+    }
 };
+
+// The hardware's exponential and reciprocal alone (relative error about 2^-22): results below 2^-126 are zero.
+__device__ __forceinline__ float exp2_hw(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float rcp_hw(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
 
 __device__ __forceinline__ float max_nan(float a, float b) {   // NaN if either is NaN
     float r;
