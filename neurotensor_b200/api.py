@@ -981,6 +981,7 @@ def matmult_host(a, b, c, transpose_a=False, transpose_b=False, accumulate=True)
 # ---- the residual feed-forward block: norm, linear with activation and residual, distillation loss -------------------
 
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+_FLOAT_CODES = {t: _TORCH_TO_CODE[t] for t in _FLOATS}
 _ACTIVATIONS = {"none": _lib.ACT_NONE, None: _lib.ACT_NONE, "relu": _lib.ACT_RELU, "gelu": _lib.ACT_GELU,
                 "gelu_tanh": _lib.ACT_GELU_TANH, "silu": _lib.ACT_SILU}
 
@@ -1029,53 +1030,64 @@ def _activation(name):
 
 
 def _norm_operands(what, x, weight, residual):
-    if x.dtype not in _FLOATS:
-        raise ValueError("%s: expected Float32, Float16 or BFloat16 but got %s" % (what, x.dtype))
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError("%s: expected rows of at least one element but got shape %s" % (what, tuple(x.shape)))
-    if weight is not None and (weight.dim() != 1 or weight.shape[0] != x.shape[-1] or weight.dtype != x.dtype):
-        raise ValueError("%s: expected a weight of %d values of %s but got %s of %s"
-                         % (what, x.shape[-1], x.dtype, tuple(weight.shape), weight.dtype))
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+    """(dtype code, raw stream) of checked operands."""
+    dtype, shape = x.dtype, x.shape
+    code = _FLOAT_CODES.get(dtype)
+    if code is None:
+        raise ValueError("%s: expected Float32, Float16 or BFloat16 but got %s" % (what, dtype))
+    if not shape or shape[-1] < 1:
+        raise ValueError("%s: expected rows of at least one element but got shape %s" % (what, tuple(shape)))
+    if weight is not None and (weight.shape != shape[-1:] or weight.dtype is not dtype):
+        raise ValueError("%s: expected a weight of %d values of %s but got %s of %s" % (what, shape[-1], dtype, tuple(weight.shape), weight.dtype))
+    if residual is not None and (residual.shape != shape or residual.dtype is not dtype):
         raise ValueError("%s: expected a residual of shape %s and %s but got %s and %s"
-                         % (what, tuple(x.shape), x.dtype, tuple(residual.shape), residual.dtype))
+                         % (what, tuple(shape), dtype, tuple(residual.shape), residual.dtype))
+    return code, _on_device(what, x, weight, residual)
+
+
+def _like(t):
+    """A contiguous tensor of t's shape and dtype."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
+def _row_values(t, rows):
+    """One Float32 for each row of t."""
+    return t.new_empty(rows if t.dim() == 2 else t.shape[:-1], dtype=torch.float32)
 
 
 def rms_norm(x, weight, eps=1e-6, residual=None):
     """h = x + residual, y = h * rstd * weight over the last dim, rstd = (mean(h^2) + eps)^-1/2.
     Returns (y, h, rstd): h is x itself without a residual, rstd (fp32, one per row) is what rms_norm_backward takes.
     The norm uses the unrounded sum h."""
-    _norm_operands("rms_norm", x, weight, residual)
-    stream = _on_device("rms_norm", x, weight, residual)
-    shape = x.shape
+    code, stream = _norm_operands("rms_norm", x, weight, residual)
     xr, rows, x_rs = _rows_of(x)
-    y = x.new_empty(shape)
-    rstd = x.new_empty(shape[:-1], dtype=torch.float32)
-    h, rr, r_rs = x, None, 0
-    if residual is not None:
-        h = x.new_empty(shape)
-        rr, _, r_rs = _rows_of(residual)
     w = weight if weight.is_contiguous() else weight.contiguous()
-    check(lib().ntb200_rms_norm(_TORCH_TO_CODE[x.dtype], xr.data_ptr(), x_rs, None if rr is None else rr.data_ptr(), r_rs, w.data_ptr(),
-                                y.data_ptr(), None if rr is None else h.data_ptr(), rstd.data_ptr(), rows, shape[-1], eps, stream))
+    y, rstd = _like(x), _row_values(x, rows)
+    if residual is None:
+        h, hp, rr, rp, r_rs = x, None, None, None, 0
+    else:
+        h = _like(x)
+        rr, _, r_rs = _rows_of(residual)
+        hp, rp = h.data_ptr(), rr.data_ptr()
+    check(lib().ntb200_rms_norm(code, xr.data_ptr(), x_rs, rp, r_rs, w.data_ptr(), y.data_ptr(), hp, rstd.data_ptr(), rows, x.shape[-1], eps,
+                                stream))
     return y, h, rstd
 
 
 def rms_norm_int8(x, weight, eps=1e-6, residual=None):
     """rms_norm whose output leaves as Int8 rows with one fp32 scale each (y = q * scale): what linear_int8 reads.
     Returns (q, scale, h)."""
-    _norm_operands("rms_norm_int8", x, weight, residual)
-    stream = _on_device("rms_norm_int8", x, weight, residual)
+    code, stream = _norm_operands("rms_norm_int8", x, weight, residual)
     xr, rows, x_rs = _rows_of(x)
-    q = x.new_empty(x.shape, dtype=torch.int8)
-    scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
-    h, rr, r_rs = x, None, 0
-    if residual is not None:
-        h = x.new_empty(x.shape)
-        rr, _, r_rs = _rows_of(residual)
     w = weight if weight.is_contiguous() else weight.contiguous()
-    check(lib().ntb200_rms_norm_int8(_TORCH_TO_CODE[x.dtype], xr.data_ptr(), x_rs, None if rr is None else rr.data_ptr(), r_rs, w.data_ptr(),
-                                     q.data_ptr(), scale.data_ptr(), None if rr is None else h.data_ptr(), rows, x.shape[-1], eps,
+    q, scale = x.new_empty(x.shape, dtype=torch.int8), _row_values(x, rows)
+    if residual is None:
+        h, hp, rr, rp, r_rs = x, None, None, None, 0
+    else:
+        h = _like(x)
+        rr, _, r_rs = _rows_of(residual)
+        hp, rp = h.data_ptr(), rr.data_ptr()
+    check(lib().ntb200_rms_norm_int8(code, xr.data_ptr(), x_rs, rp, r_rs, w.data_ptr(), q.data_ptr(), scale.data_ptr(), hp, rows, x.shape[-1], eps,
                                      stream))
     return q, scale, h
 
@@ -1083,39 +1095,38 @@ def rms_norm_int8(x, weight, eps=1e-6, residual=None):
 def quantize_rows(x):
     """(q, scale): every row of the last dim as Int8 with one fp32 scale, x ~ q * scale, scale = max |row| / 127.
     For hidden activations, and once for weights kept as [out, in]."""
-    _norm_operands("quantize_rows", x, None, None)
-    stream = _on_device("quantize_rows", x)
+    code, stream = _norm_operands("quantize_rows", x, None, None)
     xr, rows, x_rs = _rows_of(x)
-    q = x.new_empty(x.shape, dtype=torch.int8)
-    scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
-    check(lib().ntb200_quantize_rows(_TORCH_TO_CODE[x.dtype], xr.data_ptr(), x_rs, q.data_ptr(), scale.data_ptr(), rows, x.shape[-1], stream))
+    q, scale = x.new_empty(x.shape, dtype=torch.int8), _row_values(x, rows)
+    check(lib().ntb200_quantize_rows(code, xr.data_ptr(), x_rs, q.data_ptr(), scale.data_ptr(), rows, x.shape[-1], stream))
     return q, scale
 
 
 def rms_norm_backward(h, weight, rstd, grad_y, grad_h=None, want_weight=True):
     """(grad_x, grad_weight) of rms_norm from its h and rstd.  grad_h is the gradient that arrives over the residual
     stream h; grad_x is also the gradient of the residual.  grad_weight is None unless wanted."""
-    _norm_operands("rms_norm_backward", h, weight, None)
+    shape, dtype = h.shape, h.dtype
     for t, name in ((grad_y, "grad_y"), (grad_h, "grad_h")):
-        if t is not None and (t.shape != h.shape or t.dtype != h.dtype):
+        if t is not None and (t.shape != shape or t.dtype is not dtype):
             raise ValueError("rms_norm_backward: expected %s of shape %s and %s but got %s and %s"
-                             % (name, tuple(h.shape), h.dtype, tuple(t.shape), t.dtype))
-    if rstd.shape != h.shape[:-1] or rstd.dtype != torch.float32:
+                             % (name, tuple(shape), dtype, tuple(t.shape), t.dtype))
+    if rstd.shape != shape[:-1] or rstd.dtype is not torch.float32:
         raise ValueError("rms_norm_backward: expected rstd of shape %s in Float32 but got %s in %s"
                          % (tuple(h.shape[:-1]), tuple(rstd.shape), rstd.dtype))
-    stream = _on_device("rms_norm_backward", h, weight, rstd, grad_y, grad_h)
-    cols = h.shape[-1]
+    code, _ = _norm_operands("rms_norm_backward", h, weight, None)
+    stream = _on_device("rms_norm_backward", h, rstd, grad_y, grad_h)
+    cols = shape[-1]
     hr, rows, h_rs = _rows_of(h)
     gr, _, g_rs = _rows_of(grad_y)
     sr, _, s_rs = _rows_of(grad_h) if grad_h is not None else (None, 0, 0)
     w = weight if weight.is_contiguous() else weight.contiguous()
     rs = rstd if rstd.is_contiguous() else rstd.contiguous()
-    gx = h.new_empty(h.shape)
+    gx = _like(h)
     gw = ws = None
     if want_weight:
-        gw = h.new_empty(cols)
+        gw = _like(w)
         ws = h.new_empty(max(1, lib().ntb200_rms_norm_backward_workspace_bytes(rows, cols)), dtype=torch.uint8)
-    check(lib().ntb200_rms_norm_backward(_TORCH_TO_CODE[h.dtype], hr.data_ptr(), h_rs, w.data_ptr(), rs.data_ptr(), gr.data_ptr(), g_rs,
+    check(lib().ntb200_rms_norm_backward(code, hr.data_ptr(), h_rs, w.data_ptr(), rs.data_ptr(), gr.data_ptr(), g_rs,
                                          None if sr is None else sr.data_ptr(), s_rs, gx.data_ptr(),
                                          None if gw is None else gw.data_ptr(), None if ws is None else ws.data_ptr(), rows, cols,
                                          stream))
@@ -1173,9 +1184,9 @@ def linear_act(x, w, bias=None, activation="none", residual=None, transpose_w=Fa
     if x.dtype not in _FLOATS or w.dtype != x.dtype:
         raise ValueError("linear_act: expected both tensors to be Float32, Float16 or BFloat16 alike but got %s and %s" % (x.dtype, w.dtype))
     d, shape, keep, stream = _linear_desc("linear_act", x, w, bias, activation, residual, transpose_w, x.dtype)
-    y = x.new_empty(shape)
+    y = x.new_empty(shape) if residual is None else _like(residual)
     if want_pre:
-        pre = x.new_empty(shape)
+        pre = _like(y)
         d.pre, d.pre_row_stride = pre.data_ptr(), d.n
         _run_linear(d, y, stream)
         return y, pre
@@ -1231,8 +1242,8 @@ def linear_act_backward(x, w, pre, grad_out, activation="none", transpose_w=Fals
     pr, p_rs = None, 0
     if act != _lib.ACT_NONE:
         pr, _, p_rs = _rows_of(pre)
-    gx = x.new_empty(x.shape) if want_x else None
-    gw = x.new_empty(w.shape) if want_w else None
+    gx = _like(x) if want_x else None
+    gw = _like(w) if want_w else None
     gb = x.new_empty(n) if want_bias else None
     w_ks, w_ns = w.stride()
     if transpose_w:
@@ -1278,13 +1289,13 @@ def distill_topk(logits, teacher, index, temperature=1.0, row_weight=None, want_
     grad, g_rs = None, 0
     if want_grad or out_grad is not None:
         if out_grad is None:
-            grad, g_rs = logits.new_empty(logits.shape), logits.shape[-1]
+            grad, g_rs = _like(logits), logits.shape[-1]
         else:
             grad, _, g_rs = _rows_of(out_grad)
             if grad.data_ptr() != out_grad.data_ptr():
                 raise ValueError("%s: out_grad needs rows with a stride" % what)
             grad = out_grad
-    row_loss = logits.new_empty(logits.shape[:-1], dtype=torch.float32)
+    row_loss = _row_values(logits, rows)
     loss = logits.new_empty((), dtype=torch.float32)
     check(lib().ntb200_distill_topk(_TORCH_TO_CODE[logits.dtype], sr.data_ptr(), s_rs, _TORCH_TO_CODE[t.dtype], t.data_ptr(),
                                     _TORCH_TO_CODE[i.dtype], i.data_ptr(), None if rw is None else rw.data_ptr(),

@@ -209,6 +209,8 @@ __global__ void __launch_bounds__(1024) norm_long_rows_kernel(const RowArgs a) {
 // copies (one per tensor and row) while the group reduces and writes the row that has landed.  Loads in flight cost no
 // registers and no barrier, so the memory system always has the next rows to fetch.  A row is read from its stage into
 // registers before the barrier of its reduction; the thread that passes that barrier refills the stage.
+constexpr int kForwardThreads = 512, kForwardBlocks = 2;   // two blocks per SM, 64 registers per thread
+constexpr uint32_t kRingBytes = 200u * 1024u;               // an SM's shared memory for stages
 struct RowRing {
     uint32_t data, bars;             // shared-memory addresses of this group's stages and their barriers
     uint32_t row_bytes;
@@ -262,7 +264,7 @@ __device__ __forceinline__ void ring_drain(const RowRing& ring, int stage, uint3
 }
 
 template <class T, int P, int kOut, bool kResidual>
-__global__ void __launch_bounds__(512) norm_ring_kernel(const RowArgs a, const RingShape rs) {
+__global__ void __launch_bounds__(kForwardThreads, kForwardBlocks) norm_ring_kernel(const RowArgs a, const RingShape rs) {
     constexpr int V = 16 / sizeof(T);
     extern __shared__ __align__(128) uint8_t ring_mem[];
     __shared__ __align__(8) unsigned long long s_bar[128];
@@ -463,8 +465,8 @@ __global__ void __launch_bounds__(1024) norm_backward_kernel(const BackArgs a, i
 }
 
 // The backward pass over the ring: h, gy and gh (kStream) of a row land together.
-template <class T, int P, bool kStream>
-__global__ void __launch_bounds__(512) norm_backward_ring_kernel(const BackArgs a, const RingShape rs) {
+template <class T, int P, bool kStream, int kThreads>
+__global__ void __launch_bounds__(kThreads) norm_backward_ring_kernel(const BackArgs a, const RingShape rs) {
     constexpr int V = 16 / sizeof(T);
     extern __shared__ __align__(128) uint8_t ring_mem[];
     __shared__ __align__(8) unsigned long long s_bar[128];
@@ -603,18 +605,20 @@ __global__ void norm_weight_long_kernel(const BackArgs a, long long slab_rows) {
     a.partial[(long long)blockIdx.y * a.cols + c] = v;
 }
 
-// out[c] = sum over the slabs of partial[s][c], in a fixed order: 8 threads per column take every eighth slab.
+// out[c] = sum over the slabs of partial[s][c], in a fixed order: 16 threads per column take every sixteenth slab.
 template <class T>
-__global__ void __launch_bounds__(256) sum_partials_kernel(const float* __restrict__ partial, T* __restrict__ out, int slabs, int cols) {
-    __shared__ float s[8][33];
+__global__ void __launch_bounds__(512) sum_partials_kernel(const float* __restrict__ partial, T* __restrict__ out, int slabs, int cols) {
+    __shared__ float s[16][33];
     const int x = threadIdx.x & 31, y = threadIdx.x >> 5, c = blockIdx.x * 32 + x;
     float v = 0.f;
-    if (c < cols)
-        for (int i = y; i < slabs; i += 8) v += partial[(long long)i * cols + c];
+    if (c < cols) {
+#pragma unroll 8
+        for (int i = y; i < slabs; i += 16) v += partial[(long long)i * cols + c];
+    }
     s[y][x] = v;
     __syncthreads();
     if (y == 0 && c < cols) {
-        for (int i = 1; i < 8; ++i) v += s[i][x];
+        for (int i = 1; i < 16; ++i) v += s[i][x];
         out[c] = RowType<T>::down(v);
     }
 }
@@ -634,21 +638,30 @@ RowPlan plan_row(int cols, int vec, bool vec_ok) {
     return r;
 }
 
-// The ring's shape for rows of `tensors` x cols elements: blocks of 512 threads (128 registers each), two vectors per
-// thread (one for rows of up to 32 vectors, four where a row needs all 512 threads), as many stages as 200 KB of shared
-// memory hold, up to 8.  stages < 2: no ring, the row is too long.
-constexpr int kRingThreads = 512;
-struct RingPlan { int p, g, stages; uint32_t smem; };
-RingPlan plan_ring(int cols, int vec, int es, int tensors) {
+// The ring's shape for rows of `tensors` x cols elements: p vectors per thread, the smallest power of two of threads per
+// row (32 or more) that covers the row, as many stages as `bytes` of shared memory hold, up to 8.  stages < 2: no ring,
+// the row is too long.
+struct RingPlan { int p, g, threads, stages; uint32_t smem; };
+RingPlan plan_ring(int cols, int vec, int es, int tensors, int p, int threads, uint32_t bytes) {
     const int nv = cols / vec;
-    RingPlan r{nv <= 32 ? 1 : 2, 32, 0, 0};
-    while (r.g < kRingThreads && r.p * r.g < nv) r.g *= 2;
-    if (r.p * r.g < nv) r.p = 4;
+    RingPlan r{p, 32, threads, 0, 0};
+    while (r.g < threads && r.p * r.g < nv) r.g *= 2;
     if (r.p * r.g < nv) return r;
-    const uint32_t stage = uint32_t(tensors) * uint32_t(cols) * uint32_t(es), groups = uint32_t(kRingThreads / r.g);
-    r.stages = int(std::min<uint32_t>(8, 200u * 1024u / (stage * groups)));
+    const uint32_t stage = uint32_t(tensors) * uint32_t(cols) * uint32_t(es), groups = uint32_t(threads / r.g);
+    r.stages = int(std::min<uint32_t>(8, bytes / (stage * groups)));
     r.smem = stage * groups * uint32_t(std::max(r.stages, 1));
     return r;
+}
+RingPlan plan_forward(int cols, int vec, int es, int tensors) {
+    const int nv = cols / vec;
+    return plan_ring(cols, vec, es, tensors, nv <= 32 ? 1 : (nv <= 2 * kForwardThreads ? 2 : 4), kForwardThreads, kRingBytes / kForwardBlocks);
+}
+RingPlan plan_backward(int cols, int vec, int es, int tensors) {
+    const int nv = cols / vec;
+    // groups of more than one warp meet on named barriers, of which a block has 15: at most 8 such groups, or 16 warps
+    if (nv <= 64) return plan_ring(cols, vec, es, tensors, 1, 512, kRingBytes);
+    if (nv <= 1024) return plan_ring(cols, vec, es, tensors, 1, 1024, kRingBytes);
+    return plan_ring(cols, vec, es, tensors, 4, 512, kRingBytes);
 }
 
 // Kernel attributes are per device and kernel, and only ever raised.
@@ -662,9 +675,9 @@ template <class T, int P, int kOut, bool kResidual>
 int launch_ring(const RowArgs& a, const RingPlan& r, cudaStream_t stream) {
     auto kernel = norm_ring_kernel<T, P, kOut, kResidual>;
     if (int rc = allow_smem(reinterpret_cast<const void*>(kernel), r.smem)) return rc;
-    const int groups = kRingThreads / r.g;
-    const int grid = int(std::min<long long>((a.rows + groups - 1) / groups, sm_count()));
-    kernel<<<grid, kRingThreads, r.smem, stream>>>(a, RingShape{r.g, r.stages, device_status_word()});
+    const int groups = r.threads / r.g;
+    const int grid = int(std::min<long long>((a.rows + groups - 1) / groups, (long long)sm_count() * kForwardBlocks));
+    kernel<<<grid, r.threads, r.smem, stream>>>(a, RingShape{r.g, r.stages, device_status_word()});
     count_launch();
     NTB200_CUDA(cudaGetLastError());
     return NTB200_OK;
@@ -674,9 +687,9 @@ template <class T, int kOut>
 int launch_rows(const RowArgs& a, bool vec_ok, cudaStream_t stream) {
     constexpr int kVec = 16 / sizeof(T);
     if (vec_ok && (a.h || !a.r)) {
-        const RingPlan r = plan_ring(a.cols, kVec, int(sizeof(T)), a.r ? 2 : 1);
+        const RingPlan r = plan_forward(a.cols, kVec, int(sizeof(T)), a.r ? 2 : 1);
         // each group has several rows to stream
-        if (r.stages >= 2 && a.rows >= 4ll * sm_count() * (kRingThreads / r.g)) {
+        if (r.stages >= 2 && a.rows >= 4ll * sm_count() * (r.threads / r.g)) {
             if (a.r) {
                 if (r.p == 1) return launch_ring<T, 1, kOut, true>(a, r, stream);
                 if (r.p == 2) return launch_ring<T, 2, kOut, true>(a, r, stream);
@@ -717,14 +730,14 @@ constexpr int64_t kMaxCols = int64_t(1) << 30;
 
 // Slabs of the weight gradient's partial sums, and so the grid of the backward kernel: depends on sizes alone, so that
 // the workspace can be sized before the call.
-int backward_slabs(int64_t rows) { return int(std::max<int64_t>(1, std::min<int64_t>(rows, 2 * 148))); }
+int backward_slabs(int64_t rows) { return int(std::max<int64_t>(1, std::min<int64_t>(rows, 4 * 148))); }
 
-template <class T, int P, bool kStream>
+template <class T, int P, bool kStream, int kThreads>
 int launch_backward_ring(const BackArgs& a, const RingPlan& r, int grid, cudaStream_t stream) {
-    auto kernel = norm_backward_ring_kernel<T, P, kStream>;
-    const uint32_t smem = std::max(r.smem, uint32_t(kRingThreads / r.g - 1) * uint32_t(a.cols) * 4u);
+    auto kernel = norm_backward_ring_kernel<T, P, kStream, kThreads>;
+    const uint32_t smem = std::max(r.smem, uint32_t(r.threads / r.g - 1) * uint32_t(a.cols) * 4u);
     if (int rc = allow_smem(reinterpret_cast<const void*>(kernel), smem)) return rc;
-    kernel<<<grid, kRingThreads, smem, stream>>>(a, RingShape{r.g, r.stages, device_status_word()});
+    kernel<<<grid, r.threads, smem, stream>>>(a, RingShape{r.g, r.stages, device_status_word()});
     count_launch();
     return NTB200_OK;
 }
@@ -734,15 +747,12 @@ int launch_backward(const BackArgs& a, void* grad_weight, bool vec_ok, cudaStrea
     constexpr int kVec = 16 / sizeof(T);
     const RowPlan pl = plan_row(a.cols, kVec, vec_ok);
     int slabs = backward_slabs(a.rows);
-    const RingPlan r = vec_ok ? plan_ring(a.cols, kVec, int(sizeof(T)), a.gh ? 3 : 2) : RingPlan{};
-    const int ring_groups = r.g ? kRingThreads / r.g : 1;
-    if (r.stages >= 2 && a.rows >= 4ll * sm_count() * ring_groups) {
+    const RingPlan r = vec_ok ? plan_backward(a.cols, kVec, int(sizeof(T)), a.gh ? 3 : 2) : RingPlan{};
+    if (r.stages >= 2 && a.rows >= 4ll * sm_count() * (r.threads / r.g)) {
         slabs = std::min(slabs, sm_count());
         int rc;
-        if (a.gh) rc = r.p == 1 ? launch_backward_ring<T, 1, true>(a, r, slabs, stream)
-                     : r.p == 2 ? launch_backward_ring<T, 2, true>(a, r, slabs, stream) : launch_backward_ring<T, 4, true>(a, r, slabs, stream);
-        else rc = r.p == 1 ? launch_backward_ring<T, 1, false>(a, r, slabs, stream)
-                : r.p == 2 ? launch_backward_ring<T, 2, false>(a, r, slabs, stream) : launch_backward_ring<T, 4, false>(a, r, slabs, stream);
+        if (a.gh) rc = r.p == 1 ? launch_backward_ring<T, 1, true, 1024>(a, r, slabs, stream) : launch_backward_ring<T, 4, true, 512>(a, r, slabs, stream);
+        else rc = r.p == 1 ? launch_backward_ring<T, 1, false, 1024>(a, r, slabs, stream) : launch_backward_ring<T, 4, false, 512>(a, r, slabs, stream);
         if (rc) return rc;
     } else if (pl.g == 0) {
         if (a.partial) {   // before gx, which may take the place of gy
@@ -773,7 +783,7 @@ int launch_backward(const BackArgs& a, void* grad_weight, bool vec_ok, cudaStrea
     }
     NTB200_CUDA(cudaGetLastError());
     if (a.partial) {
-        sum_partials_kernel<T><<<unsigned((a.cols + 31) / 32), 256, 0, stream>>>(a.partial, static_cast<T*>(grad_weight), slabs, a.cols);
+        sum_partials_kernel<T><<<unsigned((a.cols + 31) / 32), 512, 0, stream>>>(a.partial, static_cast<T*>(grad_weight), slabs, a.cols);
         count_launch();
         NTB200_CUDA(cudaGetLastError());
     }
