@@ -512,9 +512,9 @@ __global__ void __launch_bounds__(kThreads) norm_backward_ring_kernel(const Back
                 if (kStream) gh[p] = ld_shared_pack<T, V>(ring.at(stage, 2) + uint32_t(c) * 16u);
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    const float g = gy[p].up(i) * (h[p].up(i) * rstd);
-                    gw[p * V + i] += g;
-                    dot += g * w[p].up(i);
+    const float hv = h[p].up(i), g = gy[p].up(i) * hv;      // the row's rstd joins the sums below
+                    gw[p * V + i] = fmaf(g, rstd, gw[p * V + i]);
+                    dot = fmaf(g, w[p].up(i), dot);
                 }
             }
         }
@@ -525,7 +525,7 @@ __global__ void __launch_bounds__(kThreads) norm_backward_ring_kernel(const Back
         if (t == 0 && row + ring.stages * step < a.rows) load(ring, stage, row + ring.stages * step);
         if (++stage == ring.stages) { stage = 0; phase ^= 1u; }
         if (warps > 1) dot = warp_sum(lane < warps ? s_dot[flip][first_warp + lane] : 0.f);
-        const float c0 = rstd * dot * inv_cols;
+        const float c0 = rstd * (rstd * dot) * inv_cols;
 #pragma unroll
         for (int p = 0; p < P; ++p) {
             const int c = t + p * G;
@@ -534,8 +534,8 @@ __global__ void __launch_bounds__(kThreads) norm_backward_ring_kernel(const Back
             float v[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                v[i] = rstd * (gy[p].up(i) * w[p].up(i) - h[p].up(i) * c0);
-                if (kStream) v[i] += gh[p].up(i);
+                const float d = fmaf(-h[p].up(i), c0, gy[p].up(i) * w[p].up(i));
+                v[i] = kStream ? fmaf(rstd, d, gh[p].up(i)) : rstd * d;
             }
             o.put(v);
             reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.gx) + row * a.cols)[c] = o;
@@ -660,7 +660,7 @@ RingPlan plan_backward(int cols, int vec, int es, int tensors) {
     const int nv = cols / vec;
     // groups of more than one warp meet on named barriers, of which a block has 15: at most 8 such groups, or 16 warps
     if (nv <= 64) return plan_ring(cols, vec, es, tensors, 1, 512, kRingBytes);
-    if (nv <= 1024) return plan_ring(cols, vec, es, tensors, 1, 1024, kRingBytes);
+    if (nv <= 1024) return plan_ring(cols, vec, es, tensors, 2, 512, kRingBytes);
     return plan_ring(cols, vec, es, tensors, 4, 512, kRingBytes);
 }
 
@@ -751,8 +751,10 @@ int launch_backward(const BackArgs& a, void* grad_weight, bool vec_ok, cudaStrea
     if (r.stages >= 2 && a.rows >= 4ll * sm_count() * (r.threads / r.g)) {
         slabs = std::min(slabs, sm_count());
         int rc;
-        if (a.gh) rc = r.p == 1 ? launch_backward_ring<T, 1, true, 1024>(a, r, slabs, stream) : launch_backward_ring<T, 4, true, 512>(a, r, slabs, stream);
-        else rc = r.p == 1 ? launch_backward_ring<T, 1, false, 1024>(a, r, slabs, stream) : launch_backward_ring<T, 4, false, 512>(a, r, slabs, stream);
+        if (a.gh) rc = r.p == 1 ? launch_backward_ring<T, 1, true, 512>(a, r, slabs, stream)
+                     : r.p == 2 ? launch_backward_ring<T, 2, true, 512>(a, r, slabs, stream) : launch_backward_ring<T, 4, true, 512>(a, r, slabs, stream);
+        else rc = r.p == 1 ? launch_backward_ring<T, 1, false, 512>(a, r, slabs, stream)
+                : r.p == 2 ? launch_backward_ring<T, 2, false, 512>(a, r, slabs, stream) : launch_backward_ring<T, 4, false, 512>(a, r, slabs, stream);
         if (rc) return rc;
     } else if (pl.g == 0) {
         if (a.partial) {   // before gx, which may take the place of gy

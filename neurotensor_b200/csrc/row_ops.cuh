@@ -27,7 +27,19 @@ template <> struct RowType<__nv_bfloat16> {
 template <class T, int V>
 struct __align__(sizeof(T) * V) Pack {
     T e[V];
-    __device__ __forceinline__ float up(int i) const { return RowType<T>::up(e[i]); }
+    // one instruction per value: a BFloat16 is the upper half of a Float32, so the pair's word is shifted or masked
+    // (extracting the 16 bits first costs a second one)
+    __device__ __forceinline__ float up(int i) const {
+        if constexpr (std::is_same<T, __nv_bfloat16>::value && V % 2 == 0) {
+            const uint32_t w = reinterpret_cast<const uint32_t*>(e)[i >> 1];
+            return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
+        } else if constexpr (std::is_same<T, __half>::value && V % 2 == 0) {
+            const __half2 h = reinterpret_cast<const __half2*>(e)[i >> 1];
+            return i & 1 ? __high2float(h) : __low2float(h);
+        } else {
+            return RowType<T>::up(e[i]);
+        }
+    }
     __device__ __forceinline__ void set(int i, float v) { e[i] = RowType<T>::down(v); }
     // all of them, rounded; 16-bit values two at a time (one conversion instruction a pair)
     __device__ __forceinline__ void put(const float* v) {
