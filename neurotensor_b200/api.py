@@ -1045,9 +1045,9 @@ def _norm_operands(what, x, weight, residual):
     return code, _on_device(what, x, weight, residual)
 
 
-def _like(t):
-    """A contiguous tensor of t's shape and dtype."""
-    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+def _like(t, dtype=None):
+    """A contiguous tensor of t's shape, of t's dtype unless another is given."""
+    return torch.empty_like(t, dtype=dtype) if t.is_contiguous() else t.new_empty(t.shape, dtype=dtype or t.dtype)
 
 
 def _row_values(t, rows):
@@ -1080,7 +1080,7 @@ def rms_norm_int8(x, weight, eps=1e-6, residual=None):
     code, stream = _norm_operands("rms_norm_int8", x, weight, residual)
     xr, rows, x_rs = _rows_of(x)
     w = weight if weight.is_contiguous() else weight.contiguous()
-    q, scale = x.new_empty(x.shape, dtype=torch.int8), _row_values(x, rows)
+    q, scale = _like(x, torch.int8), _row_values(x, rows)
     if residual is None:
         h, hp, rr, rp, r_rs = x, None, None, None, 0
     else:
@@ -1097,7 +1097,7 @@ def quantize_rows(x):
     For hidden activations, and once for weights kept as [out, in]."""
     code, stream = _norm_operands("quantize_rows", x, None, None)
     xr, rows, x_rs = _rows_of(x)
-    q, scale = x.new_empty(x.shape, dtype=torch.int8), _row_values(x, rows)
+    q, scale = _like(x, torch.int8), _row_values(x, rows)
     check(lib().ntb200_quantize_rows(code, xr.data_ptr(), x_rs, q.data_ptr(), scale.data_ptr(), rows, x.shape[-1], stream))
     return q, scale
 
@@ -1213,7 +1213,7 @@ def linear_int8(q, scale, w, w_scale, bias=None, activation="none", residual=Non
     s = scale if scale.is_contiguous() else scale.contiguous()
     v = w_scale if w_scale.is_contiguous() else w_scale.contiguous()
     d.x_scale, d.w_scale = s.data_ptr(), v.data_ptr()
-    y = q.new_empty(shape, dtype=dtype)
+    y = q.new_empty(shape, dtype=dtype) if residual is None else _like(residual)
     _run_linear(d, y, stream)
     return y
 

@@ -86,6 +86,7 @@ struct GemmArgs {
 // cannot be expressed as TMA tensor maps, so the caller can route elsewhere.
 bool umma_supported(const GemmArgs& g, const char** why);
 int launch_umma_gemm(const GemmArgs& g, cudaStream_t stream);
+size_t f32_linear_scratch_bytes(const GemmArgs& g);   // scratch of launch_umma_gemm for Float32 with `linear` set
 size_t umma_scratch_bytes(const GemmArgs& g);   // upper bound of the scratch launch_umma_gemm takes for 16- and 8-bit operands
 // Few rows of 16-bit floats against a large weight matrix: would the automatic route slice K over a thread-block
 // cluster (one launch, weights read once at close to the HBM rate)?

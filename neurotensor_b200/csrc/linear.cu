@@ -33,19 +33,27 @@ __global__ void linear_finish_kernel(const float* __restrict__ z, const LinearPa
     }
 }
 
-// dst[r][c] = src[r * rs + c * cs], rows of dst ld elements apart (a multiple of 16 bytes), E bytes per element.
-// One 16-byte store per thread; neighbouring threads read neighbouring elements where cs is 1.
+// dst[r][c] = src[r * rs + c * cs], rows of dst ld elements apart (a multiple of 16 bytes), for one or two matrices in one
+// launch.  One 16-byte store per thread; neighbouring threads read neighbouring elements where cs is 1.
+struct PadJob {
+    const void* src;
+    void* dst;
+    long long rs, cs, ld, rows, cols;
+};
 template <class U>
-__global__ void pad_rows_kernel(const U* __restrict__ src, long long rs, long long cs, U* __restrict__ dst, long long ld, long long rows,
-                                long long cols) {
+__global__ void pad_rows_kernel(const PadJob first, const PadJob second) {
     constexpr int V = 16 / sizeof(U);
-    const long long per_row = ld / V, total = rows * per_row;
+    const long long total_first = first.rows * (first.ld / V), total = total_first + second.rows * (second.ld / V);
     for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
-        const long long r = i / per_row, c0 = (i - r * per_row) * V;
+        const bool one = i < total_first;
+        const PadJob& j = one ? first : second;
+        const long long at = one ? i : i - total_first, per_row = j.ld / V;
+        const long long r = at / per_row, c0 = (at - r * per_row) * V;
+        const U* src = static_cast<const U*>(j.src) + r * j.rs + c0 * j.cs;
         Pack<U, V> o;
 #pragma unroll
-        for (int j = 0; j < V; ++j) o.e[j] = c0 + j < cols ? src[r * rs + (c0 + j) * cs] : U(0);
-        *reinterpret_cast<Pack<U, V>*>(dst + r * ld + c0) = o;
+        for (int k = 0; k < V; ++k) o.e[k] = c0 + k < j.cols ? src[k * j.cs] : U(0);
+        *reinterpret_cast<Pack<U, V>*>(static_cast<U*>(j.dst) + r * j.ld + c0) = o;
     }
 }
 
@@ -137,22 +145,32 @@ size_t padded_bytes(const Operand& o, int es) {
     const int64_t rows = along_k ? o.mn : o.k, cols = along_k ? o.k : o.mn, v = 16 / es;
     return round256(size_t(rows) * size_t((cols + v - 1) / v * v) * size_t(es));
 }
-int pad_operand(Operand& o, int es, cudaStream_t stream) {
+int plan_pad(Operand& o, int es, PadJob* job, cudaStream_t stream) {
+    *job = PadJob{nullptr, nullptr, 0, 0, 16, 0, 0};
     const size_t bytes = padded_bytes(o, es);
     if (bytes == 0) return NTB200_OK;
     void* copy = nullptr;
     if (int rc = scratch_acquire(&copy, bytes, stream)) return rc;
     const bool along_k = o.k_s <= o.mn_s;
     const int64_t rows = along_k ? o.mn : o.k, cols = along_k ? o.k : o.mn, v = 16 / es, ld = (cols + v - 1) / v * v;
-    const int64_t rs = along_k ? o.mn_s : o.k_s, cs = along_k ? o.k_s : o.mn_s;
-    const int blocks = int(std::min<int64_t>((rows * (ld / v) + 255) / 256, int64_t(sm_count()) * 16));
-    if (es == 1) pad_rows_kernel<uint8_t><<<blocks, 256, 0, stream>>>(static_cast<const uint8_t*>(o.p), rs, cs, static_cast<uint8_t*>(copy), ld, rows, cols);
-    else pad_rows_kernel<uint16_t><<<blocks, 256, 0, stream>>>(static_cast<const uint16_t*>(o.p), rs, cs, static_cast<uint16_t*>(copy), ld, rows, cols);
-    count_launch();
-    NTB200_CUDA(cudaGetLastError());
+    *job = PadJob{o.p, copy, along_k ? o.mn_s : o.k_s, along_k ? o.k_s : o.mn_s, ld, rows, cols};
     o.p = copy;
     o.mn_s = along_k ? ld : 1;
     o.k_s = along_k ? 1 : ld;
+    return NTB200_OK;
+}
+// Padded copies of the operands that need one.
+int pad_operands(Operand& a, Operand& b, int es, cudaStream_t stream) {
+    PadJob ja, jb;
+    if (int rc = plan_pad(a, es, &ja, stream)) return rc;
+    if (int rc = plan_pad(b, es, &jb, stream)) return rc;
+    const int64_t work = (ja.rows * ja.ld + jb.rows * jb.ld) / (16 / es);
+    if (work == 0) return NTB200_OK;
+    const int blocks = int(std::min<int64_t>((work + 255) / 256, int64_t(sm_count()) * 16));
+    if (es == 1) pad_rows_kernel<uint8_t><<<blocks, 256, 0, stream>>>(ja, jb);
+    else pad_rows_kernel<uint16_t><<<blocks, 256, 0, stream>>>(ja, jb);
+    count_launch();
+    NTB200_CUDA(cudaGetLastError());
     return NTB200_OK;
 }
 
@@ -170,16 +188,18 @@ GemmArgs gemm_of(int dtype, const Operand& a, const Operand& b, void* c, int64_t
 bool small_f32(const GemmArgs& g) { return double(g.m) * double(g.n) * double(g.k) < 6.0e7; }   // as ntb200_gemm routes it
 
 // One plain product of the backward pass: its scratch beyond padded copies.
-size_t product_bytes(const GemmArgs& g) {
-    if (g.dtype == NTB200_F32) return small_f32(g) ? 0 : 2 * size_t(g.m + g.n) * size_t(g.k + 3) * 4 + 1024;
+size_t product_bytes(GemmArgs g) {
+    if (g.dtype == NTB200_F32) {
+        const LinearParams l{};
+        g.linear = &l;
+        return small_f32(g) ? 0 : f32_linear_scratch_bytes(g);
+    }
     return umma_scratch_bytes(g) + gemv_scratch_bytes(g) + 1024;
 }
 int plain_product(int dtype, Operand a, Operand b, void* c, int64_t c_rs, cudaStream_t stream) {
     if (a.mn == 0 || b.mn == 0) return NTB200_OK;
-    if (dtype != NTB200_F32) {
-        if (int rc = pad_operand(a, 2, stream)) return rc;
-        if (int rc = pad_operand(b, 2, stream)) return rc;
-    }
+    if (dtype != NTB200_F32)
+        if (int rc = pad_operands(a, b, 2, stream)) return rc;
     GemmArgs g = gemm_of(dtype, a, b, c, c_rs);
     // Rows that TMA cannot store would leave a plain GEMM element by element, thread by thread: ntb200_linear_act's
     // epilogue moves them by rows.  Large Float32 products take its finer partial sums.
@@ -310,8 +330,10 @@ extern "C" {
 size_t ntb200_linear_act_workspace_bytes(const ntb200_linear_desc* d) {
     if (check_linear(d) || d->m == 0 || d->n == 0 || d->k == 0) return 0;
     if (d->dtype == NTB200_F32) {
-        const GemmArgs g = gemm_of(d->dtype, x_of(*d), w_of(*d), d->y, d->y_row_stride);
-        return small_f32(g) ? round256(size_t(d->m) * size_t(d->n) * 4) : 2 * size_t(d->m + d->n) * size_t(d->k + 3) * 4 + 1024;
+        GemmArgs g = gemm_of(d->dtype, x_of(*d), w_of(*d), d->y, d->y_row_stride);
+        const LinearParams l{};
+        g.linear = &l;
+        return small_f32(g) ? round256(size_t(d->m) * size_t(d->n) * 4) : f32_linear_scratch_bytes(g);
     }
     const int es = int(dtype_size(d->dtype));
     GemmArgs g = gemm_of(d->dtype, x_of(*d), w_of(*d), d->y, d->y_row_stride);
@@ -354,8 +376,7 @@ int ntb200_linear_act(const ntb200_linear_desc* d, void* workspace, size_t works
     }
     if (d->dtype != NTB200_F32) {
         const int es = int(dtype_size(d->dtype));
-        if (int rc = pad_operand(x, es, s)) return rc;
-        if (int rc = pad_operand(w, es, s)) return rc;
+        if (int rc = pad_operands(x, w, es, s)) return rc;
         g = gemm_of(d->dtype, x, w, d->y, d->y_row_stride);
     }
     g.linear = &l;
@@ -410,6 +431,8 @@ int ntb200_linear_act_backward(const ntb200_linear_backward_desc* d, void* works
     }
     Operand dx[2], dw[2];
     backward_operands(*d, gz, p.ld, dx, dw);
+    if (d->grad_x && d->grad_w && d->dtype != NTB200_F32)   // both copies in one launch
+        if (int rc = pad_operands(dx[1], dw[d->grad_w_transposed ? 1 : 0], int(es), s)) return rc;
     if (d->grad_x)
         if (int rc = plain_product(d->dtype, dx[0], dx[1], d->grad_x, d->k, s)) return rc;
     if (d->grad_w)

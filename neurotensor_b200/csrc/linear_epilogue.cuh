@@ -171,29 +171,58 @@ __device__ __forceinline__ void linear_scale_bias32(const LinearParams& l, int n
     }
 }
 
-// Everything after the product for four neighbouring products of one row (K slices: the sums come four at a time).
-__device__ __forceinline__ void linear_finish4(const LinearParams& l, int n, int row, int col, float (&f)[4]) {
-    const int dt = l.out_dtype;
-    const float rs = l.row_scale ? l.row_scale[row] : 1.f;
-    const long long y0 = (long long)row * l.y_rs + col, r0 = (long long)row * l.residual_rs + col, p0 = (long long)row * l.pre_rs + col;
-    float r[4];
+// What four neighbouring products of one row need besides themselves; K-slice kernels load it before the sums are there.
+struct LinearAhead4 {
+    float rs, cs[4], bias[4], res[4];
+};
+__device__ __forceinline__ void linear_load_ahead4(const LinearParams& l, int n, int row, int col, LinearAhead4& a) {
+    a.rs = l.row_scale ? l.row_scale[row] : 1.f;
+    const long long r0 = (long long)row * l.residual_rs + col;
+    if (l.vec_ok && col + 4 <= n) {
+        if (l.col_scale) *reinterpret_cast<float4*>(a.cs) = *reinterpret_cast<const float4*>(l.col_scale + col);
+        auto four = [&](const void* p, long long i, float (&o)[4]) {
+            if (l.out_dtype == NTB200_F32) {
+                *reinterpret_cast<float4*>(o) = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+            } else {
+                const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
+                o[0] = lin_up16(w.x & 0xffffu, l.out_dtype); o[1] = lin_up16(w.x >> 16, l.out_dtype);
+                o[2] = lin_up16(w.y & 0xffffu, l.out_dtype); o[3] = lin_up16(w.y >> 16, l.out_dtype);
+            }
+        };
+        if (l.bias) four(l.bias, col, a.bias);
+        if (l.residual) four(l.residual, r0, a.res);
+        return;
+    }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const bool in = col + j < n;
-        if (l.col_scale && in) f[j] *= rs * l.col_scale[col + j];
-        if (l.bias && in) f[j] += lin_load(l.bias, col + j, dt);
-        r[j] = l.residual && in ? lin_load(l.residual, r0 + j, dt) : 0.f;
+        if (l.col_scale) a.cs[j] = in ? l.col_scale[col + j] : 1.f;
+        if (l.bias) a.bias[j] = in ? lin_load(l.bias, col + j, l.out_dtype) : 0.f;
+        if (l.residual) a.res[j] = in ? lin_load(l.residual, r0 + j, l.out_dtype) : 0.f;
     }
-    float z[4] = {f[0], f[1], f[2], f[3]};
+}
+// Everything after the product for them, stored.
+__device__ __forceinline__ void linear_finish4(const LinearParams& l, int n, int row, int col, float (&f)[4], const LinearAhead4& a) {
+    const int dt = l.out_dtype;
+    const long long y0 = (long long)row * l.y_rs + col, p0 = (long long)row * l.pre_rs + col;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (l.col_scale) f[j] *= a.rs * a.cs[j];
+        if (l.bias) f[j] += a.bias[j];
+    }
+    const float z[4] = {f[0], f[1], f[2], f[3]};
     if (dt == NTB200_F32) act_values<false>(l.act, f);
     else act_values<true>(l.act, f);
+    if (l.residual)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] += a.res[j];
     if (l.vec_ok && col + 4 <= n) {
         if (dt == NTB200_F32) {
             if (l.pre) *reinterpret_cast<float4*>(static_cast<float*>(l.pre) + p0) = make_float4(z[0], z[1], z[2], z[3]);
-            *reinterpret_cast<float4*>(static_cast<float*>(l.y) + y0) = make_float4(f[0] + r[0], f[1] + r[1], f[2] + r[2], f[3] + r[3]);
+            *reinterpret_cast<float4*>(static_cast<float*>(l.y) + y0) = make_float4(f[0], f[1], f[2], f[3]);
         } else {
             if (l.pre) *reinterpret_cast<uint2*>(static_cast<uint16_t*>(l.pre) + p0) = make_uint2(lin_pack2(z[0], z[1], dt), lin_pack2(z[2], z[3], dt));
-            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(l.y) + y0) = make_uint2(lin_pack2(f[0] + r[0], f[1] + r[1], dt), lin_pack2(f[2] + r[2], f[3] + r[3], dt));
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(l.y) + y0) = make_uint2(lin_pack2(f[0], f[1], dt), lin_pack2(f[2], f[3], dt));
         }
         return;
     }
@@ -201,7 +230,7 @@ __device__ __forceinline__ void linear_finish4(const LinearParams& l, int n, int
     for (int j = 0; j < 4; ++j)
         if (col + j < n) {
             if (l.pre) lin_store(l.pre, p0 + j, z[j], dt);
-            lin_store(l.y, y0 + j, f[j] + r[j], dt);
+            lin_store(l.y, y0 + j, f[j], dt);
         }
 }
 
