@@ -894,9 +894,19 @@ umma_gemm_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
                     const uint32_t bar = full_bar(stage);
                     mbar_expect_tx(bar, p.s_stage_tx);
                     const int k0 = kb * p.block_k;
-                    if constexpr (kSplit) {  // the split copies are dense and K-major
-                        tma_load_3d(a_dst + p.s_a_bytes, &tma_a_lo, bar, k0, m0, b * p.a_batch_mul);
-                        tma_load_3d(b_dst + T::kBBytes, &tma_b_lo, bar, k0, n0, b * p.b_batch_mul);
+                    if constexpr (kSplit) {  // the low parts, laid out like the high ones
+                        if (!p.a_mn_major) {
+                            tma_load_3d(a_dst + p.s_a_bytes, &tma_a_lo, bar, k0, m0, b * p.a_batch_mul);
+                        } else {
+                            for (int c = 0; c < p.a_chunks; ++c)
+                                tma_load_3d(a_dst + p.s_a_bytes + c * p.chunk_bytes, &tma_a_lo, bar, m0 + c * p.chunk_mn, k0, b * p.a_batch_mul);
+                        }
+                        if (!p.b_mn_major) {
+                            tma_load_3d(b_dst + T::kBBytes, &tma_b_lo, bar, k0, n0, b * p.b_batch_mul);
+                        } else {
+                            for (int c = 0; c < p.b_chunks; ++c)
+                                tma_load_3d(b_dst + T::kBBytes + c * p.chunk_bytes, &tma_b_lo, bar, n0 + c * p.chunk_mn, k0, b * p.b_batch_mul);
+                        }
                     }
                     if (!p.a_mn_major) {
                         tma_load_3d(a_dst, &tma_a, bar, k0, m0, b * p.a_batch_mul);
@@ -1160,8 +1170,20 @@ umma_gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
                     if (leader) mbar_expect_tx(bar, 2 * kPairStageBytes);
                     const int k0 = kb * p.block_k;
                     if constexpr (kSplit) {
-                        tma_load_3d_pair(a_dst + kPairOperandBytes, &tma_a_lo, bar, k0, m0, b * p.a_batch_mul);
-                        tma_load_3d_pair(b_dst + kPairOperandBytes, &tma_b_lo, bar, k0, n0, b * p.b_batch_mul);
+                        if (!p.a_mn_major) {
+                            tma_load_3d_pair(a_dst + kPairOperandBytes, &tma_a_lo, bar, k0, m0, b * p.a_batch_mul);
+                        } else {
+                            for (int c = 0; c < p.a_chunks; ++c)
+                                tma_load_3d_pair(a_dst + kPairOperandBytes + c * p.chunk_bytes, &tma_a_lo, bar, m0 + c * p.chunk_mn, k0,
+                                                 b * p.a_batch_mul);
+                        }
+                        if (!p.b_mn_major) {
+                            tma_load_3d_pair(b_dst + kPairOperandBytes, &tma_b_lo, bar, k0, n0, b * p.b_batch_mul);
+                        } else {
+                            for (int c = 0; c < p.b_chunks; ++c)
+                                tma_load_3d_pair(b_dst + kPairOperandBytes + c * p.chunk_bytes, &tma_b_lo, bar, n0 + c * p.chunk_mn, k0,
+                                                 b * p.b_batch_mul);
+                        }
                     }
                     if (!p.a_mn_major) {
                         tma_load_3d_pair(a_dst, &tma_a, bar, k0, m0, b * p.a_batch_mul);
@@ -2521,8 +2543,8 @@ int launch_planned(const GemmArgs& g, const Planned& pl, const Side& a, const Si
         if (const char* w = plan_operand(b_lo->ptr, es, pl.dt, g.n, g.k, b_lo->mn_stride, b_lo->k_stride, g.batch, b_lo->bs,
                                          use_pair ? 128 : bn, block_k, &maps.b_lo))
             return fail(NTB200_ERR_UNSUPPORTED, "tcgen05 route, B (low part): %s", w);
-        if (maps.a.mn_major || maps.b.mn_major || maps.a_lo.mn_major || maps.b_lo.mn_major)
-            return fail(NTB200_ERR_UNSUPPORTED, "tcgen05 route: split operands must be K-major");
+        if (pl.kind == MmaKind::tf32 && (maps.a.mn_major || maps.b.mn_major || maps.a_lo.mn_major || maps.b_lo.mn_major))
+            return fail(NTB200_ERR_UNSUPPORTED, "tcgen05 route: TF32 operands must be K-major");
     } else {
         maps.a_lo = maps.a;
         maps.b_lo = maps.b;
@@ -2610,7 +2632,7 @@ int launch_planned(const GemmArgs& g, const Planned& pl, const Side& a, const Si
         p.tma_store = use_pair && l16 && l.vec_ok && !g_direct_stores && plan_store(l.y, ldt, 2, g.m, g.n, 1, l.y_rs, 0, &maps.c) &&
                       (!l.pre || plan_store(l.pre, ldt, 2, g.m, g.n, 1, l.pre_rs, 0, &maps.relu)) &&
                       (!l.residual || plan_store(const_cast<void*>(l.residual), ldt, 2, g.m, g.n, 1, l.residual_rs, 0, &maps.peers.m[0]));
-        if (pl.kind == MmaKind::tf32) return launch_linear<MmaKind::tf32, true>(maps, p, use_pair, bn, grid, a_rows_staged, stream);
+        if (pl.split) return launch_linear<MmaKind::f16, true>(maps, p, use_pair, bn, grid, a_rows_staged, stream);
         if (pl.kind == MmaKind::i8) return launch_linear<MmaKind::i8, false>(maps, p, use_pair, bn, grid, a_rows_staged, stream);
         return launch_linear<MmaKind::f16, false>(maps, p, use_pair, bn, grid, a_rows_staged, stream);
     }
@@ -2650,35 +2672,10 @@ __global__ void splitk_linear_kernel(const float* __restrict__ partial, int spli
     linear_finish4(l, n, row, col, f, ahead);
 }
 
-// ntb200_linear_act in Float32 with few tiles: K slices as batches (each writing a partial product), joined by
-// splitk_linear_kernel.  A K block of a tile moves 64 KB per SM whatever the tile, so a problem that leaves SMs idle ends
-// sooner only with more of them on the same tile: [512, 1024] x [1024, 4096] on 32 pair tiles x 2 slices instead of 128
-// single tiles took 64 -> 46 us.  1: no slices.
-struct SplitF32Plan { int slices; bool pair; };
-SplitF32Plan plan_f32_linear(const GemmArgs& g) {
-    SplitF32Plan p{1, false};
-    if (!g.linear || g.batch != 1 || g.n % 4 != 0) return p;
-    const int sms = sm_count();
-    p.pair = !g_disable_pair && g.m > 128 && g.n > 128;
-    const int64_t tiles = p.pair ? ((g.m + 255) / 256) * ((g.n + 255) / 256) : ((g.m + kBM - 1) / kBM) * ((g.n + 127) / 128);
-    const int64_t units = p.pair ? sms / 2 : sms;
-    while (p.slices < 8 && tiles * p.slices * 2 <= units && g.k / (p.slices * 2) >= 256) p.slices *= 2;
-    return p;
-}
-}  // namespace
-size_t f32_linear_scratch_bytes(const GemmArgs& g) {
-    const int slices = plan_f32_linear(g).slices;
-    return 2 * size_t(g.m + g.n) * size_t(g.k + 32 * slices) * sizeof(float) + 1024 + (slices > 1 ? size_t(slices) * size_t(g.m) * size_t(g.n) * sizeof(float) + 256 : 0);
-}
-namespace {
-
 // Float32: split both operands into dense K-major hi/lo copies in pool scratch, then one GEMM with three TF32
 // products per K step.  The scratch is returned to the pool in stream order.
 int launch_f32_split(const GemmArgs& g, cudaStream_t stream) {
-    const SplitF32Plan sp = plan_f32_linear(g);
-    const int64_t slice = sp.slices > 1 ? ((g.k + sp.slices - 1) / sp.slices + 31) / 32 * 32 : g.k;
-    // rows of the copies stay 16-byte aligned; K slices fill whole blocks with zeros
-    const int64_t kp = sp.slices > 1 ? slice * sp.slices : (g.k + 3) & ~int64_t(3);
+    const int64_t kp = (g.k + 3) & ~int64_t(3);  // rows of the copies stay 16-byte aligned
     const int64_t a_batch = (g.batch > 1 && g.a_bs != 0) ? g.batch : 1;
     const int64_t b_batch = (g.batch > 1 && g.b_bs != 0) ? g.batch : 1;
     if (a_batch > 65535 || b_batch > 65535) return fail(NTB200_ERR_UNSUPPORTED, "tcgen05 route: batch too large for the Float32 split pass");
@@ -2708,35 +2705,7 @@ int launch_f32_split(const GemmArgs& g, cudaStream_t stream) {
         const Planned pl{4, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, MmaKind::tf32, kOutF32, 1u, 2u, true, "umma_3xtf32"};
         const Side sa{a_hi, kp, 1, a_batch > 1 ? g.m * kp : 0}, sal{a_lo, kp, 1, a_batch > 1 ? g.m * kp : 0};
         const Side sb{b_hi, kp, 1, b_batch > 1 ? g.n * kp : 0}, sbl{b_lo, kp, 1, b_batch > 1 ? g.n * kp : 0};
-        // ntb200_linear_act takes the partial sums every second K block: at K = 1024 its relative error falls from 1.4e-6
-        // to that of an fp32 product
-        Planned pc = pl;
-        if (g.linear) pc.chunk = 2;
-        if (sp.slices > 1) {
-            float* partial = nullptr;
-            const int64_t slab = g.m * g.n;
-            rc = scratch_acquire(reinterpret_cast<void**>(&partial), size_t(sp.slices) * size_t(slab) * sizeof(float), stream);
-            if (rc == NTB200_OK) {
-                GemmArgs part = g;
-                part.linear = nullptr;
-                part.batch = sp.slices; part.k = slice;
-                part.c = partial; part.c_rs = g.n; part.c_bs = slab;
-                const Side ka{a_hi, kp, 1, slice}, kal{a_lo, kp, 1, slice}, kb{b_hi, kp, 1, slice}, kbl{b_lo, kp, 1, slice};
-                const TileChoice choice{sp.pair, 128};
-                pc.route = "umma_3xtf32_splitk";
-                rc = launch_planned(part, pc, ka, kb, &kal, &kbl, stream, &choice);
-                if (rc == NTB200_OK) {
-                    const long long work = (long long)g.m * (g.n / 4);
-                    splitk_linear_kernel<<<unsigned((work + 255) / 256), 256, 0, stream>>>(partial, sp.slices, slab, int(g.m), int(g.n), *g.linear);
-                    count_launch();
-                    e = cudaGetLastError();
-                    if (e != cudaSuccess) rc = cuda_fail(e, "splitk_linear_kernel");
-                }
-                scratch_release(partial, stream);
-            }
-        } else {
-            rc = launch_planned(g, pc, sa, sb, &sal, &sbl, stream);
-        }
+        rc = launch_planned(g, pl, sa, sb, &sal, &sbl, stream);
     }
     scratch_release(scratch, stream);
     return rc;
@@ -3244,6 +3213,13 @@ bool umma_cluster_k_would_run(const GemmArgs& g) {
     if (g.dtype != NTB200_F16 && g.dtype != NTB200_BF16) return false;
     if (g.m > kBM || operands_stageable(g) != nullptr) return false;
     return plan_cluster_k(g, 2).valid;
+}
+
+int launch_umma_f16x3(const GemmArgs& g, const void* a_lo, const void* b_lo, cudaStream_t stream) {
+    Planned pl{2, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, MmaKind::f16, kOutF32, 1u, 0u, true, "umma_3xf16"};
+    pl.chunk = 2;   // partial sums every 128 of K: the tensor cores' truncating adds stay below an fp32 product's error
+    const Side a{g.a, g.a_rs, g.a_cs, 0}, al{a_lo, g.a_rs, g.a_cs, 0}, b{g.b, g.b_cs, g.b_rs, 0}, bl{b_lo, g.b_cs, g.b_rs, 0};
+    return launch_planned(g, pl, a, b, &al, &bl, stream);
 }
 
 size_t umma_scratch_bytes(const GemmArgs& g) {

@@ -86,7 +86,9 @@ struct GemmArgs {
 // cannot be expressed as TMA tensor maps, so the caller can route elsewhere.
 bool umma_supported(const GemmArgs& g, const char** why);
 int launch_umma_gemm(const GemmArgs& g, cudaStream_t stream);
-size_t f32_linear_scratch_bytes(const GemmArgs& g);   // scratch of launch_umma_gemm for Float32 with `linear` set
+// ntb200_linear_act in Float32: g.a / g.b are the Float16 high parts of the operands (dtype F16), the low parts have their
+// strides; three products per multiply, fp32 out, g.linear carries the scales.
+int launch_umma_f16x3(const GemmArgs& g, const void* a_lo, const void* b_lo, cudaStream_t stream);
 size_t umma_scratch_bytes(const GemmArgs& g);   // upper bound of the scratch launch_umma_gemm takes for 16- and 8-bit operands
 // Few rows of 16-bit floats against a large weight matrix: would the automatic route slice K over a thread-block
 // cluster (one launch, weights read once at close to the HBM rate)?

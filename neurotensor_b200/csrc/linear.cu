@@ -57,6 +57,119 @@ __global__ void pad_rows_kernel(const PadJob first, const PadJob second) {
     }
 }
 
+// ---- Float32 as three Float16 products ----------------------------------------------------------------------------------
+// A row of A (a column of B) is scaled by a power of two that brings its largest finite value to [2^14, 2^15), then
+// x = hi + lo with hi = fp16(x), lo = fp16(x - hi): |x - hi - lo| <= 2^-24 |x| down to 2^-13 of the largest value and below
+// 2^-39 of it always, so a.b = hi.hi + hi.lo + lo.hi + O(2^-23 |a||b|).  kind::f16 runs at twice TF32's rate and a value's two
+// parts take 4 bytes instead of 8: [512, 1024] x [1024, 4096] took 30 us as three TF32 products.  The scales are undone by
+// the epilogue's row and column factors (powers of two, exact).  Parts keep the operand's direction (tcgen05 takes
+// Float16 tiles along either axis), so nothing is transposed.
+struct SplitF16Job {
+    const float* src;
+    __half* hi;
+    __half* lo;
+    float* unscale;                 // [mn]: what a product has to be multiplied by for this operand
+    long long mn, k, mn_s, k_s, ld; // source strides; rows of the parts (along K, or along mn) are ld elements apart
+    int along_k, blocks;
+};
+constexpr int kSplitThreads = 1024, kSplitHeld = 32;
+
+__device__ __forceinline__ float split_scale(float top, float* unscale) {
+    const int e = top > 0.f ? int(__float_as_uint(top) >> 23) : 141;
+    const int bits = min(253, 268 - e);
+    *unscale = __uint_as_float(uint32_t(254 - bits) << 23);
+    return __uint_as_float(uint32_t(bits) << 23);
+}
+__device__ __forceinline__ void split_one(float x, float scale, __half* hi, __half* lo) {
+    const float v = x * scale;
+    const __half h = __float2half_rn(v);
+    const float hf = __half2float(h);
+    *hi = h;
+    *lo = __float2half_rn(isfinite(hf) ? v - hf : 0.f);
+}
+__device__ __forceinline__ float finite_abs(float x) { return isfinite(x) ? fabsf(x) : 0.f; }
+
+__global__ void __launch_bounds__(kSplitThreads) split_f16_kernel(const SplitF16Job ja, const SplitF16Job jb) {
+    __shared__ float red[32][33];
+    const bool second = int(blockIdx.x) >= ja.blocks;
+    const SplitF16Job& j = second ? jb : ja;
+    const int block = int(blockIdx.x) - (second ? ja.blocks : 0), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (j.along_k) {   // a warp per row
+        const long long r = (long long)block * 32 + warp;
+        if (r >= j.mn) return;
+        const float* src = j.src + r * j.mn_s;
+        __half* hi = j.hi + r * j.ld;
+        __half* lo = j.lo + r * j.ld;
+        float held[kSplitHeld], top = 0.f;
+        const bool fits = j.k <= 32 * kSplitHeld;
+        if (fits) {
+#pragma unroll
+            for (int i = 0; i < kSplitHeld; ++i) {
+                const long long c = lane + 32 * i;
+                held[i] = c < j.k ? src[c * j.k_s] : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < kSplitHeld; ++i) top = fmaxf(top, finite_abs(held[i]));
+        } else {
+#pragma unroll 8
+            for (long long c = lane; c < j.k; c += 32) top = fmaxf(top, finite_abs(src[c * j.k_s]));
+        }
+        top = warp_max_nan(top);
+        float unscale;
+        const float scale = split_scale(top, &unscale);
+        if (lane == 0) j.unscale[r] = unscale;
+        if (fits) {
+#pragma unroll
+            for (int i = 0; i < kSplitHeld; ++i) {
+                const long long c = lane + 32 * i;
+                if (c < j.k) split_one(held[i], scale, hi + c, lo + c);
+            }
+        } else {
+#pragma unroll 8
+            for (long long c = lane; c < j.k; c += 32) split_one(src[c * j.k_s], scale, hi + c, lo + c);
+        }
+        return;
+    }
+    // lanes on 32 neighbouring columns, every 32nd K row per warp
+    const long long c = (long long)block * 32 + lane;
+    const bool in = c < j.mn;
+    const float* src = j.src + (in ? c : 0) * j.mn_s;
+    float held[kSplitHeld], top = 0.f;
+    const bool fits = j.k <= 32 * kSplitHeld;
+    if (fits) {
+#pragma unroll
+        for (int i = 0; i < kSplitHeld; ++i) {
+            const long long r = warp + 32 * i;
+            held[i] = in && r < j.k ? src[r * j.k_s] : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < kSplitHeld; ++i) top = fmaxf(top, finite_abs(held[i]));
+    } else if (in) {
+#pragma unroll 8
+        for (long long r = warp; r < j.k; r += 32) top = fmaxf(top, finite_abs(src[r * j.k_s]));
+    }
+    red[warp][lane] = top;
+    __syncthreads();
+    top = warp_max_nan(red[lane][warp]);   // warp w: the maximum of column w
+    __syncthreads();
+    if (lane == 0) red[0][warp] = top;
+    __syncthreads();
+    float unscale;
+    const float scale = split_scale(red[0][lane], &unscale);
+    if (!in) return;
+    if (warp == 0) j.unscale[c] = unscale;
+    if (fits) {
+#pragma unroll
+        for (int i = 0; i < kSplitHeld; ++i) {
+            const long long r = warp + 32 * i;
+            if (r < j.k) split_one(held[i], scale, j.hi + r * j.ld + c, j.lo + r * j.ld + c);
+        }
+    } else {
+#pragma unroll 8
+        for (long long r = warp; r < j.k; r += 32) split_one(src[r * j.k_s], scale, j.hi + r * j.ld + c, j.lo + r * j.ld + c);
+    }
+}
+
 // gz = gy act'(pre), and the column sums of gz of one slab of rows per blockIdx.y (partial: [slabs, n]).  32 x 8 threads,
 // each on V columns of every eighth row of the slab; the sums use gz before it is rounded.
 // kAct is the activation, decided once per launch: a switch per value costs as much as the slope.
@@ -187,13 +300,48 @@ GemmArgs gemm_of(int dtype, const Operand& a, const Operand& b, void* c, int64_t
 
 bool small_f32(const GemmArgs& g) { return double(g.m) * double(g.n) * double(g.k) < 6.0e7; }   // as ntb200_gemm routes it
 
-// One plain product of the backward pass: its scratch beyond padded copies.
-size_t product_bytes(GemmArgs g) {
-    if (g.dtype == NTB200_F32) {
-        const LinearParams l{};
-        g.linear = &l;
-        return small_f32(g) ? 0 : f32_linear_scratch_bytes(g);
+// Parts of one operand: rows along the direction in which its elements are closer together.
+size_t parts_elements(const Operand& o) {
+    const bool along_k = o.k_s <= o.mn_s;
+    const int64_t rows = along_k ? o.mn : o.k, cols = along_k ? o.k : o.mn;
+    return size_t(rows) * size_t((cols + 7) / 8 * 8);
+}
+size_t f16x3_bytes(const Operand& a, const Operand& b) {
+    return 2 * 2 * (round256(parts_elements(a)) + round256(parts_elements(b))) + 4 * round256(size_t(a.mn)) + 4 * round256(size_t(b.mn)) + 4096;
+}
+// y of `l` from Float32 operands on the tensor cores; l's scales are free.
+int f16x3_product(const Operand& a, const Operand& b, LinearParams l, cudaStream_t stream) {
+    Operand parts[2] = {a, b};
+    SplitF16Job jobs[2];
+    void* lo[2];
+    for (int i = 0; i < 2; ++i) {
+        Operand& o = parts[i];
+        const bool along_k = o.k_s <= o.mn_s;
+        const int64_t ld = ((along_k ? o.k : o.mn) + 7) / 8 * 8;
+        const size_t bytes = 2 * round256(parts_elements(o));
+        void *hi = nullptr, *unscale = nullptr;
+        if (int rc = scratch_acquire(&hi, 2 * bytes, stream)) return rc;
+        if (int rc = scratch_acquire(&unscale, 4 * size_t(o.mn), stream)) return rc;
+        lo[i] = static_cast<char*>(hi) + bytes;
+        jobs[i] = SplitF16Job{static_cast<const float*>(o.p), static_cast<__half*>(hi), static_cast<__half*>(lo[i]), static_cast<float*>(unscale),
+                              o.mn, o.k, o.mn_s, o.k_s, ld, along_k ? 1 : 0, int((o.mn + 31) / 32)};
+        o.p = hi;
+        o.mn_s = along_k ? ld : 1;
+        o.k_s = along_k ? 1 : ld;
     }
+    split_f16_kernel<<<unsigned(jobs[0].blocks + jobs[1].blocks), kSplitThreads, 0, stream>>>(jobs[0], jobs[1]);
+    count_launch();
+    NTB200_CUDA(cudaGetLastError());
+    l.row_scale = jobs[0].unscale;
+    l.col_scale = jobs[1].unscale;
+    GemmArgs g = gemm_of(NTB200_F16, parts[0], parts[1], l.y, l.y_rs);
+    g.linear = &l;
+    return launch_umma_f16x3(g, lo[0], lo[1], stream);
+}
+
+// One plain product of the backward pass: its scratch beyond padded copies.
+size_t product_bytes(const GemmArgs& g, const Operand& a, const Operand& b) {
+    if (g.dtype == NTB200_F32) return small_f32(g) ? 0 : f16x3_bytes(a, b);
     return umma_scratch_bytes(g) + gemv_scratch_bytes(g) + 1024;
 }
 int plain_product(int dtype, Operand a, Operand b, void* c, int64_t c_rs, cudaStream_t stream) {
@@ -202,10 +350,11 @@ int plain_product(int dtype, Operand a, Operand b, void* c, int64_t c_rs, cudaSt
         if (int rc = pad_operands(a, b, 2, stream)) return rc;
     GemmArgs g = gemm_of(dtype, a, b, c, c_rs);
     // Rows that TMA cannot store would leave a plain GEMM element by element, thread by thread: ntb200_linear_act's
-    // epilogue moves them by rows.  Large Float32 products take its finer partial sums.
+    // epilogue moves them by rows.  Large Float32 products are three Float16 ones.
     LinearParams l{};
     l.y = c; l.y_rs = c_rs; l.act = NTB200_ACT_NONE; l.out_dtype = dtype;
-    if (dtype == NTB200_F32 ? !small_f32(g) : c_rs % 8 != 0 || !on16(c)) {
+    if (dtype == NTB200_F32 && !small_f32(g)) return f16x3_product(a, b, l, stream);
+    if (dtype != NTB200_F32 && (c_rs % 8 != 0 || !on16(c))) {
         g.linear = &l;
         return launch_umma_gemm(g, stream);
     }
@@ -330,10 +479,8 @@ extern "C" {
 size_t ntb200_linear_act_workspace_bytes(const ntb200_linear_desc* d) {
     if (check_linear(d) || d->m == 0 || d->n == 0 || d->k == 0) return 0;
     if (d->dtype == NTB200_F32) {
-        GemmArgs g = gemm_of(d->dtype, x_of(*d), w_of(*d), d->y, d->y_row_stride);
-        const LinearParams l{};
-        g.linear = &l;
-        return small_f32(g) ? round256(size_t(d->m) * size_t(d->n) * 4) : f32_linear_scratch_bytes(g);
+        const GemmArgs g = gemm_of(d->dtype, x_of(*d), w_of(*d), d->y, d->y_row_stride);
+        return small_f32(g) ? round256(size_t(d->m) * size_t(d->n) * 4) : f16x3_bytes(x_of(*d), w_of(*d));
     }
     const int es = int(dtype_size(d->dtype));
     GemmArgs g = gemm_of(d->dtype, x_of(*d), w_of(*d), d->y, d->y_row_stride);
@@ -374,11 +521,9 @@ int ntb200_linear_act(const ntb200_linear_desc* d, void* workspace, size_t works
         NTB200_CUDA(cudaGetLastError());
         return NTB200_OK;
     }
-    if (d->dtype != NTB200_F32) {
-        const int es = int(dtype_size(d->dtype));
-        if (int rc = pad_operands(x, w, es, s)) return rc;
-        g = gemm_of(d->dtype, x, w, d->y, d->y_row_stride);
-    }
+    if (d->dtype == NTB200_F32) return f16x3_product(x, w, l, s);
+    if (int rc = pad_operands(x, w, int(dtype_size(d->dtype)), s)) return rc;
+    g = gemm_of(d->dtype, x, w, d->y, d->y_row_stride);
     g.linear = &l;
     return launch_umma_gemm(g, s);
 }
@@ -395,7 +540,7 @@ size_t ntb200_linear_act_backward_workspace_bytes(const ntb200_linear_backward_d
     for (const auto* o : {dx, dw}) {
         if (o == dx ? !d->grad_x : !d->grad_w) continue;
         if (d->dtype != NTB200_F32) bytes += padded_bytes(o[0], es) + padded_bytes(o[1], es);
-        bytes += product_bytes(gemm_of(d->dtype, o[0], o[1], nullptr, o[1].mn));
+        bytes += product_bytes(gemm_of(d->dtype, o[0], o[1], nullptr, o[1].mn), o[0], o[1]);
     }
     return bytes;
 }
