@@ -9,46 +9,55 @@
 
 namespace ntb200 {
 
-// kFast: results that are rounded to 16 bits use the hardware exponential and reciprocal (relative error about 2^-21,
-// a hundredth of half a Float16 step); Float32 results use the full-precision functions.
+// e^x for Float32 results: the hardware exponential of the rounded x log2(e), corrected to first order by what the rounding
+// left out (relative error about 2^-22; without the correction it grows with |x|).  Straight-line code: calls of expf and
+// erfcf, one value at a time, made the Float32 epilogue the longest part of its kernel.
+__device__ __forceinline__ float exp_full(float x) {
+    x = fminf(fmaxf(x, -150.f), 150.f);
+    const float t = x * 1.44269504f;
+    const float r = fmaf(x, 1.44269504f, -t) + x * 1.9259630e-8f;
+    return exp2_hw(t) * fmaf(r, 0.69314718f, 1.f);
+}
+// kFast: results that are rounded to 16 bits use the hardware exponential as it is (a hundredth of half a Float16 step).
 template <bool kFast>
 __device__ __forceinline__ float sigmoid_times(float z, float u) {   // z / (1 + e^-u)
-    if constexpr (kFast) return z * rcp_hw(1.f + exp2_hw(-1.4426950408889634f * u));
-    return z / (1.f + expf(-u));
+    return z * rcp_hw(1.f + (kFast ? exp2_hw(-1.4426950408889634f * u) : exp_full(-u)));
 }
 
 constexpr float kGeluScale = 1.5957691216057308f;   // 2 sqrt(2 / pi): z/2 (1 + tanh u) = z sigmoid(2 u)
 constexpr float kGeluCubic = 0.044715f;
 
-// Phi(z) = erfc(-z / sqrt 2) / 2 for results of 16 bits, e = e^(-z^2 / 2).  Phi(-a) = e t P(t) with t = 1 / (1 + 0.36 a): P is
-// a degree-6 fit of erfcx(a / sqrt 2) / (2 t), relative error below 1.1e-6 over 0 <= a <= 14 (least squares reweighted
-// towards the minimax, evaluated in fp32), so the tail keeps its relative precision.  15 instructions; erfcf takes 40.
-__device__ __forceinline__ float gauss_fast(float z) { return exp2_hw(-0.72134752044448170f * z * z); }   // e^(-z^2 / 2)
-__device__ __forceinline__ float phi_fast(float z, float e) {
-    const float t = rcp_hw(1.f + 0.36f * fabsf(z));
-    const float q = e * t * (0.14371304f + t * (0.14177254f + t * (0.13971882f + t * (0.026550606f + t * (0.1809521f + t * (-0.17976327f + t * 0.047055867f))))));
-    return z < 0.f ? q : 1.f - q;
+// Phi(z) = erfc(-z / sqrt 2) / 2 from e = e^(-z^2 / 2): Phi(-a) = e t P(t) with t = 1 / (1 + p a), P a fit of
+// erfcx(a / sqrt 2) / (2 t) over 0 <= a <= 14 by least squares reweighted towards the minimax of the relative error, so the
+// tail keeps its precision: degree 6, p = 0.36, error below 1.1e-6 for 16-bit results; degree 8, p = 0.21, below 1.7e-8 (and
+// 1.1e-7 rms with fp32's roundings) for Float32.
+template <bool kFast>
+__device__ __forceinline__ float gauss(float z) {
+    if constexpr (kFast) return exp2_hw(-0.72134752044448170f * z * z);
+    const float s = fminf(z * z, 400.f), low = z * z < 400.f ? fmaf(z, z, -s) : 0.f;   // the square's own rounding matters for large z
+    return exp_full(-0.5f * s) * fmaf(-0.5f, low, 1.f);
 }
-
-// Full precision, out of line: Float32 results are few and these functions long.
-static __device__ __noinline__ float act_value_full(int act, float z) {
-    switch (act) {
-        case NTB200_ACT_RELU: return z < 0.f ? 0.f : z;
-        case NTB200_ACT_GELU: return 0.5f * z * erfcf(z * -0.70710678118654752f);
-        case NTB200_ACT_GELU_TANH: return sigmoid_times<false>(z, kGeluScale * (z + kGeluCubic * z * z * z));
-        case NTB200_ACT_SILU: return sigmoid_times<false>(z, z);
-        default: return z;
+template <bool kFast>
+__device__ __forceinline__ float phi(float z, float e) {
+    float q;
+    if constexpr (kFast) {
+        const float t = rcp_hw(1.f + 0.36f * fabsf(z));
+        q = e * t * (0.14371304f + t * (0.14177254f + t * (0.13971882f + t * (0.026550606f + t * (0.1809521f + t * (-0.17976327f + t * 0.047055867f))))));
+    } else {
+        const float t = rcp_hw(1.f + 0.21f * fabsf(z));
+        q = e * t * (0.08371158f + t * (0.085068814f + t * (0.069192477f + t * (0.1248716f + t * (-0.09392268f + t * (0.34939754f + t * (-0.33025047f +
+                                                                                                                                     t * (0.28358722f + t * -0.071656048f))))))));
     }
+    return z < 0.f ? q : 1.f - q;
 }
 
 template <bool kFast>
 __device__ __forceinline__ float act_value(int act, float z) {
-    if constexpr (!kFast) return act_value_full(act, z);
     switch (act) {
         case NTB200_ACT_RELU: return z < 0.f ? 0.f : z;
-        case NTB200_ACT_GELU: return z * phi_fast(z, gauss_fast(z));
-        case NTB200_ACT_GELU_TANH: return sigmoid_times<true>(z, kGeluScale * (z + kGeluCubic * z * z * z));
-        case NTB200_ACT_SILU: return sigmoid_times<true>(z, z);
+        case NTB200_ACT_GELU: return z * phi<kFast>(z, gauss<kFast>(z));
+        case NTB200_ACT_GELU_TANH: return sigmoid_times<kFast>(z, kGeluScale * (z + kGeluCubic * z * z * z));
+        case NTB200_ACT_SILU: return sigmoid_times<kFast>(z, z);
         default: return z;
     }
 }
@@ -58,11 +67,8 @@ __device__ __forceinline__ float act_slope(int act, float z) {
     switch (act) {
         case NTB200_ACT_RELU: return z < 0.f ? 0.f : 1.f;
         case NTB200_ACT_GELU: {
-            if constexpr (kFast) {
-                const float e = gauss_fast(z);
-                return fmaf(z * 0.39894228040143268f, e, phi_fast(z, e));
-            }
-            return 0.5f * erfcf(z * -0.70710678118654752f) + z * expf(-0.5f * z * z) * 0.39894228040143268f;
+            const float e = gauss<kFast>(z);
+            return fmaf(z * 0.39894228040143268f, e, phi<kFast>(z, e));
         }
         case NTB200_ACT_GELU_TANH: {
             if (fabsf(z) > 20.f) return z > 0.f ? 1.f : 0.f;   // the tails, before z^3 can overflow
@@ -80,12 +86,6 @@ __device__ __forceinline__ float act_slope(int act, float z) {
 // The activation of N values, decided once.
 template <bool kFast, int N>
 __device__ __forceinline__ void act_values(int act, float (&f)[N]) {
-    if constexpr (!kFast) {
-        if (act == NTB200_ACT_NONE) return;
-#pragma unroll
-        for (int j = 0; j < N; ++j) f[j] = act_value_full(act, f[j]);
-        return;
-    }
 #define NTB200_ACT_CASE(A)                                            \
     case A:                                                           \
         _Pragma("unroll") for (int j = 0; j < N; ++j) f[j] = act_value<kFast>(A, f[j]); \
