@@ -266,14 +266,13 @@ __device__ __forceinline__ bool epilogue_linear(const UmmaParams& p, uint32_t tm
 }
 // The Float32 split kernels' running sums.
 template <int HC>
-__device__ __forceinline__ void finish_running(const UmmaParams& p, const float (&run)[HC], float* staged, int row0, int lane, int col_base) {
+__device__ __forceinline__ void finish_running(const UmmaParams& p, const float (&run)[HC], float* staged, int row0, int lane, int col_base, LinearAhead& ahead) {
     if (row0 >= p.m) return;
 #pragma unroll
     for (int cc = 0; cc < HC / 32; ++cc) {
         const int col0 = col_base + cc * 32;
         if (col0 >= p.n) continue;
-        LinearAhead ahead;
-        linear_load_ahead<NTB200_F32>(p.linear, p.m, p.n, row0, col0, lane, ahead);
+        if (cc > 0 || HC > 64) linear_load_ahead<NTB200_F32>(p.linear, p.m, p.n, row0, col0, lane, ahead);
         float f[32];
 #pragma unroll
         for (int j = 0; j < 32; ++j) f[j] = run[cc * 32 + j];
@@ -1001,6 +1000,8 @@ umma_gemm_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
         for (int t = blockIdx.x; alive && t < p.total_tiles; t += gridDim.x) {
             int b, mi, ni;
             tile_coords(p, t, b, mi, ni);
+            [[maybe_unused]] LinearAhead ahead;   // kLinear: requested before the sums are there, where registers allow it
+            if constexpr (kLinear && HC <= 64) linear_load_ahead<NTB200_F32>(p.linear, p.m, p.n, mi * kBM + quad * 32, ni * BN + half * HC, lane, ahead);
             for (int kb0 = 0; kb0 < p.k_blocks; kb0 += p.chunk_blocks) {
                 bool ok = mbar_wait(tfull_bar(acc), acc_phase, abort_flag);
                 ok = __all_sync(0xffffffffu, ok);
@@ -1019,7 +1020,7 @@ umma_gemm_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
             if (alive) {
                 if constexpr (kLinear)
                     finish_running<HC>(p, run, reinterpret_cast<float*>(bar_gen + T::kBarrierBytes + uint32_t(warp - 2) * kStagedBlock),
-                                       mi * kBM + quad * 32, lane, ni * BN + half * HC);
+                                       mi * kBM + quad * 32, lane, ni * BN + half * HC, ahead);
                 else
                     store_running<HC>(p, run, b, mi * kBM + row_in_tile, ni * BN + half * HC);
             }
@@ -1274,6 +1275,7 @@ umma_gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
         for (int t = pair; alive && t < p.total_tiles; t += npairs) {
             int b, mi, ni;
             tile_coords(p, t, b, mi, ni);
+            [[maybe_unused]] LinearAhead ahead;
             for (int kb0 = 0; kb0 < p.k_blocks; kb0 += p.chunk_blocks) {
                 bool ok = mbar_wait(tfull_bar(acc), acc_phase, abort_flag);
                 ok = __all_sync(0xffffffffu, ok);
@@ -1292,7 +1294,7 @@ umma_gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
             if (alive) {
                 if constexpr (kLinear)
                     finish_running<HC>(p, run, reinterpret_cast<float*>(bar_gen + 256 + uint32_t(warp - 2) * kStagedBlock),
-                                       mi * 256 + int(rank) * 128 + quad * 32, lane, ni * BN + half * HC);
+                                       mi * 256 + int(rank) * 128 + quad * 32, lane, ni * BN + half * HC, ahead);
                 else
                     store_running<HC>(p, run, b, mi * 256 + row_in_tile, ni * BN + half * HC);
             }

@@ -71,8 +71,9 @@ struct SplitF16Job {
     float* unscale;                 // [mn]: what a product has to be multiplied by for this operand
     long long mn, k, mn_s, k_s, ld; // source strides; rows of the parts (along K, or along mn) are ld elements apart
     int along_k, blocks;
+    int pairs;                      // values 2 i, 2 i + 1 of a row are neighbours and start on 8 bytes
 };
-constexpr int kSplitThreads = 1024, kSplitHeld = 32;
+constexpr int kSplitThreads = 1024;
 
 __device__ __forceinline__ float split_scale(float top, float* unscale) {
     const int e = top > 0.f ? int(__float_as_uint(top) >> 23) : 141;
@@ -80,93 +81,114 @@ __device__ __forceinline__ float split_scale(float top, float* unscale) {
     *unscale = __uint_as_float(uint32_t(254 - bits) << 23);
     return __uint_as_float(uint32_t(bits) << 23);
 }
-__device__ __forceinline__ void split_one(float x, float scale, __half* hi, __half* lo) {
-    const float v = x * scale;
-    const __half h = __float2half_rn(v);
-    const float hf = __half2float(h);
-    *hi = h;
-    *lo = __float2half_rn(isfinite(hf) ? v - hf : 0.f);
+// Both parts of a pair of values.  An infinity or a NaN stays in the high part.
+__device__ __forceinline__ void split_pair(float x, float y, float scale, __half2& hi, __half2& lo) {
+    x *= scale;
+    y *= scale;
+    hi = __floats2half2_rn(x, y);
+    const float hx = __low2float(hi), hy = __high2float(hi);
+    lo = __floats2half2_rn(fabsf(hx) < INFINITY ? x - hx : 0.f, fabsf(hy) < INFINITY ? y - hy : 0.f);
 }
-__device__ __forceinline__ float finite_abs(float x) { return isfinite(x) ? fabsf(x) : 0.f; }
+__device__ __forceinline__ float max_finite(float top, float x) {
+    const float a = fabsf(x);
+    return a < INFINITY ? fmaxf(top, a) : top;
+}
+
+// Row and column jobs alike: a thread's values come in pairs that are neighbours in memory (where the source allows it:
+// kPairs), and their parts leave as half2.
+template <bool kPairs>
+__device__ __forceinline__ float2 load_pair(const float* p, long long step, bool second) {
+    if constexpr (kPairs) return *reinterpret_cast<const float2*>(p);
+    return make_float2(p[0], second ? p[step] : 0.f);
+}
+__device__ __forceinline__ void store_parts(__half* hi, __half* lo, __half2 h, __half2 l) {   // rows of the parts are padded: a pair always fits
+    *reinterpret_cast<__half2*>(hi) = h;
+    *reinterpret_cast<__half2*>(lo) = l;
+}
+
+template <bool kPairs>
+__device__ __forceinline__ void split_rows(const SplitF16Job& j, int block, int warp, int lane) {   // a warp per row
+    const long long r = (long long)block * 32 + warp;
+    if (r >= j.mn) return;
+    const int k = int(j.k), step = int(j.k_s);
+    const float* src = j.src + r * j.mn_s;
+    __half* hi = j.hi + r * j.ld;
+    __half* lo = j.lo + r * j.ld;
+    float top = 0.f;
+#pragma unroll 8
+    for (int c = 2 * lane; c < k; c += 64) {
+        const float2 v = load_pair<kPairs>(src + (long long)c * step, step, c + 1 < k);
+        top = max_finite(max_finite(top, v.x), v.y);
+    }
+    top = warp_max_nan(top);
+    float unscale;
+    const float scale = split_scale(top, &unscale);
+    if (lane == 0) j.unscale[r] = unscale;
+#pragma unroll 8
+    for (int c = 2 * lane; c < k; c += 64) {   // from L1 / L2
+        const float2 v = load_pair<kPairs>(src + (long long)c * step, step, c + 1 < k);
+        __half2 h, l;
+        split_pair(v.x, v.y, scale, h, l);
+        store_parts(hi + c, lo + c, h, l);
+    }
+}
+
+// 32 columns per block: 16 lanes on their pairs, 64 rows of K at a time.
+template <bool kPairs>
+__device__ __forceinline__ void split_columns(const SplitF16Job& j, int block, int warp, int lane, float (*red)[33]) {
+    const int mn = int(j.mn), k = int(j.k);
+    const int at = 2 * (lane & 15), c = block * 32 + at, row0 = 2 * warp + (lane >> 4);
+    const bool in = c < mn, both = c + 1 < mn;
+    const float* src = j.src + (long long)(in ? c : 0) * j.mn_s + row0 * j.k_s;
+    const long long down = 64 * j.k_s;
+    float tx = 0.f, ty = 0.f;
+    if (in) {
+        const float* p = src;
+#pragma unroll 8
+        for (int r = row0; r < k; r += 64, p += down) {
+            const float2 v = load_pair<kPairs>(p, j.mn_s, both);
+            tx = max_finite(tx, v.x);
+            ty = max_finite(ty, v.y);
+        }
+    }
+    tx = fmaxf(tx, __shfl_xor_sync(0xffffffffu, tx, 16));
+    ty = fmaxf(ty, __shfl_xor_sync(0xffffffffu, ty, 16));
+    if (lane < 16) { red[warp][at] = tx; red[warp][at + 1] = ty; }
+    __syncthreads();
+    const float top = warp_max_nan(red[lane][warp]);   // warp w: the maximum of column w
+    __syncthreads();
+    if (lane == 0) red[0][warp] = top;
+    __syncthreads();
+    if (!in) return;
+    float ux, uy;
+    const float sx = split_scale(red[0][at], &ux), sy = split_scale(red[0][at + 1], &uy);
+    if (row0 == 0) {
+        j.unscale[c] = ux;
+        if (both) j.unscale[c + 1] = uy;
+    }
+    __half* hi = j.hi + row0 * j.ld + c;
+    __half* lo = j.lo + row0 * j.ld + c;
+    const long long out_down = 64 * j.ld;
+#pragma unroll 8
+    for (int r = row0; r < k; r += 64, src += down, hi += out_down, lo += out_down) {
+        const float2 v = load_pair<kPairs>(src, j.mn_s, both);
+        __half2 h, l;
+        split_pair(v.x * sx, v.y * sy, 1.f, h, l);
+        store_parts(hi, lo, h, l);
+    }
+}
 
 __global__ void __launch_bounds__(kSplitThreads) split_f16_kernel(const SplitF16Job ja, const SplitF16Job jb) {
     __shared__ float red[32][33];
     const bool second = int(blockIdx.x) >= ja.blocks;
-    const SplitF16Job& j = second ? jb : ja;
+    const SplitF16Job j = second ? jb : ja;
     const int block = int(blockIdx.x) - (second ? ja.blocks : 0), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (j.along_k) {   // a warp per row
-        const long long r = (long long)block * 32 + warp;
-        if (r >= j.mn) return;
-        const float* src = j.src + r * j.mn_s;
-        __half* hi = j.hi + r * j.ld;
-        __half* lo = j.lo + r * j.ld;
-        float held[kSplitHeld], top = 0.f;
-        const bool fits = j.k <= 32 * kSplitHeld;
-        if (fits) {
-#pragma unroll
-            for (int i = 0; i < kSplitHeld; ++i) {
-                const long long c = lane + 32 * i;
-                held[i] = c < j.k ? src[c * j.k_s] : 0.f;
-            }
-#pragma unroll
-            for (int i = 0; i < kSplitHeld; ++i) top = fmaxf(top, finite_abs(held[i]));
-        } else {
-#pragma unroll 8
-            for (long long c = lane; c < j.k; c += 32) top = fmaxf(top, finite_abs(src[c * j.k_s]));
-        }
-        top = warp_max_nan(top);
-        float unscale;
-        const float scale = split_scale(top, &unscale);
-        if (lane == 0) j.unscale[r] = unscale;
-        if (fits) {
-#pragma unroll
-            for (int i = 0; i < kSplitHeld; ++i) {
-                const long long c = lane + 32 * i;
-                if (c < j.k) split_one(held[i], scale, hi + c, lo + c);
-            }
-        } else {
-#pragma unroll 8
-            for (long long c = lane; c < j.k; c += 32) split_one(src[c * j.k_s], scale, hi + c, lo + c);
-        }
-        return;
-    }
-    // lanes on 32 neighbouring columns, every 32nd K row per warp
-    const long long c = (long long)block * 32 + lane;
-    const bool in = c < j.mn;
-    const float* src = j.src + (in ? c : 0) * j.mn_s;
-    float held[kSplitHeld], top = 0.f;
-    const bool fits = j.k <= 32 * kSplitHeld;
-    if (fits) {
-#pragma unroll
-        for (int i = 0; i < kSplitHeld; ++i) {
-            const long long r = warp + 32 * i;
-            held[i] = in && r < j.k ? src[r * j.k_s] : 0.f;
-        }
-#pragma unroll
-        for (int i = 0; i < kSplitHeld; ++i) top = fmaxf(top, finite_abs(held[i]));
-    } else if (in) {
-#pragma unroll 8
-        for (long long r = warp; r < j.k; r += 32) top = fmaxf(top, finite_abs(src[r * j.k_s]));
-    }
-    red[warp][lane] = top;
-    __syncthreads();
-    top = warp_max_nan(red[lane][warp]);   // warp w: the maximum of column w
-    __syncthreads();
-    if (lane == 0) red[0][warp] = top;
-    __syncthreads();
-    float unscale;
-    const float scale = split_scale(red[0][lane], &unscale);
-    if (!in) return;
-    if (warp == 0) j.unscale[c] = unscale;
-    if (fits) {
-#pragma unroll
-        for (int i = 0; i < kSplitHeld; ++i) {
-            const long long r = warp + 32 * i;
-            if (r < j.k) split_one(held[i], scale, j.hi + r * j.ld + c, j.lo + r * j.ld + c);
-        }
+    if (j.along_k) {
+        if (j.pairs) split_rows<true>(j, block, warp, lane);
+        else split_rows<false>(j, block, warp, lane);
     } else {
-#pragma unroll 8
-        for (long long r = warp; r < j.k; r += 32) split_one(src[r * j.k_s], scale, j.hi + r * j.ld + c, j.lo + r * j.ld + c);
+        if (j.pairs) split_columns<true>(j, block, warp, lane, red);
+        else split_columns<false>(j, block, warp, lane, red);
     }
 }
 
@@ -324,7 +346,9 @@ int f16x3_product(const Operand& a, const Operand& b, LinearParams l, cudaStream
         if (int rc = scratch_acquire(&unscale, 4 * size_t(o.mn), stream)) return rc;
         lo[i] = static_cast<char*>(hi) + bytes;
         jobs[i] = SplitF16Job{static_cast<const float*>(o.p), static_cast<__half*>(hi), static_cast<__half*>(lo[i]), static_cast<float*>(unscale),
-                              o.mn, o.k, o.mn_s, o.k_s, ld, along_k ? 1 : 0, int((o.mn + 31) / 32)};
+                              o.mn, o.k, o.mn_s, o.k_s, ld, along_k ? 1 : 0, int((o.mn + 31) / 32),
+                              (along_k ? o.k_s == 1 && o.mn_s % 2 == 0 && o.k % 2 == 0 : o.mn_s == 1 && o.k_s % 2 == 0 && o.mn % 2 == 0) &&
+                                      reinterpret_cast<uintptr_t>(o.p) % 8 == 0 ? 1 : 0};
         o.p = hi;
         o.mn_s = along_k ? ld : 1;
         o.k_s = along_k ? 1 : ld;

@@ -54,53 +54,87 @@ struct Quant {
     }
 };
 
-// G threads (a power of two, 32 or more) hold one row in registers, P vectors of V elements each; a block of
-// max(G, 256) threads takes blockDim / G rows at a time.  One pass over memory: load, reduce, scale, store.
-template <class T, int V, int P, int kOut>
-__global__ void __launch_bounds__(1024) norm_rows_kernel(const RowArgs a, int G) {
+// Rows that do not start on 16 bytes, but do so alike in every tensor of the call (contiguous tensors of an odd width):
+// element e of a row sits in 16-byte granule (e + lead) / V, lead being what the row's start is past a 16-byte boundary.
+// Whole granules move as vectors, the cut first and last one element by element; what they hold besides is 0.
+template <class T, int V>
+__device__ __forceinline__ Pack<T, V> load_granule(const T* row, int e0, int cols) {
+    if (e0 >= 0 && e0 + V <= cols) return *reinterpret_cast<const Pack<T, V>*>(row + e0);
+    Pack<T, V> o;
+#pragma unroll
+    for (int i = 0; i < V; ++i) o.e[i] = unsigned(e0 + i) < unsigned(cols) ? row[e0 + i] : T(0.f);
+    return o;
+}
+template <class T, int V>
+__device__ __forceinline__ void store_granule(T* row, int e0, int cols, const Pack<T, V>& v) {
+    if (e0 >= 0 && e0 + V <= cols) {
+        *reinterpret_cast<Pack<T, V>*>(row + e0) = v;
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+        if (unsigned(e0 + i) < unsigned(cols)) row[e0 + i] = v.e[i];
+}
+template <class T>
+__device__ __forceinline__ int row_lead(const T* row) { return int((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T)); }
+
+// G threads (whole warps) hold one row in registers, P vectors of V elements each; a block takes blockDim / G rows at a
+// time.  One pass over memory: load, reduce, scale, store.
+// kCut: rows laid out as above; the weight, whose start is not cut, is then read element by element (from L1).
+template <class T, int V, int P, int kOut, bool kCut, int kThreads>
+__global__ void __launch_bounds__(kThreads, kThreads == 512 && P * V <= 16 ? 2 : 1) norm_rows_kernel(const RowArgs a, int G) {
     __shared__ float s_sum[2][32], s_top[2][32];
     const int groups = blockDim.x / G, group = threadIdx.x / G, t = threadIdx.x - group * G;
     const int warps = G >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, first_warp = group * warps;
-    const int nv = a.cols / V;
-    const Pack<T, V>* w = static_cast<const Pack<T, V>*>(a.w);
+    const T* w = static_cast<const T*>(a.w);
     int flip = 0;
     for (long long base = (long long)blockIdx.x * groups; base < a.rows; base += (long long)gridDim.x * groups, flip ^= 1) {
         const long long row = base + group;
         const bool live = row < a.rows;
-        const Pack<T, V>* x = reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(a.x) + (live ? row : 0) * a.x_rs);
-        const Pack<T, V>* r = reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(a.r) + (live && a.r ? row : 0) * a.r_rs);
+        const T* x = static_cast<const T*>(a.x) + (live ? row : 0) * a.x_rs;
+        const T* r = static_cast<const T*>(a.r) + (live && a.r ? row : 0) * a.r_rs;
+        const int lead = kCut ? row_lead(x) : 0;
+        const int nv = live ? (lead + a.cols + V - 1) / V : 0;
         float f[P * V];
         Pack<T, V> px[P], pr[P];
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-            const int c = t + p * G;
-            if (live && c < nv) {
-                px[p] = x[c];
-                if (a.r) pr[p] = r[c];
+            const int c = t + p * G, e0 = c * V - lead;
+            if (c < nv) {
+                px[p] = kCut ? load_granule<T, V>(x, e0, a.cols) : *reinterpret_cast<const Pack<T, V>*>(x + e0);
+                if (a.r) pr[p] = kCut ? load_granule<T, V>(r, e0, a.cols) : *reinterpret_cast<const Pack<T, V>*>(r + e0);
             }
         }
         float sum = 0.f, top = 0.f;
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-            const int c = t + p * G;
-            const bool in = live && c < nv;
+            const int c = t + p * G, e0 = c * V - lead;
+            if (c >= nv) continue;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                float v = in ? px[p].up(i) : 0.f;
-                if (a.r && in) v = __fadd_rn(v, pr[p].up(i));
+                float v = px[p].up(i);
+                if (a.r) v = __fadd_rn(v, pr[p].up(i));
                 f[p * V + i] = v;
-                if (a.w) sum += v * v;
+                sum = fmaf(v, v, sum);
             }
-            if (a.h && in) {
+            if (a.h) {
                 Pack<T, V> o;
                 o.put(f + p * V);
-                reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.h) + row * a.cols)[c] = o;
+                T* h = static_cast<T*>(a.h) + row * a.cols;
+                if constexpr (kCut) store_granule<T, V>(h, e0, a.cols, o);
+                else *reinterpret_cast<Pack<T, V>*>(h + e0) = o;
             }
-            if (kOut == kInt8 && in) {
-                if (a.w) {
-                    const Pack<T, V> pw = w[c];
+            if (kOut == kInt8) {
+                if (w) {
+                    if constexpr (kCut) {
 #pragma unroll
-                    for (int i = 0; i < V; ++i) f[p * V + i] = __fmul_rn(f[p * V + i], pw.up(i));
+                        for (int i = 0; i < V; ++i)
+                            f[p * V + i] = unsigned(e0 + i) < unsigned(a.cols) ? __fmul_rn(f[p * V + i], RowType<T>::up(w[e0 + i])) : 0.f;
+                    } else {
+                        const Pack<T, V> pw = *reinterpret_cast<const Pack<T, V>*>(w + e0);
+#pragma unroll
+                        for (int i = 0; i < V; ++i) f[p * V + i] = __fmul_rn(f[p * V + i], pw.up(i));
+                    }
                 }
 #pragma unroll
                 for (int i = 0; i < V; ++i) top = max_nan(top, fabsf(f[p * V + i]));
@@ -121,34 +155,42 @@ __global__ void __launch_bounds__(1024) norm_rows_kernel(const RowArgs a, int G)
                 top = warp_max_nan(top);
             }
         }
-        const float rstd = a.w ? __frsqrt_rn(sum / float(a.cols) + a.eps) : 1.f;
-        if (!live) continue;
-        if (kOut == kInt8) {
-            const Quant quant(top);
+        const float rstd = w ? __frsqrt_rn(sum / float(a.cols) + a.eps) : 1.f;
+        const Quant quant(top);
 #pragma unroll
-            for (int p = 0; p < P; ++p) {
-                const int c = t + p * G;
-                if (c >= nv) continue;
+        for (int p = 0; p < P; ++p) {
+            const int c = t + p * G, e0 = c * V - lead;
+            if (c >= nv) continue;
+            if (kOut == kInt8) {
                 Pack<int8_t, V> o;
                 quant.put(o, f + p * V);
-                reinterpret_cast<Pack<int8_t, V>*>(static_cast<int8_t*>(a.y) + row * a.cols)[c] = o;
-            }
-            if (t == 0) a.stat[row] = __fdiv_rn(__fmul_rn(top, rstd), 127.f);
-        } else {
+                int8_t* q = static_cast<int8_t*>(a.y) + row * a.cols;
+                if constexpr (kCut) {
 #pragma unroll
-            for (int p = 0; p < P; ++p) {
-                const int c = t + p * G;
-                if (c >= nv) continue;
-                const Pack<T, V> pw = w[c];
+                    for (int i = 0; i < V; ++i)
+                        if (unsigned(e0 + i) < unsigned(a.cols)) q[e0 + i] = o.e[i];
+                } else {
+                    *reinterpret_cast<Pack<int8_t, V>*>(q + e0) = o;
+                }
+            } else {
+                T* y = static_cast<T*>(a.y) + row * a.cols;
                 Pack<T, V> o;
                 float v[V];
+                if constexpr (kCut) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) v[i] = f[p * V + i] * rstd * pw.up(i);
-                o.put(v);
-                reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.y) + row * a.cols)[c] = o;
+                    for (int i = 0; i < V; ++i) v[i] = unsigned(e0 + i) < unsigned(a.cols) ? f[p * V + i] * rstd * RowType<T>::up(w[e0 + i]) : 0.f;
+                    o.put(v);
+                    store_granule<T, V>(y, e0, a.cols, o);
+                } else {
+                    const Pack<T, V> pw = *reinterpret_cast<const Pack<T, V>*>(w + e0);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) v[i] = f[p * V + i] * rstd * pw.up(i);
+                    o.put(v);
+                    *reinterpret_cast<Pack<T, V>*>(y + e0) = o;
+                }
             }
-            if (a.stat && t == 0) a.stat[row] = rstd;
         }
+        if (live && t == 0 && a.stat) a.stat[row] = kOut == kInt8 ? __fdiv_rn(__fmul_rn(top, rstd), 127.f) : rstd;
     }
 }
 
@@ -371,46 +413,58 @@ struct BackArgs {
 };
 
 // The same layout; each thread keeps the sums of gy xhat of its columns in registers over all rows its block takes.
-template <class T, int V, int P>
-__global__ void __launch_bounds__(1024) norm_backward_kernel(const BackArgs a, int G) {
+// kCut: a thread's columns are the same for all rows of one lead, so a block takes rows of one lead only: rows first,
+// first + step, ... with a step that is a multiple of `period`, the number of rows after which the leads repeat.
+template <class T, int V, int P, bool kCut, int kThreads>
+__global__ void __launch_bounds__(kThreads) norm_backward_kernel(const BackArgs a, int G, int period) {
     extern __shared__ float s_gw[];      // [groups - 1][cols] while the groups of a block are joined
     __shared__ float s_dot[2][32];
     const int groups = blockDim.x / G, group = threadIdx.x / G, t = threadIdx.x - group * G;
     const int warps = G >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, first_warp = group * warps;
-    const int nv = a.cols / V;
-    const Pack<T, V>* w = static_cast<const Pack<T, V>*>(a.w);
+    const T* w = static_cast<const T*>(a.w);
+    // block b takes the rows of class b mod period: class + period (b / period * groups + group), ...
+    const long long first = blockIdx.x % period + (long long)period * ((long long)(blockIdx.x / period) * groups);
+    const long long step = (long long)gridDim.x * groups;   // gridDim is a multiple of the period
+    const int lead = kCut ? row_lead(static_cast<const T*>(a.h) + min(first, a.rows - 1) * a.h_rs) : 0;
+    const int nv = (lead + a.cols + V - 1) / V;
     float gw[P * V];
+    Pack<T, V> pw[P];
 #pragma unroll
-    for (int i = 0; i < P * V; ++i) gw[i] = 0.f;
+    for (int p = 0; p < P; ++p) {
+        const int c = t + p * G, e0 = c * V - lead;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            gw[p * V + i] = 0.f;
+            pw[p].e[i] = c < nv && unsigned(e0 + i) < unsigned(a.cols) ? w[e0 + i] : T(0.f);
+        }
+    }
     int flip = 0;
-    for (long long base = (long long)blockIdx.x * groups; base < a.rows; base += (long long)gridDim.x * groups, flip ^= 1) {
-        const long long row = base + group;
+    for (long long base = first; base < a.rows; base += step, flip ^= 1) {
+        const long long row = base + (long long)period * group;
         const bool live = row < a.rows;
-        const Pack<T, V>* h = reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(a.h) + (live ? row : 0) * a.h_rs);
-        const Pack<T, V>* gy = reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(a.gy) + (live ? row : 0) * a.gy_rs);
-        const Pack<T, V>* gh = reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(a.gh) + (live && a.gh ? row : 0) * a.gh_rs);
+        const T* h = static_cast<const T*>(a.h) + (live ? row : 0) * a.h_rs;
+        const T* gy = static_cast<const T*>(a.gy) + (live ? row : 0) * a.gy_rs;
+        const T* gh = static_cast<const T*>(a.gh) + (live && a.gh ? row : 0) * a.gh_rs;
         const float rstd = live ? a.rstd[row] : 0.f;
         Pack<T, V> ph[P], pg[P], pr[P];
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-            const int c = t + p * G;
+            const int c = t + p * G, e0 = c * V - lead;
             if (live && c < nv) {
-                ph[p] = h[c];
-                pg[p] = gy[c];
-                if (a.gh) pr[p] = gh[c];
+                ph[p] = kCut ? load_granule<T, V>(h, e0, a.cols) : *reinterpret_cast<const Pack<T, V>*>(h + e0);
+                pg[p] = kCut ? load_granule<T, V>(gy, e0, a.cols) : *reinterpret_cast<const Pack<T, V>*>(gy + e0);
+                if (a.gh) pr[p] = kCut ? load_granule<T, V>(gh, e0, a.cols) : *reinterpret_cast<const Pack<T, V>*>(gh + e0);
             }
         }
         float dot = 0.f;
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-            const int c = t + p * G;
-            if (!live || c >= nv) continue;
-            const Pack<T, V> pw = w[c];
+            if (!live || t + p * G >= nv) continue;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float gx = pg[p].up(i) * (ph[p].up(i) * rstd);
-                gw[p * V + i] += gx;
-                dot += gx * pw.up(i);
+                const float g = pg[p].up(i) * ph[p].up(i);      // the row's rstd joins the sums below
+                gw[p * V + i] = fmaf(g, rstd, gw[p * V + i]);
+                dot = fmaf(g, pw[p].up(i), dot);
             }
         }
         dot = warp_sum(dot);
@@ -420,20 +474,22 @@ __global__ void __launch_bounds__(1024) norm_backward_kernel(const BackArgs a, i
             dot = warp_sum(lane < warps ? s_dot[flip][first_warp + lane] : 0.f);
         }
         if (!live) continue;
-        dot /= float(a.cols);
+        const float c0 = rstd * (rstd * dot) / float(a.cols);
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-            const int c = t + p * G;
+            const int c = t + p * G, e0 = c * V - lead;
             if (c >= nv) continue;
-            const Pack<T, V> pw = w[c];
             Pack<T, V> o;
+            float v[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                float v = rstd * (pg[p].up(i) * pw.up(i) - ph[p].up(i) * rstd * dot);
-                if (a.gh) v += pr[p].up(i);
-                o.set(i, v);
+                const float d = fmaf(-ph[p].up(i), c0, pg[p].up(i) * pw[p].up(i));
+                v[i] = a.gh ? fmaf(rstd, d, pr[p].up(i)) : rstd * d;
             }
-            reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.gx) + row * a.cols)[c] = o;
+            o.put(v);
+            T* gx = static_cast<T*>(a.gx) + row * a.cols;
+            if constexpr (kCut) store_granule<T, V>(gx, e0, a.cols, o);
+            else *reinterpret_cast<Pack<T, V>*>(gx + e0) = o;
         }
     }
     if (!a.partial) return;
@@ -442,23 +498,23 @@ __global__ void __launch_bounds__(1024) norm_backward_kernel(const BackArgs a, i
     if (group > 0) {
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-            const int c = t + p * G;
-            if (c < nv)
+            const int e0 = (t + p * G) * V - lead;
 #pragma unroll
-                for (int i = 0; i < V; ++i) s_gw[(group - 1) * a.cols + c * V + i] = gw[p * V + i];
+            for (int i = 0; i < V; ++i)
+                if (unsigned(e0 + i) < unsigned(a.cols)) s_gw[(group - 1) * a.cols + e0 + i] = gw[p * V + i];
         }
     }
     __syncthreads();
     if (group == 0) {
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-            const int c = t + p * G;
-            if (c >= nv) continue;
+            const int e0 = (t + p * G) * V - lead;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
+                if (unsigned(e0 + i) >= unsigned(a.cols)) continue;
                 float v = gw[p * V + i];
-                for (int g = 1; g < groups; ++g) v += s_gw[(g - 1) * a.cols + c * V + i];
-                a.partial[(long long)blockIdx.x * a.cols + c * V + i] = v;
+                for (int g = 1; g < groups; ++g) v += s_gw[(g - 1) * a.cols + e0 + i];
+                a.partial[(long long)blockIdx.x * a.cols + e0 + i] = v;
             }
         }
     }
@@ -625,16 +681,52 @@ __global__ void __launch_bounds__(512) sum_partials_kernel(const float* __restri
 
 bool aligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
 
-// How a row is laid over threads: V elements per vector (16 bytes where every row starts on 16 bytes, else one), P
-// vectors per thread, G threads per row.  G = 0: too long for registers.
-struct RowPlan { int v, p, g; };
-RowPlan plan_row(int cols, int vec, bool vec_ok) {
-    RowPlan r{vec_ok ? vec : 1, 0, 0};
-    const int nv = cols / r.v;
-    const int most = vec_ok ? 4 : 16;
-    for (int p = vec_ok ? 1 : 4; p <= most; p *= 2)
-        for (int g = 32; g <= (vec_ok || p == most ? 1024 : 256); g *= 2)
-            if ((long long)p * g >= nv) return RowPlan{r.v, p, g};
+// How rows meet 16-byte boundaries: every row of every tensor starts on one, or all tensors' rows start alike past one (see
+// load_granule; period: the rows after which that repeats), or neither.
+enum Layout : int { kAligned, kCutAlike, kScattered };
+struct RowLayout {
+    Layout kind = kAligned;
+    int period = 1;
+    long long lead = -1, step = -1;
+    void add(const void* p, long long row_bytes) {   // one tensor of the call
+        if (!p) return;
+        const long long l = reinterpret_cast<uintptr_t>(p) % 16, s = row_bytes % 16;
+        if (lead < 0) { lead = l; step = s; }
+        else if (l != lead || s != step) kind = kScattered;
+    }
+    void finish(int es) {
+        if (kind == kScattered || lead < 0) return;
+        if (lead == 0 && step == 0) return;
+        if (lead % es || step % es) { kind = kScattered; return; }
+        kind = kCutAlike;
+        while (step * period % 16) period *= 2;
+    }
+};
+
+// How a row is laid over threads: V elements per vector (16 bytes, or one where rows are scattered), P vectors per thread,
+// G threads per row, `threads` per block.  Few vectors per thread as long as 512 threads hold the row; a row that needs
+// more than 128 threads has a block of its own, of just the warps it needs (4095 BFloat16 on 1024 threads left half of
+// them idle: 314 us for 16384 rows), shorter ones share blocks of 256.  g = 0: too long for registers.
+struct RowPlan { int v, p, g, threads; };
+RowPlan plan_row(int cols, int vec, Layout layout) {
+    RowPlan r{layout == kScattered ? 1 : vec, 0, 0, 0};
+    const int nv = cols / r.v + (layout == kCutAlike ? 2 : 0);   // two cut granules at most
+    const int least = layout == kScattered ? 4 : 1, most = layout == kScattered ? 16 : 4;
+    for (int limit : {512, 1024}) {
+        const int last = limit == 512 ? most / 2 : most;   // the most vectors per thread only where 1024 threads need them
+        for (r.p = limit == 512 ? least : most / 2; r.p <= last; r.p *= 2) {
+            const int need = (nv + r.p - 1) / r.p;
+            if (need > limit) continue;
+            if (need > 128) {
+                r.g = r.threads = (need + 31) / 32 * 32;
+            } else {
+                for (r.g = 32; r.g < need; r.g *= 2) {}
+                r.threads = 256;
+            }
+            return r;
+        }
+    }
+    r.g = 0;
     return r;
 }
 
@@ -684,9 +776,9 @@ int launch_ring(const RowArgs& a, const RingPlan& r, cudaStream_t stream) {
 }
 
 template <class T, int kOut>
-int launch_rows(const RowArgs& a, bool vec_ok, cudaStream_t stream) {
+int launch_rows(const RowArgs& a, Layout layout, cudaStream_t stream) {
     constexpr int kVec = 16 / sizeof(T);
-    if (vec_ok && (a.h || !a.r)) {
+    if (layout == kAligned && (a.h || !a.r)) {
         const RingPlan r = plan_forward(a.cols, kVec, int(sizeof(T)), a.r ? 2 : 1);
         // each group has several rows to stream
         if (r.stages >= 2 && a.rows >= 4ll * sm_count() * (r.threads / r.g)) {
@@ -700,24 +792,31 @@ int launch_rows(const RowArgs& a, bool vec_ok, cudaStream_t stream) {
             return launch_ring<T, 4, kOut, false>(a, r, stream);
         }
     }
-    const RowPlan pl = plan_row(a.cols, kVec, vec_ok);
+    const RowPlan pl = plan_row(a.cols, kVec, layout);
     const int sms = sm_count();
     if (pl.g == 0) {
         const int grid = int(std::min<long long>(a.rows, 2ll * sms));
         norm_long_rows_kernel<T, kOut><<<grid, 1024, 0, stream>>>(a);
     } else {
-        const int threads = std::max(pl.g, 256), groups = threads / pl.g;
+        const int threads = pl.threads, groups = threads / pl.g;
         const long long want = (a.rows + groups - 1) / groups;
         const int grid = int(std::min<long long>(want, (long long)sms * 16));
-#define NTB200_ROWS(VV, PP) norm_rows_kernel<T, VV, PP, kOut><<<grid, threads, 0, stream>>>(a, pl.g)
-        if (pl.v > 1) {
-            if (pl.p == 1) NTB200_ROWS(kVec, 1);
-            else if (pl.p == 2) NTB200_ROWS(kVec, 2);
-            else NTB200_ROWS(kVec, 4);
+#define NTB200_ROWS(VV, PP, CUT, TT) norm_rows_kernel<T, VV, PP, kOut, CUT, TT><<<grid, threads, 0, stream>>>(a, pl.g)
+        if (layout == kAligned) {
+            if (threads > 512 && pl.p == 2) NTB200_ROWS(kVec, 2, false, 1024);
+            else if (threads > 512) NTB200_ROWS(kVec, 4, false, 1024);
+            else if (pl.p == 1) NTB200_ROWS(kVec, 1, false, 512);
+            else NTB200_ROWS(kVec, 2, false, 512);
+        } else if (layout == kCutAlike) {
+            if (threads > 512 && pl.p == 2) NTB200_ROWS(kVec, 2, true, 1024);
+            else if (threads > 512) NTB200_ROWS(kVec, 4, true, 1024);
+            else if (pl.p == 1) NTB200_ROWS(kVec, 1, true, 512);
+            else NTB200_ROWS(kVec, 2, true, 512);
         } else {
-            if (pl.p == 4) NTB200_ROWS(1, 4);
-            else if (pl.p == 8) NTB200_ROWS(1, 8);
-            else NTB200_ROWS(1, 16);
+            if (threads > 512 && pl.p == 8) NTB200_ROWS(1, 8, false, 1024);
+            else if (threads > 512) NTB200_ROWS(1, 16, false, 1024);
+            else if (pl.p == 4) NTB200_ROWS(1, 4, false, 512);
+            else NTB200_ROWS(1, 8, false, 512);
         }
 #undef NTB200_ROWS
     }
@@ -730,7 +829,7 @@ constexpr int64_t kMaxCols = int64_t(1) << 30;
 
 // Slabs of the weight gradient's partial sums, and so the grid of the backward kernel: depends on sizes alone, so that
 // the workspace can be sized before the call.
-int backward_slabs(int64_t rows) { return int(std::max<int64_t>(1, std::min<int64_t>(rows, 4 * 148))); }
+int backward_slabs(int64_t rows) { return int(std::max<int64_t>(1, std::min<int64_t>(rows, 2 * 148))); }
 
 template <class T, int P, bool kStream, int kThreads>
 int launch_backward_ring(const BackArgs& a, const RingPlan& r, int grid, cudaStream_t stream) {
@@ -743,11 +842,11 @@ int launch_backward_ring(const BackArgs& a, const RingPlan& r, int grid, cudaStr
 }
 
 template <class T>
-int launch_backward(const BackArgs& a, void* grad_weight, bool vec_ok, cudaStream_t stream) {
+int launch_backward(const BackArgs& a, void* grad_weight, const RowLayout& layout, cudaStream_t stream) {
     constexpr int kVec = 16 / sizeof(T);
-    const RowPlan pl = plan_row(a.cols, kVec, vec_ok);
+    const RowPlan pl = plan_row(a.cols, kVec, layout.kind);
     int slabs = backward_slabs(a.rows);
-    const RingPlan r = vec_ok ? plan_backward(a.cols, kVec, int(sizeof(T)), a.gh ? 3 : 2) : RingPlan{};
+    const RingPlan r = layout.kind == kAligned ? plan_backward(a.cols, kVec, int(sizeof(T)), a.gh ? 3 : 2) : RingPlan{};
     if (r.stages >= 2 && a.rows >= 4ll * sm_count() * (r.threads / r.g)) {
         slabs = std::min(slabs, sm_count());
         int rc;
@@ -766,19 +865,29 @@ int launch_backward(const BackArgs& a, void* grad_weight, bool vec_ok, cudaStrea
         norm_backward_long_kernel<T><<<int(std::min<long long>(a.rows, 2ll * sm_count())), 1024, 0, stream>>>(a);
         count_launch();
     } else {
-        const int threads = std::max(pl.g, 256), groups = threads / pl.g;
-        slabs = int(std::min<long long>(slabs, (a.rows + groups - 1) / groups));
-        // at most 7 groups of 1024 columns: 28 KB
+        const int threads = pl.threads, groups = threads / pl.g;
+        const int period = layout.kind == kCutAlike ? layout.period : 1;
+        // two blocks per SM; a whole number of blocks for every class of rows (a class without rows leaves sums of zero)
+        slabs = int(std::min<long long>(std::min(slabs, 2 * sm_count()), (a.rows + groups - 1) / groups));
+        slabs = (slabs + period - 1) / period * period;
+        // at most 7 groups of 512 columns
         const size_t smem = a.partial ? size_t(groups - 1) * a.cols * sizeof(float) : 0;
-#define NTB200_BACK(VV, PP) norm_backward_kernel<T, VV, PP><<<slabs, threads, smem, stream>>>(a, pl.g)
-        if (pl.v > 1) {
-            if (pl.p == 1) NTB200_BACK(kVec, 1);
-            else if (pl.p == 2) NTB200_BACK(kVec, 2);
-            else NTB200_BACK(kVec, 4);
+#define NTB200_BACK(VV, PP, CUT, TT) norm_backward_kernel<T, VV, PP, CUT, TT><<<slabs, threads, smem, stream>>>(a, pl.g, period)
+        if (layout.kind == kAligned) {
+            if (threads > 512 && pl.p == 2) NTB200_BACK(kVec, 2, false, 1024);
+            else if (threads > 512) NTB200_BACK(kVec, 4, false, 1024);
+            else if (pl.p == 1) NTB200_BACK(kVec, 1, false, 512);
+            else NTB200_BACK(kVec, 2, false, 512);
+        } else if (layout.kind == kCutAlike) {
+            if (threads > 512 && pl.p == 2) NTB200_BACK(kVec, 2, true, 1024);
+            else if (threads > 512) NTB200_BACK(kVec, 4, true, 1024);
+            else if (pl.p == 1) NTB200_BACK(kVec, 1, true, 512);
+            else NTB200_BACK(kVec, 2, true, 512);
         } else {
-            if (pl.p == 4) NTB200_BACK(1, 4);
-            else if (pl.p == 8) NTB200_BACK(1, 8);
-            else NTB200_BACK(1, 16);
+            if (threads > 512 && pl.p == 8) NTB200_BACK(1, 8, false, 1024);
+            else if (threads > 512) NTB200_BACK(1, 16, false, 1024);
+            else if (pl.p == 4) NTB200_BACK(1, 4, false, 512);
+            else NTB200_BACK(1, 8, false, 512);
         }
 #undef NTB200_BACK
         count_launch();
@@ -822,12 +931,18 @@ static int norm_forward(const char* what, int dtype, const void* x, int64_t x_rs
     if ((rows > 1 && x_rs < cols) || (r && rows > 1 && r_rs < cols))
         return fail(NTB200_ERR_INVALID_ARG, "%s: a row stride is shorter than a row", what);
     const int es = int(dtype_size(dtype));
-    const bool vec_ok = cols * es % 16 == 0 && x_rs * es % 16 == 0 && (!r || r_rs * es % 16 == 0) && aligned(x, 16) && aligned(r, 16) &&
-                        aligned(w, 16) && aligned(y, int8 ? size_t(16 / es) : 16) && aligned(h, 16);
+    RowLayout layout;
+    layout.add(x, x_rs * es);
+    layout.add(r, r_rs * es);
+    if (!int8) layout.add(y, cols * es);
+    layout.add(h, cols * es);
+    layout.finish(es);
+    // Int8 rows start where `cols` bytes end: vectors of them need whole vectors of x, and the weight its own boundary
+    if (layout.kind == kAligned && ((cols * es) % 16 != 0 || !aligned(w, 16) || (int8 && !aligned(y, size_t(16 / es))))) layout.kind = kScattered;
     const RowArgs a{x, x_rs, r, r_rs, w, y, h, stat, rows, int(cols), float(eps)};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (int8) { NTB200_ROW_SWITCH(dtype, (launch_rows<T, kInt8>(a, vec_ok, s))) }
-    NTB200_ROW_SWITCH(dtype, (launch_rows<T, kSame>(a, vec_ok, s)))
+    if (int8) { NTB200_ROW_SWITCH(dtype, (launch_rows<T, kInt8>(a, layout.kind, s))) }
+    NTB200_ROW_SWITCH(dtype, (launch_rows<T, kSame>(a, layout.kind, s)))
 }
 
 int ntb200_rms_norm(int dtype, const void* x, int64_t x_row_stride, const void* residual, int64_t residual_row_stride, const void* weight,
@@ -849,7 +964,7 @@ int ntb200_quantize_rows(int dtype, const void* x, int64_t x_row_stride, int8_t*
 
 size_t ntb200_rms_norm_backward_workspace_bytes(int64_t rows, int64_t cols) {
     if (rows <= 0 || cols <= 0) return 0;
-    return size_t(backward_slabs(rows)) * size_t(cols) * sizeof(float);
+    return size_t(backward_slabs(rows) + 8) * size_t(cols) * sizeof(float);   // whole classes of up to 8 rows
 }
 
 int ntb200_rms_norm_backward(int dtype, const void* h, int64_t h_row_stride, const void* weight, const float* rstd, const void* grad_y,
@@ -867,12 +982,16 @@ int ntb200_rms_norm_backward(int dtype, const void* h, int64_t h_row_stride, con
     if (rows > 1 && (h_row_stride < cols || grad_y_row_stride < cols || (grad_h && grad_h_row_stride < cols)))
         return fail(NTB200_ERR_INVALID_ARG, "%s: a row stride is shorter than a row", what);
     const int es = int(dtype_size(dtype));
-    const bool vec_ok = cols * es % 16 == 0 && h_row_stride * es % 16 == 0 && grad_y_row_stride * es % 16 == 0 &&
-                        (!grad_h || grad_h_row_stride * es % 16 == 0) && aligned(h, 16) && aligned(weight, 16) && aligned(grad_y, 16) &&
-                        aligned(grad_h, 16) && aligned(grad_x, 16);
+    RowLayout layout;
+    layout.add(h, h_row_stride * es);
+    layout.add(grad_y, grad_y_row_stride * es);
+    layout.add(grad_h, grad_h_row_stride * es);
+    layout.add(grad_x, cols * es);
+    layout.finish(es);
+    if (layout.kind == kAligned && ((cols * es) % 16 != 0 || !aligned(weight, 16))) layout.kind = kScattered;
     const BackArgs a{h, h_row_stride, weight, rstd, grad_y, grad_y_row_stride, grad_h, grad_h_row_stride, grad_x,
                      grad_weight ? static_cast<float*>(workspace) : nullptr, rows, int(cols)};
-    NTB200_ROW_SWITCH(dtype, (launch_backward<T>(a, grad_weight, vec_ok, s)))
+    NTB200_ROW_SWITCH(dtype, (launch_backward<T>(a, grad_weight, layout, s)))
 }
 
 }  // extern "C"

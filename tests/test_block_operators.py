@@ -168,7 +168,8 @@ def test_distill_refusals():
 # ---- norm -----------------------------------------------------------------------------------------------------------
 
 NORM_SHAPES = [(1, 1), (3, 5), (7, 64), (130, 200), (1, 4096), (37, 1999), (5, 8192), (3, 16384), (2, 16383), (2, 40000), (300, 33), (1000, 256),
-               (9700, 64), (9600, 264), (2600, 2048), (1300, 4104), (700, 8192), (650, 16384)]     # enough rows to stream
+               (9700, 64), (9600, 264), (2600, 2048), (1300, 4104), (700, 8192), (650, 16384),     # enough rows to stream
+               (1000, 1001), (260, 14054)]
 
 
 def norm_inputs(rows, n, dtype, residual, seed=0):
