@@ -1511,8 +1511,8 @@ __device__ __forceinline__ void cluster_reduce_store(const UmmaParams& p, const 
     }
 }
 
-// The same for ntb200_linear_act: everything after the product.  `ready` spills this CTA's partial tile and meets the
-// cluster; the scales, bias and residual of a thread's first items are requested before it, while the main loop runs.
+// The same for ntb200_linear_act: everything after the product.  `ready` runs the main loop, spills this CTA's partial tile
+// and meets the cluster; the scales, bias and residual of a thread's first items are requested before it.
 // kInt: the slices' s32 sums stay whole numbers until they are one.
 template <int S, int U, bool kInt, class Ready>
 __device__ __forceinline__ void cluster_reduce_linear(const UmmaParams& p, const ClusterKParams& cp, uint32_t tile_base, int rows, int m_base, int n_base,
@@ -1637,6 +1637,7 @@ umma_gemm_cluster_k_kernel(const __grid_constant__ CUtensorMap tma_a, const __gr
     tcgen05_fence_after();
     const uint32_t tmem_base = *tmem_slot;
 
+    auto roles = [&]() {
     if (warp == 0) {
         // ------------------------------------------------------------------ TMA producer: this slice's K blocks
         if (lane == 0) {
@@ -1685,7 +1686,9 @@ umma_gemm_cluster_k_kernel(const __grid_constant__ CUtensorMap tma_a, const __gr
             if (ok) umma_commit<1>(tfull_bar);   // this slice's partial tile is complete
         }
     }
-    __syncwarp();   // the other lanes of the producer and MMA warps wait here until their lane 0 is through its loop
+    };
+    if constexpr (!kLinear) roles();
+    if constexpr (!kLinear) __syncwarp();   // the other lanes of the producer and MMA warps wait here until their lane 0 is through its loop
     auto spill = [&]() {
         // ------------------------------------------------------------------ spill the partial tile to shared memory
         // A warp reads the 32 tensor-memory lanes of quadrant warp % 4, so rows 0-63 have two warps each (0 and 4, 1
@@ -1721,6 +1724,8 @@ umma_gemm_cluster_k_kernel(const __grid_constant__ CUtensorMap tma_a, const __gr
         const int cols_mine = BN / cp.slices;
         const int rows = min(kBM, p.m - m0);
         auto ready = [&]() {
+            roles();
+            __syncwarp();
             spill();
             __syncwarp();
             cluster_sync_all();

@@ -36,20 +36,29 @@ struct Quant {
         up = top < 0x1p-100f ? 0x1p100f : 1.f;
         inv = top > 0.f ? __fdiv_rn(127.f, __fmul_rn(top, up)) : (top == 0.f ? 0.f : top);
     }
-    // V values, packed.  127 (1 + 2^-22) at most reaches the conversion, so it needs no clamp; x * 1 is exact.
+    // V values, packed.  Adding 1.5 2^23 rounds to a whole number (ties to even, as rint does) and leaves it in the low byte
+    // of the sum's bits: no conversion, which the hardware does at a quarter of the rate.  127 (1 + 2^-22) at most comes out
+    // of the product, so no value needs a clamp; a NaN's quotient is replaced, its low byte could be anything.
     template <int V>
     __device__ __forceinline__ void put(Pack<int8_t, V>& o, const float* u) const {
-        int q[V];
+        uint32_t q[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) q[i] = __float2int_rn(__fmul_rn(up == 1.f ? u[i] : __fmul_rn(u[i], up), inv));
+        for (int i = 0; i < V; ++i) q[i] = __float_as_uint(__fadd_rn(__fmul_rn(u[i], inv), 12582912.f));
+        if (up != 1.f) {   // a tiny row
+#pragma unroll
+            for (int i = 0; i < V; ++i) q[i] = __float_as_uint(__fadd_rn(__fmul_rn(__fmul_rn(u[i], up), inv), 12582912.f));
+        }
+        if (!(fabsf(inv) < INFINITY)) {   // a NaN in the row
+#pragma unroll
+            for (int i = 0; i < V; ++i) q[i] = 0;
+        }
         if constexpr (V % 4 == 0) {
             uint32_t* w = reinterpret_cast<uint32_t*>(o.e);
 #pragma unroll
-            for (int i = 0; i < V; i += 4)
-                w[i / 4] = __byte_perm(__byte_perm(uint32_t(q[i]), uint32_t(q[i + 1]), 0x0040), __byte_perm(uint32_t(q[i + 2]), uint32_t(q[i + 3]), 0x0040), 0x5410);
+            for (int i = 0; i < V; i += 4) w[i / 4] = __byte_perm(__byte_perm(q[i], q[i + 1], 0x0040), __byte_perm(q[i + 2], q[i + 3], 0x0040), 0x5410);
         } else {
 #pragma unroll
-            for (int i = 0; i < V; ++i) o.e[i] = int8_t(q[i]);
+            for (int i = 0; i < V; ++i) o.e[i] = int8_t(q[i] & 0xffu);
         }
     }
 };
