@@ -551,7 +551,8 @@ def distill64(s, t, i, T, rw):
 @pytest.mark.gpu
 @pytest.mark.parametrize("T", [0.5, 1.0, 3.0])
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
-@pytest.mark.parametrize("rows,vocab,top", [(1, 1, 1), (3, 5, 2), (9, 1000, 8), (5, 4099, 64), (4, 32000, 33), (2, 131072, 128), (3, 300001, 5), (2, 2048, 1024), (700, 257, 4)])
+@pytest.mark.parametrize("rows,vocab,top", [(1, 1, 1), (3, 5, 2), (9, 1000, 8), (5, 4099, 64), (4, 32000, 33), (2, 131072, 128), (3, 300001, 5), (2, 2048, 1024), (700, 257, 4),
+                                            (1300, 1001, 40), (460, 40007, 7), (450, 131072, 64), (450, 98304, 128)])     # enough rows to stream
 def test_distill(rows, vocab, top, dtype, T):
     from neurotensor_b200 import api
     gen = generator(rows + vocab + top)
