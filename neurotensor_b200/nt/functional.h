@@ -413,5 +413,124 @@ inline void to_numpy(const Tensor& t, const std::string& path) {
     f.write(reinterpret_cast<const char*>(v.data()), std::streamsize(v.size() * 4));
 }
 
+// ---- the residual feed-forward block (no counterpart in the reference) ----------------------------------------------
+enum class Activation : int { None = NTB200_ACT_NONE, ReLU = NTB200_ACT_RELU, GELU = NTB200_ACT_GELU, GELUTanh = NTB200_ACT_GELU_TANH, SiLU = NTB200_ACT_SILU };
+
+namespace detail {
+// Rows of the last dim, contiguous.
+inline Tensor rows_of(const Tensor& t, const char* what) {
+    utils::throw_exception(!t.is_null() && t.device() == DeviceType::CUDA, what, ": expected tensors on DeviceType::CUDA");
+    utils::throw_exception(t.dims() >= 1 && t.shape()[-1] >= 1, what, ": expected rows of at least one element but got ", t.shape());
+    return t.contiguous();
+}
+inline SizeRef row_shape(const Tensor& t) {
+    std::vector<int64_t> s(t.shape().Vec().begin(), t.shape().Vec().end() - 1);
+    if (s.empty()) s.push_back(1);
+    return SizeRef(s);
+}
+inline void check_norm(const Tensor& x, const Tensor& weight, const Tensor* residual, const char* what) {
+    utils::throw_exception(weight.dims() == 1 && weight.shape()[0] == x.shape()[-1] && weight.dtype() == x.dtype(), what, ": expected a weight of ",
+                           x.shape()[-1], " values of ", dtype_name(x.dtype()), " but got ", weight.shape());
+    utils::throw_exception(!residual || (residual->shape() == x.shape() && residual->dtype() == x.dtype()), what,
+                           ": expected the residual to be shaped and typed like the input");
+}
+}  // namespace detail
+
+struct RMSNormResult {
+    Tensor y, h, rstd;   // h: x + residual (x itself without one); rstd: one Float32 per row, for the backward pass
+};
+// h = x + residual, y = h * rstd * weight, rstd = (mean(h^2) + eps)^-1/2 over the last dim.
+inline RMSNormResult rms_norm(const Tensor& x, const Tensor& weight, double eps = 1e-6, const Tensor& residual = Tensor()) {
+    Tensor xc = detail::rows_of(x, "rms_norm"), wc = weight.contiguous();
+    const Tensor* r = residual.is_null() ? nullptr : &residual;
+    detail::check_norm(xc, wc, r, "rms_norm");
+    Tensor rc = r ? r->contiguous() : Tensor();
+    const int64_t cols = xc.shape()[-1], rows = xc.numel() / cols;
+    RMSNormResult o{Tensor(xc.shape(), xc.dtype(), DeviceType::CUDA), r ? Tensor(xc.shape(), xc.dtype(), DeviceType::CUDA) : xc,
+                    Tensor(detail::row_shape(xc), DType::Float32, DeviceType::CUDA)};
+    utils::check(ntb200_rms_norm(dtype_code(xc.dtype()), xc.data_ptr(), cols, r ? rc.data_ptr() : nullptr, cols, wc.data_ptr(), o.y.data_ptr(),
+                                 r ? o.h.data_ptr() : nullptr, static_cast<float*>(o.rstd.data_ptr()), rows, cols, eps, nullptr));
+    return o;
+}
+
+struct Int8Rows {
+    Tensor q, scale, h;   // Int8 rows, one Float32 scale per row; h as in RMSNormResult (null for quantize_rows)
+};
+inline Int8Rows rms_norm_int8(const Tensor& x, const Tensor& weight, double eps = 1e-6, const Tensor& residual = Tensor()) {
+    Tensor xc = detail::rows_of(x, "rms_norm_int8"), wc = weight.contiguous();
+    const Tensor* r = residual.is_null() ? nullptr : &residual;
+    detail::check_norm(xc, wc, r, "rms_norm_int8");
+    Tensor rc = r ? r->contiguous() : Tensor();
+    const int64_t cols = xc.shape()[-1], rows = xc.numel() / cols;
+    Int8Rows o{Tensor(xc.shape(), DType::int8, DeviceType::CUDA), Tensor(detail::row_shape(xc), DType::Float32, DeviceType::CUDA),
+               r ? Tensor(xc.shape(), xc.dtype(), DeviceType::CUDA) : xc};
+    utils::check(ntb200_rms_norm_int8(dtype_code(xc.dtype()), xc.data_ptr(), cols, r ? rc.data_ptr() : nullptr, cols, wc.data_ptr(),
+                                      static_cast<int8_t*>(o.q.data_ptr()), static_cast<float*>(o.scale.data_ptr()), r ? o.h.data_ptr() : nullptr, rows,
+                                      cols, eps, nullptr));
+    return o;
+}
+inline Int8Rows quantize_rows(const Tensor& x) {
+    Tensor xc = detail::rows_of(x, "quantize_rows");
+    const int64_t cols = xc.shape()[-1], rows = xc.numel() / cols;
+    Int8Rows o{Tensor(xc.shape(), DType::int8, DeviceType::CUDA), Tensor(detail::row_shape(xc), DType::Float32, DeviceType::CUDA), Tensor()};
+    utils::check(ntb200_quantize_rows(dtype_code(xc.dtype()), xc.data_ptr(), cols, static_cast<int8_t*>(o.q.data_ptr()),
+                                      static_cast<float*>(o.scale.data_ptr()), rows, cols, nullptr));
+    return o;
+}
+
+namespace detail {
+inline Tensor run_linear(const char* what, const Tensor& x, const Tensor& weight, const Tensor& bias, Activation act, const Tensor& residual,
+                         bool trans_weight, DType out, const Tensor* x_scale, const Tensor* w_scale, Tensor* pre) {
+    Tensor xc = rows_of(x, what);
+    utils::throw_exception(weight.dims() == 2 && weight.device() == DeviceType::CUDA && weight.dtype() == x.dtype(), what,
+                           ": expected a 2-D weight of ", dtype_name(x.dtype()), " but got ", weight.shape());
+    const int64_t k = trans_weight ? weight.shape()[1] : weight.shape()[0], n = trans_weight ? weight.shape()[0] : weight.shape()[1];
+    utils::throw_exception(xc.shape()[-1] == k, what, ": expected the weight to take ", xc.shape()[-1], " inputs when it took ", k);
+    std::vector<int64_t> s(xc.shape().Vec());
+    s.back() = n;
+    const SizeRef shape(s);
+    Tensor bc = bias.is_null() ? Tensor() : bias.contiguous(), rc = residual.is_null() ? Tensor() : residual.contiguous();
+    utils::throw_exception(bc.is_null() || (bc.numel() == n && bc.dtype() == out), what, ": expected a bias of ", n, " values of ", dtype_name(out));
+    utils::throw_exception(rc.is_null() || (rc.shape() == shape && rc.dtype() == out), what, ": expected a residual of shape ", shape);
+    Tensor y(shape, out, DeviceType::CUDA);
+    ntb200_linear_desc d{};
+    d.dtype = dtype_code(x.dtype()); d.out_dtype = dtype_code(out); d.activation = int(act);
+    d.m = xc.numel() / k; d.n = n; d.k = k;
+    d.x = xc.data_ptr(); d.x_row_stride = k; d.x_col_stride = 1;
+    d.w = weight.data_ptr();
+    d.w_row_stride = trans_weight ? weight.stride(1) : weight.stride(0); d.w_col_stride = trans_weight ? weight.stride(0) : weight.stride(1);
+    d.x_scale = x_scale ? static_cast<const float*>(x_scale->data_ptr()) : nullptr;
+    d.w_scale = w_scale ? static_cast<const float*>(w_scale->data_ptr()) : nullptr;
+    d.bias = bc.is_null() ? nullptr : bc.data_ptr();
+    d.residual = rc.is_null() ? nullptr : rc.data_ptr(); d.residual_row_stride = n;
+    d.y = y.data_ptr(); d.y_row_stride = n;
+    if (pre) {
+        *pre = Tensor(shape, out, DeviceType::CUDA);
+        d.pre = pre->data_ptr(); d.pre_row_stride = n;
+    }
+    const size_t need = ntb200_linear_act_workspace_bytes(&d);
+    Tensor ws({int64_t(need ? need : 1)}, DType::uint8, DeviceType::CUDA);
+    utils::check(ntb200_linear_act(&d, ws.data_ptr(), need, nullptr));
+    return y;
+}
+}  // namespace detail
+
+// act(x . weight + bias) + residual in one GEMM; weight [in, out], or [out, in] with trans_weight.  `pre` receives
+// x . weight + bias, which the backward pass takes.
+inline Tensor linear_act(const Tensor& x, const Tensor& weight, const Tensor& bias = Tensor(), Activation act = Activation::None,
+                         const Tensor& residual = Tensor(), bool trans_weight = false, Tensor* pre = nullptr) {
+    return detail::run_linear("linear_act", x, weight, bias, act, residual, trans_weight, x.dtype(), nullptr, nullptr, pre);
+}
+// The same for Int8 rows and an Int8 weight with a Float32 scale per row and per output; the result has `out`'s type.
+inline Tensor linear_int8(const Tensor& q, const Tensor& scale, const Tensor& weight, const Tensor& weight_scale, const Tensor& bias = Tensor(),
+                          Activation act = Activation::None, const Tensor& residual = Tensor(), bool trans_weight = false, DType out = DType::BFloat16) {
+    utils::throw_exception(q.dtype() == DType::int8 && scale.dtype() == DType::Float32 && weight_scale.dtype() == DType::Float32,
+                           "linear_int8: expected Int8 operands with Float32 scales");
+    Tensor sc = scale.contiguous(), wc = weight_scale.contiguous();
+    utils::throw_exception(sc.numel() * q.shape()[-1] == q.numel() && weight.dims() == 2 && wc.numel() == weight.shape()[trans_weight ? 0 : 1],
+                           "linear_int8: expected a scale for each row and each output");
+    return detail::run_linear("linear_int8", q, weight, bias, act, residual, trans_weight, out, &sc, &wc, nullptr);
+}
+
 }  // namespace functional
 }  // namespace nt

@@ -216,6 +216,71 @@ inline TensorGrad conv2d(const TensorGrad& image, const TensorGrad& kernel, cons
         });
 }
 
+// Norm with the residual's addition, tracked: y's gradient runs through h, whose own gradient (the residual stream's) adds
+// to it and then goes to x and to the residual alike.
+struct RMSNormGrad {
+    TensorGrad y, h;
+};
+inline RMSNormGrad rms_norm(const TensorGrad& x, const TensorGrad& weight, double eps = 1e-6, const TensorGrad& residual = TensorGrad()) {
+    const bool add = !residual.is_null();
+    Tensor W = weight.detach();
+    RMSNormResult f = rms_norm(x.detach(), W, eps, residual.detach());
+    TensorGrad h = !add ? x
+                        : TensorGrad::make_result(f.h, {x.node(), residual.node()}, [](const Tensor& g, GraphParents& parents) {
+                              for (auto& p : parents)
+                                  if (p->requires_grad) p->accumulate_gradient(g);
+                          });
+    Tensor H = f.h, rstd = f.rstd;
+    TensorGrad y = TensorGrad::make_result(f.y, {h.node(), weight.node()}, [H, W, rstd](const Tensor& g_in, GraphParents& parents) {
+        Tensor g = g_in.contiguous(), w = W.contiguous();
+        const int64_t cols = H.shape()[-1], rows = H.numel() / cols;
+        Tensor gx(H.shape(), H.dtype(), DeviceType::CUDA), gw;
+        Tensor ws({int64_t(ntb200_rms_norm_backward_workspace_bytes(rows, cols) + 1)}, DType::uint8, DeviceType::CUDA);
+        if (parents[1]->requires_grad) gw = Tensor(W.shape(), W.dtype(), DeviceType::CUDA);
+        utils::check(ntb200_rms_norm_backward(dtype_code(H.dtype()), H.data_ptr(), cols, w.data_ptr(), static_cast<const float*>(rstd.data_ptr()),
+                                              g.data_ptr(), cols, nullptr, 0, gx.data_ptr(), gw.is_null() ? nullptr : gw.data_ptr(), ws.data_ptr(), rows,
+                                              cols, nullptr));
+        if (parents[0]->requires_grad) parents[0]->accumulate_gradient(gx);
+        if (parents[1]->requires_grad) parents[1]->accumulate_gradient(gw);
+    });
+    return RMSNormGrad{y, h};
+}
+
+// act(input . weight + bias) + residual, tracked.
+inline TensorGrad linear_act(const TensorGrad& input, const TensorGrad& weight, const TensorGrad& bias, Activation act,
+                             const TensorGrad& residual = TensorGrad(), bool trans_weight = false) {
+    Tensor X = input.detach().contiguous(), W = weight.detach(), pre;
+    const bool keep = act != Activation::None;
+    Tensor out = linear_act(X, W, bias.detach(), act, residual.detach(), trans_weight, keep ? &pre : nullptr);
+    return TensorGrad::make_result(out, {input.node(), weight.node(), bias.node(), residual.node()},
+        [X, W, pre, act, trans_weight](const Tensor& g_in, GraphParents& parents) {
+            Tensor g = g_in.contiguous();
+            const int64_t k = X.shape()[-1], n = g.shape()[-1];
+            Tensor dX, dW, dB;
+            if (parents[0]->requires_grad) dX = Tensor(X.shape(), X.dtype(), DeviceType::CUDA);
+            if (parents[1]->requires_grad) dW = Tensor(W.shape(), X.dtype(), DeviceType::CUDA);
+            if (parents[2]->requires_grad) dB = Tensor({n}, X.dtype(), DeviceType::CUDA);
+            ntb200_linear_backward_desc d{};
+            d.dtype = dtype_code(X.dtype()); d.activation = int(act); d.grad_w_transposed = trans_weight ? 1 : 0;
+            d.m = X.numel() / k; d.n = n; d.k = k;
+            d.x = X.data_ptr(); d.x_row_stride = k; d.x_col_stride = 1;
+            d.w = W.data_ptr();
+            d.w_row_stride = trans_weight ? W.stride(1) : W.stride(0); d.w_col_stride = trans_weight ? W.stride(0) : W.stride(1);
+            d.pre = pre.is_null() ? nullptr : pre.data_ptr(); d.pre_row_stride = n;
+            d.grad_out = g.data_ptr(); d.grad_out_row_stride = n;
+            d.grad_x = dX.is_null() ? nullptr : dX.data_ptr();
+            d.grad_w = dW.is_null() ? nullptr : dW.data_ptr();
+            d.grad_bias = dB.is_null() ? nullptr : dB.data_ptr();
+            const size_t need = ntb200_linear_act_backward_workspace_bytes(&d);
+            Tensor ws({int64_t(need ? need : 1)}, DType::uint8, DeviceType::CUDA);
+            utils::check(ntb200_linear_act_backward(&d, ws.data_ptr(), need, nullptr));
+            if (!dX.is_null()) parents[0]->accumulate_gradient(dX);
+            if (!dW.is_null()) parents[1]->accumulate_gradient(dW);
+            if (!dB.is_null()) parents[2]->accumulate_gradient(dB);
+            if (parents[3]->requires_grad) parents[3]->accumulate_gradient(g);
+        });
+}
+
 }  // namespace functional
 
 // Seeded normal initialisation on the host (the reference's randn is a softmax of random integers seeded from
@@ -244,7 +309,28 @@ class Linear {
         if (use_bias) Bias.detach().set_mutability(false);
     }
     TensorGrad forward(const TensorGrad& x) { return functional::linear(x, Weight, Bias); }
+    // act(x . Weight + Bias) + residual in one GEMM
+    TensorGrad forward(const TensorGrad& x, functional::Activation act, const TensorGrad& residual = TensorGrad()) {
+        return functional::linear_act(x, Weight, Bias, act, residual);
+    }
     TensorGrad operator()(const TensorGrad& x) { return forward(x); }
+};
+// Root-mean-square norm over the last dim, with the residual stream's addition: returns y and the new stream h.
+class RMSNorm {
+   public:
+    double eps;
+    TensorGrad Weight;
+    explicit RMSNorm(int64_t channels, DType dt = DType::Float32, double eps = 1e-6)
+        : eps(eps), Weight([&] {
+              std::vector<float> ones(size_t(channels), 1.f);
+              Tensor t = Tensor::from_host(ones.data(), {channels}, DType::Float32);
+              return dt == DType::Float32 ? t : t.to(dt);
+          }()) {
+        Weight.detach().set_mutability(false);
+    }
+    functional::RMSNormGrad forward(const TensorGrad& x, const TensorGrad& residual = TensorGrad()) {
+        return functional::rms_norm(x, Weight, eps, residual);
+    }
 };
 // Conv2D (nn/layers/Conv2D.cpp:11-44): Weight [out, in / groups, kh, kw], Bias [out, 1, 1]; forward is
 // conv2d(x, Weight, stride, padding, dilation, groups) + Bias, the bias being a separate elementwise step whose
@@ -366,6 +452,24 @@ inline ScalarGrad MSE(const TensorGrad& output, const Tensor& target) {
     Tensor loss_t({1}, DType::Float32, DeviceType::CUDA);
     utils::check(ntb200_mse(dtype_code(o.dtype()), oc.data_ptr(), tc.data_ptr(), dx.data_ptr(), static_cast<float*>(loss_t.data_ptr()),
                             o.numel(), nullptr));
+    float v = 0.f;
+    loss_t.to_host(&v);
+    return ScalarGrad(double(v), dx, output);
+}
+// Divergence from a teacher known by its top logits (values and int32 / int64 columns, [rows, top]); the mean over rows
+// unless row_weight ([rows], Float32) says otherwise.
+inline ScalarGrad DistillTopK(const TensorGrad& output, const Tensor& teacher, const Tensor& index, double temperature = 1.0,
+                              const Tensor& row_weight = Tensor()) {
+    Tensor o = functional::detail::rows_of(output.detach(), "DistillTopK"), t = teacher.contiguous(), i = index.contiguous();
+    const int64_t vocab = o.shape()[-1], rows = o.numel() / vocab, top = t.shape()[-1];
+    utils::throw_exception(t.shape() == i.shape() && t.numel() == rows * top, "DistillTopK: shapes ", o.shape(), ", ", t.shape(), " and ", i.shape(),
+                           " do not belong together");
+    Tensor rw = row_weight.is_null() ? Tensor() : row_weight.contiguous();
+    utils::throw_exception(rw.is_null() || (rw.numel() == rows && rw.dtype() == DType::Float32), "DistillTopK: expected a Float32 weight for each row");
+    Tensor dx(o.shape(), o.dtype(), DeviceType::CUDA), row_loss({rows}, DType::Float32, DeviceType::CUDA), loss_t({1}, DType::Float32, DeviceType::CUDA);
+    utils::check(ntb200_distill_topk(dtype_code(o.dtype()), o.data_ptr(), vocab, dtype_code(t.dtype()), t.data_ptr(), dtype_code(i.dtype()), i.data_ptr(),
+                                     rw.is_null() ? nullptr : static_cast<const float*>(rw.data_ptr()), dx.data_ptr(), vocab,
+                                     static_cast<float*>(row_loss.data_ptr()), static_cast<float*>(loss_t.data_ptr()), rows, vocab, top, temperature, nullptr));
     float v = 0.f;
     loss_t.to_host(&v);
     return ScalarGrad(double(v), dx, output);
