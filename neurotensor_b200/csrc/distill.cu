@@ -77,21 +77,22 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
 }
 
 // ---- one cluster per row: the row stays in shared memory ------------------------------------------------------------
-// The C blocks of a cluster hold one row, a piece each, fetched once by untiled bulk copies in four parts; maximum, sum and
+// The C blocks of a cluster hold one row, a piece each, fetched once by an untiled bulk copy; maximum, sum and
 // gradient then come from shared memory, and only (max, sum, teacher's share) of each piece crosses the cluster.  A block
 // that re-read its row from L2 instead took 623 us for 4096 x 131072 bf16 logits: the rows in flight (592 x 256 KB) do not
 // fit L2, so the second read went to memory again.  Pieces are at most 72 KB where C <= 8 allows it, so that three blocks
-// per SM overlap loading, arithmetic and storing.
+// per SM overlap loading, arithmetic and storing (36 KB: 562 us, 512 threads per block: 566 us; four barriers per copy to
+// start earlier: 488 against 477 us).
 // Rows need not start on 16 bytes: the piece's whole 16-byte granules are copied, the elements of a cut first or last
 // granule are loaded one by one, and what else lies in those two granules is set to -inf, which adds nothing.
-constexpr int kPieceThreads = 256, kParts = 4, kMaxCluster = 8;
+constexpr int kPieceThreads = 256, kMaxCluster = 8;
 
 // Behind the piece in dynamic shared memory: three arrays of `top` entries (the teacher's probabilities, the student's
 // logits at the same places, the columns within this piece, -1: not there or in another block's piece).
 struct PieceShared {
     float red[3][kPieceThreads / 32];
     float4 share[kMaxCluster];           // (max, sum, sum p (x - max), sum p) of every block's piece, by rank
-    unsigned long long bar[kParts];
+    unsigned long long bar;
     uint32_t abort_flag;
 };
 
@@ -157,8 +158,9 @@ __device__ __forceinline__ void st_cluster_f4(uint32_t local_addr, uint32_t cta_
         ::"r"(local_addr), "r"(cta_rank), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
 }
 
-template <class T>
-__global__ void __launch_bounds__(kPieceThreads, 3) distill_piece_kernel(const DistillArgs a, int C, int piece, bool same_align, unsigned int* status) {
+// kBlocks: blocks per SM that registers shall allow (shared memory allows three of 72 KB, five of 42 KB).
+template <class T, int kBlocks>
+__global__ void __launch_bounds__(kPieceThreads, kBlocks) distill_piece_kernel(const DistillArgs a, int C, int piece, bool same_align, unsigned int* status) {
     constexpr int V = 16 / sizeof(T);
     extern __shared__ __align__(128) uint8_t piece_mem[];
     __shared__ PieceShared sh;
@@ -193,17 +195,14 @@ __global__ void __launch_bounds__(kPieceThreads, 3) distill_piece_kernel(const D
         return;
     }
     T* mem = reinterpret_cast<T*>(piece_mem);
-    const int part = g1 > g0 ? (g1 - g0 + kParts - 1) / kParts : 0;   // granules per part
     if (tid == 0) {
         sh.abort_flag = 0;
-        for (int i = 0; i < kParts; ++i) mbar_init(smem_u32(&sh.bar[i]), 1);
+        mbar_init(smem_u32(&sh.bar), 1);
         fence_barrier_init();
         fence_proxy_async_smem();
-        for (int i = 0; i < kParts; ++i) {
-            const int b = g0 + i * part, e = min(g1, b + part);
-            if (b >= e) continue;
-            mbar_expect_tx(smem_u32(&sh.bar[i]), uint32_t(e - b) * 16u);
-            bulk_load(smem_u32(piece_mem) + uint32_t(b) * 16u, s + (b * V - lead), uint32_t(e - b) * 16u, smem_u32(&sh.bar[i]));
+        if (g1 > g0) {
+            mbar_expect_tx(smem_u32(&sh.bar), uint32_t(g1 - g0) * 16u);
+            bulk_load(smem_u32(piece_mem) + uint32_t(g0) * 16u, s + (g0 * V - lead), uint32_t(g1 - g0) * 16u, smem_u32(&sh.bar));
         }
     }
     if (tid < V && granules) {   // the cut granules
@@ -226,19 +225,12 @@ __global__ void __launch_bounds__(kPieceThreads, 3) distill_piece_kernel(const D
     }
     present = __syncthreads_or(present);
     if (C > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // this block runs: its shared memory may be written
-    bool landed = true;
-    auto wait_part = [&](int i) {
-        if (g0 + i * part < min(g1, g0 + (i + 1) * part)) landed = mbar_wait(smem_u32(&sh.bar[i]), 0, &sh.abort_flag) && landed;
-    };
     float m = -INFINITY;
     if (granules > g1 && granules - 1 >= g0 && tid < V) m = RowType<T>::up(mem[(granules - 1) * V + tid]);
     if (g0 == 1 && tid < V) m = fmaxf(m, RowType<T>::up(mem[tid]));
-    for (int i = 0; i < kParts; ++i) {
-        wait_part(i);
-        for (int v = g0 + i * part + tid; v < min(g1, g0 + (i + 1) * part); v += kPieceThreads) {
-            m = fmaxf(m, pack_max(reinterpret_cast<const Pack<T, V>*>(mem)[v]));
-        }
-    }
+    const bool landed = g1 <= g0 || mbar_wait(smem_u32(&sh.bar), 0, &sh.abort_flag);
+#pragma unroll 4
+    for (int v = g0 + tid; v < g1; v += kPieceThreads) m = fmaxf(m, pack_max(reinterpret_cast<const Pack<T, V>*>(mem)[v]));
     if (!landed && lane == 0) {
         sh.abort_flag = 1;
         atomicExch(status, 0x151u);
@@ -293,9 +285,7 @@ __global__ void __launch_bounds__(kPieceThreads, 3) distill_piece_kernel(const D
     }
     if (sh.abort_flag) {   // a copy did not land in time (the status word tells): it may still, so the block waits once more
         volatile uint32_t never = 0;
-        if (tid == 0)
-            for (int i = 0; i < kParts; ++i)
-                if (g0 + i * part < min(g1, g0 + (i + 1) * part)) (void)mbar_wait(smem_u32(&sh.bar[i]), 0, &never);
+        if (tid == 0 && g1 > g0) (void)mbar_wait(smem_u32(&sh.bar), 0, &never);
         __syncthreads();
         return;
     }
@@ -513,15 +503,8 @@ int launch_distill(const DistillArgs& a, bool vec_ok, float* loss, cudaStream_t 
         const uint32_t smem = uint32_t(piece) * uint32_t(sizeof(T)) + 32u + 12u * uint32_t(a.top);
         const bool same_align = a.grad && (reinterpret_cast<uintptr_t>(a.grad) - reinterpret_cast<uintptr_t>(a.s)) % 16 == 0 &&
                                 ((a.g_rs - a.s_rs) * (long long)sizeof(T)) % 16 == 0;
-        auto kernel = distill_piece_kernel<T>;
-        static std::atomic<bool> set[64];
-        int dev = 0;
-        (void)cudaGetDevice(&dev);
-        if (dev < 0 || dev >= 64) dev = 0;
-        if (!set[dev].load(std::memory_order_acquire)) {
-            NTB200_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 213 * 1024));
-            set[dev].store(true, std::memory_order_release);
-        }
+        auto kernel = smem <= 42 * 1024 ? distill_piece_kernel<T, 5> : distill_piece_kernel<T, 3>;
+        NTB200_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 213 * 1024));
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(unsigned(a.rows * C), 1, 1);
         cfg.blockDim = dim3(kPieceThreads, 1, 1);
