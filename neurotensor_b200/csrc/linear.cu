@@ -110,14 +110,15 @@ template <bool kPairs>
 __device__ __forceinline__ void split_rows(const SplitF16Job& j, int block, int warp, int lane) {   // a warp per row
     const long long r = (long long)block * 32 + warp;
     if (r >= j.mn) return;
-    const int k = int(j.k), step = int(j.k_s);
+    const int k = int(j.k);
+    const long long step = j.k_s;
     const float* src = j.src + r * j.mn_s;
     __half* hi = j.hi + r * j.ld;
     __half* lo = j.lo + r * j.ld;
     float top = 0.f;
 #pragma unroll 8
     for (int c = 2 * lane; c < k; c += 64) {
-        const float2 v = load_pair<kPairs>(src + (long long)c * step, step, c + 1 < k);
+        const float2 v = load_pair<kPairs>(src + c * step, step, c + 1 < k);
         top = max_finite(max_finite(top, v.x), v.y);
     }
     top = warp_max_nan(top);
@@ -126,7 +127,7 @@ __device__ __forceinline__ void split_rows(const SplitF16Job& j, int block, int 
     if (lane == 0) j.unscale[r] = unscale;
 #pragma unroll 8
     for (int c = 2 * lane; c < k; c += 64) {   // from L1 / L2
-        const float2 v = load_pair<kPairs>(src + (long long)c * step, step, c + 1 < k);
+        const float2 v = load_pair<kPairs>(src + c * step, step, c + 1 < k);
         __half2 h, l;
         split_pair(v.x, v.y, scale, h, l);
         store_parts(hi + c, lo + c, h, l);
@@ -269,9 +270,12 @@ struct Operand {
     const void* p;
     int64_t mn, k, mn_s, k_s;
 };
+// TMA can address it: one direction dense, the other in steps of 16 bytes that do not overlap (an expanded matrix repeats
+// one row with a step of 0).
 bool tma_ready(const Operand& o, int es) {
     if (!on16(o.p)) return false;
-    return ((o.k_s == 1 || o.k == 1) && (o.mn == 1 || o.mn_s * es % 16 == 0)) || ((o.mn_s == 1 || o.mn == 1) && (o.k == 1 || o.k_s * es % 16 == 0));
+    return ((o.k_s == 1 || o.k == 1) && (o.mn == 1 || (o.mn_s * es % 16 == 0 && o.mn_s >= o.k))) ||
+           ((o.mn_s == 1 || o.mn == 1) && (o.k == 1 || (o.k_s * es % 16 == 0 && o.k_s >= o.mn)));
 }
 // Bytes of the padded copy (0: none needed).
 size_t padded_bytes(const Operand& o, int es) {

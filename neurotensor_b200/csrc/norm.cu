@@ -939,6 +939,8 @@ static int norm_forward(const char* what, int dtype, const void* x, int64_t x_rs
     if (!(eps >= 0)) return fail(NTB200_ERR_INVALID_ARG, "%s: epsilon must not be negative", what);
     if ((rows > 1 && x_rs < cols) || (r && rows > 1 && r_rs < cols))
         return fail(NTB200_ERR_INVALID_ARG, "%s: a row stride is shorter than a row", what);
+    if (rows > 1 && h && ((h == x && x_rs != cols) || (h == r && r_rs != cols)))
+        return fail(NTB200_ERR_INVALID_ARG, "%s: h in the place of an input must have its row stride (h is contiguous)", what);
     const int es = int(dtype_size(dtype));
     RowLayout layout;
     layout.add(x, x_rs * es);
@@ -990,6 +992,9 @@ int ntb200_rms_norm_backward(int dtype, const void* h, int64_t h_row_stride, con
         return fail(NTB200_ERR_INVALID_ARG, "%s: null pointer", what);
     if (rows > 1 && (h_row_stride < cols || grad_y_row_stride < cols || (grad_h && grad_h_row_stride < cols)))
         return fail(NTB200_ERR_INVALID_ARG, "%s: a row stride is shorter than a row", what);
+    if (rows > 1 && ((grad_x == h && h_row_stride != cols) || (grad_x == grad_y && grad_y_row_stride != cols) ||
+                     (grad_h && grad_x == grad_h && grad_h_row_stride != cols)))
+        return fail(NTB200_ERR_INVALID_ARG, "%s: grad_x in the place of an input must have its row stride (grad_x is contiguous)", what);
     const int es = int(dtype_size(dtype));
     RowLayout layout;
     layout.add(h, h_row_stride * es);

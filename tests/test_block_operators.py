@@ -79,6 +79,9 @@ def test_norm_refusals():
                  lambda: L.ntb200_rms_norm(_lib.F32, one, 8, None, 0, one, one, None, None, 1, 8, float("nan"), None),
                  lambda: L.ntb200_rms_norm(_lib.F32, one, 7, None, 0, one, one, None, None, 2, 8, 1e-6, None),
                  lambda: L.ntb200_rms_norm(_lib.F32, one, 8, one, 7, one, one, None, None, 2, 8, 1e-6, None),
+                 lambda: L.ntb200_rms_norm(_lib.F32, one, 9, None, 0, one, ctypes.c_void_p(64), one, None, 2, 8, 1e-6, None),
+                 lambda: L.ntb200_rms_norm(_lib.F32, ctypes.c_void_p(32), 8, one, 9, one, ctypes.c_void_p(64), one, None, 2, 8, 1e-6, None),
+                 lambda: L.ntb200_rms_norm_backward(_lib.F32, ctypes.c_void_p(32), 8, one, one, one, 9, None, 0, one, None, None, 2, 8, None),
                  lambda: L.ntb200_rms_norm_int8(_lib.F32, one, 8, None, 0, one, one, None, None, 2, 8, 1e-6, None),
                  lambda: L.ntb200_rms_norm_backward(_lib.F32, one, 8, one, one, one, 8, None, 0, one, one, None, 2, 8, None),
                  lambda: L.ntb200_rms_norm_backward(_lib.F32, one, 8, one, one, one, 8, one, 7, one, None, None, 2, 8, None)):
@@ -512,6 +515,51 @@ def test_linear_layouts():
         gx, gw, gb = api.linear_act_backward(big[:0, 0, :96], w, torch.empty(0, 72, device="cuda", dtype=dtype),
                                              torch.empty(0, 72, device="cuda", dtype=dtype), "gelu")
         assert gx.shape == (0, 96) and not bool(gw.any()) and not bool(gb.any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_linear_unusual_weights(dtype):
+    """Weights that repeat one row, that skip elements, and that are windows of a larger matrix."""
+    from neurotensor_b200 import api
+    gen = generator(41)
+    big, x = randn(gen, 200, 300, scale=0.1, dtype=dtype), randn(gen, 70, 64, dtype=dtype)
+    for w in (big[0, :96].expand(64, 96), big[:64, 0:288:3], big[1:129:2, 3:99], big[:96, :64].t(), big[:192:3, 5]):
+        w = w if w.dim() == 2 else w[:, None].expand(64, 96)
+        want = api.linear_act(x, w.contiguous(), None, "relu", want_pre=True)
+        got = api.linear_act(x, w, None, "relu", want_pre=True)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        a, b = api.linear_act_backward(x, w, got[1], got[0], "relu"), api.linear_act_backward(x, w.contiguous(), got[1], got[0], "relu")
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once():
+    """The same operators on two streams and from two host threads, each with its own inputs."""
+    import threading
+    from neurotensor_b200 import api
+    args = [block_inputs(generator(s), BF16, rows=200) for s in (51, 52)]
+    want = [block_step(api, *a, "silu") for a in args]
+    torch.cuda.synchronize()
+    got, failed = [None, None], []
+
+    def work(k):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(10):
+                    got[k] = block_step(api, *args[k], "silu")
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:      # pragma: no cover
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    for k in (0, 1):
+        assert all(torch.equal(got[k][n], want[k][n]) for n in want[k])
 
 
 @pytest.mark.gpu
