@@ -19,6 +19,7 @@ namespace {
 
 constexpr int kMaxTop = 1024;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kModerate = 64.f;   // |m c| up to which an exponent's error is below 2^-18
 
 struct DistillArgs {
     const void* s; long long s_rs;
@@ -170,7 +171,7 @@ __global__ void __launch_bounds__(kPieceThreads, kBlocks) distill_piece_kernel(c
     const int tid = threadIdx.x, lane = tid & 31;
     const uint32_t rank = C > 1 ? cluster_cta_rank() : 0u;
     const long long row = blockIdx.x / C;
-    const float c = kLog2e / a.temp;
+    const float c = kLog2e / a.temp, inv_temp = 1.f / a.temp;
     const int first = int(rank) * piece, count = max(0, min(piece, a.vocab - first));
     const T* s = static_cast<const T*>(a.s) + row * a.s_rs + first;
     T* grad = a.grad ? static_cast<T*>(a.grad) + row * a.g_rs + first : nullptr;
@@ -237,23 +238,38 @@ __global__ void __launch_bounds__(kPieceThreads, kBlocks) distill_piece_kernel(c
     }
     piece_max2(tmax, m, sh);
     const float ref = m == -INFINITY ? 0.f : m, mc = ref * c;
+    // 16-bit logits take one multiply-add to the exponent, x c - m c, as long as the rounding of m c (2^-24 of it) stays far
+    // below the gradient's own; not so where all of a piece is masked by the type's lowest value
+    const bool moderate = sizeof(T) == 2 && fabsf(mc) <= kModerate;
     float sums[2] = {0.f, 0.f};          // the teacher's and the student's
     for (int j = tid; j < a.top; j += kPieceThreads) sums[0] += sh_p[j] == -INFINITY ? 0.f : exp2f((sh_p[j] - tmax) * c);
     float z0 = 0.f, z1 = 0.f;
+    if (moderate) {
 #pragma unroll 2
-    for (int v = tid; v < granules; v += kPieceThreads) {
-        const Pack<T, V> x = reinterpret_cast<const Pack<T, V>*>(mem)[v];
+        for (int v = tid; v < granules; v += kPieceThreads) {
+            const Pack<T, V> x = reinterpret_cast<const Pack<T, V>*>(mem)[v];
 #pragma unroll
-        for (int k = 0; k < V; k += 2) {
-            z0 += exp2_hw(sizeof(T) == 4 ? (x.up(k) - ref) * c : fmaf(x.up(k), c, -mc));
-            z1 += exp2_hw(sizeof(T) == 4 ? (x.up(k + 1) - ref) * c : fmaf(x.up(k + 1), c, -mc));
+            for (int k = 0; k < V; k += 2) {
+                z0 += exp2_hw(fmaf(x.up(k), c, -mc));
+                z1 += exp2_hw(fmaf(x.up(k + 1), c, -mc));
+            }
+        }
+    } else {
+#pragma unroll 2
+        for (int v = tid; v < granules; v += kPieceThreads) {
+            const Pack<T, V> x = reinterpret_cast<const Pack<T, V>*>(mem)[v];
+#pragma unroll
+            for (int k = 0; k < V; k += 2) {
+                z0 += exp2_hw((x.up(k) - ref) * c);
+                z1 += exp2_hw((x.up(k + 1) - ref) * c);
+            }
         }
     }
     sums[1] = z0 + z1;
     piece_sums(sums, sh);
     const float tsum = sums[0], z = sums[1];
     // probabilities
-    float parts[3] = {0.f, 0.f, 0.f};    // sum p log p, sum p and sum p (x - m) of this piece
+    float parts[3] = {0.f, 0.f, 0.f};    // sum p log2 p, and sum p and sum p (x - m) / T of this piece
     const float log2t = log2f(tsum);
     for (int j = tid; j < a.top; j += kPieceThreads) {
         const float t = sh_p[j];
@@ -268,7 +284,7 @@ __global__ void __launch_bounds__(kPieceThreads, kBlocks) distill_piece_kernel(c
             const float x = RowType<T>::up(mem[sh_at[j] + lead]);
             sh_x[j] = x;
             parts[1] += p;
-            parts[2] += p * ((x - ref) * c);
+            parts[2] += p * ((x - ref) * inv_temp);
         } else if (sh_at[j] >= 0) {
             sh_x[j] = RowType<T>::up(mem[sh_at[j] + lead]);
         }
@@ -293,9 +309,9 @@ __global__ void __launch_bounds__(kPieceThreads, kBlocks) distill_piece_kernel(c
     for (int i = 0; i < C; ++i) gm = fmaxf(gm, sh.share[i].x);
     for (int i = 0; i < C; ++i) {
         const float4 q = sh.share[i];
-        const float d = q.x == -INFINITY ? 0.f : (q.x - gm) * c;
-        gz += q.x == -INFINITY && gm != -INFINITY ? 0.f : q.y * exp2f(d);
-        cross += q.z + q.w * d;          // sum p (x - gm) c
+        const float d = q.x == -INFINITY ? 0.f : q.x - gm;
+        gz += q.x == -INFINITY && gm != -INFINITY ? 0.f : q.y * exp2f(d * c);
+        cross += q.w == 0.f ? q.z : q.z + q.w * (d * inv_temp);   // sum p (x - gm) / T; a piece far below may have an infinite d
     }
     if (gm == -INFINITY) gz = NAN;       // every column of the student masked out
     if (!present) {
@@ -303,13 +319,13 @@ __global__ void __launch_bounds__(kPieceThreads, kBlocks) distill_piece_kernel(c
         if (rank == 0 && tid == 0) a.row_loss[row] = 0.f;
         return;
     }
-    if (rank == 0 && tid == 0) a.row_loss[row] = a.temp * a.temp * (entropy - cross + log2f(gz)) / kLog2e;
+    if (rank == 0 && tid == 0) a.row_loss[row] = a.temp * a.temp * ((entropy + log2f(gz)) / kLog2e - cross);
     if (!grad) return;
     const float coef = weight * a.temp, scale = coef / gz;
     // q times its factor: for 16-bit gradients one multiply-add and one exponential, the factor inside the exponent
-    const bool fold = sizeof(T) == 2 && scale > 0.f;
-    const float off = fold ? fmaf(-gm, c, log2f(scale)) : -gm * c, mul = fold ? 1.f : scale;
-    auto value = [&](float x) { return (sizeof(T) == 4 ? exp2_hw((x - gm) * c) : exp2_hw(fmaf(x, c, off))) * mul; };
+    const bool fold = sizeof(T) == 2 && scale > 0.f && fabsf(gm) * c <= kModerate;
+    const float off = fold ? fmaf(-gm, c, log2f(scale)) : 0.f;
+    auto value = [&](float x) { return fold ? exp2_hw(fmaf(x, c, off)) : exp2_hw((x - gm) * c) * scale; };
     if (same_align && fold) {
         Pack<T, V>* gv = reinterpret_cast<Pack<T, V>*>(grad - lead);
 #pragma unroll 2
@@ -439,13 +455,13 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(const DistillArgs a) 
             if (sh.at[j] >= 0) {
                 const float lt = (sh.p[j] - tmax) * c;
                 p = exp2f(lt) / tsum;
-                if (p > 0.f) loss += p * ((lt - log2f(tsum)) - ((sh.x[j] - m) * c - log2z));
+                if (p > 0.f) loss += p * (((lt - log2f(tsum)) + log2z) / kLog2e - (sh.x[j] - m) / a.temp);
                 else if (!(p == 0.f)) loss = p;
             }
             sh.p[j] = p;
         }
         loss = block_sum<kThreads>(loss, sh.red_z);
-        if (tid == 0) a.row_loss[row] = a.temp * a.temp * loss / kLog2e;
+        if (tid == 0) a.row_loss[row] = a.temp * a.temp * loss;
         if (!grad) continue;
         const float coef = weight * a.temp, scale = coef / z;
         for (int v = tid; v < nv; v += kThreads) {
@@ -548,7 +564,8 @@ extern "C" int ntb200_distill_topk(int dtype, const void* logits, int64_t logits
         return fail(NTB200_ERR_UNSUPPORTED, "%s: the teacher's columns must be Int32 or Int64, got %s", what, dtype_name(index_dtype));
     if (rows < 0 || vocab <= 0 || vocab > (int64_t(1) << 30) || top <= 0) return fail(NTB200_ERR_INVALID_ARG, "%s: bad extent", what);
     if (top > kMaxTop) return fail(NTB200_ERR_INVALID_ARG, "%s: at most %d teacher entries per row, got %lld", what, kMaxTop, (long long)top);
-    if (!(temperature > 0) || !(temperature < 1e30)) return fail(NTB200_ERR_INVALID_ARG, "%s: the temperature must be positive and finite", what);
+    if (!(temperature >= 1e-30) || !(temperature <= 1e30))
+        return fail(NTB200_ERR_INVALID_ARG, "%s: the temperature must be positive and finite (1e-30 to 1e30)", what);
     if (!loss) return fail(NTB200_ERR_INVALID_ARG, "%s: null pointer", what);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (rows == 0) {
