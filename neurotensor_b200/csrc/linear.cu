@@ -412,6 +412,8 @@ int check_linear(const ntb200_linear_desc* d) {
     if (!int8 && (d->x_scale || d->w_scale)) return fail(NTB200_ERR_INVALID_ARG, "%s: scales belong to Int8 operands", what);
     if (d->pre && (d->pre == d->y || d->pre == d->residual))
         return fail(NTB200_ERR_INVALID_ARG, "%s: the pre-activation needs memory of its own", what);
+    if (d->y == d->x || d->y == d->w || (d->pre && (d->pre == d->x || d->pre == d->w)))
+        return fail(NTB200_ERR_INVALID_ARG, "%s: an output in an operand's place", what);
     if (d->residual && d->residual == d->y && d->residual_row_stride != d->y_row_stride)
         return fail(NTB200_ERR_INVALID_ARG, "%s: an output in the residual's place must have its row stride", what);
     return NTB200_OK;
@@ -435,6 +437,9 @@ int check_backward(const ntb200_linear_backward_desc* d) {
     if (d->m == 0) return NTB200_OK;
     if (!d->grad_out || (d->activation != NTB200_ACT_NONE && !d->pre) || (d->grad_x && !d->w) || (d->grad_w && !d->x))
         return fail(NTB200_ERR_INVALID_ARG, "%s: null pointer", what);
+    for (const void* out : {static_cast<const void*>(d->grad_x), static_cast<const void*>(d->grad_w), static_cast<const void*>(d->grad_bias)})
+        if (out && (out == d->grad_out || out == d->pre || out == d->x || out == d->w))
+            return fail(NTB200_ERR_INVALID_ARG, "%s: a gradient in an input's place", what);
     return NTB200_OK;
 }
 

@@ -144,20 +144,40 @@ __device__ __forceinline__ void lin_add32(const void* p, long long i, int dtype,
     }
 }
 
+// A product times its row's and its column's scale.  kWide (Float32 results, whose operands' scales span the type's whole
+// range): in an order whose steps neither overflow nor vanish unless the result does.
+template <bool kWide>
+__device__ __forceinline__ float scaled(float v, float rs, float cs) {
+    if constexpr (!kWide) return v * rs * cs;
+    const bool apart = (rs < 1.f) != (cs < 1.f);
+    return v * (apart ? rs * cs : rs) * (apart ? 1.f : cs);
+}
+
 // Scales and bias of 32 consecutive products of one row; wide: every column is there and the vectors start on 16 bytes.
 __device__ __forceinline__ void linear_scale_bias32(const LinearParams& l, int n, int col0, float rs, bool wide, float (&f)[32]) {
     if (l.col_scale) {
         if (wide) {
             const float4* cs = reinterpret_cast<const float4*>(l.col_scale + col0);
+            if (l.out_dtype == NTB200_F32) {
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
-                const float4 o = cs[q];
-                f[4 * q] *= rs * o.x; f[4 * q + 1] *= rs * o.y; f[4 * q + 2] *= rs * o.z; f[4 * q + 3] *= rs * o.w;
+                for (int q = 0; q < 8; ++q) {
+                    const float4 o = cs[q];
+                    f[4 * q] = scaled<true>(f[4 * q], rs, o.x); f[4 * q + 1] = scaled<true>(f[4 * q + 1], rs, o.y);
+                    f[4 * q + 2] = scaled<true>(f[4 * q + 2], rs, o.z); f[4 * q + 3] = scaled<true>(f[4 * q + 3], rs, o.w);
+                }
+            } else {
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    const float4 o = cs[q];
+                    f[4 * q] = scaled<false>(f[4 * q], rs, o.x); f[4 * q + 1] = scaled<false>(f[4 * q + 1], rs, o.y);
+                    f[4 * q + 2] = scaled<false>(f[4 * q + 2], rs, o.z); f[4 * q + 3] = scaled<false>(f[4 * q + 3], rs, o.w);
+                }
             }
         } else {
 #pragma unroll
             for (int j = 0; j < 32; ++j)
-                if (col0 + j < n) f[j] *= rs * l.col_scale[col0 + j];
+                if (col0 + j < n)
+                    f[j] = l.out_dtype == NTB200_F32 ? scaled<true>(f[j], rs, l.col_scale[col0 + j]) : scaled<false>(f[j], rs, l.col_scale[col0 + j]);
         }
     }
     if (l.bias) {
@@ -207,7 +227,7 @@ __device__ __forceinline__ void linear_finish4(const LinearParams& l, int n, int
     const long long y0 = (long long)row * l.y_rs + col, p0 = (long long)row * l.pre_rs + col;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        if (l.col_scale) f[j] *= a.rs * a.cs[j];
+        if (l.col_scale) f[j] = dt == NTB200_F32 ? scaled<true>(f[j], a.rs, a.cs[j]) : scaled<false>(f[j], a.rs, a.cs[j]);
         if (l.bias) f[j] += a.bias[j];
     }
     const float z[4] = {f[0], f[1], f[2], f[3]};
@@ -291,7 +311,7 @@ __device__ __forceinline__ void linear_finish_block(const LinearParams& l, int m
         for (int i = 0; i < 8; ++i) {
             const int r = first + r0 + i;
             f[i] = staged[(r0 + i) * 33 + lane];
-            if (l.row_scale) f[i] *= (row0 + r < m ? l.row_scale[row0 + r] : 0.f) * a.cs;
+            if (l.row_scale) f[i] = scaled<kDt == NTB200_F32>(f[i], row0 + r < m ? l.row_scale[row0 + r] : 0.f, a.cs);
             f[i] += a.bias;
             if (l.pre && in && row0 + r < m) lin_set<kDt>(pre, f[i]);
             pre += pre_step;

@@ -107,7 +107,7 @@ def test_linear_refusals():
     def call(**kw):
         d = _lib.LinearDesc()
         base = dict(dtype=_lib.F16, out_dtype=_lib.F16, activation=0, m=4, n=8, k=8, x=16, x_row_stride=8, x_col_stride=1, w=16,
-                    w_row_stride=8, w_col_stride=1, y=16, y_row_stride=8)
+                    w_row_stride=8, w_col_stride=1, y=48, y_row_stride=8)
         base.update(kw)
         for name, v in base.items():
             setattr(d, name, v)
@@ -117,15 +117,15 @@ def test_linear_refusals():
     assert call(dtype=_lib.F64, out_dtype=_lib.F64) == _lib.ERR_UNSUPPORTED
     for kw in (dict(out_dtype=_lib.F32), dict(activation=9), dict(m=-1), dict(x_row_stride=-8), dict(y_row_stride=7), dict(y=None),
                dict(x=None), dict(dtype=_lib.I8), dict(dtype=_lib.I8, x_scale=16, w_scale=16, k=131072, x_row_stride=131072),
-               dict(x_scale=16, w_scale=16), dict(pre=16, pre_row_stride=8), dict(residual=32, residual_row_stride=4),
-               dict(residual=16, residual_row_stride=16), dict(dtype=_lib.I8, out_dtype=_lib.I8, x_scale=16, w_scale=16)):
+               dict(x_scale=16, w_scale=16), dict(pre=48, pre_row_stride=8), dict(residual=32, residual_row_stride=4), dict(y=16), dict(pre=16, pre_row_stride=8),
+               dict(residual=48, residual_row_stride=16), dict(dtype=_lib.I8, out_dtype=_lib.I8, x_scale=16, w_scale=16)):
         assert call(**kw) == _lib.ERR_INVALID_ARG, kw
     assert call(m=0) == _lib.OK and call(n=0) == _lib.OK
 
     def back(**kw):
         d = _lib.LinearBackwardDesc()
         base = dict(dtype=_lib.F16, activation=1, m=4, n=8, k=8, x=16, x_row_stride=8, x_col_stride=1, w=16, w_row_stride=8,
-                    w_col_stride=1, pre=16, pre_row_stride=8, grad_out=16, grad_out_row_stride=8, grad_x=16, grad_w=16, grad_bias=16)
+                    w_col_stride=1, pre=16, pre_row_stride=8, grad_out=16, grad_out_row_stride=8, grad_x=48, grad_w=64, grad_bias=80)
         base.update(kw)
         for name, v in base.items():
             setattr(d, name, v)
@@ -133,7 +133,7 @@ def test_linear_refusals():
 
     assert back(dtype=_lib.I8) == _lib.ERR_UNSUPPORTED
     for kw in (dict(pre=None), dict(grad_out=None), dict(w=None), dict(x=None), dict(activation=-1), dict(grad_out_row_stride=3),
-               dict(k=0)):
+               dict(k=0), dict(grad_x=16), dict(grad_w=16), dict(grad_bias=16)):
         assert back(**kw) == _lib.ERR_INVALID_ARG, kw
 
     x, w = torch.zeros(3, 4), torch.zeros(4, 5)
@@ -156,7 +156,7 @@ def test_distill_refusals():
         return L.ntb200_distill_topk(dtype, logits, s_rs, tdt, 16, idt, 16, None, grad, g_rs, 16, loss, rows, vocab, top, temp, None)
 
     assert call(dtype=_lib.I32) == _lib.ERR_UNSUPPORTED and call(tdt=_lib.F64) == _lib.ERR_UNSUPPORTED and call(idt=_lib.I16) == _lib.ERR_UNSUPPORTED
-    for kw in (dict(rows=-1), dict(vocab=0), dict(top=0), dict(top=1025), dict(temp=0.0), dict(temp=-1.0), dict(temp=float("inf")),
+    for kw in (dict(rows=-1), dict(vocab=0), dict(top=0), dict(top=1025), dict(temp=0.0), dict(temp=-1.0), dict(temp=1e-31), dict(temp=float("inf")),
                dict(temp=float("nan")), dict(s_rs=7), dict(g_rs=7), dict(logits=None), dict(loss=None), dict(grad=16, g_rs=16)):
         assert call(**kw) == _lib.ERR_INVALID_ARG, kw
     s, t, i = torch.zeros(2, 8), torch.zeros(2, 3), torch.zeros(2, 3, dtype=torch.int32)
@@ -518,6 +518,30 @@ def test_linear_layouts():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("ex,ew", [(100, 20), (-70, -50), (120, -120), (-100, 90)])
+@pytest.mark.parametrize("n", [1024, 1001])
+def test_linear_float32_range(n, ex, ew):
+    """Float32 operands far from 1: the product of their scales leaves the type's range, their products do not."""
+    from neurotensor_b200 import api
+    gen = generator(ex)
+    x, w = randn(gen, 256, 512), randn(gen, 512, n)
+    x[3], w[:, 5] = 0.0, 0.0
+    x[4, :256], w[256:, 6] = 0.0, 0.0                       # a sum of nothing but zeros
+    want = api.linear_act(x, w)
+    got = api.linear_act(x * 2.0 ** ex, w * 2.0 ** ew)
+    # Powers of two change no digit, and the results are the same: but a weight below 2^-126 is rounded to a multiple of
+    # 2^-149 before the call.  Then the exact sums differ by |x| . lost, and each side's are off by 2^-21 |x| . |w| at most
+    # (2^-22 from the parts of the operands, the rest fp32 sums of 512 terms that cancel at random).
+    lost = ((w * 2.0 ** ew).double() * 2.0 ** -ew - w.double()).abs()
+    slack = (x.double().abs() @ lost + 2.0 ** -20 * (x.double().abs() @ w.double().abs())) * float(lost.max() > 0)
+    assert float(lost.max()) == 0 or ew == -120
+    within(got.double() * 2.0 ** -(ex + ew), want.double(), slack, "scaled")
+    big, small = torch.zeros(256, 512, device="cuda"), torch.zeros(512, n, device="cuda")
+    big[:, 0], small[1] = 2.0 ** 120, 2.0 ** 120
+    assert torch.equal(api.linear_act(big, small), torch.zeros(256, n, device="cuda"))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F16, F32])
 def test_linear_unusual_weights(dtype):
     """Weights that repeat one row, that skip elements, and that are windows of a larger matrix."""
@@ -633,6 +657,31 @@ def test_distill(rows, vocab, top, dtype, T):
     place = s.clone()
     loss2, _, g2 = api.distill_topk(place, t, i, temperature=T, row_weight=rw, out_grad=place)
     assert g2 is place and torch.equal(place, grad) and torch.equal(loss2, loss)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("vocab", [64, 1001, 40000, 131072, 400001])
+def test_distill_masked_by_the_lowest_value(vocab, dtype):
+    """Columns masked out of the student by the type's lowest value: half of a row, all of it, and one the teacher names."""
+    from neurotensor_b200 import api
+    gen = generator(vocab)
+    lowest = torch.finfo(dtype).min
+    s = randn(gen, 6, vocab, scale=3.0, dtype=dtype)
+    t, i = randn(gen, 6, 4, scale=2.0), torch.randint(0, vocab // 2, (6, 4), generator=gen, device="cuda")
+    s[1:4, vocab // 2:] = lowest
+    s[0] = lowest
+    s[4, :vocab - 1] = lowest
+    i[4] = vocab - 1
+    i[2, 1] = vocab - 1
+    i[5] = -1
+    rw = torch.full((6,), 0.125, device="cuda")
+    loss, row, grad = api.distill_topk(s, t, i, row_weight=rw)
+    loss64, row64, grad64, size = distill64(s, t, i, 1.0, rw)
+    e = 2.0 ** -17 + 2.0 ** -24 * min(vocab, 4096)
+    within(grad, grad64, half_step(dtype) * grad64.abs() * (1 + 2.0 ** -9) + e * size + smallest(dtype), "grad")
+    within(row, row64, e * (row64.abs() + 100), "row")     # the others' logits and logarithms stay below 50
+    within(loss, loss64, e * (loss64.abs() + 100), "loss")
 
 
 @pytest.mark.gpu
