@@ -1274,8 +1274,8 @@ def distill_topk(logits, teacher, index, temperature=1.0, row_weight=None, want_
     top = teacher.shape[-1]
     if not 1 <= top <= 1024:
         raise ValueError("%s: expected 1 to 1024 teacher entries per row but got %d" % (what, top))
-    if not 0 < temperature < 1e30:
-        raise ValueError("%s: the temperature must be positive and finite but got %r" % (what, temperature))
+    if not 1e-30 <= temperature <= 1e30:
+        raise ValueError("%s: the temperature must be positive and finite (1e-30 to 1e30) but got %r" % (what, temperature))
     if row_weight is not None and (row_weight.shape != logits.shape[:-1] or row_weight.dtype != torch.float32):
         raise ValueError("%s: expected row weights of shape %s in Float32 but got %s in %s"
                          % (what, tuple(logits.shape[:-1]), tuple(row_weight.shape), row_weight.dtype))
