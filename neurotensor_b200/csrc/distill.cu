@@ -91,27 +91,25 @@ constexpr int kPieceThreads = 256, kMaxCluster = 8;
 // Behind the piece in dynamic shared memory: three arrays of `top` entries (the teacher's probabilities, the student's
 // logits at the same places, the columns within this piece, -1: not there or in another block's piece).
 struct PieceShared {
-    float red[3][kPieceThreads / 32];
+    float red[4][kPieceThreads / 32];
     float4 share[kMaxCluster];           // (max, sum, sum p (x - max), sum p) of every block's piece, by rank
     unsigned long long bar;
     uint32_t abort_flag;
 };
 
-// Two maxima, or up to three sums, over the block in one exchange.
-__device__ __forceinline__ void piece_max2(float& u, float& v, PieceShared& sh) {
+// A maximum, or up to four sums, over the block in one exchange.
+__device__ __forceinline__ float piece_max(float u, PieceShared& sh) {
     constexpr int W = kPieceThreads / 32;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        u = fmaxf(u, __shfl_xor_sync(0xffffffffu, u, o));
-        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    }
-    if (lane == 0) { sh.red[0][warp] = u; sh.red[1][warp] = v; }
+    for (int o = 16; o; o >>= 1) u = fmaxf(u, __shfl_xor_sync(0xffffffffu, u, o));
+    if (lane == 0) sh.red[0][warp] = u;
     __syncthreads();
-    u = sh.red[0][0]; v = sh.red[1][0];
+    u = sh.red[0][0];
 #pragma unroll
-    for (int i = 1; i < W; ++i) { u = fmaxf(u, sh.red[0][i]); v = fmaxf(v, sh.red[1][i]); }
+    for (int i = 1; i < W; ++i) u = fmaxf(u, sh.red[0][i]);
     __syncthreads();
+    return u;
 }
 template <int N>
 __device__ __forceinline__ void piece_sums(float (&u)[N], PieceShared& sh) {
@@ -224,7 +222,24 @@ __global__ void __launch_bounds__(kPieceThreads, kBlocks) distill_piece_kernel(c
         present |= t != -INFINITY;
         tmax = fmaxf(tmax, t);
     }
+    // their probabilities, while the piece is on its way
     present = __syncthreads_or(present);
+    tmax = piece_max(tmax, sh);
+    float tsums[1] = {0.f};
+    for (int j = tid; j < a.top; j += kPieceThreads) tsums[0] += sh_p[j] == -INFINITY ? 0.f : exp2f((sh_p[j] - tmax) * c);
+    piece_sums(tsums, sh);
+    float sums[4] = {0.f, 0.f, 0.f, 0.f};   // sum p log2 p, and this piece's z, sum p and sum p (x - m) / T
+    const float log2t = log2f(tsums[0]);
+    for (int j = tid; j < a.top; j += kPieceThreads) {
+        const float t = sh_p[j];
+        float p = 0.f;
+        if (t != -INFINITY) {
+            const float lt = (t - tmax) * c;
+            p = exp2f(lt) / tsums[0];
+            if (p != 0.f) sums[0] += p * (lt - log2t);
+        }
+        sh_p[j] = p;
+    }
     if (C > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // this block runs: its shared memory may be written
     float m = -INFINITY;
     if (granules > g1 && granules - 1 >= g0 && tid < V) m = RowType<T>::up(mem[(granules - 1) * V + tid]);
@@ -236,13 +251,21 @@ __global__ void __launch_bounds__(kPieceThreads, kBlocks) distill_piece_kernel(c
         sh.abort_flag = 1;
         atomicExch(status, 0x151u);
     }
-    piece_max2(tmax, m, sh);
+    m = piece_max(m, sh);
     const float ref = m == -INFINITY ? 0.f : m, mc = ref * c;
     // 16-bit logits take one multiply-add to the exponent, x c - m c, as long as the rounding of m c (2^-24 of it) stays far
     // below the gradient's own; not so where all of a piece is masked by the type's lowest value
     const bool moderate = sizeof(T) == 2 && fabsf(mc) <= kModerate;
-    float sums[2] = {0.f, 0.f};          // the teacher's and the student's
-    for (int j = tid; j < a.top; j += kPieceThreads) sums[0] += sh_p[j] == -INFINITY ? 0.f : exp2f((sh_p[j] - tmax) * c);
+    for (int j = tid; j < a.top; j += kPieceThreads) {   // a thread's own entries of above
+        const float p = sh_p[j];
+        if (sh_at[j] < 0) continue;
+        const float x = RowType<T>::up(mem[sh_at[j] + lead]);
+        sh_x[j] = x;
+        if (p != 0.f) {
+            sums[2] += p;
+            sums[3] += p * ((x - ref) * inv_temp);
+        }
+    }
     float z0 = 0.f, z1 = 0.f;
     if (moderate) {
 #pragma unroll 2
@@ -267,30 +290,7 @@ __global__ void __launch_bounds__(kPieceThreads, kBlocks) distill_piece_kernel(c
     }
     sums[1] = z0 + z1;
     piece_sums(sums, sh);
-    const float tsum = sums[0], z = sums[1];
-    // probabilities
-    float parts[3] = {0.f, 0.f, 0.f};    // sum p log2 p, and sum p and sum p (x - m) / T of this piece
-    const float log2t = log2f(tsum);
-    for (int j = tid; j < a.top; j += kPieceThreads) {
-        const float t = sh_p[j];
-        float p = 0.f;
-        if (t != -INFINITY) {
-            const float lt = (t - tmax) * c;
-            p = exp2f(lt) / tsum;
-            if (p != 0.f) parts[0] += p * (lt - log2t);
-        }
-        sh_p[j] = p;
-        if (sh_at[j] >= 0 && p != 0.f) {
-            const float x = RowType<T>::up(mem[sh_at[j] + lead]);
-            sh_x[j] = x;
-            parts[1] += p;
-            parts[2] += p * ((x - ref) * inv_temp);
-        } else if (sh_at[j] >= 0) {
-            sh_x[j] = RowType<T>::up(mem[sh_at[j] + lead]);
-        }
-    }
-    piece_sums(parts, sh);
-    const float entropy = parts[0], own_p = parts[1], own_x = parts[2];
+    const float entropy = sums[0], z = sums[1], own_p = sums[2], own_x = sums[3];
     if (C > 1) {
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
         if (tid < C) st_cluster_f4(smem_u32(&sh.share[rank]), uint32_t(tid), make_float4(m, z, own_x, own_p));
@@ -358,16 +358,18 @@ __global__ void __launch_bounds__(kPieceThreads, kBlocks) distill_piece_kernel(c
         for (int v = tid; v < count; v += kPieceThreads) grad[v] = RowType<T>::down(value(RowType<T>::up(mem[v + lead])));
     }
     __syncthreads();
-    for (int j = tid; j < a.top; j += kPieceThreads) {
+    // the teacher's places, a warp per entry: the first entry of a column writes it, with the probabilities of all its entries
+    for (int j = tid >> 5; j < a.top; j += kPieceThreads / 32) {
         const int at = sh_at[j];
         if (at < 0) continue;
-        bool one = true;
-        for (int k = 0; k < j; ++k) one = one && sh_at[k] != at;
-        if (!one) continue;
-        float p = sh_p[j];
-        for (int k = j + 1; k < a.top; ++k)
-            if (sh_at[k] == at) p += sh_p[k];
-        grad[at] = RowType<T>::down(scale * exp2f((sh_x[j] - gm) * c) - coef * p);
+        float p = 0.f;
+        bool first_one = true;
+        for (int k0 = 0; k0 < a.top; k0 += 32) {
+            unsigned same = __ballot_sync(0xffffffffu, k0 + lane < a.top && sh_at[min(k0 + lane, a.top - 1)] == at);
+            if (same && k0 + __ffs(same) - 1 < j) first_one = false;
+            for (; same; same &= same - 1) p += sh_p[k0 + __ffs(same) - 1];
+        }
+        if (first_one && lane == 0) grad[at] = RowType<T>::down(scale * exp2f((sh_x[j] - gm) * c) - coef * p);
     }
 }
 
