@@ -88,8 +88,9 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
 // granule are loaded one by one, and what else lies in those two granules is set to -inf, which adds nothing.
 constexpr int kPieceThreads = 256, kMaxCluster = 8;
 
-// Behind the piece in dynamic shared memory: three arrays of `top` entries (the teacher's probabilities, the student's
-// logits at the same places, the columns within this piece, -1: not there or in another block's piece).
+// Behind the piece in dynamic shared memory: three arrays of `top` entries (the teacher's probabilities; the same with
+// those of a column's later entries added to its first, -1 for the later ones; the columns within this piece, -1: not there or
+// in another block's piece).
 struct PieceShared {
     float red[4][kPieceThreads / 32];
     float4 share[kMaxCluster];           // (max, sum, sum p (x - max), sum p) of every block's piece, by rank
@@ -164,8 +165,8 @@ __global__ void __launch_bounds__(kPieceThreads, kBlocks) distill_piece_kernel(c
     extern __shared__ __align__(128) uint8_t piece_mem[];
     __shared__ PieceShared sh;
     float* sh_p = reinterpret_cast<float*>(piece_mem + (size_t(piece) * sizeof(T) + 32));
-    float* sh_x = sh_p + a.top;
-    int* sh_at = reinterpret_cast<int*>(sh_x + a.top);
+    float* sh_q = sh_p + a.top;
+    int* sh_at = reinterpret_cast<int*>(sh_q + a.top);
     const int tid = threadIdx.x, lane = tid & 31;
     const uint32_t rank = C > 1 ? cluster_cta_rank() : 0u;
     const long long row = blockIdx.x / C;
@@ -216,7 +217,8 @@ __global__ void __launch_bounds__(kPieceThreads, kBlocks) distill_piece_kernel(c
     int present = 0;
     for (int j = tid; j < a.top; j += kPieceThreads) {
         const long long i = a.idx64 ? static_cast<const long long*>(a.idx)[row * a.top + j] : static_cast<const int*>(a.idx)[row * a.top + j];
-        const float t = i >= 0 && i < a.vocab ? teacher_value(a, row * a.top + j) : -INFINITY;
+        const float value = teacher_value(a, row * a.top + j);   // on its way together with the column
+        const float t = i >= 0 && i < a.vocab ? value : -INFINITY;
         sh_at[j] = t != -INFINITY && i >= first && i < first + count ? int(i - first) : -1;
         sh_p[j] = t;
         present |= t != -INFINITY;
@@ -259,11 +261,9 @@ __global__ void __launch_bounds__(kPieceThreads, kBlocks) distill_piece_kernel(c
     for (int j = tid; j < a.top; j += kPieceThreads) {   // a thread's own entries of above
         const float p = sh_p[j];
         if (sh_at[j] < 0) continue;
-        const float x = RowType<T>::up(mem[sh_at[j] + lead]);
-        sh_x[j] = x;
         if (p != 0.f) {
             sums[2] += p;
-            sums[3] += p * ((x - ref) * inv_temp);
+            sums[3] += p * ((RowType<T>::up(mem[sh_at[j] + lead]) - ref) * inv_temp);
         }
     }
     float z0 = 0.f, z1 = 0.f;
@@ -294,7 +294,23 @@ __global__ void __launch_bounds__(kPieceThreads, kBlocks) distill_piece_kernel(c
     if (C > 1) {
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
         if (tid < C) st_cluster_f4(smem_u32(&sh.share[rank]), uint32_t(tid), make_float4(m, z, own_x, own_p));
-        cluster_sync_all();
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    }
+    // while the cluster meets: of a column's entries the first will write it, with the probabilities of all; a warp per entry
+    for (int j = tid >> 5; grad && j < a.top; j += kPieceThreads / 32) {
+        const int at = sh_at[j];
+        if (at < 0) continue;
+        float p = 0.f;
+        bool first_one = true;
+        for (int k0 = 0; k0 < a.top; k0 += 32) {
+            unsigned same = __ballot_sync(0xffffffffu, k0 + lane < a.top && sh_at[min(k0 + lane, a.top - 1)] == at);
+            if (same && k0 + __ffs(same) - 1 < j) first_one = false;
+            for (; same; same &= same - 1) p += sh_p[k0 + __ffs(same) - 1];
+        }
+        if (lane == 0) sh_q[j] = first_one ? p : -1.f;
+    }
+    if (C > 1) {
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     } else {
         if (tid == 0) sh.share[0] = make_float4(m, z, own_x, own_p);
         __syncthreads();
@@ -358,18 +374,9 @@ __global__ void __launch_bounds__(kPieceThreads, kBlocks) distill_piece_kernel(c
         for (int v = tid; v < count; v += kPieceThreads) grad[v] = RowType<T>::down(value(RowType<T>::up(mem[v + lead])));
     }
     __syncthreads();
-    // the teacher's places, a warp per entry: the first entry of a column writes it, with the probabilities of all its entries
-    for (int j = tid >> 5; j < a.top; j += kPieceThreads / 32) {
+    for (int j = tid; j < a.top; j += kPieceThreads) {   // the teacher's places
         const int at = sh_at[j];
-        if (at < 0) continue;
-        float p = 0.f;
-        bool first_one = true;
-        for (int k0 = 0; k0 < a.top; k0 += 32) {
-            unsigned same = __ballot_sync(0xffffffffu, k0 + lane < a.top && sh_at[min(k0 + lane, a.top - 1)] == at);
-            if (same && k0 + __ffs(same) - 1 < j) first_one = false;
-            for (; same; same &= same - 1) p += sh_p[k0 + __ffs(same) - 1];
-        }
-        if (first_one && lane == 0) grad[at] = RowType<T>::down(scale * exp2f((sh_x[j] - gm) * c) - coef * p);
+        if (at >= 0 && !(sh_q[j] < 0.f)) grad[at] = RowType<T>::down(scale * exp2f((RowType<T>::up(mem[at + lead]) - gm) * c) - coef * sh_q[j]);
     }
 }
 
