@@ -83,7 +83,10 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
 // that re-read its row from L2 instead took 623 us for 4096 x 131072 bf16 logits: the rows in flight (592 x 256 KB) do not
 // fit L2, so the second read went to memory again.  Pieces are at most 72 KB where C <= 8 allows it, so that three blocks
 // per SM overlap loading, arithmetic and storing (36 KB: 562 us, 512 threads per block: 566 us; four barriers per copy to
-// start earlier: 488 against 477 us).
+// start earlier: 488 against 477 us; the gradient formed in shared memory and sent by a bulk store: 502 against 474).  Measured:
+// 4096 x 131072 bf16 with 64 entries 466 - 506 us (4.2 - 4.6 TB/s), loss alone 297 us; bound by the chain a block goes through
+// (load, maximum, sum, exchange, store) with three blocks per SM, not by the exponential unit (a polynomial for a quarter of the
+// exponentials: 469 us).
 // Rows need not start on 16 bytes: the piece's whole 16-byte granules are copied, the elements of a cut first or last
 // granule are loaded one by one, and what else lies in those two granules is set to -inf, which adds nothing.
 constexpr int kPieceThreads = 256, kMaxCluster = 8;
