@@ -63,8 +63,8 @@ __global__ void pad_rows_kernel(const PadJob first, const PadJob second) {
 // 2^-39 of it always, so a.b = hi.hi + hi.lo + lo.hi + O(2^-23 |a||b|).  kind::f16 runs at twice TF32's rate and a value's two
 // parts take 4 bytes instead of 8: [512, 1024] x [1024, 4096] took 30 us as three TF32 products.  The scales are undone by
 // the epilogue's row and column factors (powers of two, exact).  Parts keep the operand's direction (tcgen05 takes
-// Float16 tiles along either axis), so nothing is transposed.  [512, 1024] x [1024, 4096] with gelu: 35 us, of which this split is
-// about 7.
+// Float16 tiles along either axis), so nothing is transposed.  [512, 1024] x [1024, 4096] with gelu: 34 us (46 when the split read
+// its operands twice).
 struct SplitF16Job {
     const float* src;
     __half* hi;
@@ -107,6 +107,10 @@ __device__ __forceinline__ void store_parts(__half* hi, __half* lo, __half2 h, _
     *reinterpret_cast<__half2*>(lo) = l;
 }
 
+// Up to kHeld pairs of a thread stay in registers between the maximum and the split (K <= 1024): one read, all of it on its way at
+// once.  Longer ones are read twice, the second time from L1 / L2.
+constexpr int kHeld = 16, kHeldK = kHeld * 64;
+
 template <bool kPairs>
 __device__ __forceinline__ void split_rows(const SplitF16Job& j, int block, int warp, int lane) {   // a warp per row
     const long long r = (long long)block * 32 + warp;
@@ -117,6 +121,28 @@ __device__ __forceinline__ void split_rows(const SplitF16Job& j, int block, int 
     __half* hi = j.hi + r * j.ld;
     __half* lo = j.lo + r * j.ld;
     float top = 0.f;
+    if (k <= kHeldK) {
+        float2 v[kHeld];
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            const int c = 2 * lane + 64 * i;
+            v[i] = c < k ? load_pair<kPairs>(src + c * step, step, c + 1 < k) : make_float2(0.f, 0.f);
+        }
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) top = max_finite(max_finite(top, v[i].x), v[i].y);
+        top = warp_max_nan(top);
+        float unscale;
+        const float scale = split_scale(top, &unscale);
+        if (lane == 0) j.unscale[r] = unscale;
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            const int c = 2 * lane + 64 * i;
+            __half2 h, l;
+            split_pair(v[i].x, v[i].y, scale, h, l);
+            if (c < k) store_parts(hi + c, lo + c, h, l);
+        }
+        return;
+    }
 #pragma unroll 8
     for (int c = 2 * lane; c < k; c += 64) {
         const float2 v = load_pair<kPairs>(src + c * step, step, c + 1 < k);
@@ -144,7 +170,17 @@ __device__ __forceinline__ void split_columns(const SplitF16Job& j, int block, i
     const float* src = j.src + (long long)(in ? c : 0) * j.mn_s + row0 * j.k_s;
     const long long down = 64 * j.k_s;
     float tx = 0.f, ty = 0.f;
-    if (in) {
+    const bool held = k <= kHeldK;
+    float2 kept[kHeld];
+    if (held) {
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) kept[i] = in && row0 + 64 * i < k ? load_pair<kPairs>(src + i * down, j.mn_s, both) : make_float2(0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            tx = max_finite(tx, kept[i].x);
+            ty = max_finite(ty, kept[i].y);
+        }
+    } else if (in) {
         const float* p = src;
 #pragma unroll 8
         for (int r = row0; r < k; r += 64, p += down) {
@@ -171,6 +207,15 @@ __device__ __forceinline__ void split_columns(const SplitF16Job& j, int block, i
     __half* hi = j.hi + row0 * j.ld + c;
     __half* lo = j.lo + row0 * j.ld + c;
     const long long out_down = 64 * j.ld;
+    if (held) {
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            __half2 h, l;
+            split_pair(kept[i].x * sx, kept[i].y * sy, 1.f, h, l);
+            if (row0 + 64 * i < k) store_parts(hi + i * out_down, lo + i * out_down, h, l);
+        }
+        return;
+    }
 #pragma unroll 8
     for (int r = row0; r < k; r += 64, src += down, hi += out_down, lo += out_down) {
         const float2 v = load_pair<kPairs>(src, j.mn_s, both);
