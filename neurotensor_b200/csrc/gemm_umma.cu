@@ -264,74 +264,73 @@ __device__ __forceinline__ bool epilogue_linear(const UmmaParams& p, uint32_t tm
     if (kInt && p.linear.out_dtype == NTB200_F32) return epilogue_linear<BN, kInt, kRows, NTB200_F32>(p, tmem_acc, staged, row0, lane, n0, wait);
     return epilogue_linear<BN, kInt, kRows, NTB200_BF16>(p, tmem_acc, staged, row0, lane, n0, wait);
 }
-// 16 sums of one row of a Float32 result, from the thread's own 64 bytes of shared memory: one copy of the activations' code
-// for all chunks of a tile.
+// 16 sums of one row of a Float32 result (`count` of them inside it), from the thread's own 64 bytes of shared memory: one copy of
+// the activations' code for all chunks of a tile.  kVec: rows and vectors start on 16 bytes and all 16 are there.
+template <bool kVec>
 __device__ __noinline__ void finish_row16(float* y, float* pre, const float* res, const float* cs, const float* bias, float rs, int act,
-                                          const float4* own, int swizzle) {
+                                          const float4* own, int swizzle, int count) {
 #pragma unroll 1
     for (int q = 0; q < 4; q += 2) {
         float f[8];
-        auto each4 = [&](const float* src, auto op) {
+        auto each = [&](const float* src, auto op) {
+            if constexpr (kVec) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const float4 o = reinterpret_cast<const float4*>(src)[q + h];
-                op(f[4 * h], o.x); op(f[4 * h + 1], o.y); op(f[4 * h + 2], o.z); op(f[4 * h + 3], o.w);
+                for (int h = 0; h < 2; ++h) {
+                    const float4 o = reinterpret_cast<const float4*>(src)[q + h];
+                    op(f[4 * h], o.x); op(f[4 * h + 1], o.y); op(f[4 * h + 2], o.z); op(f[4 * h + 3], o.w);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) op(f[i], 4 * q + i < count ? src[4 * q + i] : 0.f);
             }
         };
         auto store = [&](float* dst) {
+            if constexpr (kVec) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) reinterpret_cast<float4*>(dst)[q + h] = make_float4(f[4 * h], f[4 * h + 1], f[4 * h + 2], f[4 * h + 3]);
+                for (int h = 0; h < 2; ++h) reinterpret_cast<float4*>(dst)[q + h] = make_float4(f[4 * h], f[4 * h + 1], f[4 * h + 2], f[4 * h + 3]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (4 * q + i < count) dst[4 * q + i] = f[i];
+            }
         };
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const float4 o = own[(q + h) ^ swizzle];
             f[4 * h] = o.x; f[4 * h + 1] = o.y; f[4 * h + 2] = o.z; f[4 * h + 3] = o.w;
         }
-        each4(cs, [&](float& v, float c) { v = scaled<true>(v, rs, c); });
-        if (bias) each4(bias, [](float& v, float b) { v += b; });
+        each(cs, [&](float& v, float c) { v = scaled<true>(v, rs, c); });
+        if (bias) each(bias, [](float& v, float b) { v += b; });
         if (pre) store(pre);
         act_values<false>(act, f);
-        if (res) each4(res, [](float& v, float r) { v += r; });
+        if (res) each(res, [](float& v, float r) { v += r; });
         store(y);
     }
 }
 
-// The Float32 split kernels' running sums.  Where rows start on 16 bytes a thread finishes its own row: a warp that took
-// column by column through shared memory instead (as it does for other rows) left [8192, 1024] x [1024, 4096] at 387 us, with
-// gelu at 517, its few warps waiting for one row after another; now 259 and 303 (three products: 0.21 PFLOP, 129 us at the
-// measured rate of Float16 products; the rest is the split pass and the sums taken over every 128 of K).
+// The Float32 split kernels' running sums: each thread finishes its own row.  A warp that took column by column through shared
+// memory instead left [8192, 1024] x [1024, 4096] at 387 us, with gelu at 517, its few warps waiting for one row after another;
+// now 247 and 294 (three products: 0.21 PFLOP, 129 us at the measured rate of Float16 products; the rest is the split pass and
+// the sums taken over every 128 of K).
 template <int HC>
-__device__ __forceinline__ void finish_running(const UmmaParams& p, const float (&run)[HC], float* staged, int row0, int lane, int col_base, LinearAhead& ahead) {
-    if (row0 >= p.m) return;
+__device__ __forceinline__ void finish_running(const UmmaParams& p, const float (&run)[HC], float* staged, int row0, int lane, int col_base) {
     const LinearParams& l = p.linear;
     const int row = row0 + lane;
-    const float rs = row < p.m ? l.row_scale[row] : 1.f;
+    if (row >= p.m) return;
+    const float rs = l.row_scale[row];
+    float4* own = reinterpret_cast<float4*>(staged) + lane * 4;
+    const int swizzle = (lane >> 1) & 3;
 #pragma unroll
-    for (int cc = 0; cc < HC / 32; ++cc) {
-        const int col0 = col_base + cc * 32;
+    for (int c = 0; c < HC; c += 16) {
+        const int col0 = col_base + c;
         if (col0 >= p.n) continue;
-        if (l.vec_ok && col0 + 32 <= p.n) {
-            float4* own = reinterpret_cast<float4*>(staged) + lane * 4;
-            const int swizzle = (lane >> 1) & 3;
-            auto at = [&](const void* base, long long rs_elements) { return base ? const_cast<float*>(static_cast<const float*>(base)) + row * rs_elements + col0 : nullptr; };
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const float* v = &run[cc * 32 + h * 16];
-#pragma unroll
-                for (int q = 0; q < 4; ++q) own[q ^ swizzle] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-                float *y = at(l.y, l.y_rs), *pre = at(l.pre, l.pre_rs);
-                const float *res = at(l.residual, l.residual_rs), *bias = static_cast<const float*>(l.bias);
-                if (row < p.m)
-                    finish_row16(y + h * 16, pre ? pre + h * 16 : nullptr, res ? res + h * 16 : nullptr, l.col_scale + col0 + h * 16,
-                                 bias ? bias + col0 + h * 16 : nullptr, rs, l.act, own, swizzle);
-            }
-            continue;
-        }
-        if (cc > 0 || HC > 64) linear_load_ahead<NTB200_F32>(p.linear, p.m, p.n, row0, col0, lane, ahead);
-        float f[32];
-#pragma unroll
-        for (int j = 0; j < 32; ++j) f[j] = run[cc * 32 + j];
-        finish_chunk<16, NTB200_F32>(p, f, staged, row0, lane, col0, ahead);
+        for (int q = 0; q < 4; ++q) own[q ^ swizzle] = make_float4(run[c + 4 * q], run[c + 4 * q + 1], run[c + 4 * q + 2], run[c + 4 * q + 3]);
+        auto at = [&](const void* base, long long stride) { return base ? const_cast<float*>(static_cast<const float*>(base)) + row * stride + col0 : nullptr; };
+        float *y = at(l.y, l.y_rs), *pre = at(l.pre, l.pre_rs);
+        const float *res = at(l.residual, l.residual_rs), *bias = at(l.bias, 0), *cs = at(l.col_scale, 0);
+        if (l.vec_ok && col0 + 16 <= p.n) finish_row16<true>(y, pre, res, cs, bias, rs, l.act, own, swizzle, 16);
+        else finish_row16<false>(y, pre, res, cs, bias, rs, l.act, own, swizzle, p.n - col0);
     }
 }
 
@@ -1057,8 +1056,6 @@ umma_gemm_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
         for (int t = blockIdx.x; alive && t < p.total_tiles; t += gridDim.x) {
             int b, mi, ni;
             tile_coords(p, t, b, mi, ni);
-            [[maybe_unused]] LinearAhead ahead;   // kLinear: requested before the sums are there, where registers allow it
-            if constexpr (kLinear && HC <= 64) linear_load_ahead<NTB200_F32>(p.linear, p.m, p.n, mi * kBM + quad * 32, ni * BN + half * HC, lane, ahead);
             for (int kb0 = 0; kb0 < p.k_blocks; kb0 += p.chunk_blocks) {
                 bool ok = mbar_wait(tfull_bar(acc), acc_phase, abort_flag);
                 ok = __all_sync(0xffffffffu, ok);
@@ -1077,7 +1074,7 @@ umma_gemm_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constan
             if (alive) {
                 if constexpr (kLinear)
                     finish_running<HC>(p, run, reinterpret_cast<float*>(bar_gen + T::kBarrierBytes + uint32_t(warp - 2) * kStagedBlock),
-                                       mi * kBM + quad * 32, lane, ni * BN + half * HC, ahead);
+                                       mi * kBM + quad * 32, lane, ni * BN + half * HC);
                 else
                     store_running<HC>(p, run, b, mi * kBM + row_in_tile, ni * BN + half * HC);
             }
@@ -1332,7 +1329,6 @@ umma_gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
         for (int t = pair; alive && t < p.total_tiles; t += npairs) {
             int b, mi, ni;
             tile_coords(p, t, b, mi, ni);
-            [[maybe_unused]] LinearAhead ahead;
             for (int kb0 = 0; kb0 < p.k_blocks; kb0 += p.chunk_blocks) {
                 bool ok = mbar_wait(tfull_bar(acc), acc_phase, abort_flag);
                 ok = __all_sync(0xffffffffu, ok);
@@ -1351,7 +1347,7 @@ umma_gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
             if (alive) {
                 if constexpr (kLinear)
                     finish_running<HC>(p, run, reinterpret_cast<float*>(bar_gen + 256 + uint32_t(warp - 2) * kStagedBlock),
-                                       mi * 256 + int(rank) * 128 + quad * 32, lane, ni * BN + half * HC, ahead);
+                                       mi * 256 + int(rank) * 128 + quad * 32, lane, ni * BN + half * HC);
                 else
                     store_running<HC>(p, run, b, mi * 256 + row_in_tile, ni * BN + half * HC);
             }
