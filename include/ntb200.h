@@ -475,10 +475,10 @@ int ntb200_rms_norm_backward(int dtype, const void* h, int64_t h_row_stride, con
  * column of w (fp32), the product is exact in s32, and bias, residual, pre and y have out_dtype (F32 / F16 / BF16).
  * GELU is z Phi(z) with the normal distribution's Phi, GELU_TANH its usual tanh form, SILU z / (1 + e^-z).
  * y may be the residual itself (same row stride).  16-bit and Int8 products always run on the tensor cores: operands
- * whose rows do not start on 16 bytes are copied into the workspace first.  F32 products of 6e7 multiply-adds and more
- * run there too, as three products of Float16 parts: an fp32 product's error as long as the values of a row of x (a column
- * of w) lie within 2^13 of its largest one; smaller ones keep 2^-39 of that largest one.  An infinite operand may give a
- * NaN where its product alone is infinite. */
+ * whose rows do not start on 16 bytes are copied into the workspace first.  F32 products over K > 32, or of 6e7
+ * multiply-adds and more, run there too, as three products of Float16 parts: an fp32 product's error as long as the
+ * values of a row of x (a column of w) lie within 2^13 of its largest one; smaller ones keep 2^-39 of that largest one.
+ * An infinite operand may give a NaN where its product alone is infinite. */
 typedef enum ntb200_activation {
     NTB200_ACT_NONE = 0,
     NTB200_ACT_RELU = 1,

@@ -6,6 +6,8 @@
 // bytes) are copied once into padded rows in the caller's workspace; a small Float32 product runs on the exact
 // CUDA-core kernel and is finished by an elementwise pass.
 #include <algorithm>
+#include <cstdlib>
+#include <cstring>
 
 #include "internal.h"
 #include "linear_epilogue.cuh"
@@ -371,7 +373,13 @@ GemmArgs gemm_of(int dtype, const Operand& a, const Operand& b, void* c, int64_t
     return g;
 }
 
-bool small_f32(const GemmArgs& g) { return double(g.m) * double(g.n) * double(g.k) < 6.0e7; }   // as ntb200_gemm routes it
+// Float32 products for the exact CUDA-core kernel: few sums of few terms.  Its time grows with K alone while its tiles do not fill
+// the GPU ([45, 2048] x [2048, 448]: 291 us, 42 on the tensor cores; K = 128: 27 and 17, K = 64: 19 and 17).
+// NTB200_FP32_MODE=ffma asks for that kernel always.
+bool small_f32(const GemmArgs& g) {
+    static const bool exact_only = [] { const char* e = getenv("NTB200_FP32_MODE"); return e && std::strcmp(e, "ffma") == 0; }();
+    return exact_only || (g.k <= 32 && double(g.m) * double(g.n) * double(g.k) < 6.0e7);
+}
 
 // Parts of one operand: rows along the direction in which its elements are closer together.
 size_t parts_elements(const Operand& o) {
