@@ -20,13 +20,15 @@ bool linear_float(int d) { return d == NTB200_F32 || d == NTB200_F16 || d == NTB
 bool on16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 size_t round256(size_t b) { return (b + 255) & ~size_t(255); }
 
-// y = act(z + bias) + residual, pre = z + bias, from an fp32 product (or none: z null, K = 0).
-__global__ void linear_finish_kernel(const float* __restrict__ z, const LinearParams l, long long m, int n) {
+// y = act(z + bias) + residual, pre = z + bias, from an fp32 product in `slabs` partial sums (0: K = 0), added in their order.
+__global__ void linear_finish_kernel(const float* __restrict__ z, int slabs, const LinearParams l, long long m, int n) {
     const long long total = m * n;
     for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
         const long long row = i / n;
         const int col = int(i - row * n);
-        float v = z ? z[i] : 0.f;
+        float v = 0.f;
+#pragma unroll 8
+        for (int s = 0; s < slabs; ++s) v += z[s * total + i];
         if (l.bias) v += lin_load(l.bias, col, l.out_dtype);
         if (l.pre) lin_store(l.pre, row * l.pre_rs + col, v, l.out_dtype);
         v = l.out_dtype == NTB200_F32 ? act_value<false>(l.act, v) : act_value<true>(l.act, v);
@@ -56,6 +58,91 @@ __global__ void pad_rows_kernel(const PadJob first, const PadJob second) {
 #pragma unroll
         for (int k = 0; k < V; ++k) o.e[k] = c0 + k < j.cols ? src[k * j.cs] : U(0);
         *reinterpret_cast<Pack<U, V>*>(static_cast<U*>(j.dst) + r * j.ld + c0) = o;
+    }
+}
+
+// ---- Float32, few rows ---------------------------------------------------------------------------------------------------
+// y of up to 64 rows: the weight is what has to be read, so it is read as it is, 16 rows to a pass, and multiplied on the CUDA
+// cores; splitting it first would cost three times its bytes, and few tiles would walk a long K one after another
+// ([8, 4096] x [4096, 4096]: 101 us as three Float16 products).  K is cut into slices of whole 128s until there are six blocks per
+// SM; their sums go to the workspace and are added in order by linear_finish_kernel.
+struct FewRows {
+    const float* a; long long a_ms, a_ks;
+    const float* b; long long b_s;          // elements from one row (kAlongN) or column of b to the next
+    float* partial;                         // [slices][m][n]
+    int m, n, k, slice;
+};
+constexpr int kFewRows = 16, kFewStep = 128, kFewThreads = 128;
+
+// kAlongN: the weight's rows are dense along n; a thread takes two columns.  Otherwise dense along k: a warp takes four columns,
+// its lanes 32 neighbouring k.
+template <bool kAlongN>
+__global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const FewRows f) {
+    __shared__ float xs[kAlongN ? kFewStep * (kFewRows + 4) : kFewRows * kFewStep];
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int r0 = int(blockIdx.z) * kFewRows, rows = min(kFewRows, f.m - r0);
+    const int k0 = int(blockIdx.y) * f.slice, k1 = min(f.k, k0 + f.slice);
+    constexpr int kCols = kAlongN ? 2 : 4;
+    const int col = kAlongN ? int(blockIdx.x) * (2 * kFewThreads) + tid : (int(blockIdx.x) * (kFewThreads / 32) + (tid >> 5)) * 4;
+    constexpr int kNext = kAlongN ? kFewThreads : 1;   // from one of a thread's columns to its next
+    float acc[kCols][kFewRows];
+#pragma unroll
+    for (int c = 0; c < kCols; ++c)
+#pragma unroll
+        for (int r = 0; r < kFewRows; ++r) acc[c][r] = 0.f;
+    for (int kb = k0; kb < k1; kb += kFewStep) {
+        __syncthreads();
+        for (int r = 0; r < kFewRows; ++r)
+            xs[kAlongN ? tid * (kFewRows + 4) + r : r * kFewStep + tid] = r < rows && kb + tid < k1 ? f.a[(r0 + r) * f.a_ms + (kb + tid) * f.a_ks] : 0.f;
+        __syncthreads();
+        if constexpr (kAlongN) {
+            for (int kk = 0; kk < kFewStep && kb + kk < k1; kk += 8) {
+                float w[2][8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+                        w[c][u] = kb + kk + u < k1 && col + c * kNext < f.n ? f.b[(kb + kk + u) * f.b_s + col + c * kNext] : 0.f;
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+#pragma unroll
+                    for (int r = 0; r < kFewRows; r += 4) {
+                        const float4 x = *reinterpret_cast<const float4*>(&xs[(kk + u) * (kFewRows + 4) + r]);
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            acc[c][r] = fmaf(w[c][u], x.x, acc[c][r]);
+                            acc[c][r + 1] = fmaf(w[c][u], x.y, acc[c][r + 1]);
+                            acc[c][r + 2] = fmaf(w[c][u], x.z, acc[c][r + 2]);
+                            acc[c][r + 3] = fmaf(w[c][u], x.w, acc[c][r + 3]);
+                        }
+                    }
+            }
+        } else {
+            float w[kFewStep / 32][4];
+#pragma unroll
+            for (int u = 0; u < kFewStep / 32; ++u)
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    w[u][c] = kb + lane + 32 * u < k1 && col + c < f.n ? f.b[(col + c) * f.b_s + kb + lane + 32 * u] : 0.f;
+#pragma unroll
+            for (int u = 0; u < kFewStep / 32; ++u)
+#pragma unroll
+                for (int r = 0; r < kFewRows; ++r) {
+                    const float x = xs[r * kFewStep + lane + 32 * u];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) acc[c][r] = fmaf(w[u][c], x, acc[c][r]);
+                }
+        }
+    }
+    float* out = f.partial + ((long long)blockIdx.y * f.m + r0) * f.n;
+#pragma unroll
+    for (int r = 0; r < kFewRows; ++r) {
+        if (r >= rows) break;
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) {
+            const float v = kAlongN ? acc[c][r] : warp_sum(acc[c][r]);
+            if ((kAlongN || lane == 0) && col + c * kNext < f.n) out[(long long)r * f.n + col + c * kNext] = v;
+        }
     }
 }
 
@@ -380,6 +467,35 @@ bool small_f32(const GemmArgs& g) {
     static const bool exact_only = [] { const char* e = getenv("NTB200_FP32_MODE"); return e && std::strcmp(e, "ffma") == 0; }();
     return exact_only || (g.k <= 32 && double(g.m) * double(g.n) * double(g.k) < 6.0e7);
 }
+// Slices of K for few_rows_kernel, 0 where another kernel takes the product.  3e8 multiply-adds are about 25 us of it; at
+// [64, 2048] x [2048, 2048] three Float16 products take as long.
+struct FewPlan { int slices, slice; };
+FewPlan plan_few(const Operand& a, const Operand& b) {
+    if (a.mn > 64 || (b.mn_s != 1 && b.k_s != 1) || double(a.mn) * double(b.mn) * double(a.k) >= 3.0e8) return {0, 0};
+    const int64_t cols = b.mn_s == 1 ? 2 * kFewThreads : 16, steps = (a.k + kFewStep - 1) / kFewStep;
+    const int64_t blocks = (b.mn + cols - 1) / cols * ((a.mn + kFewRows - 1) / kFewRows);
+    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(steps, 148 * 6 / blocks)), per = (steps + want - 1) / want;
+    return {int((steps + per - 1) / per), int(per * kFewStep)};
+}
+size_t few_bytes(const FewPlan& p, int64_t m, int64_t n) { return round256(size_t(p.slices) * size_t(m) * size_t(n) * 4); }
+int few_product(const Operand& a, const Operand& b, const FewPlan& p, const LinearParams& l, cudaStream_t stream) {
+    void* partial = nullptr;
+    if (int rc = scratch_acquire(&partial, few_bytes(p, a.mn, b.mn), stream)) return rc;
+    const bool along_n = b.mn_s == 1;
+    const FewRows f{static_cast<const float*>(a.p), a.mn_s, a.k_s, static_cast<const float*>(b.p), along_n ? b.k_s : b.mn_s,
+                    static_cast<float*>(partial), int(a.mn), int(b.mn), int(a.k), p.slice};
+    const int cols = along_n ? 2 * kFewThreads : 16;
+    const dim3 grid(unsigned((b.mn + cols - 1) / cols), unsigned(p.slices), unsigned((a.mn + kFewRows - 1) / kFewRows));
+    if (along_n) few_rows_kernel<true><<<grid, kFewThreads, 0, stream>>>(f);
+    else few_rows_kernel<false><<<grid, kFewThreads, 0, stream>>>(f);
+    count_launch();
+    NTB200_CUDA(cudaGetLastError());
+    const int blocks = int(std::min<int64_t>((a.mn * b.mn + 255) / 256, int64_t(sm_count()) * 16));
+    linear_finish_kernel<<<blocks, 256, 0, stream>>>(static_cast<const float*>(partial), p.slices, l, a.mn, int(b.mn));
+    count_launch();
+    NTB200_CUDA(cudaGetLastError());
+    return NTB200_OK;
+}
 
 // Parts of one operand: rows along the direction in which its elements are closer together.
 size_t parts_elements(const Operand& o) {
@@ -424,7 +540,11 @@ int f16x3_product(const Operand& a, const Operand& b, LinearParams l, cudaStream
 
 // One plain product of the backward pass: its scratch beyond padded copies.
 size_t product_bytes(const GemmArgs& g, const Operand& a, const Operand& b) {
-    if (g.dtype == NTB200_F32) return small_f32(g) ? 0 : f16x3_bytes(a, b);
+    if (g.dtype == NTB200_F32) {
+        if (small_f32(g)) return 0;
+        const FewPlan few = plan_few(a, b);
+        return few.slices ? few_bytes(few, a.mn, b.mn) : f16x3_bytes(a, b);
+    }
     return umma_scratch_bytes(g) + gemv_scratch_bytes(g) + 1024;
 }
 int plain_product(int dtype, Operand a, Operand b, void* c, int64_t c_rs, cudaStream_t stream) {
@@ -436,7 +556,10 @@ int plain_product(int dtype, Operand a, Operand b, void* c, int64_t c_rs, cudaSt
     // epilogue moves them by rows.  Large Float32 products are three Float16 ones.
     LinearParams l{};
     l.y = c; l.y_rs = c_rs; l.act = NTB200_ACT_NONE; l.out_dtype = dtype;
-    if (dtype == NTB200_F32 && !small_f32(g)) return f16x3_product(a, b, l, stream);
+    if (dtype == NTB200_F32 && !small_f32(g)) {
+        const FewPlan few = plan_few(a, b);
+        return few.slices ? few_product(a, b, few, l, stream) : f16x3_product(a, b, l, stream);
+    }
     if (dtype != NTB200_F32 && (c_rs % 8 != 0 || !on16(c))) {
         g.linear = &l;
         return launch_umma_gemm(g, stream);
@@ -568,7 +691,9 @@ size_t ntb200_linear_act_workspace_bytes(const ntb200_linear_desc* d) {
     if (check_linear(d) || d->m == 0 || d->n == 0 || d->k == 0) return 0;
     if (d->dtype == NTB200_F32) {
         const GemmArgs g = gemm_of(d->dtype, x_of(*d), w_of(*d), d->y, d->y_row_stride);
-        return small_f32(g) ? round256(size_t(d->m) * size_t(d->n) * 4) : f16x3_bytes(x_of(*d), w_of(*d));
+        if (small_f32(g)) return round256(size_t(d->m) * size_t(d->n) * 4);
+        const FewPlan few = plan_few(x_of(*d), w_of(*d));
+        return few.slices ? few_bytes(few, d->m, d->n) : f16x3_bytes(x_of(*d), w_of(*d));
     }
     const int es = int(dtype_size(d->dtype));
     GemmArgs g = gemm_of(d->dtype, x_of(*d), w_of(*d), d->y, d->y_row_stride);
@@ -604,12 +729,15 @@ int ntb200_linear_act(const ntb200_linear_desc* d, void* workspace, size_t works
             if (int rc = launch_simt_gemm(g, s)) return rc;
         }
         const int blocks = int(std::min<int64_t>((d->m * d->n + 255) / 256, int64_t(sm_count()) * 16));
-        linear_finish_kernel<<<blocks, 256, 0, s>>>(static_cast<const float*>(z), l, d->m, int(d->n));
+        linear_finish_kernel<<<blocks, 256, 0, s>>>(static_cast<const float*>(z), z ? 1 : 0, l, d->m, int(d->n));
         count_launch();
         NTB200_CUDA(cudaGetLastError());
         return NTB200_OK;
     }
-    if (d->dtype == NTB200_F32) return f16x3_product(x, w, l, s);
+    if (d->dtype == NTB200_F32) {
+        const FewPlan few = plan_few(x, w);
+        return few.slices ? few_product(x, w, few, l, s) : f16x3_product(x, w, l, s);
+    }
     if (int rc = pad_operands(x, w, int(dtype_size(d->dtype)), s)) return rc;
     g = gemm_of(d->dtype, x, w, d->y, d->y_row_stride);
     g.linear = &l;
