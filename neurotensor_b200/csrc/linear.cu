@@ -69,7 +69,7 @@ __global__ void pad_rows_kernel(const PadJob first, const PadJob second) {
 struct FewRows {
     const float* a; long long a_ms, a_ks;
     const float* b; long long b_s;          // elements from one row (kAlongN) or column of b to the next
-    float* partial;                         // [slices][m][n]
+    float* out; long long out_rs;           // [slices][m] rows of n
     int m, n, k, slice;
 };
 constexpr int kFewRows = 16, kFewStep = 128, kFewThreads = 128;
@@ -134,14 +134,14 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const FewRows f) 
                 }
         }
     }
-    float* out = f.partial + ((long long)blockIdx.y * f.m + r0) * f.n;
+    float* out = f.out + ((long long)blockIdx.y * f.m + r0) * f.out_rs;
 #pragma unroll
     for (int r = 0; r < kFewRows; ++r) {
         if (r >= rows) break;
 #pragma unroll
         for (int c = 0; c < kCols; ++c) {
             const float v = kAlongN ? acc[c][r] : warp_sum(acc[c][r]);
-            if ((kAlongN || lane == 0) && col + c * kNext < f.n) out[(long long)r * f.n + col + c * kNext] = v;
+            if ((kAlongN || lane == 0) && col + c * kNext < f.n) out[r * f.out_rs + col + c * kNext] = v;
         }
     }
 }
@@ -463,33 +463,41 @@ GemmArgs gemm_of(int dtype, const Operand& a, const Operand& b, void* c, int64_t
 // Float32 products for the exact CUDA-core kernel: few sums of few terms.  Its time grows with K alone while its tiles do not fill
 // the GPU ([45, 2048] x [2048, 448]: 291 us, 42 on the tensor cores; K = 128: 27 and 17, K = 64: 19 and 17).
 // NTB200_FP32_MODE=ffma asks for that kernel always.
-bool small_f32(const GemmArgs& g) {
+bool f32_exact_only() {
     static const bool exact_only = [] { const char* e = getenv("NTB200_FP32_MODE"); return e && std::strcmp(e, "ffma") == 0; }();
-    return exact_only || (g.k <= 32 && double(g.m) * double(g.n) * double(g.k) < 6.0e7);
+    return exact_only;
 }
-// Slices of K for few_rows_kernel, 0 where another kernel takes the product.  3e8 multiply-adds are about 25 us of it; at
-// [64, 2048] x [2048, 2048] three Float16 products take as long.
-struct FewPlan { int slices, slice; };
-FewPlan plan_few(const Operand& a, const Operand& b) {
-    if (a.mn > 64 || (b.mn_s != 1 && b.k_s != 1) || double(a.mn) * double(b.mn) * double(a.k) >= 3.0e8) return {0, 0};
+bool small_f32(const GemmArgs& g) { return f32_exact_only() || (g.k <= 32 && double(g.m) * double(g.n) * double(g.k) < 6.0e7); }
+// Slices of K for few_rows_kernel, 0 where another kernel takes the product.  Few rows: 3e8 multiply-adds are about 25 us of it; at
+// [64, 2048] x [2048, 2048] three Float16 products take as long.  Few terms (plain: the weight's gradient of few rows): the result
+// is what has to be written, and it is written once, straight to its place.
+struct FewPlan { int slices, slice; bool direct; };
+FewPlan plan_few(const Operand& a, const Operand& b, bool plain) {
+    const double work = double(a.mn) * double(b.mn) * double(a.k);
+    if (f32_exact_only() || a.k == 0) return {0, 0, false};
+    if (plain && a.k <= 32 && b.mn_s == 1 && work < 2.0e9 && a.mn <= 65535 * kFewRows) return {1, kFewStep, true};
+    if (a.mn > 64 || (b.mn_s != 1 && b.k_s != 1) || work >= 3.0e8) return {0, 0, false};
     const int64_t cols = b.mn_s == 1 ? 2 * kFewThreads : 16, steps = (a.k + kFewStep - 1) / kFewStep;
     const int64_t blocks = (b.mn + cols - 1) / cols * ((a.mn + kFewRows - 1) / kFewRows);
     const int64_t want = std::max<int64_t>(1, std::min<int64_t>(steps, 148 * 6 / blocks)), per = (steps + want - 1) / want;
-    return {int((steps + per - 1) / per), int(per * kFewStep)};
+    const int slices = int((steps + per - 1) / per);
+    return {slices, int(per * kFewStep), plain && slices == 1};
 }
-size_t few_bytes(const FewPlan& p, int64_t m, int64_t n) { return round256(size_t(p.slices) * size_t(m) * size_t(n) * 4); }
+size_t few_bytes(const FewPlan& p, int64_t m, int64_t n) { return p.direct ? 0 : round256(size_t(p.slices) * size_t(m) * size_t(n) * 4); }
 int few_product(const Operand& a, const Operand& b, const FewPlan& p, const LinearParams& l, cudaStream_t stream) {
-    void* partial = nullptr;
-    if (int rc = scratch_acquire(&partial, few_bytes(p, a.mn, b.mn), stream)) return rc;
+    void* partial = l.y;
+    if (!p.direct)
+        if (int rc = scratch_acquire(&partial, few_bytes(p, a.mn, b.mn), stream)) return rc;
     const bool along_n = b.mn_s == 1;
     const FewRows f{static_cast<const float*>(a.p), a.mn_s, a.k_s, static_cast<const float*>(b.p), along_n ? b.k_s : b.mn_s,
-                    static_cast<float*>(partial), int(a.mn), int(b.mn), int(a.k), p.slice};
+                    static_cast<float*>(partial), p.direct ? l.y_rs : b.mn, int(a.mn), int(b.mn), int(a.k), p.slice};
     const int cols = along_n ? 2 * kFewThreads : 16;
     const dim3 grid(unsigned((b.mn + cols - 1) / cols), unsigned(p.slices), unsigned((a.mn + kFewRows - 1) / kFewRows));
     if (along_n) few_rows_kernel<true><<<grid, kFewThreads, 0, stream>>>(f);
     else few_rows_kernel<false><<<grid, kFewThreads, 0, stream>>>(f);
     count_launch();
     NTB200_CUDA(cudaGetLastError());
+    if (p.direct) return NTB200_OK;
     const int blocks = int(std::min<int64_t>((a.mn * b.mn + 255) / 256, int64_t(sm_count()) * 16));
     linear_finish_kernel<<<blocks, 256, 0, stream>>>(static_cast<const float*>(partial), p.slices, l, a.mn, int(b.mn));
     count_launch();
@@ -541,9 +549,8 @@ int f16x3_product(const Operand& a, const Operand& b, LinearParams l, cudaStream
 // One plain product of the backward pass: its scratch beyond padded copies.
 size_t product_bytes(const GemmArgs& g, const Operand& a, const Operand& b) {
     if (g.dtype == NTB200_F32) {
-        if (small_f32(g)) return 0;
-        const FewPlan few = plan_few(a, b);
-        return few.slices ? few_bytes(few, a.mn, b.mn) : f16x3_bytes(a, b);
+        const FewPlan few = plan_few(a, b, true);
+        return few.slices ? few_bytes(few, a.mn, b.mn) : small_f32(g) ? 0 : f16x3_bytes(a, b);
     }
     return umma_scratch_bytes(g) + gemv_scratch_bytes(g) + 1024;
 }
@@ -556,9 +563,10 @@ int plain_product(int dtype, Operand a, Operand b, void* c, int64_t c_rs, cudaSt
     // epilogue moves them by rows.  Large Float32 products are three Float16 ones.
     LinearParams l{};
     l.y = c; l.y_rs = c_rs; l.act = NTB200_ACT_NONE; l.out_dtype = dtype;
-    if (dtype == NTB200_F32 && !small_f32(g)) {
-        const FewPlan few = plan_few(a, b);
-        return few.slices ? few_product(a, b, few, l, stream) : f16x3_product(a, b, l, stream);
+    if (dtype == NTB200_F32) {
+        const FewPlan few = plan_few(a, b, true);
+        if (few.slices) return few_product(a, b, few, l, stream);
+        if (!small_f32(g)) return f16x3_product(a, b, l, stream);
     }
     if (dtype != NTB200_F32 && (c_rs % 8 != 0 || !on16(c))) {
         g.linear = &l;
@@ -691,9 +699,8 @@ size_t ntb200_linear_act_workspace_bytes(const ntb200_linear_desc* d) {
     if (check_linear(d) || d->m == 0 || d->n == 0 || d->k == 0) return 0;
     if (d->dtype == NTB200_F32) {
         const GemmArgs g = gemm_of(d->dtype, x_of(*d), w_of(*d), d->y, d->y_row_stride);
-        if (small_f32(g)) return round256(size_t(d->m) * size_t(d->n) * 4);
-        const FewPlan few = plan_few(x_of(*d), w_of(*d));
-        return few.slices ? few_bytes(few, d->m, d->n) : f16x3_bytes(x_of(*d), w_of(*d));
+        const FewPlan few = plan_few(x_of(*d), w_of(*d), false);
+        return few.slices ? few_bytes(few, d->m, d->n) : small_f32(g) ? round256(size_t(d->m) * size_t(d->n) * 4) : f16x3_bytes(x_of(*d), w_of(*d));
     }
     const int es = int(dtype_size(d->dtype));
     GemmArgs g = gemm_of(d->dtype, x_of(*d), w_of(*d), d->y, d->y_row_stride);
@@ -721,6 +728,8 @@ int ntb200_linear_act(const ntb200_linear_desc* d, void* workspace, size_t works
     l.vec_ok = rows16(l.y, l.y_rs) && rows16(l.residual, l.residual_rs) && rows16(l.pre, l.pre_rs) && on16(l.bias) && on16(l.col_scale);
     Operand x = x_of(*d), w = w_of(*d);
     GemmArgs g = gemm_of(d->dtype, x, w, d->y, d->y_row_stride);
+    const FewPlan few = d->dtype == NTB200_F32 ? plan_few(x, w, false) : FewPlan{};
+    if (few.slices) return few_product(x, w, few, l, s);
     if (d->k == 0 || (d->dtype == NTB200_F32 && small_f32(g))) {
         void* z = nullptr;
         if (d->k > 0) {
@@ -734,10 +743,7 @@ int ntb200_linear_act(const ntb200_linear_desc* d, void* workspace, size_t works
         NTB200_CUDA(cudaGetLastError());
         return NTB200_OK;
     }
-    if (d->dtype == NTB200_F32) {
-        const FewPlan few = plan_few(x, w);
-        return few.slices ? few_product(x, w, few, l, s) : f16x3_product(x, w, l, s);
-    }
+    if (d->dtype == NTB200_F32) return f16x3_product(x, w, l, s);
     if (int rc = pad_operands(x, w, int(dtype_size(d->dtype)), s)) return rc;
     g = gemm_of(d->dtype, x, w, d->y, d->y_row_stride);
     g.linear = &l;
