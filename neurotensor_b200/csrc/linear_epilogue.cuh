@@ -266,16 +266,17 @@ __device__ __forceinline__ void lin_set(char* p, float v) {
     else *reinterpret_cast<uint16_t*>(p) = uint16_t(lin_pack2(v, 0.f, kDt));
 }
 
-// What a warp needs besides the products of 32 rows x 32 columns, lane = column: the column's scale and bias and the
-// residuals of its 32 rows.  Loaded before the products are there, all loads on their way together.
+// What a warp needs besides the products of 32 rows x 32 columns, lane = column: the column's scale and bias, the
+// residuals of its 32 rows, and (lane = row) the rows' scales.  Loaded before the products are there, all loads on their way together.
 struct LinearAhead {
-    float cs, bias, res[32];
+    float cs, bias, rs, res[32];
 };
 template <int kDt>
 __device__ __forceinline__ void linear_load_ahead(const LinearParams& l, int m, int n, int row0, int col0, int lane, LinearAhead& a) {
     constexpr int es = kDt == NTB200_F32 ? 4 : 2;
     const int col = col0 + lane;
     const bool in = col < n;
+    a.rs = l.row_scale && row0 + lane < m ? l.row_scale[row0 + lane] : 1.f;
     a.cs = l.col_scale && in ? l.col_scale[col] : 1.f;
     a.bias = l.bias && in ? lin_get<kDt>(static_cast<const char*>(l.bias) + (long long)col * es) : 0.f;
     if (l.residual && in) {
@@ -311,7 +312,7 @@ __device__ __forceinline__ void linear_finish_block(const LinearParams& l, int m
         for (int i = 0; i < 8; ++i) {
             const int r = first + r0 + i;
             f[i] = staged[(r0 + i) * 33 + lane];
-            if (l.row_scale) f[i] = scaled<kDt == NTB200_F32>(f[i], row0 + r < m ? l.row_scale[row0 + r] : 0.f, a.cs);
+            if (l.row_scale) f[i] = scaled<kDt == NTB200_F32>(f[i], __shfl_sync(0xffffffffu, a.rs, r), a.cs);
             f[i] += a.bias;
             if (l.pre && in && row0 + r < m) lin_set<kDt>(pre, f[i]);
             pre += pre_step;

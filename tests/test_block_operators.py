@@ -354,7 +354,7 @@ def linear_tolerance(x64, w64, k, dtype, y64, extra=0.0):
     """Roundings of y = act(z) + r: the fp32 sum of z through a slope of at most 1.13, the fp32 activation (a few 2^-21 of
     its value for 16-bit results, 2^-22 for Float32), the residual's add, one rounding."""
     z_err = (k + 4) * 2.0 ** -23 * (x64.abs() @ w64.abs()) + extra
-    if dtype == F32:      # three TF32 products of parts that carry 21 bits: 3 2^-22 of each product besides
+    if dtype == F32:      # three products of parts that carry 21 bits or more: 3 2^-22 of each product besides
         z_err = z_err + 3 * 2.0 ** -22 * (x64.abs() @ w64.abs())
     return 1.13 * z_err, 2.0 ** -20
 
