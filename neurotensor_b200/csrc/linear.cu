@@ -3,8 +3,9 @@
 // The product runs on the tcgen05 kernels of gemm_umma.cu, whose epilogue does everything that follows the product on
 // the fp32 accumulator (linear_epilogue.cuh): one launch, one rounding, no intermediate in memory but the
 // pre-activation that the backward pass asks for.  Operands that TMA cannot address (rows that do not start on 16
-// bytes) are copied once into padded rows in the caller's workspace; a small Float32 product runs on the exact
-// CUDA-core kernel and is finished by an elementwise pass.
+// bytes) are copied once into padded rows in the caller's workspace.  Float32 has three kernels: few rows (or few terms) on
+// the CUDA cores here, tiny K on the exact CUDA-core kernel, both finished by an elementwise pass, and everything else as
+// three Float16 products on the tensor cores.
 #include <algorithm>
 #include <cstdlib>
 #include <cstring>
@@ -468,8 +469,8 @@ bool f32_exact_only() {
     return exact_only;
 }
 bool small_f32(const GemmArgs& g) { return f32_exact_only() || (g.k <= 32 && double(g.m) * double(g.n) * double(g.k) < 6.0e7); }
-// Slices of K for few_rows_kernel, 0 where another kernel takes the product.  Few rows: 3e8 multiply-adds are about 25 us of it; at
-// [64, 2048] x [2048, 2048] three Float16 products take as long.  Few terms (plain: the weight's gradient of few rows): the result
+// Slices of K for few_rows_kernel, 0 where another kernel takes the product.  Few rows: [64, 2048] x [2048, 2048] (2.7e8 multiply-adds)
+// takes 30 us, as three Float16 products 42; further up the multiply-adds bound it.  Few terms (plain: the weight's gradient of few rows): the result
 // is what has to be written, and it is written once, straight to its place.
 struct FewPlan { int slices, slice; bool direct; };
 FewPlan plan_few(const Operand& a, const Operand& b, bool plain) {
