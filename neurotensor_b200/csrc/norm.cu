@@ -359,6 +359,7 @@ __global__ void __launch_bounds__(kForwardThreads, kForwardBlocks) norm_ring_ker
                     o.put(f + p * V);
                     reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.h) + row * a.cols)[c] = o;
                 } else {
+                    if (a.h) reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.h) + row * a.cols)[c] = x;
 #pragma unroll
                     for (int i = 0; i < V; ++i) f[p * V + i] = x.up(i);
                 }

@@ -1,0 +1,58 @@
+"""The residual feed-forward block's operators at the edges of what their documentation allows: outputs that may be left out or
+given, infinities and NaN, temperatures and operands far from 1, waits that run out, and Float32 products whose low parts matter.
+
+Tolerances.  u = finfo(dtype).eps / 2 is one rounding, relative to the value; a sum of N terms in fp32 is off by at most N 2^-24 of
+the sum of their absolute values.  Where a test says so, errors are bounded by their norm: N independent roundings add up like
+their square root."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+CODES = {F32: "F32", F16: "F16", BF16: "BF16"}
+
+
+def code(dtype):
+    from neurotensor_b200 import _lib
+    return getattr(_lib, CODES[dtype])
+
+
+def generator(seed):
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(seed)
+    return gen
+
+
+def randn(gen, *shape, scale=1.0, dtype=F32):
+    return (torch.randn(*shape, generator=gen, device="cuda") * scale).to(dtype)
+
+
+# ---- norm: h without a residual -------------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("rows,n", [(3, 64), (37, 1999), (2, 40000), (9700, 64), (9600, 264), (2600, 4096), (700, 8192)])   # the last four stream
+def test_h_without_a_residual_is_x(rows, n, dtype, int8):
+    """h = x where no residual is given: a caller that passes memory for h finds x there, whatever the number of rows."""
+    from neurotensor_b200 import _lib, api
+    gen = generator(rows + n)
+    x, w = randn(gen, rows, n, dtype=dtype), randn(gen, n, dtype=dtype)
+    h = torch.full_like(x, 7.0)
+    stat = torch.empty(rows, device="cuda")
+    L = _lib.lib()
+    if int8:
+        y = torch.empty(rows, n, dtype=torch.int8, device="cuda")
+        _lib.check(L.ntb200_rms_norm_int8(code(dtype), x.data_ptr(), n, None, 0, w.data_ptr(), y.data_ptr(), stat.data_ptr(), h.data_ptr(), rows, n,
+                                          1e-6, api._stream()))
+        want = api.rms_norm_int8(x, w)[:2]
+    else:
+        y = torch.empty_like(x)
+        _lib.check(L.ntb200_rms_norm(code(dtype), x.data_ptr(), n, None, 0, w.data_ptr(), y.data_ptr(), h.data_ptr(), stat.data_ptr(), rows, n, 1e-6,
+                                     api._stream()))
+        y_, _, rstd = api.rms_norm(x, w)
+        want = (y_, rstd)
+    assert torch.equal(h, x)
+    assert torch.equal(y, want[0]) and torch.equal(stat, want[1])
