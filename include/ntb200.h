@@ -108,6 +108,10 @@ int ntb200_check_device_status(void* stream);
  * ntb200_check_device_status reports NTB200_ERR_TIMEOUT once; the context stays usable.  Exercises the same bounded
  * wait every GEMM role uses, without faulting or hanging anything. */
 int ntb200_selftest_wait_timeout(unsigned int limit_ms, void* stream);
+/* The same for the norm kernels' rings, whose threads wait in groups of `group_threads` (32, 64, 128 or 256) that meet on
+ * barriers of their own: one block of 512 threads, half of the threads of every odd group waiting in vain at turn 3 of 8.
+ * left_at (device, [512]) receives the turn at which each thread left: 3 for all threads of the odd groups, 8 for the others. */
+int ntb200_selftest_ring_timeout(int group_threads, unsigned int limit_ms, int32_t* left_at, void* stream);
 
 /* ---- storage: replaces DeviceCPU::allocate / release (nt/memory/device.cpp:46-92) with a stream-ordered
  * pool (cudaMallocAsync) on the current device. ---------------------------------------------------------- */

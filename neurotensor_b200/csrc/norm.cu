@@ -282,10 +282,22 @@ __device__ __forceinline__ Pack<T, V> ld_shared_pack(uint32_t addr) {
     return *reinterpret_cast<Pack<T, V>*>(&v);
 }
 
-// The G threads of a group meet: a warp by itself, more than one warp on a named barrier of their own.
-__device__ __forceinline__ void group_sync(int group, int G) {
-    if (G == 32) __syncwarp();
-    else asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(G) : "memory");
+// The G threads of a group meet: a warp by itself, more than one warp on a named barrier of their own.  They agree there on
+// whether any of them gave up waiting, so that they leave together: a flag read after the barrier may be set between the reads of two
+// warps, and the one that stayed would wait at the next barrier, which has no limit, for threads that are gone.
+__device__ __forceinline__ bool group_gave_up(int group, int G, bool mine) {
+    if (G == 32) {
+        __syncwarp();
+        return __any_sync(0xffffffffu, mine);
+    }
+    uint32_t any;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "bar.red.or.pred q, %2, %3, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(any) : "r"(uint32_t(mine)), "r"(group + 1), "r"(G) : "memory");
+    return any != 0;
 }
 
 struct RingShape { int G, stages; unsigned int* status; };
@@ -304,11 +316,12 @@ __device__ __forceinline__ RowRing ring_start(const RingShape& rs, uint32_t smem
     return ring;
 }
 
-// A wait that ran out: the device status word is raised, the block's groups see the flag behind their next barrier,
-// and each group's copying thread waits (bounded again) for the copies still on their way before the block ends.
-__device__ __forceinline__ void ring_gave_up(const RingShape& rs, volatile uint32_t* abort_flag, unsigned int where) {
+// A wait that ran out: the device status word is raised, the flag ends the block's other waits that are still open, each group
+// leaves at its next barrier (group_gave_up), and its copying thread waits (bounded again) for the copies still on their way before
+// the block ends.
+__device__ __forceinline__ void ring_gave_up(unsigned int* status, volatile uint32_t* abort_flag, unsigned int where) {
     *abort_flag = 1;
-    atomicExch(rs.status, 0x100u | where);
+    atomicExch(status, 0x100u | where);
 }
 __device__ __forceinline__ void ring_drain(const RowRing& ring, int stage, uint32_t phase, long long row, long long step, long long rows) {
     volatile uint32_t never = 0;
@@ -343,7 +356,8 @@ __global__ void __launch_bounds__(kForwardThreads, kForwardBlocks) norm_ring_ker
     int flip = 0, stage = 0;
     uint32_t phase = 0;
     for (; row < a.rows; row += step, flip ^= 1) {
-        if (!mbar_wait(ring.bar(stage), phase, &s_abort)) ring_gave_up(rs, &s_abort, 0x41);
+        const bool landed = mbar_wait(ring.bar(stage), phase, &s_abort);
+        if (!landed) ring_gave_up(rs.status, &s_abort, 0x41);
         float f[P * V];
         float sum = 0.f, top = 0.f;
 #pragma unroll
@@ -384,8 +398,7 @@ __global__ void __launch_bounds__(kForwardThreads, kForwardBlocks) norm_ring_ker
             s_sum[flip][warp] = sum;
             if (kOut == kInt8) s_top[flip][warp] = top;
         }
-        group_sync(group, G);     // the row is in registers and its partial sums are in place
-        if (*static_cast<volatile uint32_t*>(&s_abort)) break;
+        if (group_gave_up(group, G, !landed)) break;     // else the row is in registers and its partial sums are in place
         if (t == 0 && row + ring.stages * step < a.rows) load(ring, stage, row + ring.stages * step);
         if (++stage == ring.stages) { stage = 0; phase ^= 1u; }
         if (warps > 1) {
@@ -415,6 +428,28 @@ __global__ void __launch_bounds__(kForwardThreads, kForwardBlocks) norm_ring_ker
         if (t == 0 && a.stat) a.stat[row] = kOut == kInt8 ? __fdiv_rn(__fmul_rn(top, rstd), 127.f) : rstd;
     }
     if (t == 0 && s_abort) ring_drain(ring, stage, phase, row, step, a.rows);
+}
+
+// Self-test of the rings' way out: in every odd group the second half of the threads waits, at turn 3, on a barrier that nothing
+// signals, while the first half has nothing to wait for.  The wait runs out, the status word is raised, and all threads of such a
+// group leave at that turn; the even groups go on to the last.  left_at[thread]: the turn at which it left.
+constexpr int kSelftestTurns = 8, kSelftestStalls = 3;
+__global__ void __launch_bounds__(512) ring_timeout_selftest_kernel(int G, unsigned long long limit_ns, unsigned int* status, int* left_at) {
+    __shared__ __align__(8) unsigned long long s_bar[16];
+    __shared__ uint32_t s_abort;
+    const int group = threadIdx.x / G, t = threadIdx.x - group * G;
+    if (t == 0) mbar_init(smem_u32(&s_bar[group]), 1);
+    if (threadIdx.x == 0) s_abort = 0;
+    fence_barrier_init();
+    __syncthreads();
+    int turn = 0;
+    for (; turn < kSelftestTurns; ++turn) {
+        const bool waits = (group & 1) && t >= G / 2 && turn == kSelftestStalls;
+        const bool landed = !waits || mbar_wait(smem_u32(&s_bar[group]), 0, &s_abort, limit_ns);
+        if (!landed) ring_gave_up(status, &s_abort, 0x43);
+        if (group_gave_up(group, G, !landed)) break;
+    }
+    left_at[threadIdx.x] = turn;
 }
 
 struct BackArgs {
@@ -572,7 +607,8 @@ __global__ void __launch_bounds__(kThreads) norm_backward_ring_kernel(const Back
     const float inv_cols = 1.f / float(a.cols);
     for (; row < a.rows; row += step, flip ^= 1) {
         const float rstd = a.rstd[row];
-        if (!mbar_wait(ring.bar(stage), phase, &s_abort)) ring_gave_up(rs, &s_abort, 0x42);
+        const bool landed = mbar_wait(ring.bar(stage), phase, &s_abort);
+        if (!landed) ring_gave_up(rs.status, &s_abort, 0x42);
         Pack<T, V> h[P], gy[P], gh[P];
         float dot = 0.f;
 #pragma unroll
@@ -592,8 +628,7 @@ __global__ void __launch_bounds__(kThreads) norm_backward_ring_kernel(const Back
         }
         dot = warp_sum(dot);
         if (warps > 1 && lane == 0) s_dot[flip][warp] = dot;
-        group_sync(group, G);
-        if (*static_cast<volatile uint32_t*>(&s_abort)) break;
+        if (group_gave_up(group, G, !landed)) break;
         if (t == 0 && row + ring.stages * step < a.rows) load(ring, stage, row + ring.stages * step);
         if (++stage == ring.stages) { stage = 0; phase ^= 1u; }
         if (warps > 1) dot = warp_sum(lane < warps ? s_dot[flip][first_warp + lane] : 0.f);
@@ -978,6 +1013,16 @@ int ntb200_rms_norm_int8(int dtype, const void* x, int64_t x_row_stride, const v
 
 int ntb200_quantize_rows(int dtype, const void* x, int64_t x_row_stride, int8_t* q, float* scale, int64_t rows, int64_t cols, void* stream) {
     return norm_forward("quantize_rows", dtype, x, x_row_stride, nullptr, 0, nullptr, q, true, nullptr, scale, rows, cols, 0.0, stream);
+}
+
+int ntb200_selftest_ring_timeout(int group_threads, unsigned int limit_ms, int32_t* left_at, void* stream) {
+    const bool known = group_threads == 32 || group_threads == 64 || group_threads == 128 || group_threads == 256;
+    if (!known || limit_ms == 0 || limit_ms > 1000 || !left_at)
+        return fail(NTB200_ERR_INVALID_ARG, "selftest_ring_timeout: groups of 32, 64, 128 or 256 threads, a limit of 1..1000 ms, and 512 results");
+    ring_timeout_selftest_kernel<<<1, 512, 0, static_cast<cudaStream_t>(stream)>>>(group_threads, 1000000ull * limit_ms, device_status_word(), left_at);
+    count_launch();
+    NTB200_CUDA(cudaGetLastError());
+    return NTB200_OK;
 }
 
 size_t ntb200_rms_norm_backward_workspace_bytes(int64_t rows, int64_t cols) {

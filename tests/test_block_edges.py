@@ -56,3 +56,27 @@ def test_h_without_a_residual_is_x(rows, n, dtype, int8):
         want = (y_, rstd)
     assert torch.equal(h, x)
     assert torch.equal(y, want[0]) and torch.equal(stat, want[1])
+
+
+# ---- norm: a wait that runs out --------------------------------------------------------------------------------------
+
+def test_ring_selftest_refusals():
+    from neurotensor_b200 import _lib
+    L = _lib.lib()
+    for args in ((48, 20, 16), (512, 20, 16), (64, 0, 16), (64, 1001, 16), (64, 20, None)):
+        assert L.ntb200_selftest_ring_timeout(*args, None) == _lib.ERR_INVALID_ARG, args
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group", [32, 64, 128, 256])
+def test_ring_groups_leave_together(group):
+    """A wait of the norm rings that runs out for some threads of a group ends the turn for all of them, and only for them."""
+    from neurotensor_b200 import _lib, api
+    L = _lib.lib()
+    left = torch.full((512,), -1, dtype=torch.int32, device="cuda")
+    _lib.check(L.ntb200_selftest_ring_timeout(group, 20, left.data_ptr(), api._stream()))
+    assert L.ntb200_check_device_status(api._stream()) == _lib.ERR_TIMEOUT
+    assert left.view(-1, group).tolist() == [[3 if g % 2 else 8] * group for g in range(512 // group)]
+    assert L.ntb200_check_device_status(api._stream()) == _lib.OK          # reported once
+    x, w = torch.ones(9600, 264, device="cuda"), torch.ones(264, device="cuda")
+    assert float((api.rms_norm(x, w)[0] - 1).abs().max()) < 1e-6           # the context works on
