@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(kPieceThreads, kBlocks) distill_piece_kernel(c
     for (int i = 0; i < C; ++i) {
         const float4 q = sh.share[i];
         const float d = q.x == -INFINITY ? 0.f : q.x - gm;
-        gz += q.x == -INFINITY && gm != -INFINITY ? 0.f : q.y * exp2f(d * c);
+        gz += q.y * exp2f(d * c);        // an empty piece's sum is 0; one of nothing but NaN has the maximum of an empty one, and a NaN
         cross += q.w == 0.f ? q.z : q.z + q.w * (d * inv_temp);   // sum p (x - gm) / T; a piece far below may have an infinite d
     }
     if (gm == -INFINITY) gz = NAN;       // every column of the student masked out

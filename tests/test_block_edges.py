@@ -80,3 +80,25 @@ def test_ring_groups_leave_together(group):
     assert L.ntb200_check_device_status(api._stream()) == _lib.OK          # reported once
     x, w = torch.ones(9600, 264, device="cuda"), torch.ones(264, device="cuda")
     assert float((api.rms_norm(x, w)[0] - 1).abs().max()) < 1e-6           # the context works on
+
+
+# ---- distillation ----------------------------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("rows,vocab", [(3, 1000), (3, 40000), (3, 131072), (500, 131072), (2, 450001)])
+@pytest.mark.parametrize("rest", ["nothing", "-inf"])
+def test_distill_nan_in_a_whole_piece(rows, vocab, dtype, rest):
+    """NaN in half of a row, alone or among -inf, is the row's answer however the row is cut into pieces; other rows keep theirs."""
+    from neurotensor_b200 import api
+    gen = generator(vocab)
+    s = randn(gen, rows, vocab, dtype=dtype)
+    t, i = randn(gen, rows, 4), torch.randint(0, vocab // 4, (rows, 4), generator=gen, device="cuda")
+    clean = api.distill_topk(s, t, i)
+    s[1, vocab // 2:] = math.nan
+    if rest == "-inf":
+        s[1, vocab // 2 + 1:] = -math.inf
+    loss, row, grad = api.distill_topk(s, t, i)
+    assert math.isnan(float(loss)) and math.isnan(float(row[1])) and bool(torch.isnan(grad[1]).all())
+    for r in (0, 2 if rows > 2 else 0):
+        assert torch.equal(row[r], clean[1][r]) and torch.equal(grad[r], clean[2][r])
