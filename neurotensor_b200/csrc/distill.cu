@@ -41,6 +41,9 @@ __device__ __forceinline__ void join(float& m, float& z, float m2, float z2, flo
     m = top;
 }
 
+// T^2 (logs - cross / T) without T^2 and x / T, which leave the type's range at temperatures and logits whose loss does not.
+__device__ __forceinline__ float row_loss_of(float temp, float logs, float cross) { return temp * (temp * logs - cross); }
+
 template <int kThreads>
 struct RowShared {
     float p[kMaxTop], x[kMaxTop];        // teacher's probabilities, the student's logits at the same places
@@ -173,7 +176,7 @@ __global__ void __launch_bounds__(kPieceThreads, kBlocks) distill_piece_kernel(c
     const int tid = threadIdx.x, lane = tid & 31;
     const uint32_t rank = C > 1 ? cluster_cta_rank() : 0u;
     const long long row = blockIdx.x / C;
-    const float c = kLog2e / a.temp, inv_temp = 1.f / a.temp;
+    const float c = kLog2e / a.temp;
     const int first = int(rank) * piece, count = max(0, min(piece, a.vocab - first));
     const T* s = static_cast<const T*>(a.s) + row * a.s_rs + first;
     T* grad = a.grad ? static_cast<T*>(a.grad) + row * a.g_rs + first : nullptr;
@@ -233,7 +236,7 @@ __global__ void __launch_bounds__(kPieceThreads, kBlocks) distill_piece_kernel(c
     float tsums[1] = {0.f};
     for (int j = tid; j < a.top; j += kPieceThreads) tsums[0] += sh_p[j] == -INFINITY ? 0.f : exp2f((sh_p[j] - tmax) * c);
     piece_sums(tsums, sh);
-    float sums[4] = {0.f, 0.f, 0.f, 0.f};   // sum p log2 p, and this piece's z, sum p and sum p (x - m) / T
+    float sums[4] = {0.f, 0.f, 0.f, 0.f};   // sum p log2 p, and this piece's z, sum p and sum p (x - m)
     const float log2t = log2f(tsums[0]);
     for (int j = tid; j < a.top; j += kPieceThreads) {
         const float t = sh_p[j];
@@ -266,7 +269,7 @@ __global__ void __launch_bounds__(kPieceThreads, kBlocks) distill_piece_kernel(c
         if (sh_at[j] < 0) continue;
         if (p != 0.f) {
             sums[2] += p;
-            sums[3] += p * ((RowType<T>::up(mem[sh_at[j] + lead]) - ref) * inv_temp);
+            sums[3] += p * (RowType<T>::up(mem[sh_at[j] + lead]) - ref);
         }
     }
     float z0 = 0.f, z1 = 0.f;
@@ -330,7 +333,7 @@ __global__ void __launch_bounds__(kPieceThreads, kBlocks) distill_piece_kernel(c
         const float4 q = sh.share[i];
         const float d = q.x == -INFINITY ? 0.f : q.x - gm;
         gz += q.y * exp2f(d * c);        // an empty piece's sum is 0; one of nothing but NaN has the maximum of an empty one, and a NaN
-        cross += q.w == 0.f ? q.z : q.z + q.w * (d * inv_temp);   // sum p (x - gm) / T; a piece far below may have an infinite d
+        cross += q.w == 0.f ? q.z : q.z + q.w * d;   // sum p (x - gm); a piece far below may have an infinite d
     }
     if (gm == -INFINITY) gz = NAN;       // every column of the student masked out
     if (!present) {
@@ -338,7 +341,7 @@ __global__ void __launch_bounds__(kPieceThreads, kBlocks) distill_piece_kernel(c
         if (rank == 0 && tid == 0) a.row_loss[row] = 0.f;
         return;
     }
-    if (rank == 0 && tid == 0) a.row_loss[row] = a.temp * a.temp * ((entropy + log2f(gz)) / kLog2e - cross);
+    if (rank == 0 && tid == 0) a.row_loss[row] = row_loss_of(a.temp, (entropy + log2f(gz)) / kLog2e, cross);
     if (!grad) return;
     const float coef = weight * a.temp, scale = coef / gz;
     // q times its factor: for 16-bit gradients one multiply-add and one exponential, the factor inside the exponent
@@ -467,13 +470,13 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(const DistillArgs a) 
             if (sh.at[j] >= 0) {
                 const float lt = (sh.p[j] - tmax) * c;
                 p = exp2f(lt) / tsum;
-                if (p > 0.f) loss += p * (((lt - log2f(tsum)) + log2z) / kLog2e - (sh.x[j] - m) / a.temp);
+                if (p > 0.f) loss += p * (a.temp * (((lt - log2f(tsum)) + log2z) / kLog2e) - (sh.x[j] - m));
                 else if (!(p == 0.f)) loss = p;
             }
             sh.p[j] = p;
         }
         loss = block_sum<kThreads>(loss, sh.red_z);
-        if (tid == 0) a.row_loss[row] = a.temp * a.temp * loss;
+        if (tid == 0) a.row_loss[row] = a.temp * loss;
         if (!grad) continue;
         const float coef = weight * a.temp, scale = coef / z;
         for (int v = tid; v < nv; v += kThreads) {

@@ -102,3 +102,54 @@ def test_distill_nan_in_a_whole_piece(rows, vocab, dtype, rest):
     assert math.isnan(float(loss)) and math.isnan(float(row[1])) and bool(torch.isnan(grad[1]).all())
     for r in (0, 2 if rows > 2 else 0):
         assert torch.equal(row[r], clean[1][r]) and torch.equal(grad[r], clean[2][r])
+
+
+def distill64(s, t, i, T, rw):
+    """(loss, row losses, gradient, the size of the gradient's two parts) in 64 bits; every entry is there."""
+    lq = torch.log_softmax(s.double() / T, 1)
+    lp = torch.log_softmax(t.double() / T, 1)
+    p = lp.exp()
+    terms = torch.where(p > 0, p * ((t.double() - t.double().amax(1, keepdim=True)) / T -
+                                    ((t.double() - t.double().amax(1, keepdim=True)) / T).exp().sum(1, keepdim=True).log() - lq.gather(1, i)), torch.zeros_like(p))
+    full = torch.zeros_like(lq).scatter_add_(1, i, p)
+    c = T * rw.double()[:, None]
+    return (T * T * terms.sum(1) * rw.double()).sum(), T * T * terms.sum(1), c * (lq.exp() - full), c * (lq.exp() + full)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("vocab", [64, 40000, 131072, 450000])
+@pytest.mark.parametrize("T", [1e-30, 1e-20, 1e-3, 1e6, 1e15])
+def test_distill_temperatures_far_from_one(T, vocab, dtype):
+    """T^2 and logits / T may leave the type's range where the loss, T^2 log V or T times a difference of logits, does not."""
+    from neurotensor_b200 import api
+    gen = generator(vocab)
+    s, t = randn(gen, 5, vocab, scale=3.0, dtype=dtype), randn(gen, 5, 6, scale=3.0)
+    i = torch.stack([torch.randperm(vocab, generator=gen, device="cuda")[:6] for _ in range(5)])
+    rw = torch.tensor([0.5, 0.25, 1.0, 0.125, 0.0625], device="cuda")
+    loss, row, grad = api.distill_topk(s, t, i, temperature=T, row_weight=rw)
+    loss64, row64, grad64, size = distill64(s, t, i, T, rw)
+    # exponents up to 2^6 matter: their fp32 rounding is 2^-18 of each probability; sums of vocab terms add their own
+    e = 2.0 ** -17 + 2.0 ** -24 * min(vocab, 4096)
+    scale = T * T * (1 + math.log(vocab + 1)) + 2 * T * float(s.float().abs().max() + t.abs().max())
+    assert bool(((row.double() - row64).abs() <= e * scale).all()), (row, row64)
+    assert abs(float(loss) - float(loss64)) <= e * scale * 2
+    u = torch.finfo(dtype).eps / 2
+    assert bool(((grad.double() - grad64).abs() <= u * (1 + 2.0 ** -7) * grad64.abs() + e * size + 2.0 ** -126).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [64, 40000, 131072, 450000])
+@pytest.mark.parametrize("T", [0.25, 0.5])
+def test_distill_teacher_names_a_column_of_the_lowest_value(T, vocab):
+    """The row's loss, T p times the lowest Float32, is finite although that logit / T is not."""
+    from neurotensor_b200 import api
+    gen = generator(vocab)
+    s = randn(gen, 2, vocab)
+    i = torch.tensor([[1, vocab - 2, 7], [3, 4, 5]], device="cuda")
+    s[0, vocab - 2] = torch.finfo(F32).min
+    t = torch.zeros(2, 3, device="cuda")
+    loss, row, grad = api.distill_topk(s, t, i, temperature=T)
+    want = -T / 3 * torch.finfo(F32).min
+    assert abs(float(row[0]) - want) <= 2.0 ** -20 * want and abs(float(loss) - want / 2) <= 2.0 ** -20 * want
+    assert bool(torch.isfinite(grad).all())
