@@ -456,7 +456,7 @@ int ntb200_sum_channels(int dtype, const void* grad, void* out, int64_t batch, i
  * contiguous.  residual, h and rstd may be NULL; h may be the residual or x itself (same row stride).
  * ntb200_rms_norm_int8: the same y as Int8 rows with one scale each: with u = h * weight and A = max |u|,
  * q = rint(u * 127 / A) and scale = A * rstd / 127, so y = q * scale.  A row of zeros has scale 0; a row with a NaN or
- * an infinity has a scale that is not finite.
+ * an infinity has values of 0 and a scale that is not finite.
  * ntb200_quantize_rows: q = rint(x * 127 / A), scale = A / 127 without any norm (hidden activations; weights, once).
  * ntb200_rms_norm_backward: from h and rstd of the forward call, grad_y = dL/dy and grad_h = dL/dh over the residual
  * stream (NULL: nothing arrives there): grad_x = dL/dx, which is also the residual's gradient, and grad_weight (may be

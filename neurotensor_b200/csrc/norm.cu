@@ -30,17 +30,18 @@ struct RowArgs {
     float eps;
 };
 
-// q = rint(u * 127 / A), which lies within +-127 but for roundings; a row of zeros gives zeros, a NaN gives 0 (its row's
-// scale is NaN, so the product that reads it still is).  A below 2^-100 is scaled up first: 127 / A would overflow.
+// q = rint(u * 127 / A), which lies within +-127 but for roundings; a row of zeros gives zeros, and so does a row with a NaN or
+// an infinity (its scale is not finite, so the product that reads it is NaN).  A below 2^-100 is scaled up first: 127 / A would
+// overflow.
 struct Quant {
     float up, inv;
     __device__ __forceinline__ explicit Quant(float top) {
         up = top < 0x1p-100f ? 0x1p100f : 1.f;
-        inv = top > 0.f ? __fdiv_rn(127.f, __fmul_rn(top, up)) : (top == 0.f ? 0.f : top);
+        inv = top > 0.f && top < INFINITY ? __fdiv_rn(127.f, __fmul_rn(top, up)) : (top == 0.f ? 0.f : NAN);
     }
     // V values, packed.  Adding 1.5 2^23 rounds to a whole number (ties to even, as rint does) and leaves it in the low byte
     // of the sum's bits: no conversion, which the hardware does at a quarter of the rate.  127 (1 + 2^-22) at most comes out
-    // of the product, so no value needs a clamp; a NaN's quotient is replaced, its low byte could be anything.
+    // of the product, so no value needs a clamp; NaN quotients are replaced, their low byte could be anything.
     template <int V>
     __device__ __forceinline__ void put(Pack<int8_t, V>& o, const float* u) const {
         uint32_t q[V];
@@ -50,7 +51,7 @@ struct Quant {
 #pragma unroll
             for (int i = 0; i < V; ++i) q[i] = __float_as_uint(__fadd_rn(__fmul_rn(__fmul_rn(u[i], up), inv), 12582912.f));
         }
-        if (!(fabsf(inv) < INFINITY)) {   // a NaN in the row
+        if (!(fabsf(inv) < INFINITY)) {   // a NaN or an infinity in the row
 #pragma unroll
             for (int i = 0; i < V; ++i) q[i] = 0;
         }

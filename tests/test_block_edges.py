@@ -58,6 +58,25 @@ def test_h_without_a_residual_is_x(rows, n, dtype, int8):
     assert torch.equal(y, want[0]) and torch.equal(stat, want[1])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("rows,n", [(3, 64), (37, 1999), (3, 40000), (9600, 264), (2600, 4096)])
+def test_int8_row_that_is_not_finite(rows, n, dtype, bad, norm):
+    """Its values are zeros and its scale is not finite, so everything that is made from it is NaN, never an infinity of a sign of its own."""
+    from neurotensor_b200 import api
+    gen = generator(n)
+    x = randn(gen, rows, n, dtype=dtype)
+    x[1, n - 1] = bad
+    q, scale = api.rms_norm_int8(x, randn(gen, n, dtype=dtype))[:2] if norm else api.quantize_rows(x)
+    assert not bool(q[1].any()) and not math.isfinite(float(scale[1]))
+    assert bool(q[0].any()) and bool(q[2].any()) and bool(torch.isfinite(scale[0])) and bool(torch.isfinite(scale[2]))
+    w = torch.ones(4, n, dtype=torch.int8, device="cuda")
+    y = api.linear_int8(q[:3], scale[:3], w, torch.ones(4, device="cuda"), transpose_w=True)
+    assert bool(torch.isnan(y[1]).all()) and bool(torch.isfinite(y[0]).all()) and bool(torch.isfinite(y[2]).all())
+
+
 # ---- norm: a wait that runs out --------------------------------------------------------------------------------------
 
 def test_ring_selftest_refusals():
