@@ -482,7 +482,8 @@ int ntb200_rms_norm_backward(int dtype, const void* h, int64_t h_row_stride, con
  * whose rows do not start on 16 bytes are copied into the workspace first.  F32 products over K > 32, or of 6e7
  * multiply-adds and more, run there too, as three products of Float16 parts: an fp32 product's error as long as the
  * values of a row of x (a column of w) lie within 2^13 of its largest one; smaller ones keep 2^-39 of that largest one.
- * An infinite operand may give a NaN where its product alone is infinite. */
+ * An infinite value times one of those below 2^-39 of its row's (column's) largest may give NaN there; all other products with
+ * infinities and NaN are those of fp32. */
 typedef enum ntb200_activation {
     NTB200_ACT_NONE = 0,
     NTB200_ACT_RELU = 1,

@@ -172,13 +172,14 @@ __device__ __forceinline__ float split_scale(float top, float* unscale) {
     *unscale = __uint_as_float(uint32_t(254 - bits) << 23);
     return __uint_as_float(uint32_t(bits) << 23);
 }
-// Both parts of a pair of values.  An infinity or a NaN stays in the high part.
+// Both parts of a pair of values.  An infinity is the largest Float16 of its sign and an infinite low part: its one infinite
+// product is with the other value's high part, so the sum is the product's infinity (infinite high parts would meet low parts of
+// zero or of the other sign).  A NaN's low part is NaN.
 __device__ __forceinline__ void split_pair(float x, float y, float scale, __half2& hi, __half2& lo) {
     x *= scale;
     y *= scale;
-    hi = __floats2half2_rn(x, y);
-    const float hx = __low2float(hi), hy = __high2float(hi);
-    lo = __floats2half2_rn(fabsf(hx) < INFINITY ? x - hx : 0.f, fabsf(hy) < INFINITY ? y - hy : 0.f);
+    hi = __floats2half2_rn(fminf(fmaxf(x, -65504.f), 65504.f), fminf(fmaxf(y, -65504.f), 65504.f));
+    lo = __floats2half2_rn(x - __low2float(hi), y - __high2float(hi));
 }
 __device__ __forceinline__ float max_finite(float top, float x) {
     const float a = fabsf(x);

@@ -172,3 +172,47 @@ def test_distill_teacher_names_a_column_of_the_lowest_value(T, vocab):
     want = -T / 3 * torch.finfo(F32).min
     assert abs(float(row[0]) - want) <= 2.0 ** -20 * want and abs(float(loss) - want / 2) <= 2.0 ** -20 * want
     assert bool(torch.isfinite(grad).all())
+
+
+# ---- linear in Float32 -----------------------------------------------------------------------------------------------
+
+def infinite_pattern(x, w):
+    """x @ w in 64 bits; where a row of x or a column of w holds infinities or NaN, from its products one by one."""
+    y = torch.nan_to_num(x, 0, 0, 0).double() @ torch.nan_to_num(w, 0, 0, 0).double()
+    for r in (~torch.isfinite(x)).any(1).nonzero().flatten().tolist():
+        y[r] = (x[r].double()[:, None] * w.double()).sum(0)
+    for c in (~torch.isfinite(w)).any(0).nonzero().flatten().tolist():
+        y[:, c] = (x.double() * w[:, c].double()).sum(1)
+    return y
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("transpose", [False, True])
+@pytest.mark.parametrize("m,k,n", [(5, 40, 33), (100, 24, 33), (200, 257, 300), (300, 2048, 513), (2600, 300, 4104)])
+def test_float32_infinities(m, k, n, transpose):
+    """Infinite and NaN operands give what fp32 products and sums give, on every route that a size may take."""
+    from neurotensor_b200 import api
+    gen = generator(m + k)
+    x, w = randn(gen, m, k), randn(gen, k, n)
+    w = torch.where(w.abs() < 2.0 ** -10, torch.ones_like(w), w)      # far from the low parts' end
+    x = torch.where(x.abs() < 2.0 ** -10, torch.ones_like(x), x)
+    x[0, 3], x[1, k - 1], x[2, 0], x[2, 9], x[3, 5], x[3, 6], x[4, 11] = math.inf, -math.inf, math.inf, math.inf, math.inf, -math.inf, math.nan
+    w[3, 7] = 0.0                                                      # inf times 0
+    w[3, 1], w[8, 2] = math.inf, -math.inf                             # one of them meets x[0, 3]
+    y = api.linear_act(x, w.t().contiguous() if transpose else w, transpose_w=transpose)
+    want = infinite_pattern(x, w)
+    for kind in (torch.isnan, torch.isposinf, torch.isneginf):
+        assert torch.equal(kind(y), kind(want)), kind.__name__
+    fine = torch.isfinite(want)
+    size = torch.nan_to_num(x, 0, 0, 0).double().abs() @ torch.nan_to_num(w, 0, 0, 0).double().abs()
+    assert bool(((y.double() - want).abs()[fine] <= ((k + 4) * 2.0 ** -23 + 3 * 2.0 ** -22) * size[fine]).all())
+    # a gradient that overflowed: columns of gx's terms are infinite
+    gy = randn(gen, m, n)
+    gy = torch.where(gy.abs() < 2.0 ** -10, torch.ones_like(gy), gy)
+    gy[0, 0] = math.inf
+    clean = torch.nan_to_num(w, 1.0, 1.0, 1.0)
+    gx, gw, gb = api.linear_act_backward(torch.nan_to_num(x, 1.0, 1.0, 1.0), clean.t().contiguous() if transpose else clean, None, gy, transpose_w=transpose)
+    assert torch.equal(gx[0].double(), math.inf * clean[:, 0].double()) and bool(torch.isfinite(gx[1:]).all())
+    gw = gw.t() if transpose else gw
+    assert torch.equal(gw[:, 0].double(), math.inf * torch.nan_to_num(x, 1.0, 1.0, 1.0)[0].double()) and bool(torch.isfinite(gw[:, 1:]).all())
+    assert math.isinf(float(gb[0])) and bool(torch.isfinite(gb[1:]).all())
