@@ -417,6 +417,11 @@ inline void to_numpy(const Tensor& t, const std::string& path) {
 enum class Activation : int { None = NTB200_ACT_NONE, ReLU = NTB200_ACT_RELU, GELU = NTB200_ACT_GELU, GELUTanh = NTB200_ACT_GELU_TANH, SiLU = NTB200_ACT_SILU };
 
 namespace detail {
+// The kernels read their operands' addresses on the device: a host tensor among them (nullptr or a null one: not given) is refused.
+inline void check_on_device(const char* what, std::initializer_list<const Tensor*> given) {
+    for (const Tensor* t : given)
+        utils::throw_exception(!t || t->is_null() || t->device() == DeviceType::CUDA, what, ": expected tensors on DeviceType::CUDA");
+}
 // Rows of the last dim, contiguous.
 inline Tensor rows_of(const Tensor& t, const char* what) {
     utils::throw_exception(!t.is_null() && t.device() == DeviceType::CUDA, what, ": expected tensors on DeviceType::CUDA");
@@ -429,6 +434,7 @@ inline SizeRef row_shape(const Tensor& t) {
     return SizeRef(s);
 }
 inline void check_norm(const Tensor& x, const Tensor& weight, const Tensor* residual, const char* what) {
+    check_on_device(what, {&weight, residual});
     utils::throw_exception(weight.dims() == 1 && weight.shape()[0] == x.shape()[-1] && weight.dtype() == x.dtype(), what, ": expected a weight of ",
                            x.shape()[-1], " values of ", dtype_name(x.dtype()), " but got ", weight.shape());
     utils::throw_exception(!residual || (residual->shape() == x.shape() && residual->dtype() == x.dtype()), what,
@@ -482,6 +488,7 @@ namespace detail {
 inline Tensor run_linear(const char* what, const Tensor& x, const Tensor& weight, const Tensor& bias, Activation act, const Tensor& residual,
                          bool trans_weight, DType out, const Tensor* x_scale, const Tensor* w_scale, Tensor* pre) {
     Tensor xc = rows_of(x, what);
+    check_on_device(what, {&bias, &residual, x_scale, w_scale});
     utils::throw_exception(weight.dims() == 2 && weight.device() == DeviceType::CUDA && weight.dtype() == x.dtype(), what,
                            ": expected a 2-D weight of ", dtype_name(x.dtype()), " but got ", weight.shape());
     const int64_t k = trans_weight ? weight.shape()[1] : weight.shape()[0], n = trans_weight ? weight.shape()[0] : weight.shape()[1];

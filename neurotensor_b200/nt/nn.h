@@ -461,6 +461,7 @@ inline ScalarGrad MSE(const TensorGrad& output, const Tensor& target) {
 inline ScalarGrad DistillTopK(const TensorGrad& output, const Tensor& teacher, const Tensor& index, double temperature = 1.0,
                               const Tensor& row_weight = Tensor()) {
     Tensor o = functional::detail::rows_of(output.detach(), "DistillTopK"), t = teacher.contiguous(), i = index.contiguous();
+    functional::detail::check_on_device("DistillTopK", {&teacher, &index, &row_weight});
     const int64_t vocab = o.shape()[-1], rows = o.numel() / vocab, top = t.shape()[-1];
     utils::throw_exception(t.shape() == i.shape() && t.numel() == rows * top, "DistillTopK: shapes ", o.shape(), ", ", t.shape(), " and ", i.shape(),
                            " do not belong together");
