@@ -453,7 +453,7 @@ int ntb200_sum_channels(int dtype, const void* grad, void* out, int64_t batch, i
  *
  * ntb200_rms_norm: h = x + residual (h = x without one), rstd = (mean(h^2) + eps)^-1/2, y = h * rstd * weight for each
  * of `rows` rows.  Sums and the norm use the unrounded fp32 h; y and h are rounded once.  F32, F16, BF16; y and h are
- * contiguous.  residual, h and rstd may be NULL; h may be the residual or x itself (same row stride).
+ * contiguous.  residual, h and rstd may be NULL; h, or else y, may be the residual or x itself (same row stride).
  * ntb200_rms_norm_int8: the same y as Int8 rows with one scale each: with u = h * weight and A = max |u|,
  * q = rint(u * 127 / A) and scale = A * rstd / 127, so y = q * scale.  A row of zeros has scale 0; a row with a NaN or
  * an infinity has values of 0 and a scale that is not finite.

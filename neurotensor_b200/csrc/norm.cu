@@ -984,6 +984,8 @@ static int norm_forward(const char* what, int dtype, const void* x, int64_t x_rs
         return fail(NTB200_ERR_INVALID_ARG, "%s: a row stride is shorter than a row", what);
     if (rows > 1 && h && ((h == x && x_rs != cols) || (h == r && r_rs != cols)))
         return fail(NTB200_ERR_INVALID_ARG, "%s: h in the place of an input must have its row stride (h is contiguous)", what);
+    if (y == h || (int8 && (y == x || y == r)) || (rows > 1 && ((y == x && x_rs != cols) || (y == r && r_rs != cols))))
+        return fail(NTB200_ERR_INVALID_ARG, "%s: the output in the place of h, or of an input whose rows lie elsewhere", what);
     const int es = int(dtype_size(dtype));
     RowLayout layout;
     layout.add(x, x_rs * es);

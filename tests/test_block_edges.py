@@ -29,6 +29,41 @@ def randn(gen, *shape, scale=1.0, dtype=F32):
     return (torch.randn(*shape, generator=gen, device="cuda") * scale).to(dtype)
 
 
+# ---- norm: outputs in the place of others ----------------------------------------------------------------------------
+
+def test_norm_outputs_that_overlap_are_refused():
+    from neurotensor_b200 import _lib
+    L = _lib.lib()
+    a, b, c, w, s = (ctypes.c_void_p(64 * k) for k in range(1, 6))
+    calls = {"y is h": lambda: L.ntb200_rms_norm(_lib.F32, a, 8, b, 8, w, c, c, s, 2, 8, 1e-6, None),
+             "y is x, rows apart": lambda: L.ntb200_rms_norm(_lib.F32, a, 9, None, 0, w, a, None, s, 2, 8, 1e-6, None),
+             "y is the residual, rows apart": lambda: L.ntb200_rms_norm(_lib.F32, a, 8, b, 9, w, b, None, s, 2, 8, 1e-6, None),
+             "q is x": lambda: L.ntb200_rms_norm_int8(_lib.F32, a, 8, None, 0, w, a, s, None, 2, 8, 1e-6, None),
+             "q is the residual": lambda: L.ntb200_rms_norm_int8(_lib.F32, a, 8, b, 8, w, b, s, None, 2, 8, 1e-6, None),
+             "q is h": lambda: L.ntb200_rms_norm_int8(_lib.F32, a, 8, b, 8, w, c, s, c, 2, 8, 1e-6, None),
+             "q is the quantised rows": lambda: L.ntb200_quantize_rows(_lib.F16, a, 8, a, s, 2, 8, None)}
+    for what, call in calls.items():
+        assert call() == _lib.ERR_INVALID_ARG, what
+        assert b"in the place of" in L.ntb200_last_error_string(), what
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,n", [(5, 64), (5, 16383), (3, 40000), (2600, 4096), (9600, 264)])
+@pytest.mark.parametrize("place", ["x", "residual"])
+def test_norm_in_place_of_an_input(rows, n, place):
+    """y may be x or the residual itself."""
+    from neurotensor_b200 import _lib, api
+    gen = generator(n)
+    x, r, w = randn(gen, rows, n, dtype=BF16), randn(gen, rows, n, dtype=BF16), randn(gen, n, dtype=BF16)
+    results = []
+    for y in (torch.empty_like(x), x if place == "x" else r):
+        rstd = torch.empty(rows, device="cuda")
+        _lib.check(_lib.lib().ntb200_rms_norm(_lib.BF16, x.data_ptr(), n, r.data_ptr(), n, w.data_ptr(), y.data_ptr(), None, rstd.data_ptr(), rows, n,
+                                              1e-6, api._stream()))
+        results.append((y, rstd))
+    assert torch.equal(results[0][0], results[1][0]) and torch.equal(results[0][1], results[1][1])
+
+
 # ---- norm: h without a residual -------------------------------------------------------------------------------------
 
 @pytest.mark.gpu
