@@ -251,3 +251,99 @@ def test_float32_infinities(m, k, n, transpose):
     gw = gw.t() if transpose else gw
     assert torch.equal(gw[:, 0].double(), math.inf * torch.nan_to_num(x, 1.0, 1.0, 1.0)[0].double()) and bool(torch.isfinite(gw[:, 1:]).all())
     assert math.isinf(float(gb[0])) and bool(torch.isfinite(gb[1:]).all())
+
+
+def f16_parts(x, dim):
+    """The two Float16 parts (in fp32) of a matrix whose rows along `dim` are scaled so that their largest value lies in [2^14, 2^15)."""
+    scale = 2.0 ** (14 - torch.floor(torch.log2(x.abs().amax(dim, keepdim=True))))
+    v = x * scale
+    hi = v.half().float()
+    return hi / scale, (v - hi).half().float() / scale
+
+
+# Error of a Float32 product as three Float16 products, by its norm, relative to the result's.  A partial sum takes 24 adds (8 steps of
+# 16 along K, three products each), each cut off after 24 bits, by half a step of 2^-23 on average, while it grows to its size, so
+# that an add meets 2/3 of it on average: 24 * 2^-24 * 2/3 = 2^-20.  The parts (2^-23 a value), lo.lo and the fp32 adds of the
+# partial sums stay below 2^-22 together, errors of independent terms being summed by their squares.
+THREE_PRODUCTS = 2.0 ** -20 + 2.0 ** -22
+
+
+def relative_norm(got, want):
+    return float((got.double() - want).norm() / want.norm())
+
+
+def test_float32_bound_sees_a_lost_low_part():
+    """Without the low part of either operand, or of an eighth of its terms, the product misses that bound by far."""
+    gen = torch.Generator().manual_seed(1)
+    x, w = torch.randn(64, 1024, generator=gen), torch.randn(1024, 64, generator=gen)
+    want = x.double() @ w.double()
+    (xh, xl), (wh, wl) = ([p.double() for p in f16_parts(v, d)] for v, d in ((x, 1), (w, 0)))
+    assert relative_norm(xh @ wh + xh @ wl + xl @ wh, want) < THREE_PRODUCTS / 4
+    assert relative_norm(xh @ wh + xh @ wl, want) > 50 * THREE_PRODUCTS
+    assert relative_norm(xh @ wh + xl @ wh, want) > 50 * THREE_PRODUCTS
+    xl[:, :128] = 0
+    assert relative_norm(xh @ wh + xh @ wl + xl @ wh, want) > 20 * THREE_PRODUCTS
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("transpose", [False, True])
+@pytest.mark.parametrize("m,k,n", [(100, 100, 130), (200, 257, 300), (300, 640, 513), (128, 4096, 2048), (256, 4096, 512), (590, 832, 1792),
+                                   (45, 2048, 448), (64, 2048, 2048), (7, 4095, 33),                                # few rows
+                                   (2600, 600, 4104), (2600, 130, 4103), (2601, 1000, 4104), (1100, 2048, 3001)])   # CTA pairs, several partial sums
+def test_float32_products(m, k, n, transpose):
+    """Forward, pre-activation and both gradients against 64 bits by the norm of the error."""
+    from neurotensor_b200 import api
+    gen = generator(m + k + n)
+    x, w, gy = randn(gen, m, k), randn(gen, k, n), randn(gen, m, n)
+    wt = w.t().contiguous() if transpose else w
+    want = x.double() @ w.double()
+    assert relative_norm(api.linear_act(x, wt, transpose_w=transpose), want) < THREE_PRODUCTS
+    _, pre = api.linear_act(x, wt, None, "silu", transpose_w=transpose, want_pre=True)
+    assert relative_norm(pre, want) < THREE_PRODUCTS
+    gx, gw, gb = api.linear_act_backward(x, wt, None, gy, transpose_w=transpose)
+    assert relative_norm(gx, gy.double() @ w.double().t()) < THREE_PRODUCTS
+    assert relative_norm(gw.t() if transpose else gw, x.double().t() @ gy.double()) < THREE_PRODUCTS
+    assert relative_norm(gb, gy.double().sum(0)) < THREE_PRODUCTS
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("up", [13, 20, 26])
+@pytest.mark.parametrize("m,k,n", [(200, 1024, 300), (2600, 600, 4104)])
+def test_float32_values_far_below_their_rows_largest(m, k, n, up):
+    """One value of 2^up in each row of x meets weights of 0: what the others lose is at most 2^-39 of it each."""
+    from neurotensor_b200 import api
+    gen = generator(up)
+    x, w = randn(gen, m, k).clamp(-8, 8), randn(gen, k, n)
+    x[:, 5], w[5] = 2.0 ** up, 0.0
+    want = x.double() @ w.double()
+    lost = 2.0 ** (up - 39) * w.double().abs().sum(0, keepdim=True).expand_as(want)
+    assert float((api.linear_act(x, w).double() - want).norm()) <= THREE_PRODUCTS * float(want.norm()) + float(lost.norm())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pre", [False, True])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16, torch.int8])
+@pytest.mark.parametrize("m,k,n", [(2600, 72, 4104), (2600, 72, 4103), (300, 512, 1024), (16, 4096, 4096)])
+def test_linear_in_place_of_its_residual(m, k, n, dtype, pre):
+    """y in the residual's place, on the epilogues of CTA pairs (residuals by TMA or by rows), single tiles and K slices."""
+    from neurotensor_b200 import _lib, api
+    gen = generator(m + n)
+    out = BF16 if dtype == torch.int8 else dtype
+    bias, r = randn(gen, n, dtype=out), randn(gen, m, n, dtype=out)
+    if dtype == torch.int8:
+        x = torch.randint(-127, 128, (m, k), generator=gen, device="cuda", dtype=dtype)
+        w = torch.randint(-127, 128, (k, n), generator=gen, device="cuda", dtype=dtype)
+        s, v = torch.rand(m, generator=gen, device="cuda") * 0.01, torch.rand(n, generator=gen, device="cuda") * 0.01
+    else:
+        x, w = randn(gen, m, k, dtype=dtype), randn(gen, k, n, scale=k ** -0.5, dtype=dtype)
+    results = []
+    for y in (torch.empty_like(r), r):
+        d, _, keep, stream = api._linear_desc("linear", x, w, bias, "gelu", r, False, out)
+        if dtype == torch.int8:
+            d.x_scale, d.w_scale = s.data_ptr(), v.data_ptr()
+        z = torch.empty_like(r)
+        if pre:
+            d.pre, d.pre_row_stride = z.data_ptr(), n
+        api._run_linear(d, y, stream)
+        results.append((y.clone(), z))
+    assert torch.equal(results[0][0], results[1][0]) and (not pre or torch.equal(results[0][1], results[1][1]))

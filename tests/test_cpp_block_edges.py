@@ -27,3 +27,8 @@ def run(binary, case):
 
 def test_cpp_host_operands_are_refused(binary):
     run(binary, "refusals")
+
+
+@pytest.mark.gpu
+def test_cpp_block_in_16_bits(binary):
+    run(binary, "block16")
