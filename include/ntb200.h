@@ -477,11 +477,14 @@ int ntb200_rms_norm_backward(int dtype, const void* h, int64_t h_row_stride, con
  * whose epilogue does the rest on the fp32 sums; pre (may be NULL) receives x w + bias for the backward pass.
  * dtype F32 / F16 / BF16: everything has that type.  dtype I8: x and w are Int8 with a scale for each row of x and each
  * column of w (fp32), the product is exact in s32, and bias, residual, pre and y have out_dtype (F32 / F16 / BF16).
- * GELU is z Phi(z) with the normal distribution's Phi, GELU_TANH its usual tanh form, SILU z / (1 + e^-z).
+ * GELU is z Phi(z) with the normal distribution's Phi, GELU_TANH its usual tanh form, SILU z / (1 + e^-z); a factor of z
+ * below 2^-126 counts as 0 (silu from z = -87.3 down, where it is 1e-36 and less).
  * y may be the residual itself (same row stride).  16-bit and Int8 products always run on the tensor cores: operands
- * whose rows do not start on 16 bytes are copied into the workspace first.  F32 products over K > 32, or of 6e7
- * multiply-adds and more, run there too, as three products of Float16 parts: an fp32 product's error as long as the
- * values of a row of x (a column of w) lie within 2^13 of its largest one; smaller ones keep 2^-39 of that largest one.
+ * whose rows do not start on 16 bytes are copied into the workspace first.  F32 products run on the CUDA cores, in fp32,
+ * for up to 64 rows below 3e8 multiply-adds (w with a unit stride), for K <= 32 below 6e7 (gradients that sum up to 32
+ * terms: below 2e9), and always under NTB200_FP32_MODE=ffma.  All others run on the tensor cores as three products of
+ * Float16 parts: an fp32 product's error as long as the values of a row of x (a column of w) lie within 2^16 of its
+ * largest one; smaller ones are off by up to 2^-39 of that largest one.
  * An infinite value times one of those below 2^-39 of its row's (column's) largest may give NaN there; all other products with
  * infinities and NaN are those of fp32. */
 typedef enum ntb200_activation {
@@ -529,6 +532,7 @@ int ntb200_linear_act_backward(const ntb200_linear_backward_desc* desc, void* wo
  * p = softmax over the row's entries of teacher / T and q = softmax(logits / T) over all columns,
  *   row_loss = T^2 sum_j p_j (log p_j - log q_{i_j}),   *loss = sum over rows of row_weight * row_loss,
  *   grad = d loss / d logits = row_weight T (q - p)   (a column named twice takes the sum of its p).
+ * The row's loss is a difference of logarithms times T^2: its rounding error is about 2^-23 T^2 log(vocab).
  * A row without entries or with weight 0 has loss 0 and a gradient of zeros.  row_weight [rows] fp32, NULL: 1 / rows (the
  * mean).  grad may be NULL (loss only) or the logits themselves.  At most 1024 entries per row. */
 int ntb200_distill_topk(int dtype, const void* logits, int64_t logits_row_stride, int teacher_dtype, const void* teacher,

@@ -310,7 +310,7 @@ __device__ __noinline__ void finish_row16(float* y, float* pre, const float* res
 
 // The Float32 split kernels' running sums: each thread finishes its own row.  A warp that took column by column through shared
 // memory instead left [8192, 1024] x [1024, 4096] at 387 us, with gelu at 517, its few warps waiting for one row after another;
-// now 247 and 294 (three products: 0.21 PFLOP, 129 us at the measured rate of Float16 products; the rest is the split pass and
+// now 237 and 306 (three products: 0.21 PFLOP, 129 us at the measured rate of Float16 products; the rest is the split pass and
 // the sums taken over every 128 of K).
 template <int HC>
 __device__ __forceinline__ void finish_running(const UmmaParams& p, const float (&run)[HC], float* staged, int row0, int lane, int col_base) {

@@ -149,8 +149,9 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const FewRows f) 
 
 // ---- Float32 as three Float16 products ----------------------------------------------------------------------------------
 // A row of A (a column of B) is scaled by a power of two that brings its largest finite value to [2^14, 2^15), then
-// x = hi + lo with hi = fp16(x), lo = fp16(x - hi): |x - hi - lo| <= 2^-24 |x| down to 2^-13 of the largest value and below
-// 2^-39 of it always, so a.b = hi.hi + hi.lo + lo.hi + O(2^-23 |a||b|).  kind::f16 runs at twice TF32's rate and a value's two
+// x = hi + lo with hi = fp16(x), lo = fp16(x - hi): |x - hi| <= 2^-11 |x| and |x - hi - lo| <= 2^-23 |x| down to 2^-16 of the
+// largest value (below that lo is subnormal: the error stays below 2^-39 of the largest value).  a.b = hi.hi + hi.lo + lo.hi, less
+// lo.lo, up to 2^-22 |a||b|, and the parts' own errors, up to 2^-22 together; by their norm the three come to about 1e-7.  kind::f16 runs at twice TF32's rate and a value's two
 // parts take 4 bytes instead of 8: [512, 1024] x [1024, 4096] took 30 us as three TF32 products.  The scales are undone by
 // the epilogue's row and column factors (powers of two, exact).  Parts keep the operand's direction (tcgen05 takes
 // Float16 tiles along either axis), so nothing is transposed.  [512, 1024] x [1024, 4096] with gelu: 34 us (46 when the split read
@@ -396,7 +397,8 @@ __global__ void __launch_bounds__(256) join_slabs_kernel(const float* __restrict
     }
 }
 
-// Slabs of rows of the bias gradient's partial sums: four blocks per SM, all resident at once, of at least 64 rows each.
+// Slabs of rows of the bias gradient's partial sums: four blocks per SM, all resident at once, of at least 64 rows each.  148 SMs
+// here and in plan_few: the workspace's size, which follows, depends on the call's sizes alone.
 long long act_slabs(int64_t m, int64_t n, int vec) {
     const int64_t col_blocks = (n + 32 * vec - 1) / (32 * vec);
     int64_t slabs = std::max<int64_t>(1, std::min<int64_t>((m + 63) / 64, 148 * 4 / std::min<int64_t>(col_blocks, 148 * 4)));

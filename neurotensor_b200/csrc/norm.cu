@@ -465,8 +465,11 @@ struct BackArgs {
 // The same layout; each thread keeps the sums of gy xhat of its columns in registers over all rows its block takes.
 // kCut: a thread's columns are the same for all rows of one lead, so a block takes rows of one lead only: rows first,
 // first + step, ... with a step that is a multiple of `period`, the number of rows after which the leads repeat.
-// 3406 x 14054 bf16 (rows 12 bytes past a boundary, then 8, ...): forward 136 us, backward 205 us, bound by the cut granules'
-// instructions and the weight's single loads; element by element the two took 851 us.
+// 3406 x 14054 bf16 (rows 12 bytes past a boundary, then 8, ...): forward 136 us, backward 205 us; element by element the two took
+// 851 us.  What bounds them: the cut granules' instructions and the weight's single loads, and in the backward pass registers: at
+// 1024 threads a thread's two granules, their weights and sums do not fit the 64 it may have (spill stores of <.., 8, 2, true, 1024>
+// 220 bytes in BFloat16, 896 in Float16, which the compiler holds to 32 registers; of <.., 8, 4, *, 1024>, rows above 16384, 1108 to
+// 1768).
 template <class T, int V, int P, bool kCut, int kThreads>
 __global__ void __launch_bounds__(kThreads) norm_backward_kernel(const BackArgs a, int G, int period) {
     extern __shared__ float s_gw[];      // [groups - 1][cols] while the groups of a block are joined
