@@ -5,10 +5,9 @@
 //   L = T^2 sum_j p_j (log p_j - log q_{i_j})                    loss = sum over rows of weight L
 //   dloss/ds_v = weight T (q_v - sum_{j: i_j = v} p_j)
 //
-// A row without entries, or with weight 0, has L = 0 and a zero gradient, whatever its logits are (those of a row of weight 0 are
-// not read).  The softmax
-// statistics are fp32: a running maximum and sum per thread, joined in a fixed order.  The kernel moves bytes: the
-// logits once in, the gradient once out.
+// A row without entries, or with weight 0, has L = 0 and a zero gradient, whatever its logits are (those of a row of weight 0
+// are not read).  The softmax statistics are fp32: a running maximum and sum per thread, joined in a fixed order.  The kernel
+// moves bytes: the logits once in, the gradient once out.
 #include <algorithm>
 
 #include "internal.h"

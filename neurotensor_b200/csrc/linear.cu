@@ -151,11 +151,11 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const FewRows f) 
 // A row of A (a column of B) is scaled by a power of two that brings its largest finite value to [2^14, 2^15), then
 // x = hi + lo with hi = fp16(x), lo = fp16(x - hi): |x - hi| <= 2^-11 |x| and |x - hi - lo| <= 2^-23 |x| down to 2^-16 of the
 // largest value (below that lo is subnormal: the error stays below 2^-39 of the largest value).  a.b = hi.hi + hi.lo + lo.hi, less
-// lo.lo, up to 2^-22 |a||b|, and the parts' own errors, up to 2^-22 together; by their norm the three come to about 1e-7.  kind::f16 runs at twice TF32's rate and a value's two
-// parts take 4 bytes instead of 8: [512, 1024] x [1024, 4096] took 30 us as three TF32 products.  The scales are undone by
-// the epilogue's row and column factors (powers of two, exact).  Parts keep the operand's direction (tcgen05 takes
-// Float16 tiles along either axis), so nothing is transposed.  [512, 1024] x [1024, 4096] with gelu: 34 us (46 when the split read
-// its operands twice).
+// lo.lo, up to 2^-22 |a||b|, and the parts' own errors, up to 2^-22 together; by their norm the three come to 8e-8 of the result.
+// kind::f16 runs at twice TF32's rate and a value's two parts take 4 bytes instead of 8: [512, 1024] x [1024, 4096] took 30 us as
+// three TF32 products.  The scales are undone by the epilogue's row and column factors (powers of two, exact).  Parts keep the
+// operand's direction (tcgen05 takes Float16 tiles along either axis), so nothing is transposed.  [512, 1024] x [1024, 4096] with
+// gelu: 34 us (46 when the split read its operands twice).
 struct SplitF16Job {
     const float* src;
     __half* hi;

@@ -64,6 +64,29 @@ def test_norm_in_place_of_an_input(rows, n, place):
     assert torch.equal(results[0][0], results[1][0]) and torch.equal(results[0][1], results[1][1])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,n", [(5, 1001), (2600, 4096), (9600, 264)])      # the last two stream
+def test_norm_stream_in_place(rows, n, dtype):
+    """h in the place of x or of the residual, grad_x in the place of h, grad_y or grad_h."""
+    from neurotensor_b200 import _lib, api
+    L, gen = _lib.lib(), generator(n)
+    x, r, w, gh = randn(gen, rows, n, dtype=dtype), randn(gen, rows, n, dtype=dtype), randn(gen, n, dtype=dtype), randn(gen, rows, n, dtype=dtype)
+    y, h, rstd = api.rms_norm(x, w, residual=r)
+    for place in (0, 1):
+        ins, out = [x.clone(), r.clone()], torch.empty_like(y)
+        _lib.check(L.ntb200_rms_norm(code(dtype), ins[0].data_ptr(), n, ins[1].data_ptr(), n, w.data_ptr(), out.data_ptr(), ins[place].data_ptr(), None, rows,
+                                     n, 1e-6, api._stream()))
+        assert torch.equal(out, y) and torch.equal(ins[place], h) and torch.equal(ins[1 - place], (x, r)[1 - place])
+    gx, gw = api.rms_norm_backward(h, w, rstd, x, grad_h=gh)
+    ws = torch.empty(L.ntb200_rms_norm_backward_workspace_bytes(rows, n), dtype=torch.uint8, device="cuda")
+    for place in (0, 1, 2):
+        ins, gw2 = [h.clone(), x.clone(), gh.clone()], torch.empty_like(gw)
+        _lib.check(L.ntb200_rms_norm_backward(code(dtype), ins[0].data_ptr(), n, w.data_ptr(), rstd.data_ptr(), ins[1].data_ptr(), n, ins[2].data_ptr(), n,
+                                              ins[place].data_ptr(), gw2.data_ptr(), ws.data_ptr(), rows, n, api._stream()))
+        assert torch.equal(ins[place], gx) and torch.equal(gw2, gw)
+
+
 # ---- norm: h without a residual -------------------------------------------------------------------------------------
 
 @pytest.mark.gpu
