@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(kPieceThreads, kBlocks) distill_piece_kernel(c
     float m = -INFINITY;
     if (granules > g1 && granules - 1 >= g0 && tid < V) m = RowType<T>::up(mem[(granules - 1) * V + tid]);
     if (g0 == 1 && tid < V) m = fmaxf(m, RowType<T>::up(mem[tid]));
-    const bool landed = g1 <= g0 || mbar_wait(smem_u32(&sh.bar), 0, &sh.abort_flag);
+    const bool landed = __all_sync(0xffffffffu, g1 <= g0 || mbar_wait(smem_u32(&sh.bar), 0, &sh.abort_flag));   // for every lane of the warp
 #pragma unroll 4
     for (int v = g0 + tid; v < g1; v += kPieceThreads) m = fmaxf(m, pack_max(reinterpret_cast<const Pack<T, V>*>(mem)[v]));
     if (!landed && lane == 0) {
